@@ -13,7 +13,9 @@ Drop-in ops with the reference's call signatures (ref_torch / v4mlx), each a tor
 There is no CPU path: the ops raise on CPU tensors and when libdsv4.so is missing.
 """
 from . import _lib
-from .compressor import CompressorStep, compressor_decode_pair, compressor_decode_step, compressor_prefill
+from .chunk import chunk_attention, chunk_commit, chunk_rows
+from .compressor import (CompressorStep, compressor_chunk, compressor_decode_pair, compressor_decode_step,
+                         compressor_prefill)
 from .decode import DecodeRunner, SparseMLACache, decode_attention, window_attention
 from .hc import hc_head, hc_post, hc_pre
 from .indexer import indexer_scores, indexer_topk, indexer_topk_into
@@ -23,13 +25,15 @@ from .prefill import (CompressorWeights, PrefillStaging, ShardedPrefill, attend_
                       sparse_mla_prefill_host)
 from .mla import (N_GROUPS, N_HEADS, HEAD_DIM, O_LORA, ROPE_HD, QuantWeight, kv_proj, linear, linear_multi, o_grouped,
                   q_down, q_up, quantize_int8_g64)
+from .pages import pages_compact, pages_fork, pages_free, pages_reserve
 from .norm_rope import (apply_rotary_emb, norm_rope, perhead_norm, precompute_freqs, precompute_freqs_cis,
                         rmsnorm, rope, rope_freqs)
 from .sparse_attn import get_window_topk_idxs, sparse_attn, sparse_attn_rope
 
 __all__ = [
     "sparse_attn", "sparse_attn_rope", "get_window_topk_idxs", "compressor_prefill", "compressor_decode_step",
-    "compressor_decode_pair", "CompressorStep",
+    "compressor_decode_pair", "CompressorStep", "compressor_chunk", "chunk_attention", "chunk_rows", "chunk_commit",
+    "pages_reserve", "pages_free", "pages_fork", "pages_compact",
     "rmsnorm", "perhead_norm", "apply_rotary_emb", "precompute_freqs", "precompute_freqs_cis", "norm_rope",
     "rope", "rope_freqs", "indexer_topk", "indexer_scores", "indexer_topk_into", "linear", "linear_multi", "q_down", "q_up",
     "kv_proj", "o_grouped", "QuantWeight", "quantize_int8_g64", "SparseMLACache", "decode_attention", "DecodeRunner",

@@ -16,7 +16,7 @@ _DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.int32: I32, torch.int6
           torch.int8: I8}
 
 STATUS = {0: "OK", 1: "INVALID_ARGUMENT", 2: "UNSUPPORTED_DTYPE", 3: "CUDA", 4: "INDEX_OUT_OF_RANGE",
-          5: "WAIT_TIMEOUT", 6: "WORKSPACE"}
+          5: "WAIT_TIMEOUT", 6: "WORKSPACE", 7: "NO_PAGES"}
 
 vp, i32, i64, f32, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 
@@ -114,6 +114,27 @@ class DecodeRowsParams(ctypes.Structure):
                 ("bt_stride", i32), ("max_comp", i32)]
 
 
+class Chunk(ctypes.Structure):
+    _fields_ = [("cu_seqlens", vp), ("start", vp), ("seqs", vp), ("win_base", vp), ("block_table", vp),
+                ("comp_base", i64), ("stage_base", i64), ("pool_rows", i64), ("n", i32), ("total", i32), ("slots", i32),
+                ("window", i32), ("ratio", i32), ("page", i32), ("bt_stride", i32), ("max_comp", i32)]
+
+
+class CompressorChunkParams(ctypes.Structure):
+    _fields_ = [("kv", vp), ("score", vp), ("ape", vp), ("norm_w", vp), ("ring_kv", vp), ("ring_score", vp), ("out", vp),
+                ("freqs", vp), ("cu_seqlens", vp), ("start", vp), ("seqs", vp), ("block_table", vp), ("out_base", i64),
+                ("out_rows", i64), ("n", i32), ("total", i32), ("slots", i32), ("bt_stride", i32), ("page", i32), ("max_comp", i32),
+                ("head_dim", i32), ("ratio", i32), ("rope_dim", i32), ("norm_dtype", i32), ("out_dtype", i32),
+                ("act_quant", i32), ("eps", f32), ("key_image", vp), ("key_inv", vp), ("key_norm_max", vp)]
+
+
+class Pages(ctypes.Structure):
+    _fields_ = [("pool", vp), ("win_base", vp), ("block_table", vp), ("refs", vp), ("k_idx", vp), ("key_image", vp),
+                ("key_inv", vp), ("key_norm_max", vp), ("ring_kv", vp), ("ring_score", vp), ("ring_k_idx", vp),
+                ("ring_s_idx", vp), ("comp_base", i64), ("slots", i32), ("n_pages", i32), ("bt_stride", i32),
+                ("page", i32), ("max_comp", i32), ("window", i32), ("head_dim", i32), ("idx_dim", i32), ("ratio", i32)]
+
+
 # every symbol include/dsv4.h declares, with its ctypes signature
 SIGNATURES = {
     "dsv4_last_error": (ctypes.c_char_p, []),
@@ -136,6 +157,14 @@ SIGNATURES = {
     "dsv4_compressor_decode": (ctypes.c_int, [ctypes.POINTER(CompressorDecodeParams), vp]),
     "dsv4_compressor_decode_pair": (ctypes.c_int, [ctypes.POINTER(CompressorDecodeParams),
                                                    ctypes.POINTER(CompressorDecodeParams), vp]),
+    "dsv4_chunk_rows": (ctypes.c_int, [ctypes.POINTER(Chunk), vp, vp, vp, i64, i32, vp, vp]),
+    "dsv4_chunk_commit": (ctypes.c_int, [ctypes.POINTER(Chunk), vp, i32, vp]),
+    "dsv4_compressor_chunk": (ctypes.c_int, [ctypes.POINTER(CompressorChunkParams), vp]),
+    "dsv4_pages_workspace_size": (sz, [ctypes.POINTER(Pages), i32]),
+    "dsv4_pages_free": (ctypes.c_int, [ctypes.POINTER(Pages), vp, i32, vp]),
+    "dsv4_pages_reserve": (ctypes.c_int, [ctypes.POINTER(Pages), vp, vp, i32, i32, vp, sz, vp]),
+    "dsv4_pages_fork": (ctypes.c_int, [ctypes.POINTER(Pages), vp, vp, vp, i32, vp, sz, vp]),
+    "dsv4_pages_compact": (ctypes.c_int, [ctypes.POINTER(Pages), vp, vp, sz, vp]),
     "dsv4_decode_rows": (ctypes.c_int, [ctypes.POINTER(DecodeRowsParams), vp]),
     "dsv4_hc_pre": (ctypes.c_int, [ctypes.POINTER(HcParams), vp]),
     "dsv4_hc_workspace_size": (ctypes.c_size_t, [i64, i32, i32, i32]),
@@ -199,6 +228,22 @@ def dtype_code(t):
 
 def stream_of(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        return False
+
+
+_HERE_ALREADY = _Here()
+
+
+def device_of(t):
+    """A context in which `t`'s device is the current one (kernels launch on the current device)."""
+    return _HERE_ALREADY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def require_cuda(*ts):

@@ -1,0 +1,132 @@
+"""A chunk of new tokens per sequence over the device-resident state (`SparseMLACache`).
+
+The reference extends its state one token at a time (oracle/v4_fast.py:82-122) or builds it from
+position 0 (oracle/v4_prefill.py). These ops take the step between: several new tokens of each
+sequence on top of what the cache holds, for a prompt taken in chunks, a further turn of a
+conversation, or drafted tokens that are checked at once. The order of a layer's chunk is
+
+  positions, rows = chunk_rows(cache, cu_seqlens, start, total)   where the tokens are
+  norm_rope into the pool at `rows`                               their kv rows, staged
+  compressor_chunk(...)                                           the compressed rows they complete
+  o = chunk_attention(cache, q, sink, cu_seqlens, start)          window + compressed rows of each token
+  chunk_commit(cache, cu_seqlens, start, total)                   the staged rows into the window rings
+
+`DecodeBlock.extend` runs it. Sequence b has the tokens [cu_seqlens[b], cu_seqlens[b+1]) of the batch,
+the first of them at position start[b] of cache slot seqs[b] (default b). Rows of the batch behind
+cu_seqlens[-1] belong to no sequence (a padded batch).
+"""
+import ctypes
+
+import torch
+
+from . import _lib as L
+from .norm_rope import rope_freqs
+from .sparse_attn import sparse_attn_into
+
+
+def _index_tensor(name, t, dev, n=None):
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.dim() != 1:
+        raise TypeError(f"{name} must be a 1-d int32 tensor")
+    L.require_cuda(t)
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+    if n is not None and t.numel() != n:
+        raise ValueError(f"{name} has {t.numel()} values, the chunk has {n} sequences")
+    return t.to(torch.int32).contiguous()
+
+
+def _chunk(cache, cu_seqlens, start, seqs, total):
+    """dsv4_chunk of the cache, and the tensors it points to."""
+    dev = cache.kv_pool.device
+    cu = _index_tensor("cu_seqlens", cu_seqlens, dev)
+    n = cu.numel() - 1
+    if n < 0:
+        raise ValueError("cu_seqlens holds one value more than there are sequences")
+    start = _index_tensor("start", start, dev, n)
+    seqs = None if seqs is None else _index_tensor("seqs", seqs, dev, n)
+    if seqs is None and n > cache.batch:
+        raise ValueError(f"a chunk of {n} sequences, the cache has {cache.batch} slots")
+    if total > cache.max_chunk:
+        raise ValueError(f"a chunk of {total} tokens, the cache stages {cache.max_chunk} (SparseMLACache(max_chunk=...))")
+    c = L.Chunk()
+    c.cu_seqlens, c.start, c.seqs = cu.data_ptr(), start.data_ptr(), None if seqs is None else seqs.data_ptr()
+    c.win_base, c.block_table = cache.win_base.data_ptr(), cache.block_table.data_ptr() if cache.compressed else None
+    c.comp_base, c.stage_base, c.pool_rows = cache.comp_base, cache.stage_base, cache.kv_pool.shape[0]
+    c.n, c.total, c.slots, c.window = n, total, cache.batch, cache.window
+    c.ratio, c.page, c.bt_stride, c.max_comp = cache.ratio, cache.page, cache.block_table.shape[1], cache.max_comp
+    return c, (cu, start, seqs)
+
+
+def chunk_rows(cache, cu_seqlens, start, total, seqs=None):
+    """(positions int32 [total], rows int64 [total]): the position of each token of the chunk and the
+    pool row where its kv row is staged. Positions behind the last sequence are 0."""
+    c, keep = _chunk(cache, cu_seqlens, start, seqs, total)
+    dev = cache.kv_pool.device
+    positions = torch.zeros(total, dtype=torch.int32, device=dev) if c.n == 0 else \
+        torch.empty(total, dtype=torch.int32, device=dev)
+    rows = torch.empty(total, dtype=torch.int64, device=dev)
+    with L.device_of(positions):
+        if c.n == 0:
+            return positions, torch.arange(cache.stage_base, cache.stage_base + total, device=dev)
+        L.check(L.lib().dsv4_chunk_rows(ctypes.byref(c), L.ptr(positions), L.ptr(rows), None, 0, 0, None,
+                                        L.stream_of(positions)))
+    return positions, rows
+
+
+def chunk_commit(cache, cu_seqlens, start, total, seqs=None):
+    """Move the chunk's rows into the window rings (the last `window` of each sequence), after its
+    attention: what the decode steps and the next chunk see."""
+    c, keep = _chunk(cache, cu_seqlens, start, seqs, total)
+    with L.device_of(cache.kv_pool):
+        L.check(L.lib().dsv4_chunk_commit(ctypes.byref(c), L.ptr(cache.kv_pool), cache.head_dim,
+                                          L.stream_of(cache.kv_pool)))
+
+
+def _attend(cache, c, q, sink, rows, scale, freqs, out_dtype):
+    """Every token's list as an index tensor, and the sparse attention over it."""
+    total = q.shape[0]
+    cols = cache.max_comp if rows is None else rows.shape[1]
+    idx = torch.empty((total, cache.window + cols), dtype=torch.int32, device=q.device)
+    pos = torch.empty(total, dtype=torch.int32, device=q.device)
+    L.check(L.lib().dsv4_chunk_rows(ctypes.byref(c), L.ptr(pos), None, L.ptr(idx), idx.shape[1], cols, L.ptr(rows),
+                                    L.stream_of(q)))
+    out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    return sparse_attn_into(out, q, cache.kv_pool, sink, idx, scale, freqs, pos, 2 * freqs.numel())
+
+
+def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, scale=None, freqs=None,
+                    out_dtype=torch.bfloat16):
+    """Attention of a chunk of new tokens over the cache, their kv rows staged (`chunk_rows`) and their
+    compressed rows written (`compressor_chunk`).
+
+    q [total, 64, 512] bf16 after the per-head norm and RoPE (`norm_rope`), sink [64]. The token at
+    position p sees the window rows of positions p-window+1 .. p, from the ring before the chunk and from
+    the stage in it, and every compressed entry j < (p+1) // ratio (the list of
+    oracle/decode_engine.py:110-116), or with `rows` (int32 [total, k] pool rows, -1 for none: the
+    indexer's selection) those instead. Returns o [total, 64, 512] after the inverse RoPE; what it holds
+    behind the last sequence is not defined."""
+    L.require_cuda(q, sink, rows, freqs)
+    if q.dim() != 3 or q.shape[2] != cache.head_dim:
+        raise ValueError(f"chunk_attention: q must be [total, heads, {cache.head_dim}], got {tuple(q.shape)}")
+    if q.dtype != torch.bfloat16:
+        raise TypeError(f"chunk_attention: q is the bf16 output of norm_rope, got {q.dtype}")
+    if q.shape[1] != 64 or sink.numel() != 64:
+        raise ValueError(f"chunk_attention: 64 heads, got q {tuple(q.shape)} and {sink.numel()} sinks")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"chunk_attention: out_dtype must be bfloat16 or float32, got {out_dtype}")
+    if q.device != cache.kv_pool.device or sink.device != q.device or (rows is not None and rows.device != q.device):
+        raise ValueError("chunk_attention: q, sink and rows must be on the cache's device")
+    total = q.shape[0]
+    if rows is not None:
+        if rows.dim() != 2 or rows.shape[0] != total or rows.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"chunk_attention: rows must be int32 [{total}, k], got {rows.dtype} {tuple(rows.shape)}")
+        rows = rows.to(torch.int32).contiguous()
+    freqs = rope_freqs(64, q.device) if freqs is None else freqs.float().contiguous()
+    if freqs.numel() > cache.head_dim // 2:
+        raise ValueError("chunk_attention: more rotation frequencies than pairs of dims")
+    scale = cache.head_dim ** -0.5 if scale is None else float(scale)
+    c, keep = _chunk(cache, cu_seqlens, start, seqs, total)
+    if total == 0 or c.n == 0:
+        return torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    with L.device_of(q):
+        return _attend(cache, c, q.contiguous(), sink.float().contiguous(), rows, scale, freqs, out_dtype)

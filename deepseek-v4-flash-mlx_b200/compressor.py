@@ -248,3 +248,97 @@ def compressor_decode_pair(a: CompressorStep, b: CompressorStep, positions, rati
                                int(a.head_dim), int(a.act_quant),
                                b.proj[0], b.proj[1], b.ape, b.norm_w, b.ring_kv, b.ring_score, b.out, b.out_rows,
                                int(b.head_dim), int(b.act_quant), img, inv, nmax, int(stride))
+
+
+@torch.library.custom_op("dsv4::compressor_chunk",
+                         mutates_args=("ring_kv", "ring_score", "out", "key_image", "key_inv", "key_norm_max"),
+                         device_types="cuda")
+def _compressor_chunk_op(kv: torch.Tensor, score: torch.Tensor, cu_seqlens: torch.Tensor, start: torch.Tensor,
+                         seqs: torch.Tensor | None, ape: torch.Tensor, norm_w: torch.Tensor | None, ring_kv: torch.Tensor,
+                         ring_score: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor | None, page: int,
+                         out_base: int, max_comp: int, head_dim: int, ratio: int, rope_head_dim: int, freqs: torch.Tensor,
+                         eps: float, key_image: torch.Tensor | None, key_inv: torch.Tensor | None,
+                         key_norm_max: torch.Tensor | None, act_quant: int) -> None:
+    _chunk_into(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, page, out_base,
+                max_comp, head_dim, ratio, rope_head_dim, freqs, eps, key_image, key_inv, key_norm_max, act_quant)
+
+
+@_compressor_chunk_op.register_fake
+def _(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, page, out_base, max_comp,
+      head_dim, ratio, rope_head_dim, freqs, eps, key_image, key_inv, key_norm_max, act_quant):
+    return None
+
+
+def _chunk_into(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, page, out_base,
+                max_comp, head_dim, ratio, rope_head_dim, freqs, eps, key_image, key_inv, key_norm_max, act_quant):
+    p = L.CompressorChunkParams()
+    p.kv, p.score, p.ape, p.norm_w = L.ptr(kv), L.ptr(score), L.ptr(ape), L.ptr(norm_w)
+    p.ring_kv, p.ring_score, p.out, p.freqs = L.ptr(ring_kv), L.ptr(ring_score), L.ptr(out), L.ptr(freqs)
+    p.cu_seqlens, p.start, p.seqs, p.block_table = L.ptr(cu_seqlens), L.ptr(start), L.ptr(seqs), L.ptr(block_table)
+    p.out_base, p.out_rows = out_base, out.numel() // head_dim
+    p.n, p.total, p.slots = cu_seqlens.numel() - 1, kv.shape[0], ring_kv.shape[0]
+    p.bt_stride, p.page = (block_table.shape[1], page) if block_table is not None else (0, 1)
+    p.max_comp, p.head_dim, p.ratio, p.rope_dim = max_comp, head_dim, ratio, rope_head_dim
+    p.norm_dtype = L.dtype_code(norm_w) if norm_w is not None else L.F32
+    p.out_dtype, p.act_quant, p.eps = L.dtype_code(out), act_quant, eps
+    p.key_image, p.key_inv, p.key_norm_max = L.ptr(key_image), L.ptr(key_inv), L.ptr(key_norm_max)
+    with L.device_of(kv):
+        L.check(L.lib().dsv4_compressor_chunk(ctypes.byref(p), L.stream_of(kv)))
+
+
+def compressor_chunk(proj, cu_seqlens, start, ape, norm_w, ring_kv, ring_score, out, max_comp, block_table=None, page=0,
+                     out_base=0, seqs=None, head_dim=512, ratio=4, rope_head_dim=64, freqs=None, eps=1e-6, key_image=None,
+                     act_quant=False, rotate=False):
+    """A chunk of new tokens of each sequence through its compressor: what `compressor_decode_step` on
+    one token after the other leaves in the rings and the emitted rows (oracle/decode_engine.py:96-105),
+    in one launch.
+
+    proj = (kv, score) fp32 [total, 2*head_dim], the projections of the tokens; sequence b has the
+    tokens [cu_seqlens[b], cu_seqlens[b+1]), the first at position start[b] of slot seqs[b] (default b),
+    int32 tensors on the device. Entry j of slot s goes to row out_base + block_table[s, j // page] *
+    page + j % page of `out`, or without a table (the indexer keys) to row out_base + s * max_comp + j.
+    An entry past max_comp, or whose page the table does not have, raises INDEX_OUT_OF_RANGE on the
+    device error word and is not stored. `key_image` (image, inv, norm_max: the cache's), `act_quant` and
+    `rotate` as in `compressor_decode_step`. The custom op `dsv4::compressor_chunk`."""
+    kv, score = proj
+    L.require_cuda(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, freqs)
+    if kv.dtype != torch.float32 or score.dtype != torch.float32 or kv.shape != score.shape or kv.dim() != 2 or \
+            kv.shape[1] != 2 * head_dim:
+        raise ValueError(f"compressor_chunk: kv and score must be float32 [total, {2 * head_dim}]")
+    for name, r in (("ring_kv", ring_kv), ("ring_score", ring_score)):
+        if r.dtype != torch.float32 or r.dim() != 3 or r.shape[1:] != (2 * ratio, 2 * head_dim) or not r.is_contiguous():
+            raise ValueError(f"compressor_chunk: {name} must be contiguous float32 [slots, {2 * ratio}, {2 * head_dim}]")
+    if ring_kv.shape[0] != ring_score.shape[0]:
+        raise ValueError("compressor_chunk: ring_kv and ring_score have different slots")
+    if out.shape[-1] != head_dim or not out.is_contiguous() or out.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"compressor_chunk: out must be contiguous rows of {head_dim} float32 or bfloat16")
+    n, slots = cu_seqlens.numel() - 1, ring_kv.shape[0]
+    if n < 0 or start.numel() != n or (seqs is not None and seqs.numel() != n) or (seqs is None and n > slots):
+        raise ValueError(f"compressor_chunk: cu_seqlens, start and seqs name {n}, {start.numel()} and "
+                         f"{None if seqs is None else seqs.numel()} sequences ({slots} slots)")
+    for name, t in (("cu_seqlens", cu_seqlens), ("start", start), ("seqs", seqs), ("block_table", block_table)):
+        if t is not None and t.dtype != torch.int32:
+            raise TypeError(f"compressor_chunk: {name} must be int32, got {t.dtype}")
+    if block_table is not None and (block_table.dim() != 2 or block_table.shape[0] < slots or page <= 0 or
+                                    not block_table.is_contiguous()):
+        raise ValueError("compressor_chunk: block_table must be contiguous int32 [slots, pages] with a page size")
+    rows = out.numel() // head_dim
+    if block_table is None and out_base + slots * max_comp > rows:
+        raise ValueError(f"compressor_chunk: out has {rows} rows, {slots} slots of {max_comp} entries need "
+                         f"{out_base + slots * max_comp}")
+    if ape.shape != (ratio, 2 * head_dim) or ape.dtype != torch.float32:
+        raise ValueError(f"compressor_chunk: ape must be float32 [{ratio}, {2 * head_dim}]")
+    if norm_w is not None and norm_w.numel() != head_dim:
+        raise ValueError(f"compressor_chunk: norm_w must have {head_dim} values")
+    freqs = rope_freqs(rope_head_dim, kv.device) if freqs is None else freqs.float().contiguous()
+    if 2 * freqs.numel() < rope_head_dim:
+        raise ValueError("compressor_chunk: fewer rotation frequencies than rope_head_dim needs")
+    if norm_w is not None and norm_w.dtype not in (torch.float32, torch.bfloat16):
+        norm_w = norm_w.float()
+    img, inv, nmax = key_image if key_image is not None else (None, None, None)
+    # traced programs see the custom op; an eager call goes straight to it
+    f = _compressor_chunk_op if torch.compiler.is_compiling() else _chunk_into
+    f(kv.contiguous(), score.contiguous(), cu_seqlens.contiguous(), start.contiguous(),
+      None if seqs is None else seqs.contiguous(), ape.contiguous(), None if norm_w is None else norm_w.contiguous(),
+      ring_kv, ring_score, out, block_table, int(page), int(out_base), int(max_comp), int(head_dim), int(ratio),
+      int(rope_head_dim), freqs, float(eps), img, inv, nmax, 2 if rotate else int(act_quant))

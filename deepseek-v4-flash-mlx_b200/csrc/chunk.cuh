@@ -1,0 +1,52 @@
+// A chunk of new tokens over the paged cache, as the kernels read it (dsv4_chunk of dsv4.h).
+#pragma once
+#include "common.cuh"
+
+namespace dsv4 {
+
+struct ChunkToken {
+  int seq;    // index of the chunk's sequence, -1 behind the last one
+  int first;  // its first token
+  int start;  // position of that token
+  int pos;    // position of this token
+};
+
+// cache slot of the chunk's sequence b; -1 (and the error word) when seqs names none
+__device__ __forceinline__ int chunk_slot(const dsv4_chunk& c, int b) {
+  const int s = c.seqs ? c.seqs[b] : b;
+  if (s < 0 || s >= c.slots) {
+    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+    return -1;
+  }
+  return s;
+}
+
+// the sequence of token t: the last b with cu_seqlens[b] <= t (empty sequences own no token)
+__device__ __forceinline__ ChunkToken chunk_token(const dsv4_chunk& c, int t) {
+  ChunkToken k = {-1, 0, 0, 0};
+  if (t >= c.cu_seqlens[c.n]) return k;
+  int lo = 0, hi = c.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (c.cu_seqlens[mid] <= t)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  k.first = c.cu_seqlens[lo];
+  k.start = c.start[lo];
+  k.pos = k.start + (t - k.first);
+  if (t >= k.first && k.start >= 0 && (c.seqs == nullptr || (c.seqs[lo] >= 0 && c.seqs[lo] < c.slots))) k.seq = lo;
+  return k;
+}
+
+// compressed entries seen at position pos
+__device__ __forceinline__ int chunk_seen(const dsv4_chunk& c, int pos) {
+  if (c.max_comp == 0) return 0;
+  const int e = (pos + 1) / c.ratio;
+  return e < c.max_comp ? e : c.max_comp;
+}
+
+int check_chunk(const dsv4_chunk* c, const char* who);
+
+}  // namespace dsv4

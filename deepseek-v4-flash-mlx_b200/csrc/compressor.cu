@@ -50,6 +50,7 @@ __device__ __forceinline__ float block_max(float v, float* red) {
 }
 
 __device__ __forceinline__ void store_pair(float v0, float v1, int c, int d, void* out, int64_t orow, int out_dtype) {
+  if (orow < 0) return;  // an entry whose page is not assigned: dsv4_decode_rows has raised the error word
   const int64_t off = orow * d + c;
   if (out_dtype == DSV4_BF16)
     *reinterpret_cast<uint32_t*>(reinterpret_cast<__nv_bfloat16*>(out) + off) = pack_bf16x2(v0, v1);
@@ -268,32 +269,38 @@ __device__ __forceinline__ void st2(float* p, float2 v) { *reinterpret_cast<floa
 // the emitted row (indexer key, head_dim 128 = 64 pairs held by threads 0..63, fp32 values as
 // stored) added to the key image: scaled and split as dsv4_indexer_key_image does it, its inverse
 // scale, and the entry's norm maximum raised
-template <int NP>
-__device__ __forceinline__ void append_key_image(const dsv4_compressor_decode_params& p, const float (&vals)[NP][2],
-                                                 float* red) {
+__device__ __forceinline__ void append_key_row(float v0, float v1, int head_dim, uint8_t* key_image, float* key_inv,
+                                               float* key_norm_max, int64_t image_stride, int64_t seq, int64_t j,
+                                               float* red) {
   const int tid = threadIdx.x;
-  const bool mine = 2 * tid < p.head_dim;
-  const float v0 = mine ? vals[0][0] : 0.f, v1 = mine ? vals[0][1] : 0.f;
+  const bool mine = 2 * tid < head_dim;
+  if (!mine) v0 = v1 = 0.f;
   const float mx = block_max(fmaxf(fabsf(v0), fabsf(v1)), red);
   const float ss = block_sum(fmaf(v1, v1, v0 * v0), red);
-  const int64_t orow = p.out_rows[blockIdx.x];
-  const int64_t seq = orow / p.image_stride, j = orow % p.image_stride;
-  const int64_t tiles = (p.image_stride + 127) / 128;
+  const int64_t tiles = (image_stride + 127) / 128;
   const int sh = itc::row_shift(mx);
   if (mine) {
     uint32_t hi, lo;
     const float up = itc::pow2(sh);
     itc::split2(v0 * up, v1 * up, &hi, &lo);
     const int c = 2 * tid;
-    uint8_t* img = p.key_image + (seq * tiles + j / 128) * itc::IMG_TILE_BYTES;
+    uint8_t* img = key_image + (seq * tiles + j / 128) * itc::IMG_TILE_BYTES;
     const uint32_t off = itc::key_off(static_cast<int>(j % 128), c >> 2) + ((c >> 1) & 1) * 4;
     *reinterpret_cast<uint32_t*>(img + off) = hi;
     *reinterpret_cast<uint32_t*>(img + off + itc::IMG_SLAB_K) = lo;
   }
   if (tid == 0) {
-    p.key_inv[seq * tiles * 128 + j] = itc::pow2(-sh);
-    atomicMax(reinterpret_cast<unsigned int*>(p.key_norm_max + seq), __float_as_uint(sqrtf(ss)));
+    key_inv[seq * tiles * 128 + j] = itc::pow2(-sh);
+    atomicMax(reinterpret_cast<unsigned int*>(key_norm_max + seq), __float_as_uint(sqrtf(ss)));
   }
+}
+template <int NP>
+__device__ __forceinline__ void append_key_image(const dsv4_compressor_decode_params& p, const float (&vals)[NP][2],
+                                                 float* red) {
+  const bool mine = 2 * static_cast<int>(threadIdx.x) < p.head_dim;
+  const int64_t orow = p.out_rows[blockIdx.x];
+  append_key_row(mine ? vals[0][0] : 0.f, mine ? vals[0][1] : 0.f, p.head_dim, p.key_image, p.key_inv, p.key_norm_max,
+                 p.image_stride, orow / p.image_stride, orow % p.image_stride, red);
 }
 
 // the ratio-4 step of sequence blockIdx.x for one compressor (the body of decode_r4_kernel)
@@ -480,6 +487,191 @@ __global__ void __launch_bounds__(THREADS) decode_kernel(dsv4_compressor_decode_
     }
 }
 
+// ---- a chunk of new tokens per sequence (dsv4_compressor_chunk): what R = ratio calls of the
+// decode step per emitted row would leave, in one launch. Block g of a sequence is emitted when its
+// last token, position R g + R - 1, is in the chunk; its tokens and those of block g - 1 come from
+// the chunk where it has them and from the ring otherwise (rows [0, R): the last complete block,
+// rows R + p % R: the tokens of the block begun before the chunk).
+//
+// Every element of the projections is used once (the first half of a token's columns by the next
+// block's row, the second half by its own), so the kernel is a stream of 16 * head_dim bytes per
+// token and bound by HBM. A CTA takes the rows emitted by four neighbouring tokens, one in a long
+// chunk, up to four where every sequence has a token or two; each thread owns pairs of columns and
+// has all 4 R of its loads in flight before the first is used. The rows that read the ring (at most
+// the first two of a sequence) and the ring's own update belong to one CTA per sequence, so no
+// order between CTAs is needed: a thread reads the ring's columns it owns before it writes them.
+// The prefix grid (the sequences' CTAs, the slowest) is launched first.
+template <int R>
+struct ChunkSeq {
+  int first, n, start, slot;  // first token, tokens, position of the first, cache slot
+};
+
+template <int R>
+__device__ __forceinline__ void chunk_emit(const dsv4_compressor_chunk_params& p, const ChunkSeq<R>& q, int g,
+                                           float* red, float* xch) {
+  const int d = p.head_dim, d2 = 2 * d;
+  const float* rk = p.ring_kv + static_cast<int64_t>(q.slot) * 2 * R * d2;
+  const float* rs = p.ring_score + static_cast<int64_t>(q.slot) * 2 * R * d2;
+  const int block = q.start / R * R;  // the block the chunk begins in
+  float vals[2][2];
+  float ss = 0.f;
+#pragma unroll
+  for (int np = 0; np < 2; ++np) {
+    const int c = 2 * (threadIdx.x + np * THREADS);
+    if (c >= d) continue;
+    float2 K[2 * R], S[2 * R];
+#pragma unroll
+    for (int i = 0; i < 2 * R; ++i) {
+      const int pos = (g - 1) * R + i;  // slots [0, R): block g - 1, first half of the columns
+      const int col = c + (i < R ? 0 : d);
+      if (pos >= q.start) {
+        const int64_t off = static_cast<int64_t>(q.first + (pos - q.start)) * d2 + col;
+        K[i] = ld2(p.kv + off);
+        const float2 s = ld2(p.score + off), a = ld2(p.ape + (i % R) * d2 + col);
+        S[i] = make_float2(s.x + a.x, s.y + a.y);
+      } else {
+        const int row = (pos >= block ? R : 0) + i % R;  // positions below 0 are the ring's empty rows
+        K[i] = ld2(rk + row * d2 + col);
+        S[i] = ld2(rs + row * d2 + col);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float m = e ? S[0].y : S[0].x;
+#pragma unroll
+      for (int i = 1; i < 2 * R; ++i) m = fmaxf(m, e ? S[i].y : S[i].x);
+      float den = 0.f, num = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * R; ++i) {
+        const float ex = expf((e ? S[i].y : S[i].x) - m);
+        den += ex;
+        num = fmaf(ex, e ? K[i].y : K[i].x, num);
+      }
+      vals[np][e] = num / den;
+      ss = fmaf(vals[np][e], vals[np][e], ss);
+    }
+  }
+  ss = block_sum(ss, red);
+  const float rinv = rsqrtf(ss / static_cast<float>(d) + p.eps);
+  int64_t orow = -1;
+  if (g >= p.max_comp) {
+    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+  } else if (p.block_table == nullptr) {
+    orow = p.out_base + static_cast<int64_t>(q.slot) * p.max_comp + g;
+  } else {
+    const int32_t pg = p.block_table[static_cast<int64_t>(q.slot) * p.bt_stride + g / p.page];
+    if (pg >= 0)
+      orow = p.out_base + static_cast<int64_t>(pg) * p.page + g % p.page;
+    else
+      raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+  }
+  if (orow >= p.out_rows) {
+    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+    orow = -1;
+  }
+#pragma unroll
+  for (int np = 0; np < 2; ++np) {
+    const int c = 2 * (threadIdx.x + np * THREADS);
+    if (c >= d) continue;
+    finish_pair(vals[np][0], vals[np][1], c, d, p.rope_dim, p.norm_w, p.norm_dtype, rinv, p.freqs, R * g, p.out, orow,
+                p.out_dtype, p.act_quant);
+  }
+  if (p.act_quant == 2) {  // head_dim 128: threads 0..63 hold the row (uniform over the CTA)
+    hadamard_fp4_128(vals[0][0], vals[0][1], xch);
+    if (threadIdx.x < 64) store_pair(vals[0][0], vals[0][1], 2 * threadIdx.x, d, p.out, orow, p.out_dtype);
+  }
+  if (p.key_image && g < p.max_comp)
+    append_key_row(vals[0][0], vals[0][1], d, p.key_image, p.key_inv, p.key_norm_max, p.max_comp, q.slot, g, red);
+  __syncthreads();  // red and xch are free for the next row
+}
+
+// the chunk's sequence b; n == 0 where there is nothing to do or the chunk is not a valid one
+template <int R>
+__device__ __forceinline__ ChunkSeq<R> chunk_seq(const dsv4_compressor_chunk_params& p, int b) {
+  ChunkSeq<R> q;
+  q.first = p.cu_seqlens[b];
+  q.n = p.cu_seqlens[b + 1] - q.first;
+  q.start = p.start[b];
+  q.slot = p.seqs ? p.seqs[b] : b;
+  if (q.first < 0 || q.first + q.n > p.total || q.start < 0 || q.slot < 0 || q.slot >= p.slots) {
+    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+    q.n = 0;
+  }
+  return q;
+}
+
+template <int R>
+__global__ void __launch_bounds__(THREADS) chunk_kernel(dsv4_compressor_chunk_params p) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float red[33];
+  __shared__ float xch[128];
+  __shared__ int own[4];  // sequence of each of the four tokens, -1: nothing to emit
+  if (static_cast<int>(blockIdx.x) >= p.n) {
+    const int t = 4 * (blockIdx.x - p.n) + threadIdx.x;
+    if (threadIdx.x < 4) {
+      int b = -1;
+      if (t < p.total && t < p.cu_seqlens[p.n]) {
+        int lo = 0, hi = p.n - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (p.cu_seqlens[mid] <= t)
+            lo = mid;
+          else
+            hi = mid - 1;
+        }
+        // a block whose row needs no token of before the chunk
+        const int start = p.start[lo], pos = start + (t - p.cu_seqlens[lo]);
+        if ((pos + 1) % R == 0 && pos + 1 - 2 * R >= start) b = lo;
+      }
+      own[threadIdx.x] = b;
+    }
+    __syncthreads();
+    for (int i = 0; i < 4; ++i) {
+      const int b = own[i];
+      if (b < 0) continue;
+      const ChunkSeq<R> q = chunk_seq<R>(p, b);
+      const int pos = q.start + (4 * (static_cast<int>(blockIdx.x) - p.n) + i - q.first);
+      if (q.n > 0) chunk_emit<R>(p, q, pos / R, red, xch);
+    }
+    return;
+  }
+  const ChunkSeq<R> q = chunk_seq<R>(p, blockIdx.x);
+  if (q.n <= 0) return;
+  const int end = q.start + q.n, g0 = q.start / R, g1 = end / R;
+  for (int g = g0; g < g1 && (g - 1) * R < q.start; ++g) chunk_emit<R>(p, q, g, red, xch);
+  // the ring after the chunk: rows [0, R) the last complete block, rows R + p % R the newest token
+  const int d2 = 2 * p.head_dim;
+  float* rk = p.ring_kv + static_cast<int64_t>(q.slot) * 2 * R * d2;
+  float* rs = p.ring_score + static_cast<int64_t>(q.slot) * 2 * R * d2;
+  for (int c = 2 * threadIdx.x; c < d2; c += 2 * blockDim.x) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int last = end - 1 - (end - 1 - i + R) % R;  // newest position with p % R == i
+      if (g1 > g0) {
+        const int pos = (g1 - 1) * R + i;
+        if (pos >= q.start) {
+          const int64_t off = static_cast<int64_t>(q.first + (pos - q.start)) * d2 + c;
+          const float2 s = ld2(p.score + off), a = ld2(p.ape + i * d2 + c);
+          st2(rk + i * d2 + c, ld2(p.kv + off));
+          st2(rs + i * d2 + c, make_float2(s.x + a.x, s.y + a.y));
+        } else {
+          st2(rk + i * d2 + c, ld2(rk + (R + i) * d2 + c));
+          st2(rs + i * d2 + c, ld2(rs + (R + i) * d2 + c));
+        }
+      }
+      if (last >= q.start) {
+        const int64_t off = static_cast<int64_t>(q.first + (last - q.start)) * d2 + c;
+        const float2 s = ld2(p.score + off), a = ld2(p.ape + i * d2 + c);
+        st2(rk + (R + i) * d2 + c, ld2(p.kv + off));
+        st2(rs + (R + i) * d2 + c, make_float2(s.x + a.x, s.y + a.y));
+      }
+    }
+  }
+}
+
+DSV4_ERROR_READER(compressor)
+
 }  // namespace cmp
 }  // namespace dsv4
 
@@ -564,5 +756,53 @@ extern "C" int dsv4_compressor_decode_pair(const dsv4_compressor_decode_params* 
   DSV4_CUDA_CHECK(launch_pdl(cmp::decode_r4_pair_kernel<1>, dim3(a->b, 2), dim3(cmp::THREADS), 0, as_stream(stream),
                              *a, *b));
   DSV4_LAUNCH_CHECK("compressor decode_r4_pair_kernel");
+  return DSV4_OK;
+}
+
+extern "C" int dsv4_compressor_chunk(const dsv4_compressor_chunk_params* p, void* stream) {
+  DSV4_CHECK_ARG(p && p->kv && p->score && p->ape && p->ring_kv && p->ring_score && p->out && p->freqs && p->cu_seqlens &&
+                     p->start,
+                 "dsv4_compressor_chunk: NULL tensor");
+  DSV4_CHECK_ARG(p->act_quant == 0 ||
+                     (p->act_quant == 1 && p->head_dim % 64 == 0 && (p->head_dim - p->rope_dim) % 64 == 0) ||
+                     (p->act_quant == 2 && p->head_dim == 128),
+                 "dsv4_compressor_chunk: act_quant 1 needs head_dim and head_dim - rope_dim multiples of 64, "
+                 "act_quant 2 (Hadamard + fp4) head_dim 128");
+  DSV4_CHECK_ARG(p->n >= 0 && p->total >= 0 && p->slots > 0 && p->max_comp >= 0 && p->ratio > 0 && p->ratio <= 8,
+                 "dsv4_compressor_chunk: bad sizes (ratio 1 to 8)");
+  DSV4_CHECK_ARG(p->head_dim > 0 && p->head_dim % 2 == 0 && p->head_dim <= 4 * cmp::THREADS && p->rope_dim >= 0 &&
+                     p->rope_dim % 2 == 0 && p->rope_dim <= p->head_dim,
+                 "dsv4_compressor_chunk: head_dim %d, rope_dim %d unsupported", p->head_dim, p->rope_dim);
+  DSV4_CHECK_ARG(p->seqs || p->n <= p->slots, "dsv4_compressor_chunk: more sequences than the ring has slots");
+  DSV4_CHECK_ARG(p->block_table == nullptr ||
+                     (p->page > 0 && p->bt_stride * static_cast<int64_t>(p->page) >= p->max_comp),
+                 "dsv4_compressor_chunk: the block table does not cover max_comp");
+  DSV4_CHECK_DTYPE(p->out_dtype == DSV4_F32 || p->out_dtype == DSV4_BF16, "dsv4_compressor_chunk: out dtype");
+  DSV4_CHECK_DTYPE(p->norm_w == nullptr || p->norm_dtype == DSV4_F32 || p->norm_dtype == DSV4_BF16,
+                   "dsv4_compressor_chunk: norm dtype");
+  DSV4_CHECK_ARG(((reinterpret_cast<uintptr_t>(p->kv) | reinterpret_cast<uintptr_t>(p->score) |
+                   reinterpret_cast<uintptr_t>(p->ape) | reinterpret_cast<uintptr_t>(p->ring_kv) |
+                   reinterpret_cast<uintptr_t>(p->ring_score) | reinterpret_cast<uintptr_t>(p->out)) & 7) == 0,
+                 "dsv4_compressor_chunk: tensors must be 8-byte aligned");
+  DSV4_CHECK_ARG(p->key_image == nullptr || (p->key_inv && p->key_norm_max && p->max_comp > 0 && p->head_dim == 128 &&
+                                              p->out_dtype == DSV4_F32 &&
+                                              reinterpret_cast<uintptr_t>(p->key_image) % 16 == 0),
+                 "dsv4_compressor_chunk: a key image needs head_dim 128, fp32 out, inv, norm_max and a 16-byte aligned image");
+  if (p->n == 0 || p->total == 0) return DSV4_OK;
+  const int threads = std::min(cmp::THREADS, (p->head_dim / 2 + 31) / 32 * 32);
+  const dim3 grid(p->n + (p->total + 3) / 4);
+  void (*k)(dsv4_compressor_chunk_params) = nullptr;
+  switch (p->ratio) {
+    case 1: k = cmp::chunk_kernel<1>; break;
+    case 2: k = cmp::chunk_kernel<2>; break;
+    case 3: k = cmp::chunk_kernel<3>; break;
+    case 4: k = cmp::chunk_kernel<4>; break;
+    case 5: k = cmp::chunk_kernel<5>; break;
+    case 6: k = cmp::chunk_kernel<6>; break;
+    case 7: k = cmp::chunk_kernel<7>; break;
+    default: k = cmp::chunk_kernel<8>; break;
+  }
+  DSV4_CUDA_CHECK(launch_pdl(k, grid, dim3(threads), 0, as_stream(stream), *p));
+  DSV4_LAUNCH_CHECK("compressor chunk_kernel");
   return DSV4_OK;
 }

@@ -36,7 +36,9 @@ __global__ void decode_rows_kernel(dsv4_decode_rows_params p) {
         entry = p.max_comp - 1;
       }
       const int64_t blk = p.block_table[static_cast<int64_t>(i) * p.bt_stride + entry / p.page];
-      p.comp_rows[i] = p.comp_base + blk * p.page + entry % p.page;
+      // a paged cache may not have the page: an error where the step emits into it, else nothing is stored
+      if (blk < 0 && (pos + 1) % p.ratio == 0) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+      p.comp_rows[i] = blk < 0 ? -1 : p.comp_base + blk * p.page + entry % p.page;
       p.key_rows[i] = static_cast<int64_t>(i) * p.max_comp + entry;
     }
   }

@@ -13,6 +13,11 @@ HBM and is addressed by index:
   k_idx       fp32 [batch, max_comp, 128]: indexer keys of the compressed entries
   ring_kv / ring_score fp32 [batch, 2*ratio, 1024]: the compressor's decode ring
 
+With `n_pages` the cache is paged: the table starts empty (-1), pages are handed out as sequences grow
+(`reserve`), given back (`free`), shared between branches (`fork`) and moved together (`compact`);
+page_refs int32 [n_pages] counts the table cells that hold each page. With `max_chunk` the pool has that
+many rows more, behind the pages, where a chunk of new tokens is staged (chunk.py).
+
 `decode_attention` is the measured decode path: on one stream, chained with programmatic dependent
 launch, the indexer scores, the top-k selection straight into the attention index list (mapped
 through the block table), sparse attention — whose window tiles, computed from the positions, run
@@ -28,6 +33,7 @@ import torch
 from . import _lib as L
 from .indexer import build_key_image, indexer_topk_into, key_image_buffers
 from .norm_rope import norm_rope, rope_freqs
+from .pages import pages_compact, pages_fork, pages_free, pages_reserve
 from .sparse_attn import sparse_attn_decode, sparse_attn_into, sparse_attn_rope
 
 # below this batch the decode step fuses q's norm + RoPE into the attention kernel (the head-group
@@ -37,18 +43,30 @@ FUSED_Q_MAX_BATCH = 16
 
 class SparseMLACache:
     def __init__(self, batch, max_comp, window=128, head_dim=512, idx_dim=128, ratio=4, page=64,
-                 device="cuda", page_order=None):
+                 device="cuda", page_order=None, n_pages=None, max_chunk=0):
         self.batch, self.window, self.head_dim, self.ratio, self.page = batch, window, head_dim, ratio, page
         self.max_comp = max_comp
         self.pages_per_seq = math.ceil(max_comp / page)
-        n_pages = batch * self.pages_per_seq
+        paged = n_pages is not None and max_comp > 0
+        if n_pages is not None and (n_pages < 0 or page_order is not None):
+            raise ValueError("SparseMLACache: n_pages is a number of pages, and a paged cache hands them out itself "
+                             "(no page_order)")
+        n_pages = n_pages if n_pages is not None else batch * self.pages_per_seq
         self.comp_base = batch * window
-        self.kv_pool = torch.zeros((self.comp_base + n_pages * page, head_dim), dtype=torch.bfloat16,
+        self.max_chunk = int(max_chunk)
+        if self.max_chunk < 0:
+            raise ValueError("SparseMLACache: max_chunk is a number of tokens")
+        self.stage_base = self.comp_base + n_pages * page
+        self.kv_pool = torch.zeros((self.stage_base + self.max_chunk, head_dim), dtype=torch.bfloat16,
                                    device=device)
+        self.page_refs = torch.zeros(n_pages, dtype=torch.int32, device=device) if paged else None
         self.win_base = (torch.arange(batch, dtype=torch.int64) * window).to(device)
-        if page_order is None:
-            page_order = torch.arange(n_pages, dtype=torch.int32)
-        self.block_table = page_order.to(torch.int32).reshape(batch, self.pages_per_seq).to(device)
+        if paged:
+            self.block_table = torch.full((batch, self.pages_per_seq), -1, dtype=torch.int32, device=device)
+        else:
+            if page_order is None:
+                page_order = torch.arange(batch * self.pages_per_seq, dtype=torch.int32)
+            self.block_table = page_order.to(torch.int32).reshape(batch, self.pages_per_seq).to(device)
         self.image_stale = False
         # max_comp == 0: a window-only layer (ratio 0, and the ratio-128 layers, which the reference
         # runs with neither a compressor ring nor compressed rows, oracle/v4_fast.py:42-43, 114)
@@ -69,8 +87,8 @@ class SparseMLACache:
 
     # ---- checkpoint / resume (the reference copies its per-layer state with clone_states,
     # oracle/v4_fast.py:150-159, and copy.deepcopy, oracle/decode_engine.py:167) ----
-    _STATE = ("kv_pool", "win_base", "block_table", "k_idx", "key_image", "ring_kv", "ring_score", "ring_k_idx",
-              "ring_s_idx")
+    _STATE = ("kv_pool", "win_base", "block_table", "page_refs", "k_idx", "key_image", "ring_kv", "ring_score",
+              "ring_k_idx", "ring_s_idx")
 
     def state_dict(self):
         """The whole decode state as tensors (on the cache's device), for torch.save; the key image
@@ -93,6 +111,8 @@ class SparseMLACache:
         meta = st["meta"].tolist()
         if meta[:6] != [self.batch, self.max_comp, self.window, self.head_dim, self.ratio, self.page]:
             raise ValueError(f"SparseMLACache.load_state_dict: saved layout {meta[:6]} differs from this cache's")
+        if ("page_refs" in st) != (self.page_refs is not None) or st["kv_pool"].shape != self.kv_pool.shape:
+            raise ValueError("SparseMLACache.load_state_dict: the saved pool is paged or staged otherwise than this cache's")
         for name in self._STATE:
             v = getattr(self, name)
             if name == "key_image" and v is not None:
@@ -113,6 +133,23 @@ class SparseMLACache:
             elif v is not None:
                 setattr(c, name, v.clone())
         return c
+
+    # ---- pages (a paged cache; see pages.py) ----
+    def reserve(self, seqs, tokens, add=0):
+        """Pages for `tokens + add` tokens of slots `seqs` (pages_reserve)."""
+        pages_reserve(self, seqs, tokens, add)
+
+    def free(self, seqs):
+        """Give back the pages of slots `seqs` (pages_free)."""
+        pages_free(self, seqs)
+
+    def fork(self, src, dst, tokens):
+        """Branch slot src[k], holding tokens[k] tokens, into slot dst[k] (pages_fork)."""
+        pages_fork(self, src, dst, tokens)
+
+    def compact(self):
+        """Move the pages in use to the front of the pool; their number, int32 [1] (pages_compact)."""
+        return pages_compact(self)
 
     # ---- address helpers (host side) ----
     def comp_rows(self, b, j):
@@ -156,6 +193,11 @@ class SparseMLACache:
         n = comp_rows.shape[0] if comp_rows is not None else 0
         if n > self.max_comp:
             raise ValueError(f"SparseMLACache.load_prefill: {n} compressed rows exceed the cache's {self.max_comp}")
+        if self.page_refs is not None:  # the slot's earlier pages back, new ones for the rows
+            self.free([b])
+            self.reserve([b], [n * self.ratio])
+            if n and int(self.block_table[b, (n - 1) // self.page]) < 0:
+                raise RuntimeError(f"SparseMLACache.load_prefill: too few free pages for {n} compressed rows")
         if n:
             self.fill_compressed(b, comp_rows, keys)
         # an omitted ring starts from the compressor's initial state (kv 0, scores -inf), never from

@@ -1,0 +1,109 @@
+"""Pages of a paged `SparseMLACache`: handing out, giving back, branching and compacting.
+
+The reference copies the whole state of a conversation to branch it (oracle/v4_fast.py:150-159
+clone_states). Here a branch shares the full pages of compressed rows and copies only what its tokens
+will write to (the last partial page, the window ring, the compressor rings) and the indexer keys,
+which are laid out by slot. Tables and counts stay on the device: every call is asynchronous on the
+current stream, can be captured in a CUDA graph, and gives the same tables for the same input. What a
+call cannot do for one sequence it leaves out for that sequence, and raises the device error word
+(`_lib.device_error`): NO_PAGES, or INDEX_OUT_OF_RANGE for a slot that does not exist, more tokens
+than the cache holds, or a branch onto a slot that has pages.
+"""
+import ctypes
+
+import torch
+
+from . import _lib as L
+
+
+def _params(cache):
+    if cache.page_refs is None:
+        raise ValueError("SparseMLACache: pages are handed out and shared only in a paged cache (n_pages=...)")
+    p = L.Pages()
+    p.pool, p.win_base, p.block_table, p.refs = (t.data_ptr() for t in (cache.kv_pool, cache.win_base, cache.block_table,
+                                                                       cache.page_refs))
+    p.k_idx = cache.k_idx.data_ptr()
+    p.key_image, p.key_inv, p.key_norm_max = (t.data_ptr() for t in cache.key_image)
+    p.ring_kv, p.ring_score = cache.ring_kv.data_ptr(), cache.ring_score.data_ptr()
+    p.ring_k_idx, p.ring_s_idx = cache.ring_k_idx.data_ptr(), cache.ring_s_idx.data_ptr()
+    p.comp_base, p.slots, p.n_pages = cache.comp_base, cache.batch, cache.page_refs.numel()
+    p.bt_stride, p.page, p.max_comp, p.window = cache.block_table.shape[1], cache.page, cache.max_comp, cache.window
+    p.head_dim, p.idx_dim, p.ratio = cache.head_dim, cache.k_idx.shape[-1], cache.ratio
+    return p
+
+
+def _ints(name, cache, *ts):
+    """Sequences and token counts as int32 tensors of one length on the cache's device."""
+    dev, out = cache.block_table.device, []
+    for t in ts:
+        t = torch.as_tensor(t, device=dev) if not isinstance(t, torch.Tensor) else t
+        L.require_cuda(t)
+        if t.device != dev:
+            raise ValueError(f"{name}: tensors on {t.device}, the cache is on {dev}")
+        if t.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name}: sequences and token counts are integers, got {t.dtype}")
+        out.append(t.reshape(-1).to(torch.int32).contiguous())
+    if any(t.numel() != out[0].numel() for t in out):
+        raise ValueError(f"{name}: {[t.numel() for t in out]} sequences and counts")
+    return out
+
+
+def _workspace(p, n, device):
+    nbytes = L.lib().dsv4_pages_workspace_size(ctypes.byref(p), n)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+
+
+def pages_free(cache, seqs):
+    """Give back the pages of slots `seqs` (a page shared with another slot stays with that one) and
+    empty their table rows. A slot named twice gives its pages back once."""
+    p = _params(cache)
+    seqs, = _ints("pages_free", cache, seqs)
+    with L.device_of(seqs):
+        L.check(L.lib().dsv4_pages_free(ctypes.byref(p), L.ptr(seqs), seqs.numel(), L.stream_of(seqs)))
+
+
+def pages_reserve(cache, seqs, tokens, add=0):
+    """Pages for the compressed rows of `tokens + add` tokens of slots `seqs` (None: slot k for the
+    k-th count); pages they have stay. A slot that finds too few free pages gets none."""
+    p = _params(cache)
+    if seqs is None:
+        tokens, = _ints("pages_reserve", cache, tokens)
+        if tokens.numel() > cache.batch:
+            raise ValueError(f"pages_reserve: {tokens.numel()} counts, the cache has {cache.batch} slots")
+    else:
+        seqs, tokens = _ints("pages_reserve", cache, seqs, tokens)
+    with L.device_of(tokens):
+        ws, nbytes = _workspace(p, tokens.numel(), tokens.device)
+        L.check(L.lib().dsv4_pages_reserve(ctypes.byref(p), L.ptr(seqs), L.ptr(tokens), int(add), tokens.numel(),
+                                           L.ptr(ws), nbytes, L.stream_of(tokens)))
+
+
+def pages_fork(cache, src, dst, tokens):
+    """Make slot dst[k], which has no pages, a branch of slot src[k], which holds tokens[k] tokens (all
+    that it holds: the window ring and the compressor rings are those of its latest token). A slot may
+    be the source of several branches, but not a branch twice, nor a branch and a source."""
+    p = _params(cache)
+    if cache.image_stale:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("pages_fork: the cache's key image is stale inside a stream capture; call "
+                               "cache.refresh_key_image() before capturing")
+        cache.refresh_key_image()
+    src, dst, tokens = _ints("pages_fork", cache, src, dst, tokens)
+    if src.numel() > cache.batch:
+        raise ValueError(f"pages_fork: {src.numel()} branches, the cache has {cache.batch} slots")
+    with L.device_of(src):
+        ws, nbytes = _workspace(p, src.numel(), src.device)
+        L.check(L.lib().dsv4_pages_fork(ctypes.byref(p), L.ptr(src), L.ptr(dst), L.ptr(tokens), src.numel(), L.ptr(ws),
+                                        nbytes, L.stream_of(src)))
+
+
+def pages_compact(cache):
+    """Move the pages in use to the front of the pool, the first free page taking the first page in use
+    behind the new end, and so on; tables and counts follow. Returns their number, int32 [1] on the
+    device. Page numbers that a caller keeps beside the table are no longer valid."""
+    p = _params(cache)
+    n = torch.empty(1, dtype=torch.int32, device=cache.block_table.device)
+    with L.device_of(n):
+        ws, nbytes = _workspace(p, 0, n.device)
+        L.check(L.lib().dsv4_pages_compact(ctypes.byref(p), L.ptr(n), L.ptr(ws), nbytes, L.stream_of(n)))
+    return n

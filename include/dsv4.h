@@ -52,7 +52,8 @@ typedef enum {
   DSV4_ERR_CUDA = 3,              /* a CUDA runtime call failed; message carries cudaGetErrorString */
   DSV4_ERR_INDEX_OUT_OF_RANGE = 4,/* device error word: a gathered index was outside [-1, n) */
   DSV4_ERR_WAIT_TIMEOUT = 5,      /* device error word: a bounded wait ran out */
-  DSV4_ERR_WORKSPACE = 6          /* workspace pointer missing or smaller than *_workspace_size */
+  DSV4_ERR_WORKSPACE = 6,         /* workspace pointer missing or smaller than *_workspace_size */
+  DSV4_ERR_NO_PAGES = 7           /* device error word: a paged cache has too few free pages */
 } dsv4_status;
 
 typedef enum { DSV4_F32 = 0, DSV4_BF16 = 1, DSV4_I32 = 2, DSV4_I64 = 3, DSV4_I8 = 4 } dsv4_dtype;
@@ -361,7 +362,9 @@ DSV4_API int dsv4_compressor_decode_pair(const dsv4_compressor_decode_params* a,
  *   entry        = max((p + 1) / ratio - 1, 0)                   (compressed entry the step emits)
  *   comp_rows[i] = comp_base + block_table[i*bt_stride + entry/page]*page + entry % page
  *   key_rows[i]  = i * max_comp + entry
- * An entry >= max_comp raises DSV4_ERR_INDEX_OUT_OF_RANGE on the device error word (clamped).
+ * An entry >= max_comp raises DSV4_ERR_INDEX_OUT_OF_RANGE on the device error word (clamped). An entry
+ * that the step emits into a page the sequence does not have (block_table < 0, a paged cache without
+ * dsv4_pages_reserve) raises it too, and comp_rows[i] is -1: the compressor then stores no row.
  * max_comp == 0 is a window-only cache (the ratio-0 and ratio-128 layers, which keep no compressed
  * rows, oracle/v4_fast.py:42-43, 114): comp_rows and key_rows are -1 and block_table may be NULL.
  * Replaces the host-side ring and kvbuf bookkeeping of oracle/v4_fast.py:93-118. */
@@ -376,6 +379,99 @@ typedef struct {
   int32_t b, window, ratio, page, bt_stride, max_comp;
 } dsv4_decode_rows_params;
 DSV4_API int dsv4_decode_rows(const dsv4_decode_rows_params* p, void* stream);
+
+/* ---- a chunk of new tokens over the device-resident state -----------------------------------------
+ * n sequences with cu_seqlens[b + 1] - cu_seqlens[b] new tokens each, the first at position start[b]
+ * of cache slot seqs[b]. The chunk's kv rows are staged in the pool, token i at row stage_base + i,
+ * and go into the window rings after the attention (dsv4_chunk_commit): the ring has one row per
+ * window position, so a token written early would overwrite a row that the chunk still sees. All
+ * arrays are device memory; tokens behind cu_seqlens[n] (a padded batch) belong to no sequence. */
+typedef struct {
+  const int32_t* cu_seqlens;  /* [n + 1], ascending from 0 */
+  const int32_t* start;       /* [n] */
+  const int32_t* seqs;        /* [n] cache slots, or NULL: sequence b is slot b */
+  const int64_t* win_base;    /* [slots] */
+  const int32_t* block_table; /* [slots, bt_stride], or NULL with max_comp 0 (a window-only layer) */
+  int64_t comp_base, stage_base, pool_rows;
+  int32_t n, total, slots;    /* total: rows of the call, at least cu_seqlens[n] */
+  int32_t window, ratio, page, bt_stride, max_comp;
+} dsv4_chunk;
+/* positions [total] (0 behind the last sequence) and stage_rows [total] (stage_base + i); either may
+ * be NULL. With index: row t gets [window rows of the token, oldest first | cols columns], -1 where
+ * there is none: the columns of given [total, cols] (pool rows), or with given == NULL the pool rows
+ * of every compressed entry the token sees, j < (p + 1) / ratio. The list of oracle/decode_engine.py:110-116
+ * for each token. */
+DSV4_API int dsv4_chunk_rows(const dsv4_chunk* c, int32_t* positions, int64_t* stage_rows, int32_t* index,
+                             int64_t index_stride, int32_t cols, const int32_t* given, void* stream);
+/* the chunk's last rows (at most window per sequence) from the stage into the window rings; pool is
+ * the bf16 pool of rows of dim elements */
+DSV4_API int dsv4_chunk_commit(const dsv4_chunk* c, void* pool, int32_t dim, void* stream);
+
+/* The compressor over a chunk, continuing each sequence's ring: what one dsv4_compressor_decode call
+ * per token would leave in the rings, the emitted rows and the key image, in one launch
+ * (oracle/decode_engine.py:96-105 for a run of tokens; the reference takes one token at a time). Entry g of
+ * slot s goes to row out_base + block_table[s, g / page] * page + g % page, or without a table to row
+ * out_base + s * max_comp + g (the indexer keys). An entry past max_comp or without a page raises
+ * DSV4_ERR_INDEX_OUT_OF_RANGE and is not stored. */
+typedef struct {
+  const float* kv;            /* [total, 2 * head_dim] */
+  const float* score;         /* [total, 2 * head_dim], before ape */
+  const float* ape;           /* [ratio, 2 * head_dim] */
+  const void* norm_w;         /* [head_dim] or NULL */
+  float* ring_kv;             /* [slots, 2 * ratio, 2 * head_dim] */
+  float* ring_score;
+  void* out;
+  const float* freqs;         /* [rope_dim / 2] */
+  const int32_t* cu_seqlens;  /* as dsv4_chunk */
+  const int32_t* start;
+  const int32_t* seqs;
+  const int32_t* block_table;
+  int64_t out_base, out_rows; /* out_rows: rows of out; one past them raises the error word too */
+  int32_t n, total, slots, bt_stride, page, max_comp;
+  int32_t head_dim, ratio, rope_dim, norm_dtype, out_dtype, act_quant; /* as dsv4_compressor_decode_params */
+  float eps;
+  uint8_t* key_image;         /* optional (head_dim 128, fp32 out): each key also goes to the image of its slot */
+  float* key_inv;
+  float* key_norm_max;
+} dsv4_compressor_chunk_params;
+DSV4_API int dsv4_compressor_chunk(const dsv4_compressor_chunk_params* p, void* stream);
+
+/* ---- the pages of a paged cache: block_table[slot, j] is the page of entries [j * page, (j + 1) * page),
+ * -1 where there is none, and refs[page] the number of table cells that hold it (0: free). Everything
+ * runs on the device in stream order; free pages are handed out from the lowest index up, in the order
+ * of the call, so the same calls give the same tables. What a call cannot do for one sequence (no free
+ * pages, a slot out of range, an occupied branch) it leaves out for that sequence and raises on the
+ * device error word. No reference counterpart: the reference copies whole states
+ * (oracle/v4_fast.py:150-159 clone_states). */
+typedef struct {
+  void* pool;               /* bf16 rows of head_dim: window rings at win_base, pages from comp_base */
+  const int64_t* win_base;  /* [slots] */
+  int32_t* block_table;     /* [slots, bt_stride] */
+  int32_t* refs;            /* [n_pages] */
+  float* k_idx;             /* [slots, max_comp, idx_dim] or NULL */
+  uint8_t* key_image;       /* dsv4_key_image_params layout, or NULL */
+  float* key_inv;
+  float* key_norm_max;
+  float *ring_kv, *ring_score;     /* [slots, 2 * ratio, 2 * head_dim] or NULL */
+  float *ring_k_idx, *ring_s_idx;  /* [slots, 2 * ratio, 2 * idx_dim] or NULL */
+  int64_t comp_base;
+  int32_t slots, n_pages, bt_stride, page, max_comp, window, head_dim, idx_dim, ratio;
+} dsv4_pages;
+/* bytes that a reserve, fork (n sequences) or compact call needs */
+DSV4_API size_t dsv4_pages_workspace_size(const dsv4_pages* p, int32_t n);
+/* the slots' pages given back, their table rows emptied */
+DSV4_API int dsv4_pages_free(const dsv4_pages* p, const int32_t* seqs, int32_t n, void* stream);
+/* pages for the entries of tokens[k] + add tokens of slot seqs[k] (NULL: slot k) */
+DSV4_API int dsv4_pages_reserve(const dsv4_pages* p, const int32_t* seqs, const int32_t* tokens, int32_t add, int32_t n,
+                                void* workspace, size_t workspace_bytes, void* stream);
+/* slot dst[k] (its table row empty) becomes a branch of slot src[k], which holds tokens[k] tokens: full
+ * pages shared, the last partial page, the window ring, the compressor rings, the keys and their image
+ * copied. No slot may be a dst twice, or a dst and a src. */
+DSV4_API int dsv4_pages_fork(const dsv4_pages* p, const int32_t* src, const int32_t* dst, const int32_t* tokens, int32_t n,
+                             void* workspace, size_t workspace_bytes, void* stream);
+/* the pages in use moved to [0, *n_live), in place of the free ones there (the k-th free one below
+ * *n_live takes the k-th used one above it); tables and refs follow. Rows above stay as they were. */
+DSV4_API int dsv4_pages_compact(const dsv4_pages* p, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- a6: projections. y[m, n] = sum_k x[m, k] * W[n, k] (W row-major [n, k] as the reference)
  * W is BF16, or I8 with BF16 scales per (row, group of `group` k). x BF16 or F32, y F32 or BF16.
