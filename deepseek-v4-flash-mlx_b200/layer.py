@@ -26,7 +26,8 @@ from dataclasses import dataclass, fields
 import torch
 
 from . import _lib as L
-from .compressor import CompressorStep, compressor_decode_pair, compressor_prefill
+from .chunk import chunk_attention, chunk_commit, chunk_rows
+from .compressor import CompressorStep, compressor_chunk, compressor_decode_pair, compressor_prefill
 from .configs import DIMS, LayerDims, window_only
 from .decode import SparseMLACache, decode_attention, decode_rows, window_attention
 from .hc import hc_post, hc_pre
@@ -155,13 +156,15 @@ class DecodeBlock:
     (config 5): `step(x, positions)` runs the whole attention block for one token per sequence."""
 
     def __init__(self, W: AttentionWeights, batch, max_ctx, top_k=512, dims: LayerDims = DIMS, device="cuda",
-                 page=64, cache=None, act_quant=False):
+                 page=64, cache=None, act_quant=False, n_pages=None, max_chunk=0):
+        """`n_pages`: a paged cache of that many pages (`SparseMLACache`); the block reserves the pages
+        that its tokens need. `max_chunk`: the most new tokens that one `extend` takes."""
         self.W, self.dims, self.top_k = W, dims, top_k
         self.act_quant = act_quant  # the fp8 act-quant simulation of cached rows (oracle/decode_engine.py:82, 105)
         self.window_only = window_only(dims)
         self.cache = cache if cache is not None else SparseMLACache(
             batch, 0 if self.window_only else max_ctx // dims.ratio, window=dims.window, head_dim=dims.head_dim,
-            idx_dim=dims.idx_dim, ratio=dims.ratio, page=page, device=device)
+            idx_dim=dims.idx_dim, ratio=dims.ratio, page=page, device=device, n_pages=n_pages, max_chunk=max_chunk)
         if self.window_only and self.cache.compressed:
             raise ValueError("DecodeBlock: a window-only layer (ratio 0 or 128) takes a cache without compressed rows")
         self.freqs = layer_rope_freqs(dims, device)
@@ -219,6 +222,8 @@ class DecodeBlock:
         qa = rmsnorm(qa_p, W.q_a_norm, out_dtype=torch.bfloat16)
         qraw, qi = linear_multi(qa, [W.wq_b, W.i_wq], torch.float32)
         qraw = qraw.view(b, d.n_heads, d.head_dim)
+        if c.page_refs is not None:
+            c.reserve(None, pos, 1)
         # this token's window slot, and where the compressors emit (when (p+1) % ratio == 0)
         win_rows, comp_rows, key_rows = decode_rows(c, pos)
         _norm_rope_into(kvp, W.kv_a_norm, pos, self.freqs, c.kv_pool, win_rows, d.rope_dim, self.act_quant)
@@ -236,6 +241,84 @@ class DecodeBlock:
             aux.update(q_idx=q_idx, w_idx=w_idx, idx=idx_buf)
         o = decode_attention(c, qraw, q_idx, w_idx, W.sinks, pos, self.top_k, freqs=self.freqs, idx_buf=idx_buf)
         return o_grouped(o.reshape(b, -1), W.wo_a, W.wo_b)
+
+
+    def extend(self, x, lengths, start, seqs=None, aux=None):
+        """Several new tokens of each sequence in one call: a chunk of a prompt, a further turn, drafted
+        tokens to check. x [total, dim] fp32/bf16, the tokens of the first sequence, then those of the
+        second, and so on; lengths and start: their numbers, and the position of each sequence's first new
+        token (the tokens it holds), lists of ints; seqs: their cache slots (default: the first ones).
+        Returns out [total, dim] fp32 and leaves the cache as `step` on one token after the other does
+        (oracle/v4_fast.py:82-122 in a loop); rows of x behind the last sequence (padding) give rows of no
+        meaning. The cache must stage that many tokens (`max_chunk`). `aux` as in `step`."""
+        d, W, c = self.dims, self.W, self.cache
+        total, dev = x.shape[0], x.device
+        lengths, start = [int(n) for n in lengths], [int(p) for p in start]
+        slots = list(range(len(lengths))) if seqs is None else [int(s) for s in seqs]
+        if not len(lengths) == len(start) == len(slots):
+            raise ValueError(f"extend: {len(lengths)} lengths, {len(start)} positions, {len(slots)} slots")
+        if any(n < 0 for n in lengths) or any(p < 0 for p in start) or sum(lengths) > total:
+            raise ValueError(f"extend: lengths {lengths} from positions {start} in {total} rows")
+        if len(set(slots)) < len(slots) or any(not 0 <= s < c.batch for s in slots):
+            raise ValueError(f"extend: slots {slots} of a cache with {c.batch}")
+        if total > c.max_chunk:
+            raise ValueError(f"extend: {total} rows, the cache stages {c.max_chunk} (max_chunk)")
+        if c.compressed and any((p + n) // d.ratio > c.max_comp for n, p in zip(lengths, start)):
+            raise ValueError(f"extend: a sequence grows past the cache's {c.max_comp} compressed rows")
+        meta, at = [0], 0
+        for n in lengths:
+            at += n
+            meta.append(at)
+        meta = torch.tensor(meta + start + slots + [p + n for n, p in zip(lengths, start)], dtype=torch.int32).to(dev)
+        k = len(lengths)
+        cu, start_t, seqs_t, held = meta[:k + 1], meta[k + 1:2 * k + 1], meta[2 * k + 1:3 * k + 1], meta[3 * k + 1:]
+        pos, rows = chunk_rows(c, cu, start_t, total, seqs_t)
+        xn = rmsnorm(x, W.attn_norm, out_dtype=torch.bfloat16)
+        if self.window_only:
+            qa_p, kvp = linear_multi(xn, [W.wq_a, W.wkv], torch.float32)
+            qraw = linear(rmsnorm(qa_p, W.q_a_norm, out_dtype=torch.bfloat16), W.wq_b, torch.float32)
+        else:
+            qa_p, kvp, c_kv, c_sc, w_idx, i_kv, i_sc = linear_multi(
+                xn, [W.wq_a, W.wkv, W.c_wkv, W.c_wgate, W.i_wproj, W.i_wkv, W.i_wgate], torch.float32)
+            qraw, qi = linear_multi(rmsnorm(qa_p, W.q_a_norm, out_dtype=torch.bfloat16), [W.wq_b, W.i_wq], torch.float32)
+        q = norm_rope(qraw.view(total, d.n_heads, d.head_dim), pos, self.freqs, weight=None, rope_dim=d.rope_dim)
+        _norm_rope_into(kvp, W.kv_a_norm, pos, self.freqs, c.kv_pool, rows, d.rope_dim, self.act_quant)
+        listed = None
+        if not self.window_only:
+            if c.page_refs is not None:
+                c.reserve(seqs_t, held)
+            comp = dict(seqs=seqs_t, max_comp=c.max_comp, ratio=d.ratio, rope_head_dim=d.rope_dim, freqs=self.freqs)
+            compressor_chunk((c_kv, c_sc), cu, start_t, W.c_ape, W.c_norm, c.ring_kv, c.ring_score, c.kv_pool,
+                             block_table=c.block_table, page=c.page, out_base=c.comp_base, head_dim=d.head_dim,
+                             act_quant=self.act_quant, **comp)
+            compressor_chunk((i_kv, i_sc), cu, start_t, W.i_ape, W.i_norm, c.ring_k_idx, c.ring_s_idx, c.k_idx,
+                             head_dim=d.idx_dim, key_image=c.key_image, **comp)
+            if c.max_comp > self.top_k:   # else every token sees all of its compressed rows
+                q_idx = rope(qi.view(total, d.idx_heads, d.idx_dim), pos, self.freqs, d.rope_dim)
+                listed = self._select(q_idx, w_idx, pos, lengths, slots)
+                if aux is not None:
+                    aux.update(q_idx=q_idx, w_idx=w_idx, idx=listed)
+        o = chunk_attention(c, q, W.sinks, cu, start_t, seqs_t, rows=listed, freqs=self.freqs)
+        chunk_commit(c, cu, start_t, total, seqs_t)
+        return o_grouped(o.reshape(total, -1), W.wo_a, W.wo_b)
+
+    def _select(self, q_idx, w_idx, pos, lengths, slots):
+        """The pool rows that the indexer selects for each token of a chunk, int32 [total, top_k]."""
+        c = self.cache
+        if c.image_stale:
+            c.refresh_key_image()
+        img, inv, nmax = c.key_image
+        out = torch.full((q_idx.shape[0], self.top_k), -1, dtype=torch.int32, device=q_idx.device)
+        per, at = img.numel() // c.batch, 0
+        for n, s in zip(lengths, slots):
+            if n:
+                t = slice(at, at + n)
+                indexer_topk_into(out[t][None], q_idx[t][None], w_idx[t][None], c.k_idx[s:s + 1], self.top_k,
+                                  positions=pos[t][None], ratio=c.ratio, out_offset=c.comp_base,
+                                  block_table=c.block_table[s:s + 1], page=c.page,
+                                  key_image=(img[s * per:(s + 1) * per], inv[s:s + 1], nmax[s:s + 1]))
+            at += n
+        return out
 
 
 def layer_rope_freqs(dims: LayerDims, device):

@@ -33,10 +33,10 @@ def _params(cache):
 
 
 def _ints(name, cache, *ts):
-    """Sequences and token counts as int32 tensors of one length on the cache's device."""
+    """Sequences and token counts (lists, or tensors on the cache's device) as int32 tensors of one length."""
     dev, out = cache.block_table.device, []
     for t in ts:
-        t = torch.as_tensor(t, device=dev) if not isinstance(t, torch.Tensor) else t
+        t = torch.tensor(t, dtype=torch.int32, device=dev) if not isinstance(t, torch.Tensor) else t
         L.require_cuda(t)
         if t.device != dev:
             raise ValueError(f"{name}: tensors on {t.device}, the cache is on {dev}")

@@ -1,0 +1,469 @@
+"""Chunks of new tokens over a (paged) cache: attention, compressor, row moves and whole layers, against
+plain forms in 64 bits and against one token after the other.
+
+Tolerances. The attention rounds each probability and the output to bf16, each by half a step at most,
+a relative 2^-8 (torch.finfo(bf16).eps / 2 = 2^-8); products and sums are fp32. With p_j the exact
+normalised weights, the rounded weights w_j = p_j (1 + d_j), |d_j| <= 2^-8, give
+|o' - o| <= sum_j p_j |d_j| |v_j| + |o| sum_j p_j |d_j| (the denominator's change, where the sum is of
+rounded weights) <= 2^-8 (A + |o|) <= 2^-7 A with A = sum_j p_j |v_j|, and the rounding of the output adds 2^-8 |o| <= 2^-8 A.
+So |got - exact| <= 3 * 2^-8 A per element, and before the inverse rotation; the rotation mixes two
+elements, whose bounds then add up to sqrt(2) times the larger at most: 3 * 2^-8 * (A_d + A_d').
+The fp32 parts (512-term products, exp) stay below 2^-14 of the same scale and are covered by one more 2^-8 A.
+"""
+import importlib
+
+import numpy as np
+import pytest
+import torch
+
+from helpers import rel_rms
+
+pytestmark = pytest.mark.gpu
+PKG = "deepseek-v4-flash-mlx_b200"
+H, D, W, R = 64, 512, 128, 4
+EPS = torch.finfo(torch.bfloat16).eps / 2   # 2^-8
+
+
+def _mods():
+    return importlib.import_module(PKG), importlib.import_module(PKG + ".decode"), importlib.import_module(PKG + "._lib")
+
+
+def _freqs():
+    return 1.0 / (160000.0 ** (torch.arange(0, 64, 2, dtype=torch.float32) / 64))
+
+
+def _case(lens, start, page=64, ratio=4, seed=0, paged=False, seqs=None, slots=None, pad=0, window=W):
+    """A cache with random rows, a chunk staged in it and its queries."""
+    pkg, Dm, _ = _mods()
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    total = sum(lens) + pad
+    slots = slots or len(lens)
+    seqs = seqs or list(range(len(lens)))
+    most = max(max((s + n) // ratio for n, s in zip(lens, start)), 1) if ratio else 0
+    per = -(-most // page)
+    if paged:
+        c = Dm.SparseMLACache(slots, most, page=page, ratio=ratio or 4, n_pages=slots * per + 5, max_chunk=total, window=window)
+        c.reserve(seqs, [s + n for n, s in zip(lens, start)])
+    else:
+        order = torch.randperm(slots * per, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+        c = Dm.SparseMLACache(slots, most, page=page, ratio=ratio or 4, page_order=order if most else None, max_chunk=total,
+                              window=window)
+    c.kv_pool.copy_(torch.randn(c.kv_pool.shape, generator=g, device="cuda").to(torch.bfloat16))
+    q = torch.randn(total, H, D, generator=g, device="cuda")
+    q = (q * torch.rsqrt(q.square().mean(-1, keepdim=True))).to(torch.bfloat16)
+    sink = torch.randn(H, generator=g, device="cuda")
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    return c, q, sink, cu, torch.tensor(start, dtype=torch.int32, device="cuda"), torch.tensor(seqs, dtype=torch.int32, device="cuda")
+
+
+def _rotate64(x, pos, f, sign):
+    a = (pos.float()[:, None] * f.to(pos.device)).double()[:, None, :] * sign
+    y = x.clone()
+    y[..., -64::2] = x[..., -64::2] * a.cos() - x[..., -63::2] * a.sin()
+    y[..., -63::2] = x[..., -64::2] * a.sin() + x[..., -63::2] * a.cos()
+    return y
+
+
+def _attention64(c, q, sink, lens, start, seqs, rows=None, scale=D ** -0.5):
+    """o and the bound of each element, in 64 bits, token by token."""
+    f, pool = _freqs().cuda(), c.kv_pool.double()
+    out, tol = [], []
+    at = 0
+    for n, s, b in zip(lens, start, seqs):
+        for i in range(n):
+            p = s + i
+            r = []
+            for w in range(max(0, p - c.window + 1), p + 1):
+                r.append(c.stage_base + at + w - s if w >= s else int(c.win_base[b]) + w % c.window)
+            r = torch.tensor(r, device="cuda")
+            if rows is not None:
+                mine = rows[at + i].long()
+                r = torch.cat([r, mine[mine >= 0]])
+            elif c.compressed:
+                e = torch.arange(min((p + 1) // c.ratio, c.max_comp), device="cuda")
+                if e.numel():
+                    r = torch.cat([r, c.comp_base + c.block_table[b].long()[e // c.page] * c.page + e % c.page])
+            kv = pool[r]
+            x = torch.cat([q[at + i].double() @ kv.T * scale, sink.double()[:, None]], 1)
+            w = torch.softmax(x, -1)[:, :-1]
+            o, a = w @ kv, w @ kv.abs()
+            a[:, -64:] = a[:, -64:] + a[:, -64:].reshape(H, 32, 2).flip(-1).reshape(H, 64)
+            out.append(_rotate64(o[None], torch.tensor([p], device="cuda"), f, -1)[0])
+            tol.append(4 * EPS * a)
+        at += n
+    return torch.stack(out), torch.stack(tol)
+
+
+def _check(got, want, tol):
+    got = got[:want.shape[0]].double()
+    assert torch.isfinite(got).all()
+    worst = ((got - want).abs() / tol).max().item()
+    assert worst <= 1, worst
+
+
+# lengths and starts around the ring's and the tiles' borders: empty windows, a window that the chunk
+# fills, a ring that has wrapped, one token, more than two windows of tokens, odd and even counts
+CASES = [([1], [0]), ([1], [127]), ([2], [3]), ([5], [0]), ([3], [126]), ([7, 1, 2], [300, 0, 1023]), ([64], [64]),
+         ([129], [60]), ([130, 1], [511, 4000]), ([300], [0]), ([0, 4, 0, 1], [9, 700, 1, 5000]), ([33, 34], [255, 256])]
+
+
+@pytest.mark.parametrize("lens,start", CASES)
+def test_chunk_attention(lens, start):
+    pkg, _, L = _mods()
+    c, q, sink, cu, st, _ = _case(lens, start, seed=1)
+    o = pkg.chunk_attention(c, q, sink, cu, st, freqs=_freqs().cuda())
+    assert o.dtype == torch.bfloat16 and L.device_error() == 0
+    want, tol = _attention64(c, q, sink, lens, start, range(len(lens)))
+    _check(o, want, tol)
+
+
+@pytest.mark.parametrize("page", [8, 16, 24, 32, 48, 64, 100, 128, 256])
+def test_chunk_attention_page_sizes(page):
+    """Pages smaller than, larger than and out of step with the rows taken at a time, handed out by the cache."""
+    pkg, _, L = _mods()
+    lens, start = [5, 70, 1], [611, 1200, 37]
+    c, q, sink, cu, st, _ = _case(lens, start, page=page, seed=2, paged=True)
+    o = pkg.chunk_attention(c, q, sink, cu, st, freqs=_freqs().cuda())
+    assert L.device_error() == 0
+    want, tol = _attention64(c, q, sink, lens, start, range(3))
+    _check(o, want, tol)
+
+
+def test_chunk_attention_window_only_slots_padding_and_types():
+    """A cache without compressed rows; sequences in other slots than their order; rows behind the last
+    sequence; an fp32 output; strided queries, 64-bit indices; another window."""
+    pkg, _, L = _mods()
+    f = _freqs().cuda()
+    lens, start, seqs = [9, 200, 3], [50, 1000, 0], [4, 0, 2]
+    for ratio, window in ((0, 128), (4, 128), (4, 256), (4, 64)):
+        c, q, sink, cu, st, sq = _case(lens, start, ratio=ratio, seed=3, seqs=seqs, slots=5, pad=7, window=window)
+        wide = torch.empty(q.shape[0], H, 2 * D, dtype=q.dtype, device="cuda")
+        wide[..., :D] = q
+        o = pkg.chunk_attention(c, wide[..., :D], sink, cu.long(), st.long(), seqs=sq.long(), freqs=f, out_dtype=torch.float32)
+        assert o.dtype == torch.float32 and o.shape == q.shape
+        want, tol = _attention64(c, q, sink, lens, start, seqs)
+        _check(o, want, tol)
+        assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("lens,start,k", [([40], [3000], 64), ([5, 17], [100, 2000], 33), ([2], [9], 16), ([1], [40000], 512)])
+def test_chunk_attention_listed(lens, start, k):
+    """Given rows instead of all: lists with gaps, empty lists, the first tokens without any entry."""
+    pkg, _, L = _mods()
+    c, q, sink, cu, st, _ = _case(lens, start, seed=4)
+    rng = np.random.default_rng(5)
+    rows = np.full((sum(lens), k), -1, np.int32)
+    at = 0
+    for b, (n, s) in enumerate(zip(lens, start)):
+        for i in range(n):
+            seen = (s + i + 1) // R
+            e = np.sort(rng.choice(seen, min(k, seen), replace=False)) if i % 5 != 4 else np.zeros(0, int)
+            put = np.sort(rng.choice(k, len(e), replace=False))
+            bt = c.block_table[b].cpu().numpy()
+            rows[at + i, put] = c.comp_base + bt[e // c.page] * c.page + e % c.page
+        at += n
+    rows = torch.from_numpy(rows).cuda()
+    o = pkg.chunk_attention(c, q, sink, cu, st, rows=rows, freqs=_freqs().cuda())
+    assert L.device_error() == 0
+    want, tol = _attention64(c, q, sink, lens, start, range(len(lens)), rows)
+    _check(o, want, tol)
+
+
+def test_chunk_attention_masked_rows_may_hold_anything():
+    """NaN and infinities in every row that no token of the chunk sees: ring slots out of the window,
+    entries not yet complete, other sequences' stages and pages, rows behind the stage."""
+    pkg, _, L = _mods()
+    lens, start, seqs = [3, 70], [130, 77], [0, 1]
+    c, q, sink, cu, st, _ = _case(lens, start, seed=6, slots=3, pad=60)
+    seen = torch.zeros(c.kv_pool.shape[0], dtype=torch.bool, device="cuda")
+    at = 0
+    for n, s, b in zip(lens, start, seqs):
+        seen[c.stage_base + at:c.stage_base + at + n] = True
+        w = torch.arange(max(0, s - c.window + 1), s, device="cuda")
+        seen[b * c.window + w % c.window] = True
+        e = torch.arange((s + n) // R, device="cuda")
+        seen[c.comp_base + c.block_table[b].long()[e // c.page] * c.page + e % c.page] = True
+        at += n
+    want, tol = _attention64(c, q, sink, lens, start, seqs)
+    bad = torch.tensor([float("nan"), float("inf"), float("-inf")], device="cuda").to(torch.bfloat16)
+    fill = bad[torch.arange(c.kv_pool.shape[0], device="cuda") % 3]
+    c.kv_pool[~seen] = fill[~seen][:, None]
+    q[sum(lens):] = float("nan")
+    o = pkg.chunk_attention(c, q, sink, cu, st, freqs=_freqs().cuda())
+    _check(o, want, tol)
+    assert L.device_error() == 0
+
+
+def test_chunk_attention_large_scores_and_sinks():
+    """Scores far apart (a running maximum that keeps growing along the list), sinks that swallow all or nothing."""
+    pkg, _, _ = _mods()
+    lens, start = [6], [2100]
+    c, q, sink, cu, st, _ = _case(lens, start, seed=7)
+    grow = torch.linspace(0.01, 12, c.kv_pool.shape[0], device="cuda")[:, None]
+    c.kv_pool.copy_((c.kv_pool.float() * grow).to(torch.bfloat16))
+    sink = torch.linspace(-300, 300, H, device="cuda")
+    o = pkg.chunk_attention(c, q, sink, cu, st, freqs=_freqs().cuda())
+    want, tol = _attention64(c, q, sink, lens, start, [0])
+    # scores up to 12 * 60: their fp32 rounding (512 products) moves a weight by up to 2^-24 * 512 * 720 / sqrt(512) = 2^-10
+    _check(o, want, tol * 1.25 + 1e-30)
+
+
+def test_chunk_attention_graph_streams_and_repeat():
+    """Captured and replayed with other inputs; two streams at once; the same call twice, bit for bit."""
+    pkg, _, _ = _mods()
+    f = _freqs().cuda()
+    a = _case([5, 3], [900, 40], seed=8)
+    b = _case([5, 3], [900, 40], seed=9)
+    args = lambda k: (k[0], k[1], k[2], k[3], k[4])  # noqa: E731
+    want_a, want_b = pkg.chunk_attention(*args(a), freqs=f), pkg.chunk_attention(*args(b), freqs=f)
+    assert torch.equal(want_a, pkg.chunk_attention(*args(a), freqs=f))
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(4):
+        for s, k in ((s1, a), (s2, b)):
+            with torch.cuda.stream(s):
+                outs.append(pkg.chunk_attention(*args(k), freqs=f))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want_a) for x in outs[::2]) and all(torch.equal(x, want_b) for x in outs[1::2])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = pkg.chunk_attention(*args(a), freqs=f)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, want_a)
+    a[0].kv_pool.copy_(b[0].kv_pool), a[0].block_table.copy_(b[0].block_table), a[1].copy_(b[1]), a[2].copy_(b[2])
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, want_b)
+
+
+def test_chunk_attention_refusals():
+    pkg, Dm, L = _mods()
+    c, q, sink, cu, st, sq = _case([4], [100], seed=10)
+    ok = dict(cache=c, q=q, sink=sink, cu_seqlens=cu, start=st)
+    for err, kw in ((TypeError, dict(q=q.float())), (ValueError, dict(q=q[:, :32])), (ValueError, dict(q=q[..., :256])),
+                    (ValueError, dict(sink=sink[:3])), (TypeError, dict(out_dtype=torch.float16)),
+                    (ValueError, dict(start=st.repeat(2))), (TypeError, dict(cu_seqlens=cu.float())),
+                    (ValueError, dict(seqs=sq.repeat(2))), (ValueError, dict(cu_seqlens=torch.zeros(3, dtype=torch.int32, device="cuda"),
+                                                                            start=st.repeat(2))),
+                    (ValueError, dict(rows=torch.zeros(3, 5, dtype=torch.int32, device="cuda"))),
+                    (ValueError, dict(rows=torch.zeros(4, 5, device="cuda"))), (RuntimeError, dict(sink=sink.cpu())),
+                    (ValueError, dict(q=q.repeat(2, 1, 1)))):
+        with pytest.raises(err):
+            pkg.chunk_attention(**{**ok, **kw})
+    assert pkg.chunk_attention(**{**ok, "q": q[:0], "cu_seqlens": cu * 0}).shape == (0, H, D)
+    # an entry whose page the sequence does not have: reported, and the rest of its rows still attended
+    p, q, sink, cu, st, _ = _case([4], [1000], seed=11, paged=True)
+    p.block_table[0, 2] = -1
+    o = pkg.chunk_attention(p, q, sink, cu, st, freqs=_freqs().cuda())
+    assert torch.isfinite(o).all() and L.device_error() == 4 and L.device_error() == 0
+
+
+# ---- the compressor over a chunk ----
+
+def _compress_by_step(pkg, kv, sc, lens, start, seqs, ape, nw, rk, rs, out, rows_of, d, ratio, f, **kw):
+    """One compressor_decode_step per token."""
+    at = 0
+    for n, s, b in zip(lens, start, seqs):
+        for i in range(n):
+            p = torch.tensor([s + i], dtype=torch.int32, device="cuda")
+            r = torch.tensor([rows_of(b, max((s + i + 1) // ratio - 1, 0))], device="cuda")
+            pkg.compressor_decode_step(p, kv, kv, ape, nw, rk[b:b + 1], rs[b:b + 1], p, out, r, head_dim=d, ratio=ratio, freqs=f,
+                                       proj=(kv[at + i:at + i + 1].contiguous(), sc[at + i:at + i + 1].contiguous()), **kw)
+        at += n
+
+
+@pytest.mark.parametrize("d,ratio,lens,start", [
+    (512, 4, [1], [0]), (512, 4, [1], [3]), (512, 4, [4, 4, 4, 4], [0, 1, 2, 3]), (512, 4, [9, 1, 0, 30], [0, 7, 5, 10]),
+    (128, 4, [17, 2, 3], [6, 0, 13]), (1024, 4, [21], [2]), (96, 4, [11, 8], [1, 4]), (64, 1, [5, 3], [0, 7]),
+    (512, 2, [7, 1], [1, 3]), (128, 3, [10, 2], [4, 0]), (512, 8, [37, 5], [3, 16]), (512, 5, [23], [7])])
+@pytest.mark.parametrize("quant", [0, 1, 2])
+def test_compressor_chunk_equals_the_steps(d, ratio, lens, start, quant):
+    """Rows, rings and key image bit for bit as one decode step per token leaves them (the order of the
+    operations in a row is the same)."""
+    pkg, Dm, L = _mods()
+    if (quant == 2 and d != 128) or (quant == 1 and d % 64):
+        pytest.skip("a quantisation of other widths")
+    I = importlib.import_module(PKG + ".indexer")
+    g = torch.Generator(device="cuda").manual_seed(d + ratio)
+    rope = min(64, d - 64 if quant == 1 and d > 64 else d)
+    if quant == 1 and d == 64:
+        rope = 0
+    f = (_freqs() if rope else torch.zeros(1)).cuda()
+    slots, page = len(lens) + 2, 16
+    seqs = list(range(1, len(lens) + 1))
+    most = max((s + n) // ratio for n, s in zip(lens, start)) + 3
+    per = -(-most // page)
+    table = torch.randperm(slots * per, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(slots, per).cuda()
+    total = sum(lens)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    kv, sc, ape, nw = rnd(total, 2 * d), rnd(total, 2 * d), rnd(ratio, 2 * d), 1 + 0.1 * rnd(d)
+    rk, rs = rnd(slots, 2 * ratio, 2 * d), rnd(slots, 2 * ratio, 2 * d)
+    for s, b in zip(start, seqs):
+        if s < ratio:
+            rk[b], rs[b, :ratio] = 0, float("-inf")
+            rs[b, ratio + s:] = float("-inf")
+    keys = d == 128 and ratio == 4
+    dt = torch.float32 if d == 128 else torch.bfloat16
+    out = torch.zeros((3 + slots * per * page, d), dtype=dt, device="cuda")
+    image = I.key_image_buffers(slots, most, "cuda") if keys else None
+    state = [rk, rs, out, *(image or ())]
+    mine, ref = [t.clone() for t in state], [t.clone() for t in state]
+    bt = table.cpu()
+    if keys:
+        rows_of, kw, ckw = (lambda b, e: b * most + e), dict(key_image=(*ref[3:], most)), dict(key_image=mine[3:])
+    else:
+        rows_of, kw, ckw = (lambda b, e: 3 + int(bt[b, e // page]) * page + e % page), {}, dict(block_table=table, page=page, out_base=3)
+    q = dict(act_quant=quant == 1, rotate=quant == 2, rope_head_dim=rope)
+    _compress_by_step(pkg, kv, sc, lens, start, seqs, ape, nw, ref[0], ref[1], ref[2], rows_of, d, ratio, f, **kw, **q)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    pkg.compressor_chunk((kv, sc), cu, torch.tensor(start, dtype=torch.int32, device="cuda"), ape, nw, mine[0], mine[1], mine[2],
+                         most, seqs=torch.tensor(seqs, dtype=torch.int32, device="cuda"), head_dim=d, ratio=ratio, freqs=f,
+                         **ckw, **q)
+    assert L.device_error() == 0
+    for name, a, b in zip(("ring_kv", "ring_score", "rows", "image", "inv", "norm_max"), mine, ref):
+        assert torch.equal(a, b), name
+
+
+def test_compressor_chunk_against_the_definition():
+    """Rows in 64 bits: eight-slot softmax, norm and rotation. fp32 arithmetic: at most 40 roundings of
+    2^-24 on values of the row's scale (each output is a normalised weighted mean; the norm divides by the
+    rms, 512 terms summed in a tree), plus the rotation's angle, an exact product of fp32 in both."""
+    pkg, _, L = _mods()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    n, s, d = 203, 5, 512
+    kv, sc = (torch.randn(n, 2 * d, generator=g, device="cuda") for _ in range(2))
+    ape, nw = torch.randn(4, 2 * d, generator=g, device="cuda"), torch.ones(d, device="cuda")
+    rk, rs = (torch.randn(1, 8, 2 * d, generator=g, device="cuda") for _ in range(2))
+    k = torch.cat([rk[0, :5], kv]).double()                       # positions 0..4 from the ring (block 0, then token 4)
+    x = torch.cat([rs[0, :5], sc + ape[(s + torch.arange(n, device="cuda")) % 4]]).double()
+    blocks = k.shape[0] // 4
+    k, x = k[:blocks * 4].view(blocks, 4, 2, d), x[:blocks * 4].view(blocks, 4, 2, d)
+    w = torch.softmax(torch.cat([x[:-1, :, 0], x[1:, :, 1]], 1), 1)
+    row = (w * torch.cat([k[:-1, :, 0], k[1:, :, 1]], 1)).sum(1)
+    row = row / (row.square().mean(-1, keepdim=True) + 1e-6).sqrt()
+    pos = 4 * torch.arange(1, blocks, device="cuda")
+    row = _rotate64(row[:, None], pos, _freqs(), 1)[:, 0]
+    out = torch.zeros(60, d, device="cuda")
+    pkg.compressor_chunk((kv, sc), torch.tensor([0, n], dtype=torch.int32, device="cuda"),
+                         torch.tensor([s], dtype=torch.int32, device="cuda"), ape, nw, rk, rs, out, 60, freqs=_freqs().cuda())
+    assert L.device_error() == 0
+    assert (out[0] == 0).all() and (out[blocks:] == 0).all()
+    assert ((out[1:blocks].double() - row).abs() <= 40 * 2.0 ** -24 * row.abs().amax(-1, keepdim=True)).all()
+
+
+def test_compressor_chunk_errors_and_refusals():
+    pkg, _, L = _mods()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    kv, sc = (torch.randn(12, 1024, generator=g, device="cuda") for _ in range(2))
+    ape, nw = torch.zeros(4, 1024, device="cuda"), torch.ones(512, device="cuda")
+    ring = lambda: (torch.zeros(2, 8, 1024, device="cuda"), torch.zeros(2, 8, 1024, device="cuda"))  # noqa: E731
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    # past the end of the cache, a missing page, a page outside of `out`, a slot that does not exist: reported, not stored
+    for table, most, seqs in ((i32(0).view(1, 1).repeat(2, 1), 2, None), (i32(-1).view(1, 1).repeat(2, 1), 8, None),
+                              (i32(9).view(1, 1).repeat(2, 1), 8, None), (i32(0).view(1, 1).repeat(2, 1), 8, i32(7))):
+        out = torch.zeros(16, 512, device="cuda")
+        pkg.compressor_chunk((kv, sc), i32(0, 12), i32(0), ape, nw, *ring(), out, most, block_table=table, page=8, seqs=seqs)
+        assert L.device_error() == 4
+        assert (out[2 if most == 2 else 0:] == 0).all()
+    out, r = torch.zeros(16, 512, device="cuda"), ring()
+    good = dict(proj=(kv, sc), cu_seqlens=i32(0, 12), start=i32(0), ape=ape, norm_w=nw, ring_kv=r[0], ring_score=r[1], out=out,
+                max_comp=8)
+    for err, kw in ((ValueError, dict(proj=(kv[:, :512], sc[:, :512]))), (ValueError, dict(proj=(kv.half(), sc.half()))),
+                    (ValueError, dict(ring_kv=r[0][:, :4])), (ValueError, dict(ring_score=r[1][:1])), (ValueError, dict(out=out.half())),
+                    (ValueError, dict(out=out[:, :256])), (ValueError, dict(start=i32(0, 1))), (TypeError, dict(start=i32(0).long())),
+                    (ValueError, dict(max_comp=9)), (ValueError, dict(ape=ape[:2])), (ValueError, dict(norm_w=nw[:9])),
+                    (ValueError, dict(block_table=i32(0).view(1, 1), page=8)), (RuntimeError, dict(start=torch.tensor([0], dtype=torch.int32))),
+                    (ValueError, dict(freqs=torch.ones(3, device="cuda"))), (ValueError, dict(seqs=i32(0, 1)))):
+        with pytest.raises(err):
+            pkg.compressor_chunk(**{**good, **kw})
+
+
+# ---- rows, and whole layers ----
+
+def test_chunk_rows_and_commit():
+    pkg, _, L = _mods()
+    lens, start, seqs = [300, 2, 0, 64], [10, 127, 3, 500], [1, 0, 4, 2]
+    c, q, sink, cu, st, sq = _case(lens, start, seed=12, seqs=seqs, slots=5, pad=3)
+    pos, rows = pkg.chunk_rows(c, cu, st, q.shape[0], sq)
+    want = np.concatenate([np.arange(s, s + n) for n, s in zip(lens, start)] + [np.zeros(3, int)])
+    assert (pos.cpu().numpy() == want).all()
+    assert torch.equal(rows, c.stage_base + torch.arange(q.shape[0], device="cuda"))
+    ref, at = c.kv_pool.clone(), 0
+    for n, s, b in zip(lens, start, seqs):
+        for i in range(max(0, n - W), n):
+            ref[b * W + (s + i) % W] = ref[c.stage_base + at + i]
+        at += n
+    pkg.chunk_commit(c, cu, st, q.shape[0], sq)
+    assert torch.equal(c.kv_pool, ref) and L.device_error() == 0
+
+
+def _block(ratio, batch, max_ctx, top_k, **kw):
+    Lm, C = importlib.import_module(PKG + ".layer"), importlib.import_module(PKG + ".configs")
+    dims = C.LayerDims(ratio=ratio)
+    Wt = Lm.make_attention_weights(40 + ratio, dims=dims).to("cuda")
+    return Lm.DecodeBlock(Wt, batch, max_ctx, top_k=top_k, dims=dims, **kw), Wt, dims, Lm
+
+
+# both take the same bf16 roundings at the same places; the projections' sums run in another order (fp32),
+# which moves a value across a rounding border here and there: the block bound of the layer tests
+BLOCK_REL = 1e-2
+
+
+@pytest.mark.parametrize("ratio,paged,top_k", [(4, False, 512), (4, True, 512), (4, True, 32), (0, False, 512), (128, False, 512)])
+def test_extend_equals_the_steps(ratio, paged, top_k):
+    """Chunks and single tokens on two sequences, against single tokens alone: outputs, window rings,
+    compressed rows and compressor rings."""
+    pkg, _, L = _mods()
+    kw = dict(n_pages=24) if paged else {}
+    a, Wt, dims, Lm = _block(ratio, 2, 640, top_k, max_chunk=320, page=16, **kw)
+    b, _, _, _ = _block(ratio, 2, 640, top_k, page=16, **kw)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(2, 330, 4096, generator=g, device="cuda")
+    outs = [[], []]
+    o = a.extend(torch.cat([x[0, :150], x[1, :150], x[0, :9]]), [150, 150], [0, 0])       # nine rows of padding
+    outs[0].append(o[:150]), outs[1].append(o[150:300])
+    o = a.extend(torch.cat([x[1, 150:157], x[0, 150:320]]), [7, 170], [150, 150], seqs=[1, 0])
+    outs[1].append(o[:7]), outs[0].append(o[7:])
+    o = a.extend(x[1, 157:320], [163], [157], seqs=[1])
+    outs[1].append(o)
+    o = a.step(x[:, 320], torch.full((2,), 320, dtype=torch.int32, device="cuda"))
+    outs[0].append(o[:1]), outs[1].append(o[1:])
+    ref = [b.step(x[:, p], torch.full((2,), p, dtype=torch.int32, device="cuda")) for p in range(321)]
+    ref = torch.stack(ref, 1)
+    assert L.device_error() == 0
+    for s in range(2):
+        got = torch.cat(outs[s])
+        if top_k > 80:
+            assert rel_rms(got, ref[s]) <= BLOCK_REL
+        else:   # selections from scores an fp32 rounding apart: the tokens before the first selection, and most after
+            assert rel_rms(got[:4 * top_k], ref[s][:4 * top_k]) <= BLOCK_REL
+            near = ((got - ref[s]).norm(dim=-1) / ref[s].norm(dim=-1)) <= 2 * BLOCK_REL
+            assert near.float().mean() >= 0.9
+        assert rel_rms(a.cache.kv_pool[s * W:(s + 1) * W].float(), b.cache.kv_pool[s * W:(s + 1) * W].float()) <= BLOCK_REL
+        if ratio == 4:
+            e = torch.arange(80, device="cuda")
+            assert rel_rms(a.cache.kv_pool[a.cache.comp_rows(s, e)].float(), b.cache.kv_pool[b.cache.comp_rows(s, e)].float()) <= BLOCK_REL
+            assert rel_rms(a.cache.k_idx[s, :80], b.cache.k_idx[s, :80]) <= BLOCK_REL
+            assert rel_rms(a.cache.ring_kv[s], b.cache.ring_kv[s]) <= BLOCK_REL
+
+
+def test_extend_continues_a_prefill_and_refuses():
+    """prefill_layer of a prompt, then a chunk: the rows of the whole prompt's prefill."""
+    pkg, _, L = _mods()
+    blk, Wt, dims, Lm = _block(4, 1, 640, 512, max_chunk=128, n_pages=5, page=32)
+    x = torch.randn(300, 4096, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    whole = Lm.prefill_layer(x, Wt, dims=dims)
+    _, aux = Lm.prefill_layer(x[:190], Wt, dims=dims, return_aux=True)
+    blk.load_prefill(0, aux)
+    o = blk.extend(x[190:300], [110], [190])
+    assert L.device_error() == 0 and rel_rms(o, whole[190:]) <= BLOCK_REL
+    assert blk.cache.page_refs.sum() == -(-75 // 32)
+    for kw in (dict(lengths=[3], start=[300, 1]), dict(lengths=[5], start=[300]), dict(lengths=[-1], start=[300]),
+               dict(lengths=[4], start=[-1]), dict(lengths=[1, 1], start=[3, 4], seqs=[0, 0]), dict(lengths=[4], start=[700]),
+               dict(lengths=[4], start=[300], seqs=[1])):
+        with pytest.raises(ValueError):
+            blk.extend(x[:4], **kw)
+    with pytest.raises(ValueError, match="max_chunk"):
+        blk.extend(x[:200], [200], [300])
