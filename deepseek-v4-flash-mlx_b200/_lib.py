@@ -120,6 +120,11 @@ class Chunk(ctypes.Structure):
                 ("window", i32), ("ratio", i32), ("page", i32), ("bt_stride", i32), ("max_comp", i32)]
 
 
+class ChunkAttnParams(ctypes.Structure):
+    _fields_ = [("chunk", Chunk), ("q", vp), ("pool", vp), ("sink", vp), ("out", vp), ("rope_freqs", vp), ("rope_dim", i32),
+                ("out_dtype", i32), ("scale", f32), ("num_splits", i32), ("workspace", vp), ("workspace_bytes", sz)]
+
+
 class CompressorChunkParams(ctypes.Structure):
     _fields_ = [("kv", vp), ("score", vp), ("ape", vp), ("norm_w", vp), ("ring_kv", vp), ("ring_score", vp), ("out", vp),
                 ("freqs", vp), ("cu_seqlens", vp), ("start", vp), ("seqs", vp), ("block_table", vp), ("out_base", i64),
@@ -159,6 +164,8 @@ SIGNATURES = {
                                                    ctypes.POINTER(CompressorDecodeParams), vp]),
     "dsv4_chunk_rows": (ctypes.c_int, [ctypes.POINTER(Chunk), vp, vp, vp, i64, i32, vp, vp]),
     "dsv4_chunk_commit": (ctypes.c_int, [ctypes.POINTER(Chunk), vp, i32, vp]),
+    "dsv4_chunk_attn_workspace_size": (sz, [ctypes.POINTER(ChunkAttnParams)]),
+    "dsv4_chunk_attn": (ctypes.c_int, [ctypes.POINTER(ChunkAttnParams), vp]),
     "dsv4_compressor_chunk": (ctypes.c_int, [ctypes.POINTER(CompressorChunkParams), vp]),
     "dsv4_pages_workspace_size": (sz, [ctypes.POINTER(Pages), i32]),
     "dsv4_pages_free": (ctypes.c_int, [ctypes.POINTER(Pages), vp, i32, vp]),

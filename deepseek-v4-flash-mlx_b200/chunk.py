@@ -82,7 +82,21 @@ def chunk_commit(cache, cu_seqlens, start, total, seqs=None):
                                           L.stream_of(cache.kv_pool)))
 
 
-def _attend(cache, c, q, sink, rows, scale, freqs, out_dtype):
+def _attend(cache, c, q, sink, scale, freqs, out_dtype, num_splits):
+    """All visible rows: dsv4_chunk_attn, which finds them by itself."""
+    out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    p = L.ChunkAttnParams()
+    p.chunk = c
+    p.q, p.pool, p.sink, p.out, p.rope_freqs = (t.data_ptr() for t in (q, cache.kv_pool, sink, out, freqs))
+    p.rope_dim, p.out_dtype, p.scale, p.num_splits = 2 * freqs.numel(), L.dtype_code(out), scale, num_splits
+    nbytes = L.lib().dsv4_chunk_attn_workspace_size(ctypes.byref(p))
+    ws = L.workspace(nbytes, q.device)
+    p.workspace, p.workspace_bytes = L.ptr(ws), nbytes
+    L.check(L.lib().dsv4_chunk_attn(ctypes.byref(p), L.stream_of(q)))
+    return out
+
+
+def _attend_listed(cache, c, q, sink, rows, scale, freqs, out_dtype):
     """Every token's list as an index tensor, and the sparse attention over it."""
     total = q.shape[0]
     cols = cache.max_comp if rows is None else rows.shape[1]
@@ -95,7 +109,7 @@ def _attend(cache, c, q, sink, rows, scale, freqs, out_dtype):
 
 
 def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, scale=None, freqs=None,
-                    out_dtype=torch.bfloat16):
+                    out_dtype=torch.bfloat16, num_splits=0):
     """Attention of a chunk of new tokens over the cache, their kv rows staged (`chunk_rows`) and their
     compressed rows written (`compressor_chunk`).
 
@@ -103,7 +117,8 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
     position p sees the window rows of positions p-window+1 .. p, from the ring before the chunk and from
     the stage in it, and every compressed entry j < (p+1) // ratio (the list of
     oracle/decode_engine.py:110-116), or with `rows` (int32 [total, k] pool rows, -1 for none: the
-    indexer's selection) those instead. Returns o [total, 64, 512] after the inverse RoPE; what it holds
+    indexer's selection) those instead. `num_splits`: over how many CTA pairs the rows of two tokens are split
+    (0: automatic; all visible rows only). Returns o [total, 64, 512] after the inverse RoPE; what it holds
     behind the last sequence is not defined."""
     L.require_cuda(q, sink, rows, freqs)
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
@@ -122,11 +137,18 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
             raise ValueError(f"chunk_attention: rows must be int32 [{total}, k], got {rows.dtype} {tuple(rows.shape)}")
         rows = rows.to(torch.int32).contiguous()
     freqs = rope_freqs(64, q.device) if freqs is None else freqs.float().contiguous()
-    if freqs.numel() > cache.head_dim // 2:
-        raise ValueError("chunk_attention: more rotation frequencies than pairs of dims")
+    if not 0 < freqs.numel() <= 32:
+        raise ValueError(f"chunk_attention: 1 to 32 rotation frequencies, got {freqs.numel()}")
+    if not 0 <= num_splits <= 64:
+        raise ValueError(f"chunk_attention: 0 to 64 splits, got {num_splits}")
     scale = cache.head_dim ** -0.5 if scale is None else float(scale)
     c, keep = _chunk(cache, cu_seqlens, start, seqs, total)
     if total == 0 or c.n == 0:
         return torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    q, sink = q.contiguous(), sink.float().contiguous()
     with L.device_of(q):
-        return _attend(cache, c, q.contiguous(), sink.float().contiguous(), rows, scale, freqs, out_dtype)
+        # lists differ from token to token, and pages that no box of rows divides have no run to load: those
+        # go through an index, token by token
+        if rows is None and (cache.page % 8 == 0 or not cache.compressed) and cache.window <= 1024:
+            return _attend(cache, c, q, sink, scale, freqs, out_dtype, int(num_splits))
+        return _attend_listed(cache, c, q, sink, rows, scale, freqs, out_dtype)

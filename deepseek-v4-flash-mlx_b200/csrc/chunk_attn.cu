@@ -1,0 +1,764 @@
+// Attention of a chunk of new tokens over the paged cache, every token over its window and all of its
+// compressed rows (the list of oracle/decode_engine.py:110-116), on the 5th-generation tensor cores.
+//
+// All 64 heads share the 512-wide row that is both key and value, so the tokens of a chunk are rows of
+// one matrix: two neighbouring tokens times 64 heads are the M = 128 rows of a CTA pair
+// (cta_group::2), one token in each CTA, against tiles of 128 cached rows:
+//   S[row, j]   = Q[row, :] . K[j, :]        M = 128, N = 128, K = 512   (tensor memory, two buffers)
+//   P[row, j]   = 2^(S * scale * log2 e - m[row])  as bf16               (shared memory, two buffers)
+//   O[row, :]  += P[row, :] . K[:, :]        M = 128, N = 2 x 256, K = 128 (tensor memory, 256 columns)
+// A pair because of space: O alone is 128 KB a token. M = 128 over two CTAs gives each CTA its 64 rows
+// with the columns folded over the 128 TMEM lanes (lane l: row l % 64, columns of half l / 64), so O
+// takes 256 of the 512 TMEM columns and two S buffers 128; and each operand tile is brought into the
+// pair once for S and half of it once more for O, not twice into each CTA:
+//   as K (N = 128 rows, split over the pair): CTA r holds rows 64 r .. 64 r + 63, all 512 dims;
+//   as V (N = 512 dims, split over the pair): CTA r holds dims 256 r .., all 128 rows.
+// A tile buffer has two 32 KB slots, X and Y. For S the CTA's own 64 rows are in X (dims 0-255) and Y
+// (dims 256-511). For O X holds rows 0-63 and Y rows 64-127 of the CTA's dims: of the two slots one is
+// already that (X in CTA 0, Y in CTA 1), the other is loaded again once S has been computed. 96 KB per
+// tile and CTA instead of 128, and two tiles fit beside Q (64 KB) and P (2 x 16 KB).
+//
+// Rows come in halves of 64: the ring's rows of before the chunk, in slot order; the staged rows of
+// the chunk itself; the compressed entries, page by page. Every half is a run of the pool, so TMA
+// brings it in (boxes of min(64, the power of two that divides the page) rows), coordinates past the
+// pool for what is not there (TMA fills zeros). Visibility is a 64-bit mask per half and token. Rows
+// that neither token of the pair sees are zeroed in shared memory before they are used as values, so
+// that whatever they hold stays out; a row that one of the two sees is finite or spoils both.
+//
+// Roles (11 warps a CTA): warps 0-7 softmax and epilogue (warp w: TMEM lanes 32 (w % 4) .., columns of
+// half w / 4); warp 8 loads Q and the tiles as K; warp 9 of CTA 0 issues all MMAs, whichever of the
+// next S and the next O has its operands ready; warp 10 loads the second slot as V. The running
+// maximum is lazy (raised only when a score passes it by 2^8; O and the sums are then rescaled), the
+// sums are fp32, of the rounded probabilities. P is rounded to bf16 (the MMA takes both operands in
+// the rows' type), O is rounded once at the end.
+// Long lists with few tokens are split over clusters; fp32 partials and a merging kernel follow.
+// All waits inside a CTA are bounded (1 s): DSV4_ERR_WAIT_TIMEOUT, and the pair drains and leaves.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "chunk.cuh"
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace dsv4 {
+namespace ca {
+
+using namespace tc5;
+
+constexpr int D = 512, HB = 64, BN = 128;
+constexpr int SMX_WARPS = 8, SMX_THREADS = 256, THREADS = 352;
+constexpr int SLAB = 64 * 128;           // 64 rows of 64 bf16 dims, 128-byte swizzled
+constexpr int SLOT = 4 * SLAB;           // 64 rows of 256 dims
+constexpr int TMEM_COLS = 512, COL_O = 0, COL_S = 256;
+constexpr int MAX_WINDOW = 1024;         // the ring's halves are kept as 4-bit numbers
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float RESCALE = 8.0f;          // log2 units a score may pass the running maximum by
+
+struct Smem {
+  uint8_t q[8 * SLAB];
+  uint8_t kv[2][2][SLOT];                // [tile buffer][X, Y]
+  uint8_t p[2][2 * SLAB];                // [buffer][rows 0-63 of the tile, rows 64-127]
+  float red[4][HB];
+  float rope_c[32], rope_s[32];
+  uint64_t q_full, kv_full[2], s_full[2], p_full[2], v_full[2], done[2];
+  uint32_t tmem_base;
+  int abort;
+  int unit[4];                           // sequence, first token of the pair, tokens, units in all
+};
+static_assert(sizeof(Smem) + 1024 <= 232448, "shared memory above the 227 KB a CTA may opt into");
+
+struct Params {
+  CUtensorMap pool;  // [pool_rows, 512] bf16, box 64 dims x box_rows
+  CUtensorMap q;     // [total * 64, 512] bf16, box 64 dims x 64 rows
+  dsv4_chunk c;
+  const float* sink;
+  void* out;
+  float* part;       // splits > 1: O [total][splits][64][512], then (m, l) [total][splits][64][2]
+  const float* freqs;
+  int rope_dim, out_dtype, splits, box_rows;
+  float scale_log2;
+};
+
+// ---- the pair
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+// not a waiting form: the issuer looks at two barriers in turn
+__device__ __forceinline__ bool test_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// a tile load into this CTA's shared memory that completes on a barrier of CTA 0 of the pair
+__device__ __forceinline__ void load_pair(void* dst, const void* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];\n" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc));
+}
+// arrive on `bar` of both CTAs once the MMAs issued before have completed
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {  // 2^x, relative error about 2^-22, 2^-inf = +0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void smx_bar() { asm volatile("bar.sync 1, %0;\n" ::"n"(SMX_THREADS) : "memory"); }
+__device__ __forceinline__ bool smx_any(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, 1, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(v)), "n"(SMX_THREADS)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void set_abort(Smem& sm) {
+  if (!*reinterpret_cast<volatile int*>(&sm.abort)) {
+    *reinterpret_cast<volatile int*>(&sm.abort) = 1;
+    raise_device_error(DSV4_ERR_WAIT_TIMEOUT);
+  }
+}
+
+// ---- the halves of 64 rows that a pair of tokens attends to
+struct Unit {
+  int first, start;       // the sequence's first token in the batch and its position
+  int t0, n;              // the pair's first token, tokens of the pair (1 or 2)
+  int p0;                 // its position
+  int64_t win;            // the ring's first pool row
+  const int32_t* table;
+  int stage_pos;          // position of the first staged row it sees
+  int nring, nstage, nh;  // halves: ring, stage, all
+  uint64_t ring;          // the ring's halves, 4 bits each
+  int seen[2];            // compressed entries that the first and the last token see
+};
+__device__ __forceinline__ Unit make_unit(const dsv4_chunk& c, int seq, int t0, int n) {
+  Unit u;
+  u.first = c.cu_seqlens[seq];
+  u.start = c.start[seq];
+  u.t0 = t0;
+  u.n = n;
+  u.p0 = u.start + (t0 - u.first);
+  const int slot = c.seqs ? c.seqs[seq] : seq;
+  u.win = c.win_base[slot];
+  u.table = c.block_table ? c.block_table + static_cast<int64_t>(slot) * c.bt_stride : nullptr;
+  const int lo = max(0, u.p0 - c.window + 1);  // oldest position in the first token's window
+  u.ring = 0;
+  u.nring = 0;
+  const int old = u.start - lo;                // rows of before the chunk: slots lo % window .., cyclic
+  if (old > 0)
+    for (int h = 0; h < c.window / 64; ++h) {
+      const int gap = (h * 64 - lo % c.window + c.window) % c.window;  // slots from the oldest row to the half
+      if (gap < old || gap > c.window - 64) u.ring |= static_cast<uint64_t>(h) << (4 * u.nring++);
+    }
+  u.stage_pos = max(u.start, lo);
+  u.nstage = (u.p0 + n - u.stage_pos + 63) / 64;
+  u.seen[0] = chunk_seen(c, u.p0);
+  u.seen[1] = chunk_seen(c, u.p0 + n - 1);
+  u.nh = u.nring + u.nstage + (u.seen[1] + 63) / 64;
+  return u;
+}
+// first pool row of box b of half h; the row behind the pool where there is nothing to load
+__device__ __forceinline__ int half_row(const Params& P, const Unit& u, int h, int b) {
+  const dsv4_chunk& c = P.c;
+  const int r = b * P.box_rows;
+  if (h < u.nring) return static_cast<int>(u.win) + 64 * static_cast<int>((u.ring >> (4 * h)) & 15) + r;
+  h -= u.nring;
+  if (h < u.nstage) return static_cast<int>(c.stage_base) + u.first + (u.stage_pos - u.start) + 64 * h + r;
+  const int e = 64 * (h - u.nstage) + r;
+  if (e >= u.seen[1]) return static_cast<int>(c.pool_rows);
+  const int32_t pg = u.table[e / c.page];
+  if (pg < 0) {
+    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+    return static_cast<int>(c.pool_rows);
+  }
+  const int64_t row = c.comp_base + static_cast<int64_t>(pg) * c.page + e % c.page;
+  return row < c.pool_rows ? static_cast<int>(row) : static_cast<int>(c.pool_rows);
+}
+// whether the token at position p (entries: what it sees of them) sees row j of half h
+__device__ __forceinline__ bool half_sees(const dsv4_chunk& c, const Unit& u, int h, int j, int p, int entries) {
+  if (h < u.nring) {
+    const int back = (u.start - 1 - 64 * static_cast<int>((u.ring >> (4 * h)) & 15) - j) % c.window;
+    const int pos = u.start - 1 - (back < 0 ? back + c.window : back);
+    return pos >= 0 && pos > p - c.window;
+  }
+  h -= u.nring;
+  if (h < u.nstage) {
+    const int pos = u.stage_pos + 64 * h + j;
+    return pos <= p && pos > p - c.window;
+  }
+  return 64 * (h - u.nstage) + j < entries;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_constant__ Params P) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = cluster_rank();
+  const int split = static_cast<int>(blockIdx.x >> 1) % P.splits;
+  const int want = static_cast<int>(blockIdx.x >> 1) / P.splits;
+
+  // The unit: pairs of tokens counted through the sequences. The last pairs see the most rows and
+  // are started first.
+  if (warp == 0) {
+    int total = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+      const int target = total - 1 - want;  // of the second pass
+      int before = 0, seq = -1, t0 = 0, n = 0;
+      for (int b0 = 0; b0 < P.c.n; b0 += 32) {
+        const int b = b0 + lane;
+        int cnt = 0, first = 0, len = 0;
+        if (b < P.c.n) {
+          first = P.c.cu_seqlens[b];
+          len = P.c.cu_seqlens[b + 1] - first;
+          const int slot = P.c.seqs ? P.c.seqs[b] : b;
+          const bool ok = first >= 0 && len >= 0 && first + len <= P.c.total && P.c.start[b] >= 0 && slot >= 0 && slot < P.c.slots;
+          if (!ok && pass == 0) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+          cnt = ok ? (len + 1) / 2 : 0;
+        }
+        int s = cnt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += x;
+        }
+        const int at = before + s - cnt;
+        if (pass == 1 && target >= at && target < at + cnt) {
+          seq = b;
+          t0 = first + 2 * (target - at);
+          n = min(2, first + len - t0);
+        }
+        before += __shfl_sync(0xffffffffu, s, 31);
+      }
+      if (pass == 0) {
+        total = before;
+      } else if (seq >= 0) {
+        sm.unit[0] = seq;
+        sm.unit[1] = t0;
+        sm.unit[2] = n;
+      }
+    }
+    if (lane == 0) sm.unit[3] = total;
+  }
+  __syncthreads();
+  if (want >= sm.unit[3]) return;  // the same in both CTAs
+  const Unit u = make_unit(P.c, sm.unit[0], sm.unit[1], sm.unit[2]);
+  const int tiles = (u.nh + 1) / 2;
+  const int tile0 = static_cast<int>(static_cast<int64_t>(tiles) * split / P.splits);
+  const int nt = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / P.splits) - tile0;
+  const bool mine = static_cast<int>(rank) < u.n;       // this CTA has a token
+  const int64_t token = u.t0 + rank;
+  if (nt == 0) {  // splits > 1: nothing for this one (also the same in both CTAs)
+    if (mine && tid < HB) {
+      float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + ((token * P.splits + split) * HB + tid) * 2;
+      ml[0] = -INFINITY;
+      ml[1] = 0.f;
+    }
+    return;
+  }
+
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sm.tmem_base)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  }
+  if (tid == 0) {
+    bar_init(&sm.q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sm.kv_full[i], 1);
+      bar_init(&sm.s_full[i], 1);
+      bar_init(&sm.p_full[i], 2 * SMX_WARPS);
+      bar_init(&sm.v_full[i], 1);
+      bar_init(&sm.done[i], 1);
+    }
+    sm.abort = 0;
+    bar_init_fence();
+    tma_prefetch_map(&P.pool);
+    tma_prefetch_map(&P.q);
+  }
+  if (warp == 10 && P.freqs != nullptr && lane < P.rope_dim / 2)
+    rope_cos_sin(u.p0 + static_cast<int>(rank), P.freqs[lane], &sm.rope_c[lane], &sm.rope_s[lane]);
+  before_sync();
+  __syncthreads();
+  cluster_sync();
+  after_sync();
+  const uint32_t tmem = sm.tmem_base;
+  const volatile int* abort = &sm.abort;
+  const int boxes = 64 / P.box_rows;
+  const uint32_t box_bytes = static_cast<uint32_t>(P.box_rows) * 128;
+
+  if (warp == 8) {
+    // ---------------------------------------------------------------- Q, and the tiles as K
+    if (lane == 0) {
+      const uint32_t qb = in_cta(&sm.q_full, 0);
+      if (rank == 0) bar_expect_tx(&sm.q_full, 2 * 8 * SLAB);
+      const int qrow = mine ? static_cast<int>(token) * HB : P.c.total * HB;  // behind q: zeros
+      for (int g = 0; g < 8; ++g) load_pair(sm.q + g * SLAB, &P.q, g * 64, qrow, qb);
+      bool ok = true;
+      int issued = 0;
+      for (int i = 0; i < nt; ++i) {
+        const int b = i & 1, h = 2 * (tile0 + i) + static_cast<int>(rank);
+        int row = h < u.nh ? half_row(P, u, h, 0) : static_cast<int>(P.c.pool_rows);
+        if (i >= 2 && !(ok = bar_wait_or_abort(&sm.done[b], ((i >> 1) - 1) & 1, abort))) break;
+        const uint32_t fb = in_cta(&sm.kv_full[b], 0);
+        if (rank == 0) bar_expect_tx(&sm.kv_full[b], 2 * 2 * SLOT);
+        for (int x = 0; x < boxes; ++x) {
+          if (x > 0) row = h < u.nh ? half_row(P, u, h, x) : static_cast<int>(P.c.pool_rows);
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            load_pair(sm.kv[b][g >> 2] + (g & 3) * SLAB + x * box_bytes, &P.pool, g * 64, row, fb);
+        }
+        issued = i + 1;
+      }
+      if (!ok) set_abort(sm);
+      if (!ok && rank == 0) {
+        // what both CTAs have under way into the pair's tiles lands before the pair leaves
+        bar_wait(&sm.q_full, 0);
+        for (int i = max(0, issued - 2); i < issued; ++i) bar_wait(&sm.kv_full[i & 1], (i >> 1) & 1);
+      }
+    }
+  } else if (warp == 10) {
+    // ---------------------------------------------------------------- the other half's rows as V
+    if (lane == 0) {
+      bool ok = true;
+      int issued = 0;
+      for (int i = 0; i < nt; ++i) {
+        const int b = i & 1, h = 2 * (tile0 + i) + 1 - static_cast<int>(rank);
+        int row = h < u.nh ? half_row(P, u, h, 0) : static_cast<int>(P.c.pool_rows);
+        if (!(ok = bar_wait_or_abort(&sm.s_full[b], (i >> 1) & 1, abort))) break;
+        bar_expect_tx(&sm.v_full[b], SLOT);
+        uint8_t* slot = sm.kv[b][1 - rank];  // CTA 0: Y takes rows 64-127, CTA 1: X takes rows 0-63
+        for (int x = 0; x < boxes; ++x) {
+          if (x > 0) row = h < u.nh ? half_row(P, u, h, x) : static_cast<int>(P.c.pool_rows);
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            tma_load_2d(slot + g * SLAB + x * box_bytes, &P.pool, (4 * static_cast<int>(rank) + g) * 64, row, &sm.v_full[b]);
+        }
+        issued = i + 1;
+      }
+      if (!ok) {
+        set_abort(sm);
+        for (int i = max(0, issued - 2); i < issued; ++i) bar_wait(&sm.v_full[i & 1], (i >> 1) & 1);
+      }
+    }
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- MMAs (CTA 0, one thread)
+    if (rank == 0 && lane == 0) {
+      constexpr uint32_t id_s = idesc_bf16<128, 128>(false, false);
+      constexpr uint32_t id_o = idesc_bf16<128, 256>(false, true);
+      const uint32_t qs = smem_u32(sm.q);
+      bool ok = bar_wait_or_abort(&sm.q_full, 0, abort);
+      int s = 0, o = 0;  // S and O steps issued
+      uint64_t since = global_ns();
+      while (ok && o < nt) {
+        if (s < nt && s - o < 2 && test_cluster(&sm.kv_full[s & 1], (s >> 1) & 1)) {
+          after_sync();
+          const uint32_t d = tmem + COL_S + 64 * (s & 1);
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const uint32_t ks = smem_u32(sm.kv[s & 1][g >> 2]) + (g & 3) * SLAB;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_pair(d, sdesc(qs + g * SLAB + kk * 32, 16, 1024), sdesc(ks + kk * 32, 16, 1024), id_s, (g | kk) ? 1u : 0u);
+          }
+          commit_pair(&sm.s_full[s & 1]);
+          ++s;
+          since = global_ns();
+        } else if (o < s && test_cluster(&sm.p_full[o & 1], (o >> 1) & 1)) {
+          after_sync();
+          const uint32_t ps = smem_u32(sm.p[o & 1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              const uint32_t vs = smem_u32(sm.kv[o & 1][kk >> 2]) + 2 * j * SLAB + (kk & 3) * 2048;
+              mma_pair(tmem + COL_O + 128 * j, sdesc(ps + (kk >> 2) * SLAB + (kk & 3) * 32, 16, 1024), sdesc(vs, SLAB, 1024),
+                       id_o, (o | kk) ? 1u : 0u);
+            }
+          commit_pair(&sm.done[o & 1]);
+          ++o;
+          since = global_ns();
+        } else if (*abort || global_ns() - since > WAIT_NS) {
+          ok = false;
+        }
+      }
+      if (!ok) {
+        set_abort(sm);
+        // everything issued completes before the pair leaves: one more commit on a barrier of its own
+        // phase (q_full, phase 1; both CTAs' q_full are past phase 0 or unused)
+        commit_pair(&sm.q_full);
+        bar_wait(&sm.q_full, 1);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax, epilogue (warps 0-7)
+    const int quad = warp & 3, ch = warp >> 2;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const int head = (quad & 1) * 32 + lane, kvh = quad >> 1;  // TMEM lane: head + 64 kvh
+    const int pos = u.p0 + static_cast<int>(rank);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int i = 0; i < nt; ++i) {
+      const int b = i & 1;
+      // what of this warp's 32 rows is seen, by the CTA's token and by either token of the pair
+      const int h = 2 * (tile0 + i) + kvh, j = 32 * ch + lane;
+      const bool v0 = h < u.nh && half_sees(P.c, u, h, j, u.p0, u.seen[0]);
+      const bool v1 = h < u.nh && u.n > 1 && half_sees(P.c, u, h, j, u.p0 + 1, u.seen[1]);
+      const uint32_t see = __ballot_sync(0xffffffffu, rank == 0 ? v0 : v1);
+      const uint32_t either = __ballot_sync(0xffffffffu, v0 || v1);
+      ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.s_full[b], (i >> 1) & 1, abort));
+      float x[32];
+      float mx = -INFINITY;
+      if (ok) {
+        after_sync();
+        tmem_ld16(tmem + lanes + COL_S + 64 * b + 32 * ch, x);
+        tmem_ld16(tmem + lanes + COL_S + 64 * b + 32 * ch + 16, x + 16);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          x[c] = (see >> c) & 1 ? x[c] * P.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, x[c]);
+        }
+      }
+      if (smx_any(!ok || mx > m + RESCALE)) {
+        if (smx_any(!ok)) {
+          if (lane == 0) set_abort(sm);
+          ok = false;
+          break;
+        }
+        sm.red[kvh * 2 + ch][head] = mx;
+        smx_bar();
+        const float mn = fmaxf(m, fmaxf(fmaxf(sm.red[0][head], sm.red[1][head]), fmaxf(sm.red[2][head], sm.red[3][head])));
+        const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+        const bool moved = mn != m && m != -INFINITY;
+        m = mn;
+        l *= alpha;
+        smx_bar();  // red is free again
+        if (i > 0 && __any_sync(0xffffffffu, moved)) {
+          // O of the tiles before has been added up: rescale this warp's half of its columns
+          ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.done[b ^ 1], ((i - 1) >> 1) & 1, abort));
+          if (ok) {
+            after_sync();
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+              float v[32];
+              tmem_ld16(tmem + lanes + COL_O + 128 * ch + c, v);
+              tmem_ld16(tmem + lanes + COL_O + 128 * ch + c + 16, v + 16);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] *= moved ? alpha : 1.f;
+              tmem_st16(tmem + lanes + COL_O + 128 * ch + c, v);
+              tmem_st16(tmem + lanes + COL_O + 128 * ch + c + 16, v + 16);
+            }
+            tmem_wait_st();
+          }
+        }
+      }
+      // P: 32 columns of this row, four 16-byte chunks of the 128-byte-swizzled slab
+      uint8_t* prow = sm.p[b] + kvh * SLAB + head * 128;
+      const float mm = m == -INFINITY ? 0.f : m;  // nothing seen yet: every x is -inf and p is 0
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = pack_bf16x2(ex2(x[c4 * 8 + 2 * e] - mm), ex2(x[c4 * 8 + 2 * e + 1] - mm));
+          l += __uint_as_float(w[e] << 16) + __uint_as_float(w[e] & 0xffff0000u);
+        }
+        *reinterpret_cast<uint4*>(prow + (((ch * 4 + c4) ^ (head & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.v_full[b], (i >> 1) & 1, abort));
+      if (!ok) {  // the CTA's other warps end at their next wait or at smx_any
+        if (lane == 0) set_abort(sm);
+      } else if (either != 0xffffffffu && h < u.nh) {
+        // values of rows that neither token sees: two slabs of the slot for this warp, 16 lanes a row
+        uint8_t* slab = sm.kv[b][kvh] + (2 * (quad & 1) + ((lane >> 3) & 1)) * SLAB;
+        for (int r = lane >> 4; r < 32; r += 2)
+          if (!((either >> r) & 1))
+            *reinterpret_cast<uint4*>(slab + (32 * ch + r) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_async_smem();
+      before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_at(in_cta(&sm.p_full[b], 0));
+    }
+    if (ok) ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.done[(nt - 1) & 1], ((nt - 1) >> 1) & 1, abort));
+    if (!ok && lane == 0) set_abort(sm);
+    sm.red[kvh * 2 + ch][head] = l;
+    smx_bar();
+    l = (sm.red[0][head] + sm.red[1][head]) + (sm.red[2][head] + sm.red[3][head]);
+    if (ok && !*abort && mine) {
+      after_sync();
+      const uint32_t src = tmem + lanes + COL_O + 128 * ch;
+      const int d0 = 256 * kvh + 128 * ch;
+      if (P.splits > 1) {
+        const int64_t at = (token * P.splits + split) * HB + head;
+        float* po = P.part + at * D + d0;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          float v[32];
+          tmem_ld16(src + c, v);
+          tmem_ld16(src + c + 16, v + 16);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            reinterpret_cast<float4*>(po + c)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+        }
+        if (kvh == 0 && ch == 0) {
+          float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + at * 2;
+          ml[0] = m;
+          ml[1] = l;
+        }
+      } else {
+        const float inv = 1.f / (l + exp2f(P.sink[head] * LOG2E - m));
+        const int64_t off = (token * HB + head) * D + d0;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          float v[32];
+          tmem_ld16(src + c, v);
+          tmem_ld16(src + c + 16, v + 16);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] *= inv;
+          if (P.freqs != nullptr && d0 + c + 32 > D - P.rope_dim) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const int f = (d0 + c + e - (D - P.rope_dim)) >> 1;
+              if (f >= 0) rotate_pair(v[e], v[e + 1], sm.rope_c[f], sm.rope_s[f], true, &v[e], &v[e + 1]);
+            }
+          }
+          if (P.out_dtype == DSV4_BF16) {
+            uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.out) + off + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              dst[e] = make_uint4(pack_bf16x2(v[8 * e], v[8 * e + 1]), pack_bf16x2(v[8 * e + 2], v[8 * e + 3]),
+                                  pack_bf16x2(v[8 * e + 4], v[8 * e + 5]), pack_bf16x2(v[8 * e + 6], v[8 * e + 7]));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + off + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  before_sync();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while the pair's MMAs, loads or arrivals may touch it
+  after_sync();
+  if (warp == 9)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(TMEM_COLS));
+}
+
+// One CTA per (token, head): the splits' partials weighed by 2^(m - max), the sink, the inverse
+// rotation. At most 64 splits.
+__global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ Params P) {
+  const int64_t t = blockIdx.x >> 6;
+  const int head = blockIdx.x & 63;
+  const ChunkToken k = chunk_token(P.c, static_cast<int>(t));
+  if (k.seq < 0) return;
+  __shared__ float w[64];
+  __shared__ float inv;
+  const float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D);
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    float m[2], l[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int s = lane + 32 * e;
+      const int64_t at = ((t * P.splits + s) * HB + head) * 2;
+      m[e] = s < P.splits ? ml[at] : -INFINITY;
+      l[e] = s < P.splits ? ml[at + 1] : 0.f;
+    }
+    const float M = warp_max(fmaxf(m[0], m[1]));
+    float L = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float x = m[e] == -INFINITY ? 0.f : exp2f(m[e] - M);
+      w[lane + 32 * e] = x;
+      L += x * l[e];
+    }
+    L = warp_sum(L);
+    if (lane == 0) inv = 1.f / (L + exp2f(P.sink[head] * LOG2E - M));
+  }
+  __syncthreads();
+  const int d = threadIdx.x * 4;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  const float* src = P.part + (t * P.splits * HB + head) * D + d;
+#pragma unroll 4
+  for (int s = 0; s < P.splits; ++s) {
+    const float x = w[s];
+    if (x != 0.f) {  // a split without rows has written no O
+      const float4 v = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (HB * D));
+      o[0] = fmaf(x, v.x, o[0]);
+      o[1] = fmaf(x, v.y, o[1]);
+      o[2] = fmaf(x, v.z, o[2]);
+      o[3] = fmaf(x, v.w, o[3]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= inv;
+  if (P.freqs != nullptr) {
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      const int f = (d + e - (D - P.rope_dim)) >> 1;
+      if (f >= 0) {
+        float c, s;
+        rope_cos_sin(k.pos, P.freqs[f], &c, &s);
+        rotate_pair(o[e], o[e + 1], c, s, true, &o[e], &o[e + 1]);
+      }
+    }
+  }
+  const int64_t off = (t * HB + head) * D + d;
+  if (P.out_dtype == DSV4_BF16)
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + off) =
+        make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+  else
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + off) = make_float4(o[0], o[1], o[2], o[3]);
+}
+
+DSV4_ERROR_READER(chunk_attn)
+
+static int encode(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows) {
+  static std::atomic<void*> fn{nullptr};
+  void* f = fn.load(std::memory_order_acquire);
+  if (!f) {
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      set_error("dsv4_chunk_attn: cuTensorMapEncodeTiled is not available from the driver");
+      return DSV4_ERR_CUDA;
+    }
+    fn.store(f, std::memory_order_release);
+  }
+  const cuuint64_t dims[2] = {D, rows};
+  const cuuint64_t strides[1] = {D * 2};
+  const cuuint32_t box[2] = {64, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f)(
+      map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("dsv4_chunk_attn: cuTensorMapEncodeTiled failed (%d) for %llu rows", static_cast<int>(r),
+              static_cast<unsigned long long>(rows));
+    return DSV4_ERR_CUDA;
+  }
+  return DSV4_OK;
+}
+
+// clusters of one wave shared out over the pairs of tokens, two tiles a split at least
+static int plan_splits(const dsv4_chunk_attn_params* p) {
+  const int64_t units = (static_cast<int64_t>(p->chunk.total) + p->chunk.n) / 2;
+  const int tiles = p->chunk.max_comp / BN + 1;
+  int want = p->num_splits;
+  if (want <= 0) {
+    want = static_cast<int>(std::max<int64_t>(1, num_sms() / 2 / std::max<int64_t>(1, units)));
+    want = std::min(want, std::max(1, tiles / 2));
+  }
+  return std::min(want, 64);
+}
+
+}  // namespace ca
+}  // namespace dsv4
+
+using namespace dsv4;
+
+extern "C" {
+
+size_t dsv4_chunk_attn_workspace_size(const dsv4_chunk_attn_params* p) {
+  if (p == nullptr || p->chunk.total <= 0 || p->chunk.n <= 0) return 0;
+  const int splits = ca::plan_splits(p);
+  return splits == 1 ? 0 : static_cast<size_t>(p->chunk.total) * splits * (ca::HB * ca::D + ca::HB * 2) * sizeof(float);
+}
+
+int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
+  DSV4_CHECK_ARG(p != nullptr, "dsv4_chunk_attn: params is NULL");
+  const int rc = check_chunk(&p->chunk, "dsv4_chunk_attn");
+  if (rc != DSV4_OK) return rc;
+  DSV4_CHECK_ARG(p->q && p->pool && p->sink && p->out, "dsv4_chunk_attn: NULL tensor");
+  DSV4_CHECK_ARG(((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->pool) |
+                   reinterpret_cast<uintptr_t>(p->out)) & 15) == 0,
+                 "dsv4_chunk_attn: q, pool and out must be 16-byte aligned");
+  DSV4_CHECK_ARG(p->chunk.window <= ca::MAX_WINDOW, "dsv4_chunk_attn: window %d above %d", p->chunk.window, ca::MAX_WINDOW);
+  DSV4_CHECK_ARG(p->chunk.max_comp == 0 || p->chunk.page % 8 == 0, "dsv4_chunk_attn: page %d is not a multiple of 8",
+                 p->chunk.page);
+  DSV4_CHECK_DTYPE(p->out_dtype == DSV4_F32 || p->out_dtype == DSV4_BF16, "dsv4_chunk_attn: out dtype");
+  DSV4_CHECK_ARG(p->rope_freqs == nullptr || (p->rope_dim > 0 && p->rope_dim <= 64 && p->rope_dim % 2 == 0),
+                 "dsv4_chunk_attn: 0 < rope_dim <= 64");
+  DSV4_CHECK_ARG(p->num_splits >= 0 && p->num_splits <= 64, "dsv4_chunk_attn: 0 to 64 splits");
+  DSV4_CHECK_ARG(static_cast<int64_t>(p->chunk.total) * ca::HB <= 0x7fffffffLL - ca::HB, "dsv4_chunk_attn: too many tokens");
+  if (p->chunk.n == 0 || p->chunk.total == 0) return DSV4_OK;
+  ca::Params P = {};
+  P.splits = ca::plan_splits(p);
+  const size_t need = dsv4_chunk_attn_workspace_size(p);
+  if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(p->workspace) & 15) != 0)) {
+    set_error("dsv4_chunk_attn: workspace of %zu bytes needed, %zu given", need, p->workspace_bytes);
+    return DSV4_ERR_WORKSPACE;
+  }
+  P.box_rows = 64;
+  if (p->chunk.max_comp > 0)
+    while (p->chunk.page % P.box_rows != 0) P.box_rows /= 2;
+  int st = ca::encode(&P.pool, p->pool, static_cast<uint64_t>(p->chunk.pool_rows), static_cast<uint32_t>(P.box_rows));
+  if (st != DSV4_OK) return st;
+  st = ca::encode(&P.q, p->q, static_cast<uint64_t>(p->chunk.total) * ca::HB, 64);
+  if (st != DSV4_OK) return st;
+  P.c = p->chunk;
+  P.sink = p->sink;
+  P.out = p->out;
+  P.part = reinterpret_cast<float*>(p->workspace);
+  P.freqs = p->rope_freqs;
+  P.rope_dim = p->rope_freqs ? p->rope_dim : 0;
+  P.out_dtype = p->out_dtype;
+  P.scale_log2 = p->scale * ca::LOG2E;
+  const int64_t units = (static_cast<int64_t>(P.c.total) + P.c.n) / 2;
+  DSV4_CHECK_ARG(2 * units * P.splits <= 0x7fffffffLL && static_cast<int64_t>(P.c.total) * 64 <= 0x7fffffffLL,
+                 "dsv4_chunk_attn: too many tokens");
+  static PerDeviceOnce attr;
+  const int smem = static_cast<int>(sizeof(ca::Smem)) + 1024;
+  DSV4_CUDA_CHECK(set_smem_once(attr, ca::chunk_attn_kernel, smem));
+  ca::chunk_attn_kernel<<<static_cast<unsigned>(2 * units * P.splits), ca::THREADS, smem, as_stream(stream)>>>(P);
+  DSV4_LAUNCH_CHECK("chunk_attn_kernel");
+  if (P.splits > 1) {
+    ca::chunk_merge_kernel<<<static_cast<unsigned>(P.c.total) * 64, 128, 0, as_stream(stream)>>>(P);
+    DSV4_LAUNCH_CHECK("chunk_merge_kernel");
+  }
+  return DSV4_OK;
+}
+
+}  // extern "C"

@@ -407,6 +407,29 @@ DSV4_API int dsv4_chunk_rows(const dsv4_chunk* c, int32_t* positions, int64_t* s
  * the bf16 pool of rows of dim elements */
 DSV4_API int dsv4_chunk_commit(const dsv4_chunk* c, void* pool, int32_t dim, void* stream);
 
+/* Attention of the chunk, every token over its window and all the compressed entries it sees; the
+ * rows staged and the entries written. q after the per-head norm and RoPE; o after the inverse RoPE of
+ * its last rope_dim dims (rope_freqs == NULL: none). 64 heads of 512, a window of at most 1024, pages of
+ * a multiple of 8 rows. Rows of out behind the last sequence are not written. Tokens are taken in pairs
+ * (2 i, 2 i + 1 of a sequence): a row that holds no finite numbers and is seen by one of a pair
+ * reaches both. An entry whose page the sequence does not have counts as a row of zeros and raises
+ * DSV4_ERR_INDEX_OUT_OF_RANGE. */
+typedef struct {
+  dsv4_chunk chunk;
+  const void* q;              /* [total, 64, 512] BF16 */
+  const void* pool;           /* [pool_rows, 512] BF16 */
+  const float* sink;          /* [64] */
+  void* out;                  /* [total, 64, 512] out_dtype */
+  const float* rope_freqs;    /* [rope_dim / 2] */
+  int32_t rope_dim, out_dtype;
+  float scale;
+  int32_t num_splits;         /* 0: automatic; a token pair's rows over this many CTA pairs (1 to 64) */
+  void* workspace;            /* dsv4_chunk_attn_workspace_size bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} dsv4_chunk_attn_params;
+DSV4_API size_t dsv4_chunk_attn_workspace_size(const dsv4_chunk_attn_params* p);
+DSV4_API int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream);
+
 /* The compressor over a chunk, continuing each sequence's ring: what one dsv4_compressor_decode call
  * per token would leave in the rings, the emitted rows and the key image, in one launch
  * (oracle/decode_engine.py:96-105 for a run of tokens; the reference takes one token at a time). Entry g of

@@ -13,7 +13,8 @@ import torch
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = "deepseek-v4-flash-mlx_b200"
 L = importlib.import_module(PKG + "._lib")
-PAIRS = {"dsv4_chunk": L.Chunk, "dsv4_compressor_chunk_params": L.CompressorChunkParams, "dsv4_pages": L.Pages}
+PAIRS = {"dsv4_chunk": L.Chunk, "dsv4_chunk_attn_params": L.ChunkAttnParams,
+         "dsv4_compressor_chunk_params": L.CompressorChunkParams, "dsv4_pages": L.Pages}
 
 
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="needs a host C compiler")
