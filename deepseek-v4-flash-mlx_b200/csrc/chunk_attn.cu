@@ -25,12 +25,12 @@
 // that neither token of the pair sees are zeroed in shared memory before they are used as values, so
 // that whatever they hold stays out; a row that one of the two sees is finite or spoils both.
 //
-// Roles (11 warps a CTA): warps 0-7 softmax and epilogue (warp w: TMEM lanes 32 (w % 4) .., columns of
-// half w / 4); warp 8 loads Q and the tiles as K; warp 9 of CTA 0 issues all MMAs, whichever of the
-// next S and the next O has its operands ready; warp 10 loads the second slot as V. The running
-// maximum is lazy (raised only when a score passes it by 2^8; O and the sums are then rescaled), the
-// sums are fp32, of the rounded probabilities. P is rounded to bf16 (the MMA takes both operands in
-// the rows' type), O is rounded once at the end.
+// Roles (12 warps a CTA): warps 0-7 softmax and epilogue (warp w: TMEM lanes 32 (w % 4) .., columns of
+// half w / 4); warps 8 and 11 load Q and the tiles as K, a slot each; warp 9 of CTA 0 issues all MMAs,
+// whichever of the next O and the next half of an S (a slot's dims) has its operands ready; warp 10
+// loads the second slot as V. The running maximum is lazy (raised only when a score passes it by 2^8; O
+// and the sums are then rescaled), the sums are fp32. P is rounded to bf16 (the MMA takes both operands
+// in the rows' type), O is rounded once at the end.
 // Long lists with few tokens are split over clusters; fp32 partials and a merging kernel follow.
 // All waits inside a CTA are bounded (1 s): DSV4_ERR_WAIT_TIMEOUT, and the pair drains and leaves.
 #include <cudaTypedefs.h>
@@ -48,7 +48,7 @@ namespace ca {
 using namespace tc5;
 
 constexpr int D = 512, HB = 64, BN = 128;
-constexpr int SMX_WARPS = 8, SMX_THREADS = 256, THREADS = 352;
+constexpr int SMX_WARPS = 8, SMX_THREADS = 256, THREADS = 384;
 constexpr int SLAB = 64 * 128;           // 64 rows of 64 bf16 dims, 128-byte swizzled
 constexpr int SLOT = 4 * SLAB;           // 64 rows of 256 dims
 constexpr int TMEM_COLS = 512, COL_O = 0, COL_S = 256;
@@ -62,7 +62,7 @@ struct Smem {
   uint8_t p[2][2 * SLAB];                // [buffer][rows 0-63 of the tile, rows 64-127]
   float red[4][HB];
   float rope_c[32], rope_s[32];
-  uint64_t q_full, kv_full[2], s_full[2], p_full[2], v_full[2], done[2];
+  uint64_t q_full, kv_full[2][2], kv_free[2][2], s_full[2], p_full[2], v_full[2];
   uint32_t tmem_base;
   int abort;
   int unit[4];                           // sequence, first token of the pair, tokens, units in all
@@ -82,6 +82,15 @@ struct Params {
 };
 
 // ---- the pair
+// One lane of the warp, chosen so that the compiler knows it: with the role's warp index the same in
+// every lane, the MMAs' descriptors stay in uniform registers (issued from a plain "lane == 0" branch
+// every MMA cost 70 to 130 cycles of the issuing thread, whatever its shape; this way 33 and 65 for
+// the N = 128 and N = 256 forms, their full rate).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\nselp.u32 %0, 1, 0, e;\n}\n" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
@@ -95,18 +104,11 @@ __device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
+// Arrive on a barrier of either CTA. What it tells of is read by the tensor cores from the arriving
+// CTA's own shared memory, and its writes there are complete for them once fence.proxy.async has been
+// passed, so the arrival need not release at cluster scope (which took 1000 to 1800 cycles a tile).
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
-}
-// not a waiting form: the issuer looks at two barriers in turn
-__device__ __forceinline__ bool test_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n.reg .pred p;\nmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
 // a tile load into this CTA's shared memory that completes on a barrier of CTA 0 of the pair
 __device__ __forceinline__ void load_pair(void* dst, const void* map, int x, int y, uint32_t bar) {
@@ -225,7 +227,8 @@ __device__ __forceinline__ bool half_sees(const dsv4_chunk& c, const Unit& u, in
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_constant__ Params P) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // the same register in every lane
   const uint32_t rank = cluster_rank();
   const int split = static_cast<int>(blockIdx.x >> 1) % P.splits;
   const int want = static_cast<int>(blockIdx.x >> 1) / P.splits;
@@ -298,11 +301,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
   if (tid == 0) {
     bar_init(&sm.q_full, 1);
     for (int i = 0; i < 2; ++i) {
-      bar_init(&sm.kv_full[i], 1);
+      for (int x = 0; x < 2; ++x) {
+        bar_init(&sm.kv_full[i][x], 1);
+        bar_init(&sm.kv_free[i][x], 1);
+      }
       bar_init(&sm.s_full[i], 1);
       bar_init(&sm.p_full[i], 2 * SMX_WARPS);
       bar_init(&sm.v_full[i], 1);
-      bar_init(&sm.done[i], 1);
     }
     sm.abort = 0;
     bar_init_fence();
@@ -320,39 +325,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
   const int boxes = 64 / P.box_rows;
   const uint32_t box_bytes = static_cast<uint32_t>(P.box_rows) * 128;
 
-  if (warp == 8) {
-    // ---------------------------------------------------------------- Q, and the tiles as K
-    if (lane == 0) {
-      const uint32_t qb = in_cta(&sm.q_full, 0);
-      if (rank == 0) bar_expect_tx(&sm.q_full, 2 * 8 * SLAB);
-      const int qrow = mine ? static_cast<int>(token) * HB : P.c.total * HB;  // behind q: zeros
-      for (int g = 0; g < 8; ++g) load_pair(sm.q + g * SLAB, &P.q, g * 64, qrow, qb);
+  if (warp == 8 || warp == 11) {
+    // ---------------------------------------------------------------- the tiles as K: slot X (and Q), slot Y
+    if (elect_one()) {
+      const int x = warp == 8 ? 0 : 1;
+      if (x == 0) {
+        const uint32_t qb = in_cta(&sm.q_full, 0);
+        if (rank == 0) bar_expect_tx(&sm.q_full, 2 * 8 * SLAB);
+        const int qrow = mine ? static_cast<int>(token) * HB : P.c.total * HB;  // behind q: zeros
+        for (int g = 0; g < 8; ++g) load_pair(sm.q + g * SLAB, &P.q, g * 64, qrow, qb);
+      }
       bool ok = true;
       int issued = 0;
       for (int i = 0; i < nt; ++i) {
         const int b = i & 1, h = 2 * (tile0 + i) + static_cast<int>(rank);
         int row = h < u.nh ? half_row(P, u, h, 0) : static_cast<int>(P.c.pool_rows);
-        if (i >= 2 && !(ok = bar_wait_or_abort(&sm.done[b], ((i >> 1) - 1) & 1, abort))) break;
-        const uint32_t fb = in_cta(&sm.kv_full[b], 0);
-        if (rank == 0) bar_expect_tx(&sm.kv_full[b], 2 * 2 * SLOT);
-        for (int x = 0; x < boxes; ++x) {
-          if (x > 0) row = h < u.nh ? half_row(P, u, h, x) : static_cast<int>(P.c.pool_rows);
+        if (i >= 2 && !(ok = bar_wait_or_abort(&sm.kv_free[b][x], ((i >> 1) - 1) & 1, abort))) break;
+        const uint32_t fb = in_cta(&sm.kv_full[b][x], 0);
+        if (rank == 0) bar_expect_tx(&sm.kv_full[b][x], 2 * SLOT);
+        for (int k = 0; k < boxes; ++k) {
+          if (k > 0) row = h < u.nh ? half_row(P, u, h, k) : static_cast<int>(P.c.pool_rows);
 #pragma unroll
-          for (int g = 0; g < 8; ++g)
-            load_pair(sm.kv[b][g >> 2] + (g & 3) * SLAB + x * box_bytes, &P.pool, g * 64, row, fb);
+          for (int g = 0; g < 4; ++g)
+            load_pair(sm.kv[b][x] + g * SLAB + k * box_bytes, &P.pool, (4 * x + g) * 64, row, fb);
         }
         issued = i + 1;
       }
       if (!ok) set_abort(sm);
       if (!ok && rank == 0) {
         // what both CTAs have under way into the pair's tiles lands before the pair leaves
-        bar_wait(&sm.q_full, 0);
-        for (int i = max(0, issued - 2); i < issued; ++i) bar_wait(&sm.kv_full[i & 1], (i >> 1) & 1);
+        if (x == 0) bar_wait(&sm.q_full, 0);
+        for (int i = max(0, issued - 2); i < issued; ++i) bar_wait(&sm.kv_full[i & 1][x], (i >> 1) & 1);
       }
     }
   } else if (warp == 10) {
     // ---------------------------------------------------------------- the other half's rows as V
-    if (lane == 0) {
+    if (elect_one()) {
       bool ok = true;
       int issued = 0;
       for (int i = 0; i < nt; ++i) {
@@ -361,11 +369,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
         if (!(ok = bar_wait_or_abort(&sm.s_full[b], (i >> 1) & 1, abort))) break;
         bar_expect_tx(&sm.v_full[b], SLOT);
         uint8_t* slot = sm.kv[b][1 - rank];  // CTA 0: Y takes rows 64-127, CTA 1: X takes rows 0-63
-        for (int x = 0; x < boxes; ++x) {
-          if (x > 0) row = h < u.nh ? half_row(P, u, h, x) : static_cast<int>(P.c.pool_rows);
+        for (int k = 0; k < boxes; ++k) {
+          if (k > 0) row = h < u.nh ? half_row(P, u, h, k) : static_cast<int>(P.c.pool_rows);
 #pragma unroll
           for (int g = 0; g < 4; ++g)
-            tma_load_2d(slot + g * SLAB + x * box_bytes, &P.pool, (4 * static_cast<int>(rank) + g) * 64, row, &sm.v_full[b]);
+            tma_load_2d(slot + g * SLAB + k * box_bytes, &P.pool, (4 * static_cast<int>(rank) + g) * 64, row, &sm.v_full[b]);
         }
         issued = i + 1;
       }
@@ -376,40 +384,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     }
   } else if (warp == 9) {
     // ---------------------------------------------------------------- MMAs (CTA 0, one thread)
-    if (rank == 0 && lane == 0) {
+    if (rank == 0 && elect_one()) {
       constexpr uint32_t id_s = idesc_bf16<128, 128>(false, false);
       constexpr uint32_t id_o = idesc_bf16<128, 256>(false, true);
-      const uint32_t qs = smem_u32(sm.q);
+      const uint64_t qd = sdesc(smem_u32(sm.q), 16, 1024), kd = sdesc(smem_u32(sm.kv), 16, 1024);
+      const uint64_t pd = sdesc(smem_u32(sm.p), 16, 1024), vd = sdesc(smem_u32(sm.kv), SLAB, 1024);
       bool ok = bar_wait_or_abort(&sm.q_full, 0, abort);
-      int s = 0, o = 0;  // S and O steps issued
+      int s = 0, o = 0;  // steps issued: half an S (one slot's dims), an O
       uint64_t since = global_ns();
       while (ok && o < nt) {
-        if (s < nt && s - o < 2 && test_cluster(&sm.kv_full[s & 1], (s >> 1) & 1)) {
+        const int sb = (s >> 1) & 1, x = s & 1;
+        if (2 * o < s - 1 && bar_test(&sm.p_full[o & 1], (o >> 1) & 1)) {
           after_sync();
-          const uint32_t d = tmem + COL_S + 64 * (s & 1);
+          const uint64_t a = pd + (o & 1) * (2 * SLAB >> 4), v = vd + (o & 1) * (2 * SLOT >> 4);
+          const uint32_t acc = o > 0 ? 1u : 0u;
 #pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const uint32_t ks = smem_u32(sm.kv[s & 1][g >> 2]) + (g & 3) * SLAB;
+          for (int kk = 0; kk < 8; ++kk) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_pair(d, sdesc(qs + g * SLAB + kk * 32, 16, 1024), sdesc(ks + kk * 32, 16, 1024), id_s, (g | kk) ? 1u : 0u);
+            for (int j = 0; j < 2; ++j)
+              mma_pair(tmem + COL_O + 128 * j, a + ((kk >> 2) * SLAB + (kk & 3) * 32 >> 4),
+                       v + ((kk >> 2) * SLOT + 2 * j * SLAB + (kk & 3) * 2048 >> 4), id_o, kk ? 1u : acc);
+            if (kk == 3) commit_pair(&sm.kv_free[o & 1][0]);
           }
-          commit_pair(&sm.s_full[s & 1]);
-          ++s;
-          since = global_ns();
-        } else if (o < s && test_cluster(&sm.p_full[o & 1], (o >> 1) & 1)) {
-          after_sync();
-          const uint32_t ps = smem_u32(sm.p[o & 1]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {
-              const uint32_t vs = smem_u32(sm.kv[o & 1][kk >> 2]) + 2 * j * SLAB + (kk & 3) * 2048;
-              mma_pair(tmem + COL_O + 128 * j, sdesc(ps + (kk >> 2) * SLAB + (kk & 3) * 32, 16, 1024), sdesc(vs, SLAB, 1024),
-                       id_o, (o | kk) ? 1u : 0u);
-            }
-          commit_pair(&sm.done[o & 1]);
+          commit_pair(&sm.kv_free[o & 1][1]);
           ++o;
+          since = global_ns();
+        } else if (s < 2 * nt && s < 2 * o + 4 && bar_test(&sm.kv_full[sb][x], (s >> 2) & 1)) {
+          after_sync();
+          const uint32_t d = tmem + COL_S + 64 * sb;
+          const uint64_t a = qd + x * (4 * SLAB >> 4), k = kd + (2 * sb + x) * (SLOT >> 4);
+          const uint32_t acc = x;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            mma_pair(d, a + ((e >> 2) * SLAB + (e & 3) * 32 >> 4), k + ((e >> 2) * SLAB + (e & 3) * 32 >> 4), id_s,
+                     e ? 1u : acc);
+          if (x == 1) commit_pair(&sm.s_full[sb]);
+          ++s;
           since = global_ns();
         } else if (*abort || global_ns() - since > WAIT_NS) {
           ok = false;
@@ -428,7 +438,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     const int quad = warp & 3, ch = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const int head = (quad & 1) * 32 + lane, kvh = quad >> 1;  // TMEM lane: head + 64 kvh
-    const int pos = u.p0 + static_cast<int>(rank);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int i = 0; i < nt; ++i) {
@@ -439,7 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       const bool v1 = h < u.nh && u.n > 1 && half_sees(P.c, u, h, j, u.p0 + 1, u.seen[1]);
       const uint32_t see = __ballot_sync(0xffffffffu, rank == 0 ? v0 : v1);
       const uint32_t either = __ballot_sync(0xffffffffu, v0 || v1);
-      ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.s_full[b], (i >> 1) & 1, abort));
+      ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.s_full[b], (i >> 1) & 1, abort));
       float x[32];
       float mx = -INFINITY;
       if (ok) {
@@ -448,10 +457,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
         tmem_ld16(tmem + lanes + COL_S + 64 * b + 32 * ch + 16, x + 16);
         tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          x[c] = (see >> c) & 1 ? x[c] * P.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, x[c]);
+        for (int c = 0; c < 32; ++c) x[c] *= P.scale_log2;
+        if (see != 0xffffffffu) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) x[c] = (see >> c) & 1 ? x[c] : -INFINITY;
         }
+        float mc[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mc[c] = x[c];
+#pragma unroll
+        for (int c = 4; c < 32; ++c) mc[c & 3] = fmaxf(mc[c & 3], x[c]);
+        mx = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3]));
       }
       if (smx_any(!ok || mx > m + RESCALE)) {
         if (smx_any(!ok)) {
@@ -469,7 +485,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
         smx_bar();  // red is free again
         if (i > 0 && __any_sync(0xffffffffu, moved)) {
           // O of the tiles before has been added up: rescale this warp's half of its columns
-          ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.done[b ^ 1], ((i - 1) >> 1) & 1, abort));
+          ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.kv_free[b ^ 1][1], ((i - 1) >> 1) & 1, abort));
           if (ok) {
             after_sync();
 #pragma unroll 1
@@ -490,16 +506,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       // P: 32 columns of this row, four 16-byte chunks of the 128-byte-swizzled slab
       uint8_t* prow = sm.p[b] + kvh * SLAB + head * 128;
       const float mm = m == -INFINITY ? 0.f : m;  // nothing seen yet: every x is -inf and p is 0
+      float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c4 = 0; c4 < 4; ++c4) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = pack_bf16x2(ex2(x[c4 * 8 + 2 * e] - mm), ex2(x[c4 * 8 + 2 * e + 1] - mm));
-          l += __uint_as_float(w[e] << 16) + __uint_as_float(w[e] & 0xffff0000u);
+          const float p0 = ex2(x[c4 * 8 + 2 * e] - mm), p1 = ex2(x[c4 * 8 + 2 * e + 1] - mm);
+          w[e] = pack_bf16x2(p0, p1);
+          ls[e] += p0 + p1;
         }
         *reinterpret_cast<uint4*>(prow + (((ch * 4 + c4) ^ (head & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
       ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.v_full[b], (i >> 1) & 1, abort));
       if (!ok) {  // the CTA's other warps end at their next wait or at smx_any
         if (lane == 0) set_abort(sm);
@@ -515,7 +534,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       __syncwarp();
       if (lane == 0) arrive_at(in_cta(&sm.p_full[b], 0));
     }
-    if (ok) ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.done[(nt - 1) & 1], ((nt - 1) >> 1) & 1, abort));
+    for (int x = 0; x < 2; ++x)  // both of the last commits have arrived here
+      ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.kv_free[(nt - 1) & 1][x], ((nt - 1) >> 1) & 1, abort));
     if (!ok && lane == 0) set_abort(sm);
     sm.red[kvh * 2 + ch][head] = l;
     smx_bar();
