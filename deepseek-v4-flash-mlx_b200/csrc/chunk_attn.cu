@@ -25,12 +25,16 @@
 // that neither token of the pair sees are zeroed in shared memory before they are used as values, so
 // that whatever they hold stays out; a row that one of the two sees is finite or spoils both.
 //
-// Roles (12 warps a CTA): warps 0-7 softmax and epilogue (warp w: TMEM lanes 32 (w % 4) .., columns of
-// half w / 4); warps 8 and 11 load Q and the tiles as K, a slot each; warp 9 of CTA 0 issues all MMAs,
-// whichever of the next O and the next half of an S (a slot's dims) has its operands ready; warp 10
-// loads the second slot as V. The running maximum is lazy (raised only when a score passes it by 2^8; O
-// and the sums are then rescaled), the sums are fp32. P is rounded to bf16 (the MMA takes both operands
-// in the rows' type), O is rounded once at the end.
+// The kernel is persistent: a cluster takes pairs of tokens from a static list, the longest first, and
+// the next pair's loads and S run under the last pair's epilogue.
+// Roles (13 warps a CTA): in CTA 0 one thread of warp 0 issues the S MMAs, a quarter (two slabs of a slot)
+// as its rows arrive, and one of warp 12 the O MMAs; an O frees the buffer quarter by quarter, in the order
+// in which the next S takes them. (One thread for both that looked at two barriers in turn lost 300 cycles
+// and more at each look: the MMAs keep shared memory busy, and a look waits for it.) Warps 1 and 2 load Q
+// and the tiles as K, a slot each; warp 3 loads the second slot as V; warps 4-11 softmax and epilogue (warp
+// w: TMEM lanes 32 (w % 4) .., half of the columns). The running maximum is lazy (raised only when a score
+// passes it by 2^8; O and the sums are then rescaled), the sums are fp32. P is rounded to bf16 (the MMA
+// takes both operands in the rows' type), O is rounded once at the end.
 // Long lists with few tokens are split over clusters; fp32 partials and a merging kernel follow.
 // All waits inside a CTA are bounded (1 s): DSV4_ERR_WAIT_TIMEOUT, and the pair drains and leaves.
 #include <cudaTypedefs.h>
@@ -48,7 +52,7 @@ namespace ca {
 using namespace tc5;
 
 constexpr int D = 512, HB = 64, BN = 128;
-constexpr int SMX_WARPS = 8, SMX_THREADS = 256, THREADS = 384;
+constexpr int SMX_WARPS = 8, SMX_THREADS = 256, THREADS = 416;
 constexpr int SLAB = 64 * 128;           // 64 rows of 64 bf16 dims, 128-byte swizzled
 constexpr int SLOT = 4 * SLAB;           // 64 rows of 256 dims
 constexpr int TMEM_COLS = 512, COL_O = 0, COL_S = 256;
@@ -61,11 +65,10 @@ struct Smem {
   uint8_t kv[2][2][SLOT];                // [tile buffer][X, Y]
   uint8_t p[2][2 * SLAB];                // [buffer][rows 0-63 of the tile, rows 64-127]
   float red[4][HB];
-  float rope_c[32], rope_s[32];
-  uint64_t q_full, kv_full[2][2], kv_free[2][2], s_full[2], p_full[2], v_full[2];
+  uint64_t fin[2], q_full, o_free, kv_full[2][4], kv_free[2][4], s_full[2], p_full[2], v_full[2];
   uint32_t tmem_base;
   int abort;
-  int unit[4];                           // sequence, first token of the pair, tokens, units in all
+  volatile int unit_tiles[2];            // tiles of a unit, handed to the S thread with its Q; -1: no more
 };
 static_assert(sizeof(Smem) + 1024 <= 232448, "shared memory above the 227 KB a CTA may opt into");
 
@@ -86,9 +89,10 @@ struct Params {
 // every lane, the MMAs' descriptors stay in uniform registers (issued from a plain "lane == 0" branch
 // every MMA cost 70 to 130 cycles of the issuing thread, whatever its shape; this way 33 and 65 for
 // the N = 128 and N = 256 forms, their full rate).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\nselp.u32 %0, 1, 0, e;\n}\n" : "=r"(p));
+__device__ __forceinline__ bool elect_one(uint32_t* leader = nullptr) {
+  uint32_t p, l;
+  asm volatile("{\n.reg .pred e;\nelect.sync %1|e, 0xffffffff;\nselp.u32 %0, 1, 0, e;\n}\n" : "=r"(p), "=r"(l));
+  if (leader) *leader = l;
   return p != 0;
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -131,6 +135,11 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
           smem_u32(bar)),
       "h"(static_cast<uint16_t>(3))
       : "memory");
+}
+// after an error: everything this thread issued completes (bounded) before its CTA leaves
+__device__ __forceinline__ void drain_issued(uint64_t* fin) {
+  commit_pair(fin);
+  bar_wait(fin, 0);
 }
 __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error about 2^-22, 2^-inf = +0
   float y;
@@ -224,84 +233,79 @@ __device__ __forceinline__ bool half_sees(const dsv4_chunk& c, const Unit& u, in
   return 64 * (h - u.nstage) + j < entries;
 }
 
+// Pairs of tokens, counted through the sequences. A warp looks together, 32 sequences at a time.
+// find < 0: the number of pairs in all; else *u becomes that pair's unit.
+__device__ __forceinline__ int look(const Params& P, int find, Unit* u) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int b0 = 0; b0 < P.c.n; b0 += 32) {
+    const int b = b0 + lane;
+    int cnt = 0, first = 0, len = 0;
+    if (b < P.c.n) {
+      first = P.c.cu_seqlens[b];
+      len = P.c.cu_seqlens[b + 1] - first;
+      const int slot = P.c.seqs ? P.c.seqs[b] : b;
+      const bool ok = first >= 0 && len >= 0 && first + len <= P.c.total && P.c.start[b] >= 0 && slot >= 0 && slot < P.c.slots;
+      if (!ok && find < 0) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+      cnt = ok ? (len + 1) / 2 : 0;
+    }
+    int s = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += x;
+    }
+    const int at = before + s - cnt;
+    const uint32_t hit = __ballot_sync(0xffffffffu, find >= at && find < at + cnt);
+    if (hit != 0) {
+      const int l = __ffs(hit) - 1, t0 = first + 2 * (find - at);
+      *u = make_unit(P.c, __shfl_sync(0xffffffffu, b, l), __shfl_sync(0xffffffffu, t0, l),
+                     __shfl_sync(0xffffffffu, min(2, first + len - t0), l));
+      return 0;
+    }
+    before += __shfl_sync(0xffffffffu, s, 31);
+  }
+  return before;
+}
+
+// The work of a cluster: units (pair of tokens, split) number `at`, at + clusters, ...; the pairs from the last to
+// the first, since the last see the most rows.
+struct Work {
+  Unit u;
+  int pairs, at, split, tile0, nt;
+  __device__ __forceinline__ explicit Work(const Params& P) : pairs(look(P, -1, nullptr)), at(static_cast<int>(blockIdx.x >> 1)) {}
+  __device__ __forceinline__ bool next(const Params& P) {
+    if (at >= pairs * P.splits) return false;
+    split = at % P.splits;
+    look(P, pairs - 1 - at / P.splits, &u);
+    const int tiles = (u.nh + 1) / 2;
+    tile0 = static_cast<int>(static_cast<int64_t>(tiles) * split / P.splits);
+    nt = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / P.splits) - tile0;
+    at += gridDim.x >> 1;
+    return true;
+  }
+};
+
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_constant__ Params P) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // the same register in every lane
   const uint32_t rank = cluster_rank();
-  const int split = static_cast<int>(blockIdx.x >> 1) % P.splits;
-  const int want = static_cast<int>(blockIdx.x >> 1) / P.splits;
 
-  // The unit: pairs of tokens counted through the sequences. The last pairs see the most rows and
-  // are started first.
   if (warp == 0) {
-    int total = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-      const int target = total - 1 - want;  // of the second pass
-      int before = 0, seq = -1, t0 = 0, n = 0;
-      for (int b0 = 0; b0 < P.c.n; b0 += 32) {
-        const int b = b0 + lane;
-        int cnt = 0, first = 0, len = 0;
-        if (b < P.c.n) {
-          first = P.c.cu_seqlens[b];
-          len = P.c.cu_seqlens[b + 1] - first;
-          const int slot = P.c.seqs ? P.c.seqs[b] : b;
-          const bool ok = first >= 0 && len >= 0 && first + len <= P.c.total && P.c.start[b] >= 0 && slot >= 0 && slot < P.c.slots;
-          if (!ok && pass == 0) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-          cnt = ok ? (len + 1) / 2 : 0;
-        }
-        int s = cnt;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, s, o);
-          if (lane >= o) s += x;
-        }
-        const int at = before + s - cnt;
-        if (pass == 1 && target >= at && target < at + cnt) {
-          seq = b;
-          t0 = first + 2 * (target - at);
-          n = min(2, first + len - t0);
-        }
-        before += __shfl_sync(0xffffffffu, s, 31);
-      }
-      if (pass == 0) {
-        total = before;
-      } else if (seq >= 0) {
-        sm.unit[0] = seq;
-        sm.unit[1] = t0;
-        sm.unit[2] = n;
-      }
-    }
-    if (lane == 0) sm.unit[3] = total;
-  }
-  __syncthreads();
-  if (want >= sm.unit[3]) return;  // the same in both CTAs
-  const Unit u = make_unit(P.c, sm.unit[0], sm.unit[1], sm.unit[2]);
-  const int tiles = (u.nh + 1) / 2;
-  const int tile0 = static_cast<int>(static_cast<int64_t>(tiles) * split / P.splits);
-  const int nt = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / P.splits) - tile0;
-  const bool mine = static_cast<int>(rank) < u.n;       // this CTA has a token
-  const int64_t token = u.t0 + rank;
-  if (nt == 0) {  // splits > 1: nothing for this one (also the same in both CTAs)
-    if (mine && tid < HB) {
-      float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + ((token * P.splits + split) * HB + tid) * 2;
-      ml[0] = -INFINITY;
-      ml[1] = 0.f;
-    }
-    return;
-  }
-
-  if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sm.tmem_base)),
                  "r"(TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
   }
-  if (tid == 0) {
+  if (tid == 32) {
     bar_init(&sm.q_full, 1);
+    bar_init(&sm.fin[0], 1);
+    bar_init(&sm.fin[1], 1);
+    bar_init(&sm.o_free, 2 * SMX_WARPS);
     for (int i = 0; i < 2; ++i) {
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < 4; ++x) {
         bar_init(&sm.kv_full[i][x], 1);
         bar_init(&sm.kv_free[i][x], 1);
       }
@@ -314,8 +318,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     tma_prefetch_map(&P.pool);
     tma_prefetch_map(&P.q);
   }
-  if (warp == 10 && P.freqs != nullptr && lane < P.rope_dim / 2)
-    rope_cos_sin(u.p0 + static_cast<int>(rank), P.freqs[lane], &sm.rope_c[lane], &sm.rope_s[lane]);
   before_sync();
   __syncthreads();
   cluster_sync();
@@ -325,282 +327,380 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
   const int boxes = 64 / P.box_rows;
   const uint32_t box_bytes = static_cast<uint32_t>(P.box_rows) * 128;
 
-  if (warp == 8 || warp == 11) {
+  // Tiles and units are counted through the whole work (g, ord): a barrier of two buffers is in phase
+  // (g / 2) % 2 at tile g.
+  if (warp == 1 || warp == 2) {
     // ---------------------------------------------------------------- the tiles as K: slot X (and Q), slot Y
-    if (elect_one()) {
-      const int x = warp == 8 ? 0 : 1;
-      if (x == 0) {
-        const uint32_t qb = in_cta(&sm.q_full, 0);
-        if (rank == 0) bar_expect_tx(&sm.q_full, 2 * 8 * SLAB);
-        const int qrow = mine ? static_cast<int>(token) * HB : P.c.total * HB;  // behind q: zeros
-        for (int g = 0; g < 8; ++g) load_pair(sm.q + g * SLAB, &P.q, g * 64, qrow, qb);
-      }
-      bool ok = true;
-      int issued = 0;
-      for (int i = 0; i < nt; ++i) {
-        const int b = i & 1, h = 2 * (tile0 + i) + static_cast<int>(rank);
-        int row = h < u.nh ? half_row(P, u, h, 0) : static_cast<int>(P.c.pool_rows);
-        if (i >= 2 && !(ok = bar_wait_or_abort(&sm.kv_free[b][x], ((i >> 1) - 1) & 1, abort))) break;
-        const uint32_t fb = in_cta(&sm.kv_full[b][x], 0);
-        if (rank == 0) bar_expect_tx(&sm.kv_full[b][x], 2 * SLOT);
-        for (int k = 0; k < boxes; ++k) {
-          if (k > 0) row = h < u.nh ? half_row(P, u, h, k) : static_cast<int>(P.c.pool_rows);
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            load_pair(sm.kv[b][x] + g * SLAB + k * box_bytes, &P.pool, (4 * x + g) * 64, row, fb);
+    const int x = warp - 1;
+    bool ok = true;
+    int g = 0, ord = 0, issued = 0;
+    Work w(P);
+    while (ok && w.next(P)) {
+      if (w.nt == 0) continue;
+      uint32_t leader;
+      if (elect_one(&leader)) {
+        if (x == 0) {
+          // Q follows the last S of the unit before
+          if (g > 0) ok = bar_wait_or_abort(&sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort);
+          if (ok) {
+            sm.unit_tiles[ord & 1] = w.nt;
+            const uint32_t qb = in_cta(&sm.q_full, 0);
+            if (rank == 0) bar_expect_tx(&sm.q_full, 2 * 8 * SLAB);
+            const int qrow = static_cast<int>(rank) < w.u.n ? (w.u.t0 + static_cast<int>(rank)) * HB : P.c.total * HB;
+            for (int e = 0; e < 8; ++e) load_pair(sm.q + e * SLAB, &P.q, e * 64, qrow, qb);  // behind q: zeros
+          }
         }
-        issued = i + 1;
+        for (int i = 0; i < w.nt && ok; ++i, ++g) {
+          const int b = g & 1, h = 2 * (w.tile0 + i) + static_cast<int>(rank);
+          int row = h < w.u.nh ? half_row(P, w.u, h, 0) : static_cast<int>(P.c.pool_rows);
+          for (int y = 0; y < 2; ++y) {  // two slabs at a time, as the O of the tile before last frees them
+            const int qr = 2 * y + x;
+            if (g >= 2 && !(ok = bar_wait_or_abort(&sm.kv_free[b][qr], ((g >> 1) - 1) & 1, abort))) break;
+            const uint32_t fb = in_cta(&sm.kv_full[b][qr], 0);
+            if (rank == 0) bar_expect_tx(&sm.kv_full[b][qr], 4 * SLAB);
+            for (int k = 0; k < boxes; ++k) {
+              if (boxes > 1) row = h < w.u.nh ? half_row(P, w.u, h, k) : static_cast<int>(P.c.pool_rows);
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                load_pair(sm.kv[b][x] + (2 * y + e) * SLAB + k * box_bytes, &P.pool, (4 * x + 2 * y + e) * 64, row, fb);
+            }
+            ++issued;
+          }
+        }
+        if (!ok) {
+          set_abort(sm);
+          // what both CTAs have under way into the pair's tiles lands before the pair leaves
+          if (rank == 0) {
+            if (x == 0) bar_wait(&sm.q_full, ord & 1);
+            for (int e = max(0, issued - 4); e < issued; ++e)
+              bar_wait(&sm.kv_full[(e >> 1) & 1][2 * (e & 1) + x], (e >> 2) & 1);
+          }
+        }
       }
+      ok = __shfl_sync(0xffffffffu, ok, leader);
+      g = __shfl_sync(0xffffffffu, g, leader);
+      issued = __shfl_sync(0xffffffffu, issued, leader);
+      ++ord;
+    }
+    if (x == 0 && ok && elect_one()) {
+      if (g > 0) ok = bar_wait_or_abort(&sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort);
       if (!ok) set_abort(sm);
-      if (!ok && rank == 0) {
-        // what both CTAs have under way into the pair's tiles lands before the pair leaves
-        if (x == 0) bar_wait(&sm.q_full, 0);
-        for (int i = max(0, issued - 2); i < issued; ++i) bar_wait(&sm.kv_full[i & 1][x], (i >> 1) & 1);
-      }
+      sm.unit_tiles[ord & 1] = -1;
+      bar_arrive(&sm.q_full);
     }
-  } else if (warp == 10) {
+  } else if (warp == 3) {
     // ---------------------------------------------------------------- the other half's rows as V
-    if (elect_one()) {
-      bool ok = true;
-      int issued = 0;
-      for (int i = 0; i < nt; ++i) {
-        const int b = i & 1, h = 2 * (tile0 + i) + 1 - static_cast<int>(rank);
-        int row = h < u.nh ? half_row(P, u, h, 0) : static_cast<int>(P.c.pool_rows);
-        if (!(ok = bar_wait_or_abort(&sm.s_full[b], (i >> 1) & 1, abort))) break;
-        bar_expect_tx(&sm.v_full[b], SLOT);
-        uint8_t* slot = sm.kv[b][1 - rank];  // CTA 0: Y takes rows 64-127, CTA 1: X takes rows 0-63
-        for (int k = 0; k < boxes; ++k) {
-          if (k > 0) row = h < u.nh ? half_row(P, u, h, k) : static_cast<int>(P.c.pool_rows);
+    bool ok = true;
+    int g = 0;
+    Work w(P);
+    while (ok && w.next(P)) {
+      uint32_t leader;
+      if (elect_one(&leader)) {
+        for (int i = 0; i < w.nt; ++i, ++g) {
+          const int b = g & 1, h = 2 * (w.tile0 + i) + 1 - static_cast<int>(rank);
+          int row = h < w.u.nh ? half_row(P, w.u, h, 0) : static_cast<int>(P.c.pool_rows);
+          if (!(ok = bar_wait_or_abort(&sm.s_full[b], (g >> 1) & 1, abort))) break;
+          bar_expect_tx(&sm.v_full[b], SLOT);
+          uint8_t* slot = sm.kv[b][1 - rank];  // CTA 0: Y takes rows 64-127, CTA 1: X takes rows 0-63
+          for (int k = 0; k < boxes; ++k) {
+            if (k > 0) row = h < w.u.nh ? half_row(P, w.u, h, k) : static_cast<int>(P.c.pool_rows);
 #pragma unroll
-          for (int g = 0; g < 4; ++g)
-            tma_load_2d(slot + g * SLAB + k * box_bytes, &P.pool, (4 * static_cast<int>(rank) + g) * 64, row, &sm.v_full[b]);
+            for (int e = 0; e < 4; ++e)
+              tma_load_2d(slot + e * SLAB + k * box_bytes, &P.pool, (4 * static_cast<int>(rank) + e) * 64, row, &sm.v_full[b]);
+          }
         }
-        issued = i + 1;
+        if (!ok) {
+          set_abort(sm);
+          for (int e = max(0, g - 2); e < g; ++e) bar_wait(&sm.v_full[e & 1], (e >> 1) & 1);
+        }
       }
-      if (!ok) {
-        set_abort(sm);
-        for (int i = max(0, issued - 2); i < issued; ++i) bar_wait(&sm.v_full[i & 1], (i >> 1) & 1);
-      }
+      ok = __shfl_sync(0xffffffffu, ok, leader);
+      g = __shfl_sync(0xffffffffu, g, leader);
     }
-  } else if (warp == 9) {
-    // ---------------------------------------------------------------- MMAs (CTA 0, one thread)
+  } else if (warp == 0) {
+    // ---------------------------------------------------------------- S (CTA 0, one thread)
     if (rank == 0 && elect_one()) {
       constexpr uint32_t id_s = idesc_bf16<128, 128>(false, false);
-      constexpr uint32_t id_o = idesc_bf16<128, 256>(false, true);
       const uint64_t qd = sdesc(smem_u32(sm.q), 16, 1024), kd = sdesc(smem_u32(sm.kv), 16, 1024);
-      const uint64_t pd = sdesc(smem_u32(sm.p), 16, 1024), vd = sdesc(smem_u32(sm.kv), SLAB, 1024);
-      bool ok = bar_wait_or_abort(&sm.q_full, 0, abort);
-      int s = 0, o = 0;  // steps issued: half an S (one slot's dims), an O
-      uint64_t since = global_ns();
-      while (ok && o < nt) {
-        const int sb = (s >> 1) & 1, x = s & 1;
-        if (2 * o < s - 1 && bar_test(&sm.p_full[o & 1], (o >> 1) & 1)) {
-          after_sync();
-          const uint64_t a = pd + (o & 1) * (2 * SLAB >> 4), v = vd + (o & 1) * (2 * SLOT >> 4);
-          const uint32_t acc = o > 0 ? 1u : 0u;
+      bool ok = true;
+      int g = 0;
+      for (int ord = 0; ok; ++ord) {
+        if (!(ok = bar_wait_or_abort(&sm.q_full, ord & 1, abort))) break;
+        const int n = sm.unit_tiles[ord & 1];
+        if (n < 0) break;
+        for (int i = 0; i < n && ok; ++i, ++g) {
+          const int b = g & 1;
+          const uint32_t d = tmem + COL_S + 64 * b;
+          // Quarter qr: slabs 2 (qr / 2) .. of slot qr % 2. Its rows say that the buffer of the tile before last
+          // has been through O, and so that its S has been read.
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
+          for (int qr = 0; qr < 4; ++qr) {
+            if (!(ok = bar_wait_or_abort(&sm.kv_full[b][qr], (g >> 1) & 1, abort))) break;
+            if (qr == 0) after_sync();
+            const uint64_t a = qd + ((4 * (qr & 1) + (qr & 2)) * SLAB >> 4);
+            const uint64_t k = kd + b * (2 * SLOT >> 4) + ((qr & 1) * SLOT + (qr & 2) * SLAB >> 4);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              mma_pair(tmem + COL_O + 128 * j, a + ((kk >> 2) * SLAB + (kk & 3) * 32 >> 4),
-                       v + ((kk >> 2) * SLOT + 2 * j * SLAB + (kk & 3) * 2048 >> 4), id_o, kk ? 1u : acc);
-            if (kk == 3) commit_pair(&sm.kv_free[o & 1][0]);
+            for (int e = 0; e < 8; ++e)
+              mma_pair(d, a + ((e >> 2) * SLAB + (e & 3) * 32 >> 4), k + ((e >> 2) * SLAB + (e & 3) * 32 >> 4), id_s,
+                       (qr | e) ? 1u : 0u);
           }
-          commit_pair(&sm.kv_free[o & 1][1]);
-          ++o;
-          since = global_ns();
-        } else if (s < 2 * nt && s < 2 * o + 4 && bar_test(&sm.kv_full[sb][x], (s >> 2) & 1)) {
-          after_sync();
-          const uint32_t d = tmem + COL_S + 64 * sb;
-          const uint64_t a = qd + x * (4 * SLAB >> 4), k = kd + (2 * sb + x) * (SLOT >> 4);
-          const uint32_t acc = x;
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            mma_pair(d, a + ((e >> 2) * SLAB + (e & 3) * 32 >> 4), k + ((e >> 2) * SLAB + (e & 3) * 32 >> 4), id_s,
-                     e ? 1u : acc);
-          if (x == 1) commit_pair(&sm.s_full[sb]);
-          ++s;
-          since = global_ns();
-        } else if (*abort || global_ns() - since > WAIT_NS) {
-          ok = false;
+          if (ok) commit_pair(&sm.s_full[b]);
         }
       }
       if (!ok) {
         set_abort(sm);
-        // everything issued completes before the pair leaves: one more commit on a barrier of its own
-        // phase (q_full, phase 1; both CTAs' q_full are past phase 0 or unused)
-        commit_pair(&sm.q_full);
-        bar_wait(&sm.q_full, 1);
+        drain_issued(&sm.fin[0]);
+      }
+    }
+  } else if (warp == 12) {
+    // ---------------------------------------------------------------- O (CTA 0, one thread)
+    if (rank == 0) {
+      constexpr uint32_t id_o = idesc_bf16<128, 256>(false, true);
+      const uint64_t pd = sdesc(smem_u32(sm.p), 16, 1024), vd = sdesc(smem_u32(sm.kv), SLAB, 1024);
+      bool ok = true;
+      int g = 0, ord = 0;
+      Work w(P);
+      while (ok && w.next(P)) {
+        if (w.nt == 0) continue;
+        uint32_t leader;
+        if (elect_one(&leader)) {
+          // the epilogue of the unit before has read O
+          if (ord > 0) ok = bar_wait_or_abort(&sm.o_free, (ord - 1) & 1, abort);
+          for (int i = 0; i < w.nt && ok; ++i, ++g) {
+            const int b = g & 1;
+            if (!(ok = bar_wait_or_abort(&sm.p_full[b], (g >> 1) & 1, abort))) break;
+            after_sync();
+            const uint64_t a = pd + b * (2 * SLAB >> 4), v = vd + b * (2 * SLOT >> 4);
+            const uint32_t acc = i > 0 ? 1u : 0u;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk) {
+                mma_pair(tmem + COL_O + 128 * j, a + ((kk >> 2) * SLAB + (kk & 3) * 32 >> 4),
+                         v + ((kk >> 2) * SLOT + 2 * j * SLAB + (kk & 3) * 2048 >> 4), id_o, kk ? 1u : acc);
+                if ((kk & 3) == 3) commit_pair(&sm.kv_free[b][2 * j + (kk >> 2)]);
+              }
+          }
+          if (!ok) {
+            set_abort(sm);
+            drain_issued(&sm.fin[1]);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, leader);
+        g = __shfl_sync(0xffffffffu, g, leader);
+        ++ord;
       }
     }
   } else {
-    // ---------------------------------------------------------------- softmax, epilogue (warps 0-7)
-    const int quad = warp & 3, ch = warp >> 2;
+    // ---------------------------------------------------------------- softmax, epilogue (warps 4-11)
+    const int quad = warp & 3, ch = (warp >> 2) - 1;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const int head = (quad & 1) * 32 + lane, kvh = quad >> 1;  // TMEM lane: head + 64 kvh
-    float m = -INFINITY, l = 0.f;
+    const float sink = P.sink[head] * LOG2E;
     bool ok = true;
-    for (int i = 0; i < nt; ++i) {
-      const int b = i & 1;
-      // what of this warp's 32 rows is seen, by the CTA's token and by either token of the pair
-      const int h = 2 * (tile0 + i) + kvh, j = 32 * ch + lane;
-      const bool v0 = h < u.nh && half_sees(P.c, u, h, j, u.p0, u.seen[0]);
-      const bool v1 = h < u.nh && u.n > 1 && half_sees(P.c, u, h, j, u.p0 + 1, u.seen[1]);
-      const uint32_t see = __ballot_sync(0xffffffffu, rank == 0 ? v0 : v1);
-      const uint32_t either = __ballot_sync(0xffffffffu, v0 || v1);
-      ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.s_full[b], (i >> 1) & 1, abort));
-      float x[32];
-      float mx = -INFINITY;
-      if (ok) {
-        after_sync();
-        tmem_ld16(tmem + lanes + COL_S + 64 * b + 32 * ch, x);
-        tmem_ld16(tmem + lanes + COL_S + 64 * b + 32 * ch + 16, x + 16);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; ++c) x[c] *= P.scale_log2;
-        if (see != 0xffffffffu) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) x[c] = (see >> c) & 1 ? x[c] : -INFINITY;
+    int g = 0;
+    Work w(P);
+    while (w.next(P)) {
+      const Unit& u = w.u;
+      const bool mine = static_cast<int>(rank) < u.n;  // this CTA has a token
+      const int64_t token = u.t0 + rank;
+      if (w.nt == 0) {  // splits > 1: no rows for this one, its O is not read
+        if (mine && kvh == 0 && ch == 0) {
+          float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + ((token * P.splits + w.split) * HB + head) * 2;
+          ml[0] = -INFINITY;
+          ml[1] = 0.f;
         }
-        float mc[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) mc[c] = x[c];
-#pragma unroll
-        for (int c = 4; c < 32; ++c) mc[c & 3] = fmaxf(mc[c & 3], x[c]);
-        mx = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3]));
+        continue;
       }
-      if (smx_any(!ok || mx > m + RESCALE)) {
-        if (smx_any(!ok)) {
-          if (lane == 0) set_abort(sm);
-          ok = false;
-          break;
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < w.nt; ++i, ++g) {
+        const int b = g & 1;
+        // what of this warp's 32 rows is seen, by the CTA's token and by either token of the pair: all of
+        // them, but for the ring, the stage and the last entries
+        const int h = 2 * (w.tile0 + i) + kvh;
+        uint32_t see = 0xffffffffu, either = 0xffffffffu;
+        if (h < u.nring + u.nstage || 64 * (h - u.nring - u.nstage) + 64 > u.seen[0]) {
+          const int j = 32 * ch + lane;
+          const bool v0 = h < u.nh && half_sees(P.c, u, h, j, u.p0, u.seen[0]);
+          const bool v1 = h < u.nh && u.n > 1 && half_sees(P.c, u, h, j, u.p0 + 1, u.seen[1]);
+          see = __ballot_sync(0xffffffffu, rank == 0 ? v0 : v1);
+          either = __ballot_sync(0xffffffffu, v0 || v1);
         }
-        sm.red[kvh * 2 + ch][head] = mx;
-        smx_bar();
-        const float mn = fmaxf(m, fmaxf(fmaxf(sm.red[0][head], sm.red[1][head]), fmaxf(sm.red[2][head], sm.red[3][head])));
-        const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
-        const bool moved = mn != m && m != -INFINITY;
-        m = mn;
-        l *= alpha;
-        smx_bar();  // red is free again
-        if (i > 0 && __any_sync(0xffffffffu, moved)) {
-          // O of the tiles before has been added up: rescale this warp's half of its columns
-          ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.kv_free[b ^ 1][1], ((i - 1) >> 1) & 1, abort));
-          if (ok) {
-            after_sync();
-#pragma unroll 1
-            for (int c = 0; c < 128; c += 32) {
-              float v[32];
-              tmem_ld16(tmem + lanes + COL_O + 128 * ch + c, v);
-              tmem_ld16(tmem + lanes + COL_O + 128 * ch + c + 16, v + 16);
-              tmem_wait_ld();
+        // a wait that ran out takes the CTA's warps to the end together, from the next smx_any
+        ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.s_full[b], (g >> 1) & 1, abort));
+        float x[32];
+        float mx = -INFINITY;
+        if (ok) {
+          after_sync();
+          tmem_ld16(tmem + lanes + COL_S + 64 * b + 32 * ch, x);
+          tmem_ld16(tmem + lanes + COL_S + 64 * b + 32 * ch + 16, x + 16);
+          tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] *= moved ? alpha : 1.f;
-              tmem_st16(tmem + lanes + COL_O + 128 * ch + c, v);
-              tmem_st16(tmem + lanes + COL_O + 128 * ch + c + 16, v + 16);
+          for (int c = 0; c < 32; ++c) x[c] *= P.scale_log2;
+          if (see != 0xffffffffu) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[c] = (see >> c) & 1 ? x[c] : -INFINITY;
+          }
+          float mc[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mc[c] = x[c];
+#pragma unroll
+          for (int c = 4; c < 32; ++c) mc[c & 3] = fmaxf(mc[c & 3], x[c]);
+          mx = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3]));
+        }
+        if (smx_any(!ok || mx > m + RESCALE)) {
+          if (smx_any(!ok)) {
+            if (lane == 0) set_abort(sm);
+            ok = false;
+            break;
+          }
+          sm.red[kvh * 2 + ch][head] = mx;
+          smx_bar();
+          const float mn = fmaxf(m, fmaxf(fmaxf(sm.red[0][head], sm.red[1][head]), fmaxf(sm.red[2][head], sm.red[3][head])));
+          const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+          const bool moved = mn != m && m != -INFINITY;
+          m = mn;
+          l *= alpha;
+          smx_bar();  // red is free again
+          if (i > 0 && __any_sync(0xffffffffu, moved)) {
+            // O of the tiles before has been added up: rescale this warp's half of its columns
+            ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.kv_free[b ^ 1][3], ((g - 1) >> 1) & 1, abort));
+            if (ok) {
+              after_sync();
+#pragma unroll 1
+              for (int c = 0; c < 128; c += 32) {
+                float v[32];
+                tmem_ld16(tmem + lanes + COL_O + 128 * ch + c, v);
+                tmem_ld16(tmem + lanes + COL_O + 128 * ch + c + 16, v + 16);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] *= moved ? alpha : 1.f;
+                tmem_st16(tmem + lanes + COL_O + 128 * ch + c, v);
+                tmem_st16(tmem + lanes + COL_O + 128 * ch + c + 16, v + 16);
+              }
+              tmem_wait_st();
             }
-            tmem_wait_st();
+          }
+        }
+        // P: 32 columns of this row, four 16-byte chunks of the 128-byte-swizzled slab (free: the S that was
+        // waited for needed the tile before last's O, which read it)
+        uint8_t* prow = sm.p[b] + kvh * SLAB + head * 128;
+        const float mm = m == -INFINITY ? 0.f : m;  // nothing seen yet: every x is -inf and p is 0
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+          uint32_t e2[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p0 = ex2(x[c4 * 8 + 2 * e] - mm), p1 = ex2(x[c4 * 8 + 2 * e + 1] - mm);
+            e2[e] = pack_bf16x2(p0, p1);
+            ls[e] += p0 + p1;
+          }
+          *reinterpret_cast<uint4*>(prow + (((ch * 4 + c4) ^ (head & 7)) << 4)) = make_uint4(e2[0], e2[1], e2[2], e2[3]);
+        }
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.v_full[b], (g >> 1) & 1, abort));
+        if (!ok) {  // the CTA's other warps end at their next wait or at smx_any
+          if (lane == 0) set_abort(sm);
+        } else if (either != 0xffffffffu && h < u.nh) {
+          // values of rows that neither token sees: two slabs of the slot for this warp, 16 lanes a row
+          uint8_t* slab = sm.kv[b][kvh] + (2 * (quad & 1) + ((lane >> 3) & 1)) * SLAB;
+          for (int e = lane >> 4; e < 32; e += 2)
+            if (!((either >> e) & 1))
+              *reinterpret_cast<uint4*>(slab + (32 * ch + e) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_async_smem();
+        before_sync();
+        __syncwarp();
+        if (lane == 0) arrive_at(in_cta(&sm.p_full[b], 0));
+      }
+      // the row's sum of its four parts; the unit's last O (a warp whose wait ran out goes on to the barriers)
+      if (smx_any(!ok)) {
+        if (lane == 0) set_abort(sm);
+        ok = false;
+        break;
+      }
+      sm.red[kvh * 2 + ch][head] = l;
+      smx_bar();
+      l = (sm.red[0][head] + sm.red[1][head]) + (sm.red[2][head] + sm.red[3][head]);
+      smx_bar();
+      ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.kv_free[(g - 1) & 1][3], ((g - 1) >> 1) & 1, abort));
+      after_sync();
+      if (ok && mine) {
+        const uint32_t src = tmem + lanes + COL_O + 128 * ch;
+        const int d0 = 256 * kvh + 128 * ch;
+        if (P.splits > 1) {
+          const int64_t at = (token * P.splits + w.split) * HB + head;
+          float* po = P.part + at * D + d0;
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 32) {
+            float v[32];
+            tmem_ld16(src + c, v);
+            tmem_ld16(src + c + 16, v + 16);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              reinterpret_cast<float4*>(po + c)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          }
+          if (kvh == 0 && ch == 0) {
+            float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + at * 2;
+            ml[0] = m;
+            ml[1] = l;
+          }
+        } else {
+          const float inv = 1.f / (l + exp2f(sink - m));
+          const int64_t off = (token * HB + head) * D + d0;
+          float rc = 1.f, rs = 0.f;  // lane f: the rotation of pair f
+          if (P.freqs != nullptr && d0 + 128 > D - P.rope_dim && lane < P.rope_dim / 2)
+            rope_cos_sin(u.p0 + static_cast<int>(rank), P.freqs[lane], &rc, &rs);
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 32) {
+            float v[32];
+            tmem_ld16(src + c, v);
+            tmem_ld16(src + c + 16, v + 16);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] *= inv;
+            if (d0 + c + 32 > D - P.rope_dim) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const int f = (d0 + c + e - (D - P.rope_dim)) >> 1;
+                const float cs = __shfl_sync(0xffffffffu, rc, f & 31), sn = __shfl_sync(0xffffffffu, rs, f & 31);
+                if (f >= 0) rotate_pair(v[e], v[e + 1], cs, sn, true, &v[e], &v[e + 1]);
+              }
+            }
+            if (P.out_dtype == DSV4_BF16) {
+              uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.out) + off + c);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                dst[e] = make_uint4(pack_bf16x2(v[8 * e], v[8 * e + 1]), pack_bf16x2(v[8 * e + 2], v[8 * e + 3]),
+                                    pack_bf16x2(v[8 * e + 4], v[8 * e + 5]), pack_bf16x2(v[8 * e + 6], v[8 * e + 7]));
+            } else {
+              float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + off + c);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            }
           }
         }
       }
-      // P: 32 columns of this row, four 16-byte chunks of the 128-byte-swizzled slab
-      uint8_t* prow = sm.p[b] + kvh * SLAB + head * 128;
-      const float mm = m == -INFINITY ? 0.f : m;  // nothing seen yet: every x is -inf and p is 0
-      float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c4 = 0; c4 < 4; ++c4) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = ex2(x[c4 * 8 + 2 * e] - mm), p1 = ex2(x[c4 * 8 + 2 * e + 1] - mm);
-          w[e] = pack_bf16x2(p0, p1);
-          ls[e] += p0 + p1;
-        }
-        *reinterpret_cast<uint4*>(prow + (((ch * 4 + c4) ^ (head & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-      ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.v_full[b], (i >> 1) & 1, abort));
-      if (!ok) {  // the CTA's other warps end at their next wait or at smx_any
-        if (lane == 0) set_abort(sm);
-      } else if (either != 0xffffffffu && h < u.nh) {
-        // values of rows that neither token sees: two slabs of the slot for this warp, 16 lanes a row
-        uint8_t* slab = sm.kv[b][kvh] + (2 * (quad & 1) + ((lane >> 3) & 1)) * SLAB;
-        for (int r = lane >> 4; r < 32; r += 2)
-          if (!((either >> r) & 1))
-            *reinterpret_cast<uint4*>(slab + (32 * ch + r) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-      }
-      fence_async_smem();
+      if (!ok && lane == 0) set_abort(sm);
+      // O has been read: the next unit's may be begun
       before_sync();
       __syncwarp();
-      if (lane == 0) arrive_at(in_cta(&sm.p_full[b], 0));
+      if (lane == 0) arrive_at(in_cta(&sm.o_free, 0));
     }
-    for (int x = 0; x < 2; ++x)  // both of the last commits have arrived here
-      ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.kv_free[(nt - 1) & 1][x], ((nt - 1) >> 1) & 1, abort));
+    // every commit of the last two tiles has arrived here before the CTA leaves
+    for (int e = max(0, g - 2); e < g; ++e)
+      for (int x = 0; x < 4; ++x)
+        ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.kv_free[e & 1][x], (e >> 1) & 1, abort));
     if (!ok && lane == 0) set_abort(sm);
-    sm.red[kvh * 2 + ch][head] = l;
-    smx_bar();
-    l = (sm.red[0][head] + sm.red[1][head]) + (sm.red[2][head] + sm.red[3][head]);
-    if (ok && !*abort && mine) {
-      after_sync();
-      const uint32_t src = tmem + lanes + COL_O + 128 * ch;
-      const int d0 = 256 * kvh + 128 * ch;
-      if (P.splits > 1) {
-        const int64_t at = (token * P.splits + split) * HB + head;
-        float* po = P.part + at * D + d0;
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          float v[32];
-          tmem_ld16(src + c, v);
-          tmem_ld16(src + c + 16, v + 16);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            reinterpret_cast<float4*>(po + c)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-        }
-        if (kvh == 0 && ch == 0) {
-          float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + at * 2;
-          ml[0] = m;
-          ml[1] = l;
-        }
-      } else {
-        const float inv = 1.f / (l + exp2f(P.sink[head] * LOG2E - m));
-        const int64_t off = (token * HB + head) * D + d0;
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          float v[32];
-          tmem_ld16(src + c, v);
-          tmem_ld16(src + c + 16, v + 16);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] *= inv;
-          if (P.freqs != nullptr && d0 + c + 32 > D - P.rope_dim) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const int f = (d0 + c + e - (D - P.rope_dim)) >> 1;
-              if (f >= 0) rotate_pair(v[e], v[e + 1], sm.rope_c[f], sm.rope_s[f], true, &v[e], &v[e + 1]);
-            }
-          }
-          if (P.out_dtype == DSV4_BF16) {
-            uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.out) + off + c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              dst[e] = make_uint4(pack_bf16x2(v[8 * e], v[8 * e + 1]), pack_bf16x2(v[8 * e + 2], v[8 * e + 3]),
-                                  pack_bf16x2(v[8 * e + 4], v[8 * e + 5]), pack_bf16x2(v[8 * e + 6], v[8 * e + 7]));
-          } else {
-            float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + off + c);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-          }
-        }
-      }
-    }
   }
   __syncwarp();
   before_sync();
   __syncthreads();
   cluster_sync();  // no CTA leaves while the pair's MMAs, loads or arrivals may touch it
   after_sync();
-  if (warp == 9)
+  if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(TMEM_COLS));
 }
 
@@ -766,13 +866,13 @@ int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
   P.rope_dim = p->rope_freqs ? p->rope_dim : 0;
   P.out_dtype = p->out_dtype;
   P.scale_log2 = p->scale * ca::LOG2E;
-  const int64_t units = (static_cast<int64_t>(P.c.total) + P.c.n) / 2;
-  DSV4_CHECK_ARG(2 * units * P.splits <= 0x7fffffffLL && static_cast<int64_t>(P.c.total) * 64 <= 0x7fffffffLL,
-                 "dsv4_chunk_attn: too many tokens");
+  // one cluster per pair of SMs, or per unit where there are fewer
+  const int64_t units = (static_cast<int64_t>(P.c.total) + P.c.n) / 2 * P.splits;
+  DSV4_CHECK_ARG(units <= 0x3fffffffLL, "dsv4_chunk_attn: too many tokens");
   static PerDeviceOnce attr;
   const int smem = static_cast<int>(sizeof(ca::Smem)) + 1024;
   DSV4_CUDA_CHECK(set_smem_once(attr, ca::chunk_attn_kernel, smem));
-  ca::chunk_attn_kernel<<<static_cast<unsigned>(2 * units * P.splits), ca::THREADS, smem, as_stream(stream)>>>(P);
+  ca::chunk_attn_kernel<<<static_cast<unsigned>(2 * std::min<int64_t>(units, num_sms() / 2)), ca::THREADS, smem, as_stream(stream)>>>(P);
   DSV4_LAUNCH_CHECK("chunk_attn_kernel");
   if (P.splits > 1) {
     ca::chunk_merge_kernel<<<static_cast<unsigned>(P.c.total) * 64, 128, 0, as_stream(stream)>>>(P);

@@ -92,25 +92,34 @@ __device__ __forceinline__ bool bar_test(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
+// The time limit of a wait. Reading %globaltimer takes several hundred cycles, so it is looked at only
+// every 64th unsuccessful try.
+struct WaitLimit {
+  uint32_t tries = 0;
+  uint64_t since = 0;
+  __device__ __forceinline__ bool passed() {
+    if ((++tries & 63) != 0) return false;
+    const uint64_t now = global_ns();
+    if (since == 0) since = now;
+    return now - since > WAIT_NS;
+  }
+};
 // wait for the phase with the given parity, bounded by WAIT_NS of wall time; false on timeout
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t a = smem_u32(bar);
-  if (bar_try(a, parity)) return true;
-  const uint64_t t0 = global_ns();
+  WaitLimit limit;
   while (true) {
     if (bar_try(a, parity)) return true;
-    if (global_ns() - t0 > WAIT_NS) return false;
+    if (limit.passed()) return false;
   }
 }
 // as bar_wait, but also gives up as soon as *abort (set by another thread) is nonzero
 __device__ __forceinline__ bool bar_wait_or_abort(uint64_t* bar, uint32_t parity, const volatile int* abort) {
   const uint32_t a = smem_u32(bar);
-  if (bar_try(a, parity)) return true;
-  const uint64_t t0 = global_ns();
+  WaitLimit limit;
   while (true) {
     if (bar_try(a, parity)) return true;
-    if (*abort) return false;
-    if (global_ns() - t0 > WAIT_NS) return false;
+    if (*abort || limit.passed()) return false;
   }
 }
 
