@@ -75,6 +75,7 @@ static_assert(sizeof(Smem) + 1024 <= 232448, "shared memory above the 227 KB a C
 struct Params {
   CUtensorMap pool;  // [pool_rows, 512] bf16, box 64 dims x box_rows
   CUtensorMap q;     // [total * 64, 512] bf16, box 64 dims x 64 rows
+  CUtensorMap o;     // out, if bf16: as q
   dsv4_chunk c;
   const float* sink;
   void* out;
@@ -122,6 +123,16 @@ __device__ __forceinline__ void load_pair(void* dst, const void* map, int x, int
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// a 64 x 64 tile of this CTA's shared memory to a tensor, and the wait until such tiles have been read
+__device__ __forceinline__ void store_tile(const void* map, int x, int y, const void* src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(smem_u32(src))
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+}
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
   asm volatile(
       "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
@@ -147,6 +158,8 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error about 2^
   return y;
 }
 __device__ __forceinline__ void smx_bar() { asm volatile("bar.sync 1, %0;\n" ::"n"(SMX_THREADS) : "memory"); }
+// the two warps that hold the same columns of O
+__device__ __forceinline__ void column_bar(int group) { asm volatile("bar.sync %0, 64;\n" ::"r"(2 + group) : "memory"); }
 __device__ __forceinline__ bool smx_any(bool v) {
   uint32_t r;
   asm volatile(
@@ -500,16 +513,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     bool ok = true;
     int g = 0;
     Work w(P);
-    while (w.next(P)) {
+    for (bool has = w.next(P); has;) {
       const Unit& u = w.u;
       const bool mine = static_cast<int>(rank) < u.n;  // this CTA has a token
       const int64_t token = u.t0 + rank;
+      const int pos = u.p0 + static_cast<int>(rank), split = w.split;
       if (w.nt == 0) {  // splits > 1: no rows for this one, its O is not read
         if (mine && kvh == 0 && ch == 0) {
-          float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + ((token * P.splits + w.split) * HB + head) * 2;
+          float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + ((token * P.splits + split) * HB + head) * 2;
           ml[0] = -INFINITY;
           ml[1] = 0.f;
         }
+        has = w.next(P);
         continue;
       }
       float m = -INFINITY, l = 0.f;
@@ -624,13 +639,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       smx_bar();
       l = (sm.red[0][head] + sm.red[1][head]) + (sm.red[2][head] + sm.red[3][head]);
       smx_bar();
+      has = w.next(P);  // found while the last O is being computed; u is the next unit's from here
       ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.kv_free[(g - 1) & 1][3], ((g - 1) >> 1) & 1, abort));
       after_sync();
-      if (ok && mine) {
-        const uint32_t src = tmem + lanes + COL_O + 128 * ch;
-        const int d0 = 256 * kvh + 128 * ch;
-        if (P.splits > 1) {
-          const int64_t at = (token * P.splits + w.split) * HB + head;
+      const uint32_t src = tmem + lanes + COL_O + 128 * ch;
+      const int d0 = 256 * kvh + 128 * ch, group = 2 * kvh + ch;
+      if (P.splits > 1) {
+        if (ok && mine) {
+          const int64_t at = (token * P.splits + split) * HB + head;
           float* po = P.part + at * D + d0;
 #pragma unroll 1
           for (int c = 0; c < 128; c += 32) {
@@ -642,46 +658,62 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
             for (int e = 0; e < 8; ++e)
               reinterpret_cast<float4*>(po + c)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
           }
-          if (kvh == 0 && ch == 0) {
+          if (group == 0) {
             float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + at * 2;
             ml[0] = m;
             ml[1] = l;
           }
-        } else {
-          const float inv = 1.f / (l + exp2f(sink - m));
-          const int64_t off = (token * HB + head) * D + d0;
-          float rc = 1.f, rs = 0.f;  // lane f: the rotation of pair f
-          if (P.freqs != nullptr && d0 + 128 > D - P.rope_dim && lane < P.rope_dim / 2)
-            rope_cos_sin(u.p0 + static_cast<int>(rank), P.freqs[lane], &rc, &rs);
+        }
+      } else {
+        const float inv = 1.f / (l + exp2f(sink - m));
+        const int64_t off = (token * HB + head) * D + d0;
+        float rc = 1.f, rs = 0.f;  // lane f: the rotation of pair f
+        if (P.freqs != nullptr && d0 + 128 > D - P.rope_dim && lane < P.rope_dim / 2)
+          rope_cos_sin(pos, P.freqs[lane], &rc, &rs);
+        // bf16: by way of P's space, which is out of use until the next unit's first P: 64 rows by 64 dims
+        // of two warps at a time, 128-byte swizzled, to the tensor by TMA (rows of 16 bytes a lane straight
+        // from the registers took 5700 cycles a unit)
+        uint8_t* const tile = sm.p[0] + group * SLAB;
+        const bool store = mine && P.out_dtype == DSV4_BF16;
 #pragma unroll 1
-          for (int c = 0; c < 128; c += 32) {
-            float v[32];
-            tmem_ld16(src + c, v);
-            tmem_ld16(src + c + 16, v + 16);
-            tmem_wait_ld();
+        for (int c = 0; c < 128; c += 32) {
+          float v[32];
+          tmem_ld16(src + c, v);
+          tmem_ld16(src + c + 16, v + 16);
+          tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] *= inv;
-            if (d0 + c + 32 > D - P.rope_dim) {
+          for (int e = 0; e < 32; ++e) v[e] *= inv;
+          if (d0 + c + 32 > D - P.rope_dim) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const int f = (d0 + c + e - (D - P.rope_dim)) >> 1;
-                const float cs = __shfl_sync(0xffffffffu, rc, f & 31), sn = __shfl_sync(0xffffffffu, rs, f & 31);
-                if (f >= 0) rotate_pair(v[e], v[e + 1], cs, sn, true, &v[e], &v[e + 1]);
-              }
-            }
-            if (P.out_dtype == DSV4_BF16) {
-              uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.out) + off + c);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                dst[e] = make_uint4(pack_bf16x2(v[8 * e], v[8 * e + 1]), pack_bf16x2(v[8 * e + 2], v[8 * e + 3]),
-                                    pack_bf16x2(v[8 * e + 4], v[8 * e + 5]), pack_bf16x2(v[8 * e + 6], v[8 * e + 7]));
-            } else {
-              float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + off + c);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            for (int e = 0; e < 32; e += 2) {
+              const int f = (d0 + c + e - (D - P.rope_dim)) >> 1;
+              const float cs = __shfl_sync(0xffffffffu, rc, f & 31), sn = __shfl_sync(0xffffffffu, rs, f & 31);
+              if (f >= 0) rotate_pair(v[e], v[e + 1], cs, sn, true, &v[e], &v[e + 1]);
             }
           }
+          if (P.out_dtype == DSV4_BF16) {
+            if (c == 64) {  // the first 64 dims have left the space
+              if (store && (quad & 1) == 0 && lane == 0) stores_read();
+              column_bar(group);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(tile + head * 128 + (((((c >> 3) & 4) + e) ^ (head & 7)) << 4)) =
+                  make_uint4(pack_bf16x2(v[8 * e], v[8 * e + 1]), pack_bf16x2(v[8 * e + 2], v[8 * e + 3]),
+                             pack_bf16x2(v[8 * e + 4], v[8 * e + 5]), pack_bf16x2(v[8 * e + 6], v[8 * e + 7]));
+            if (c & 32) {
+              fence_async_smem();
+              column_bar(group);
+              if (store && ok && (quad & 1) == 0 && lane == 0)
+                store_tile(&P.o, d0 + c - 32, static_cast<int>(token) * HB, tile);
+            }
+          } else if (ok && mine) {
+            float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + off + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          }
         }
+        if (store && (quad & 1) == 0 && lane == 0) stores_read();
       }
       if (!ok && lane == 0) set_abort(sm);
       // O has been read: the next unit's may be begun
@@ -689,6 +721,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       __syncwarp();
       if (lane == 0) arrive_at(in_cta(&sm.o_free, 0));
     }
+    if (lane == 0) stores_done();
     // every commit of the last two tiles has arrived here before the CTA leaves
     for (int e = max(0, g - 2); e < g; ++e)
       for (int x = 0; x < 4; ++x)
@@ -858,6 +891,10 @@ int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
   if (st != DSV4_OK) return st;
   st = ca::encode(&P.q, p->q, static_cast<uint64_t>(p->chunk.total) * ca::HB, 64);
   if (st != DSV4_OK) return st;
+  if (p->out_dtype == DSV4_BF16) {
+    st = ca::encode(&P.o, p->out, static_cast<uint64_t>(p->chunk.total) * ca::HB, 64);
+    if (st != DSV4_OK) return st;
+  }
   P.c = p->chunk;
   P.sink = p->sink;
   P.out = p->out;
