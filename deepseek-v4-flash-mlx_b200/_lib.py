@@ -233,7 +233,13 @@ def dtype_code(t):
         raise TypeError(f"dsv4: unsupported dtype {t.dtype}") from None
 
 
+# the current stream's handle without making a Stream object (a few microseconds less a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(t):
+    if _raw_stream is not None:
+        return _raw_stream(t.get_device())
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
@@ -250,7 +256,7 @@ _HERE_ALREADY = _Here()
 
 def device_of(t):
     """A context in which `t`'s device is the current one (kernels launch on the current device)."""
-    return _HERE_ALREADY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE_ALREADY if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def require_cuda(*ts):

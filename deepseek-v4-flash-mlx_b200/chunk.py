@@ -24,36 +24,39 @@ from .norm_rope import rope_freqs
 from .sparse_attn import sparse_attn_into
 
 
-def _index_tensor(name, t, dev, n=None):
+def _index_tensor(name, t, dev, n):
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.dim() != 1:
         raise TypeError(f"{name} must be a 1-d int32 tensor")
-    L.require_cuda(t)
     if t.device != dev:
+        L.require_cuda(t)
         raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
     if n is not None and t.numel() != n:
         raise ValueError(f"{name} has {t.numel()} values, the chunk has {n} sequences")
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _f32(t):
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
 def _chunk(cache, cu_seqlens, start, seqs, total):
     """dsv4_chunk of the cache, and the tensors it points to."""
-    dev = cache.kv_pool.device
-    cu = _index_tensor("cu_seqlens", cu_seqlens, dev)
+    pool, table = cache.kv_pool, cache.block_table
+    dev = pool.device
+    cu = _index_tensor("cu_seqlens", cu_seqlens, dev, None)
     n = cu.numel() - 1
     if n < 0:
         raise ValueError("cu_seqlens holds one value more than there are sequences")
     start = _index_tensor("start", start, dev, n)
-    seqs = None if seqs is None else _index_tensor("seqs", seqs, dev, n)
-    if seqs is None and n > cache.batch:
+    if seqs is not None:
+        seqs = _index_tensor("seqs", seqs, dev, n)
+    elif n > cache.batch:
         raise ValueError(f"a chunk of {n} sequences, the cache has {cache.batch} slots")
     if total > cache.max_chunk:
         raise ValueError(f"a chunk of {total} tokens, the cache stages {cache.max_chunk} (SparseMLACache(max_chunk=...))")
-    c = L.Chunk()
-    c.cu_seqlens, c.start, c.seqs = cu.data_ptr(), start.data_ptr(), None if seqs is None else seqs.data_ptr()
-    c.win_base, c.block_table = cache.win_base.data_ptr(), cache.block_table.data_ptr() if cache.compressed else None
-    c.comp_base, c.stage_base, c.pool_rows = cache.comp_base, cache.stage_base, cache.kv_pool.shape[0]
-    c.n, c.total, c.slots, c.window = n, total, cache.batch, cache.window
-    c.ratio, c.page, c.bt_stride, c.max_comp = cache.ratio, cache.page, cache.block_table.shape[1], cache.max_comp
+    c = L.Chunk(cu.data_ptr(), start.data_ptr(), None if seqs is None else seqs.data_ptr(), cache.win_base.data_ptr(),
+                table.data_ptr() if cache.compressed else None, cache.comp_base, cache.stage_base, pool.shape[0], n, total,
+                cache.batch, cache.window, cache.ratio, cache.page, table.shape[1], cache.max_comp)
     return c, (cu, start, seqs)
 
 
@@ -84,15 +87,15 @@ def chunk_commit(cache, cu_seqlens, start, total, seqs=None):
 
 def _attend(cache, c, q, sink, scale, freqs, out_dtype, num_splits):
     """All visible rows: dsv4_chunk_attn, which finds them by itself."""
-    out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    p = L.ChunkAttnParams()
-    p.chunk = c
-    p.q, p.pool, p.sink, p.out, p.rope_freqs = (t.data_ptr() for t in (q, cache.kv_pool, sink, out, freqs))
-    p.rope_dim, p.out_dtype, p.scale, p.num_splits = 2 * freqs.numel(), L.dtype_code(out), scale, num_splits
-    nbytes = L.lib().dsv4_chunk_attn_workspace_size(ctypes.byref(p))
-    ws = L.workspace(nbytes, q.device)
-    p.workspace, p.workspace_bytes = L.ptr(ws), nbytes
-    L.check(L.lib().dsv4_chunk_attn(ctypes.byref(p), L.stream_of(q)))
+    out = torch.empty_like(q, dtype=out_dtype)
+    p = L.ChunkAttnParams(c, q.data_ptr(), cache.kv_pool.data_ptr(), sink.data_ptr(), out.data_ptr(), freqs.data_ptr(),
+                          2 * freqs.numel(), L.dtype_code(out), scale, num_splits)
+    lib, ref = L.lib(), ctypes.byref(p)
+    nbytes = lib.dsv4_chunk_attn_workspace_size(ref)
+    if nbytes:
+        ws = L.workspace(nbytes, q.device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+    L.check(lib.dsv4_chunk_attn(ref, L.stream_of(q)))
     return out
 
 
@@ -129,14 +132,15 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
         raise ValueError(f"chunk_attention: 64 heads, got q {tuple(q.shape)} and {sink.numel()} sinks")
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"chunk_attention: out_dtype must be bfloat16 or float32, got {out_dtype}")
-    if q.device != cache.kv_pool.device or sink.device != q.device or (rows is not None and rows.device != q.device):
+    dev = cache.kv_pool.device
+    if q.device != dev or sink.device != dev or (rows is not None and rows.device != dev):
         raise ValueError("chunk_attention: q, sink and rows must be on the cache's device")
     total = q.shape[0]
     if rows is not None:
         if rows.dim() != 2 or rows.shape[0] != total or rows.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"chunk_attention: rows must be int32 [{total}, k], got {rows.dtype} {tuple(rows.shape)}")
         rows = rows.to(torch.int32).contiguous()
-    freqs = rope_freqs(64, q.device) if freqs is None else freqs.float().contiguous()
+    freqs = rope_freqs(64, dev) if freqs is None else _f32(freqs)
     if not 0 < freqs.numel() <= 32:
         raise ValueError(f"chunk_attention: 1 to 32 rotation frequencies, got {freqs.numel()}")
     if not 0 <= num_splits <= 64:
@@ -145,7 +149,7 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
     c, keep = _chunk(cache, cu_seqlens, start, seqs, total)
     if total == 0 or c.n == 0:
         return torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    q, sink = q.contiguous(), sink.float().contiguous()
+    q, sink = q.contiguous(), _f32(sink)
     with L.device_of(q):
         # lists differ from token to token, and pages that no box of rows divides have no run to load: those
         # go through an index, token by token

@@ -271,17 +271,14 @@ def _(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out,
 
 def _chunk_into(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, page, out_base,
                 max_comp, head_dim, ratio, rope_head_dim, freqs, eps, key_image, key_inv, key_norm_max, act_quant):
-    p = L.CompressorChunkParams()
-    p.kv, p.score, p.ape, p.norm_w = L.ptr(kv), L.ptr(score), L.ptr(ape), L.ptr(norm_w)
-    p.ring_kv, p.ring_score, p.out, p.freqs = L.ptr(ring_kv), L.ptr(ring_score), L.ptr(out), L.ptr(freqs)
-    p.cu_seqlens, p.start, p.seqs, p.block_table = L.ptr(cu_seqlens), L.ptr(start), L.ptr(seqs), L.ptr(block_table)
-    p.out_base, p.out_rows = out_base, out.numel() // head_dim
-    p.n, p.total, p.slots = cu_seqlens.numel() - 1, kv.shape[0], ring_kv.shape[0]
-    p.bt_stride, p.page = (block_table.shape[1], page) if block_table is not None else (0, 1)
-    p.max_comp, p.head_dim, p.ratio, p.rope_dim = max_comp, head_dim, ratio, rope_head_dim
-    p.norm_dtype = L.dtype_code(norm_w) if norm_w is not None else L.F32
-    p.out_dtype, p.act_quant, p.eps = L.dtype_code(out), act_quant, eps
-    p.key_image, p.key_inv, p.key_norm_max = L.ptr(key_image), L.ptr(key_inv), L.ptr(key_norm_max)
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    p = L.CompressorChunkParams(
+        kv.data_ptr(), score.data_ptr(), ape.data_ptr(), at(norm_w), ring_kv.data_ptr(), ring_score.data_ptr(), out.data_ptr(),
+        freqs.data_ptr(), cu_seqlens.data_ptr(), start.data_ptr(), at(seqs), at(block_table), out_base, out.numel() // head_dim,
+        cu_seqlens.numel() - 1, kv.shape[0], ring_kv.shape[0], block_table.shape[1] if block_table is not None else 0,
+        page if block_table is not None else 1, max_comp, head_dim, ratio, rope_head_dim,
+        L.dtype_code(norm_w) if norm_w is not None else L.F32, L.dtype_code(out), act_quant, eps, at(key_image), at(key_inv),
+        at(key_norm_max))
     with L.device_of(kv):
         L.check(L.lib().dsv4_compressor_chunk(ctypes.byref(p), L.stream_of(kv)))
 

@@ -19,32 +19,35 @@ from . import _lib as L
 def _params(cache):
     if cache.page_refs is None:
         raise ValueError("SparseMLACache: pages are handed out and shared only in a paged cache (n_pages=...)")
-    p = L.Pages()
-    p.pool, p.win_base, p.block_table, p.refs = (t.data_ptr() for t in (cache.kv_pool, cache.win_base, cache.block_table,
-                                                                       cache.page_refs))
-    p.k_idx = cache.k_idx.data_ptr()
-    p.key_image, p.key_inv, p.key_norm_max = (t.data_ptr() for t in cache.key_image)
-    p.ring_kv, p.ring_score = cache.ring_kv.data_ptr(), cache.ring_score.data_ptr()
-    p.ring_k_idx, p.ring_s_idx = cache.ring_k_idx.data_ptr(), cache.ring_s_idx.data_ptr()
-    p.comp_base, p.slots, p.n_pages = cache.comp_base, cache.batch, cache.page_refs.numel()
-    p.bt_stride, p.page, p.max_comp, p.window = cache.block_table.shape[1], cache.page, cache.max_comp, cache.window
-    p.head_dim, p.idx_dim, p.ratio = cache.head_dim, cache.k_idx.shape[-1], cache.ratio
-    return p
+    L.require_cuda(cache.kv_pool)
+    img, inv, nmax = cache.key_image
+    k, table = cache.k_idx, cache.block_table
+    return L.Pages(cache.kv_pool.data_ptr(), cache.win_base.data_ptr(), table.data_ptr(), cache.page_refs.data_ptr(),
+                   k.data_ptr(), img.data_ptr(), inv.data_ptr(), nmax.data_ptr(), cache.ring_kv.data_ptr(),
+                   cache.ring_score.data_ptr(), cache.ring_k_idx.data_ptr(), cache.ring_s_idx.data_ptr(), cache.comp_base,
+                   cache.batch, cache.page_refs.numel(), table.shape[1], cache.page, cache.max_comp, cache.window,
+                   cache.head_dim, k.shape[2], cache.ratio)
 
 
 def _ints(name, cache, *ts):
     """Sequences and token counts (lists, or tensors on the cache's device) as int32 tensors of one length."""
     dev, out = cache.block_table.device, []
     for t in ts:
-        t = torch.tensor(t, dtype=torch.int32, device=dev) if not isinstance(t, torch.Tensor) else t
-        L.require_cuda(t)
+        if not isinstance(t, torch.Tensor):
+            t = torch.tensor(t, dtype=torch.int32, device=dev)
+        elif t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            if t.dtype not in (torch.int32, torch.int64):
+                L.require_cuda(t)
+                raise TypeError(f"{name}: sequences and token counts are integers, got {t.dtype}")
+            t = t.reshape(-1).to(torch.int32).contiguous()
         if t.device != dev:
+            L.require_cuda(t)
             raise ValueError(f"{name}: tensors on {t.device}, the cache is on {dev}")
-        if t.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"{name}: sequences and token counts are integers, got {t.dtype}")
-        out.append(t.reshape(-1).to(torch.int32).contiguous())
-    if any(t.numel() != out[0].numel() for t in out):
-        raise ValueError(f"{name}: {[t.numel() for t in out]} sequences and counts")
+        out.append(t)
+    n = out[0].numel()
+    for t in out:
+        if t.numel() != n:
+            raise ValueError(f"{name}: {[t.numel() for t in out]} sequences and counts")
     return out
 
 
@@ -59,7 +62,7 @@ def pages_free(cache, seqs):
     p = _params(cache)
     seqs, = _ints("pages_free", cache, seqs)
     with L.device_of(seqs):
-        L.check(L.lib().dsv4_pages_free(ctypes.byref(p), L.ptr(seqs), seqs.numel(), L.stream_of(seqs)))
+        L.check(L.lib().dsv4_pages_free(ctypes.byref(p), seqs.data_ptr(), seqs.numel(), L.stream_of(seqs)))
 
 
 def pages_reserve(cache, seqs, tokens, add=0):
@@ -74,8 +77,8 @@ def pages_reserve(cache, seqs, tokens, add=0):
         seqs, tokens = _ints("pages_reserve", cache, seqs, tokens)
     with L.device_of(tokens):
         ws, nbytes = _workspace(p, tokens.numel(), tokens.device)
-        L.check(L.lib().dsv4_pages_reserve(ctypes.byref(p), L.ptr(seqs), L.ptr(tokens), int(add), tokens.numel(),
-                                           L.ptr(ws), nbytes, L.stream_of(tokens)))
+        L.check(L.lib().dsv4_pages_reserve(ctypes.byref(p), None if seqs is None else seqs.data_ptr(), tokens.data_ptr(),
+                                           int(add), tokens.numel(), ws.data_ptr(), nbytes, L.stream_of(tokens)))
 
 
 def pages_fork(cache, src, dst, tokens):
@@ -93,7 +96,8 @@ def pages_fork(cache, src, dst, tokens):
         raise ValueError(f"pages_fork: {src.numel()} branches, the cache has {cache.batch} slots")
     with L.device_of(src):
         ws, nbytes = _workspace(p, src.numel(), src.device)
-        L.check(L.lib().dsv4_pages_fork(ctypes.byref(p), L.ptr(src), L.ptr(dst), L.ptr(tokens), src.numel(), L.ptr(ws),
+        L.check(L.lib().dsv4_pages_fork(ctypes.byref(p), src.data_ptr(), dst.data_ptr(), tokens.data_ptr(), src.numel(),
+                                        ws.data_ptr(),
                                         nbytes, L.stream_of(src)))
 
 
@@ -105,5 +109,5 @@ def pages_compact(cache):
     n = torch.empty(1, dtype=torch.int32, device=cache.block_table.device)
     with L.device_of(n):
         ws, nbytes = _workspace(p, 0, n.device)
-        L.check(L.lib().dsv4_pages_compact(ctypes.byref(p), L.ptr(n), L.ptr(ws), nbytes, L.stream_of(n)))
+        L.check(L.lib().dsv4_pages_compact(ctypes.byref(p), n.data_ptr(), ws.data_ptr(), nbytes, L.stream_of(n)))
     return n
