@@ -31,10 +31,11 @@
 // as its rows arrive, and one of warp 12 the O MMAs; an O frees the buffer quarter by quarter, in the order
 // in which the next S takes them. (One thread for both that looked at two barriers in turn lost 300 cycles
 // and more at each look: the MMAs keep shared memory busy, and a look waits for it.) Warps 1 and 2 load Q
-// and the tiles as K, a slot each; warp 3 loads the second slot as V; warps 4-11 softmax and epilogue (warp
-// w: TMEM lanes 32 (w % 4) .., half of the columns). The running maximum is lazy (raised only when a score
-// passes it by 2^8; O and the sums are then rescaled), the sums are fp32. P is rounded to bf16 (the MMA
-// takes both operands in the rows' type), O is rounded once at the end.
+// and the tiles as K, a slot each (one warp for both: 1.04 instead of 0.97 ms at the size below); warp 3
+// loads the second slot as V; warps 4-11 softmax and epilogue (warp w: TMEM lanes 32 (w % 4) .., half of the
+// columns). The running maximum is lazy (raised only when a score passes it by 2^8; O and the sums are then
+// rescaled), the sums are fp32. P is rounded to bf16 (the MMA takes both operands in the rows' type), O is
+// rounded once at the end.
 // Long lists with few tokens are split over clusters; fp32 partials and a merging kernel follow.
 // All waits inside a CTA are bounded (1 s): DSV4_ERR_WAIT_TIMEOUT, and the pair drains and leaves.
 #include <cudaTypedefs.h>
@@ -75,7 +76,7 @@ static_assert(sizeof(Smem) + 1024 <= 232448, "shared memory above the 227 KB a C
 struct Params {
   CUtensorMap pool;  // [pool_rows, 512] bf16, box 64 dims x box_rows
   CUtensorMap q;     // [total * 64, 512] bf16, box 64 dims x 64 rows
-  CUtensorMap o;     // out, if bf16: as q
+  CUtensorMap o;     // out, if bf16: as q; the partials [total * splits * 64, 512] fp32 if split, box 32 dims x 64 rows
   dsv4_chunk c;
   const float* sink;
   void* out;
@@ -181,23 +182,20 @@ struct Unit {
   int first, start;       // the sequence's first token in the batch and its position
   int t0, n;              // the pair's first token, tokens of the pair (1 or 2)
   int p0;                 // its position
-  int64_t win;            // the ring's first pool row
-  const int32_t* table;
+  int slot;               // cache slot
   int stage_pos;          // position of the first staged row it sees
   int nring, nstage, nh;  // halves: ring, stage, all
   uint64_t ring;          // the ring's halves, 4 bits each
   int seen[2];            // compressed entries that the first and the last token see
 };
-__device__ __forceinline__ Unit make_unit(const dsv4_chunk& c, int seq, int t0, int n) {
+__device__ __forceinline__ Unit make_unit(const dsv4_chunk& c, int first, int start, int slot, int t0, int n) {
   Unit u;
-  u.first = c.cu_seqlens[seq];
-  u.start = c.start[seq];
+  u.first = first;
+  u.start = start;
   u.t0 = t0;
   u.n = n;
   u.p0 = u.start + (t0 - u.first);
-  const int slot = c.seqs ? c.seqs[seq] : seq;
-  u.win = c.win_base[slot];
-  u.table = c.block_table ? c.block_table + static_cast<int64_t>(slot) * c.bt_stride : nullptr;
+  u.slot = slot;
   const int lo = max(0, u.p0 - c.window + 1);  // oldest position in the first token's window
   u.ring = 0;
   u.nring = 0;
@@ -218,18 +216,22 @@ __device__ __forceinline__ Unit make_unit(const dsv4_chunk& c, int seq, int t0, 
 __device__ __forceinline__ int half_row(const Params& P, const Unit& u, int h, int b) {
   const dsv4_chunk& c = P.c;
   const int r = b * P.box_rows;
-  if (h < u.nring) return static_cast<int>(u.win) + 64 * static_cast<int>((u.ring >> (4 * h)) & 15) + r;
+  if (h < u.nring) return static_cast<int>(c.win_base[u.slot]) + 64 * static_cast<int>((u.ring >> (4 * h)) & 15) + r;
   h -= u.nring;
   if (h < u.nstage) return static_cast<int>(c.stage_base) + u.first + (u.stage_pos - u.start) + 64 * h + r;
   const int e = 64 * (h - u.nstage) + r;
   if (e >= u.seen[1]) return static_cast<int>(c.pool_rows);
-  const int32_t pg = u.table[e / c.page];
+  const int32_t pg = c.block_table[static_cast<int64_t>(u.slot) * c.bt_stride + e / c.page];
   if (pg < 0) {
     raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
     return static_cast<int>(c.pool_rows);
   }
   const int64_t row = c.comp_base + static_cast<int64_t>(pg) * c.page + e % c.page;
   return row < c.pool_rows ? static_cast<int>(row) : static_cast<int>(c.pool_rows);
+}
+// the same for lane `b` of a warp that loads a half together; nothing to load past the last half or box
+__device__ __forceinline__ int tile_row(const Params& P, const Unit& u, int h, int b, int boxes) {
+  return h < u.nh && b < boxes ? half_row(P, u, h, b) : static_cast<int>(P.c.pool_rows);
 }
 // whether the token at position p (entries: what it sees of them) sees row j of half h
 __device__ __forceinline__ bool half_sees(const dsv4_chunk& c, const Unit& u, int h, int j, int p, int entries) {
@@ -246,55 +248,63 @@ __device__ __forceinline__ bool half_sees(const dsv4_chunk& c, const Unit& u, in
   return 64 * (h - u.nstage) + j < entries;
 }
 
-// Pairs of tokens, counted through the sequences. A warp looks together, 32 sequences at a time.
-// find < 0: the number of pairs in all; else *u becomes that pair's unit.
-__device__ __forceinline__ int look(const Params& P, int find, Unit* u) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int b0 = 0; b0 < P.c.n; b0 += 32) {
-    const int b = b0 + lane;
-    int cnt = 0, first = 0, len = 0;
-    if (b < P.c.n) {
-      first = P.c.cu_seqlens[b];
-      len = P.c.cu_seqlens[b + 1] - first;
-      const int slot = P.c.seqs ? P.c.seqs[b] : b;
-      const bool ok = first >= 0 && len >= 0 && first + len <= P.c.total && P.c.start[b] >= 0 && slot >= 0 && slot < P.c.slots;
-      if (!ok && find < 0) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-      cnt = ok ? (len + 1) / 2 : 0;
-    }
-    int s = cnt;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += x;
-    }
-    const int at = before + s - cnt;
-    const uint32_t hit = __ballot_sync(0xffffffffu, find >= at && find < at + cnt);
-    if (hit != 0) {
-      const int l = __ffs(hit) - 1, t0 = first + 2 * (find - at);
-      *u = make_unit(P.c, __shfl_sync(0xffffffffu, b, l), __shfl_sync(0xffffffffu, t0, l),
-                     __shfl_sync(0xffffffffu, min(2, first + len - t0), l));
-      return 0;
-    }
-    before += __shfl_sync(0xffffffffu, s, 31);
-  }
-  return before;
-}
-
-// The work of a cluster: units (pair of tokens, split) number `at`, at + clusters, ...; the pairs from the last to
-// the first, since the last see the most rows.
+// The work of a cluster: units (pair of tokens, split) number `at`, at + clusters, ...; the pairs are counted
+// through the sequences and taken from the last to the first, since the last see the most rows. A warp looks
+// together, a lane per sequence, 32 at a time.
 struct Work {
   Unit u;
   int pairs, at, split, tile0, nt;
-  __device__ __forceinline__ explicit Work(const Params& P) : pairs(look(P, -1, nullptr)), at(static_cast<int>(blockIdx.x >> 1)) {}
+
+  struct Seq {
+    int first, len, start, slot, pairs;
+  };
+  // this lane's sequence of those from b0 on
+  static __device__ __forceinline__ Seq load(const Params& P, int b0) {
+    const int b = b0 + (threadIdx.x & 31);
+    Seq q = {0, 0, 0, 0, 0};
+    if (b < P.c.n) {
+      q.first = P.c.cu_seqlens[b];
+      q.len = P.c.cu_seqlens[b + 1] - q.first;
+      q.start = P.c.start[b];
+      q.slot = P.c.seqs ? P.c.seqs[b] : b;
+      if (q.first >= 0 && q.len >= 0 && q.first + q.len <= P.c.total && q.start >= 0 && q.slot >= 0 && q.slot < P.c.slots)
+        q.pairs = (q.len + 1) / 2;
+      else
+        raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+    }
+    return q;
+  }
+  __device__ __forceinline__ explicit Work(const Params& P) : pairs(0), at(static_cast<int>(blockIdx.x >> 1)) {
+    for (int b0 = 0; b0 < P.c.n; b0 += 32) pairs += __reduce_add_sync(0xffffffffu, load(P, b0).pairs);
+  }
   __device__ __forceinline__ bool next(const Params& P) {
     if (at >= pairs * P.splits) return false;
     split = at % P.splits;
-    look(P, pairs - 1 - at / P.splits, &u);
+    const int find = pairs - 1 - at / P.splits;
+    at += gridDim.x >> 1;
+    int before = 0;
+    for (int b0 = 0;; b0 += 32) {  // ends: find < pairs
+      const Seq q = load(P, b0);
+      int s = q.pairs;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, s, o);
+        if ((threadIdx.x & 31) >= o) s += x;
+      }
+      const int own = before + s - q.pairs;
+      const uint32_t hit = __ballot_sync(0xffffffffu, find >= own && find < own + q.pairs);
+      if (hit != 0) {
+        const int l = __ffs(hit) - 1, t0 = q.first + 2 * (find - own);
+        u = make_unit(P.c, __shfl_sync(0xffffffffu, q.first, l), __shfl_sync(0xffffffffu, q.start, l),
+                      __shfl_sync(0xffffffffu, q.slot, l), __shfl_sync(0xffffffffu, t0, l),
+                      __shfl_sync(0xffffffffu, min(2, q.first + q.len - t0), l));
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, s, 31);
+    }
     const int tiles = (u.nh + 1) / 2;
     tile0 = static_cast<int>(static_cast<int64_t>(tiles) * split / P.splits);
     nt = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / P.splits) - tile0;
-    at += gridDim.x >> 1;
     return true;
   }
 };
@@ -331,6 +341,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     tma_prefetch_map(&P.pool);
     tma_prefetch_map(&P.q);
   }
+  pdl_wait();  // what follows reads memory that the kernels before may have written
+  pdl_trigger();
+  Work w(P);
+  bool has = w.next(P);
   before_sync();
   __syncthreads();
   cluster_sync();
@@ -344,91 +358,90 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
   // (g / 2) % 2 at tile g.
   if (warp == 1 || warp == 2) {
     // ---------------------------------------------------------------- the tiles as K: slot X (and Q), slot Y
+    // (the warp goes together: lane k finds the row of box k, a tile ahead; one lane issues the loads)
     const int x = warp - 1;
     bool ok = true;
     int g = 0, ord = 0, issued = 0;
-    Work w(P);
-    while (ok && w.next(P)) {
+    for (; ok && has; has = w.next(P)) {
       if (w.nt == 0) continue;
-      uint32_t leader;
-      if (elect_one(&leader)) {
-        if (x == 0) {
-          // Q follows the last S of the unit before
-          if (g > 0) ok = bar_wait_or_abort(&sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort);
-          if (ok) {
-            sm.unit_tiles[ord & 1] = w.nt;
-            const uint32_t qb = in_cta(&sm.q_full, 0);
-            if (rank == 0) bar_expect_tx(&sm.q_full, 2 * 8 * SLAB);
-            const int qrow = static_cast<int>(rank) < w.u.n ? (w.u.t0 + static_cast<int>(rank)) * HB : P.c.total * HB;
-            for (int e = 0; e < 8; ++e) load_pair(sm.q + e * SLAB, &P.q, e * 64, qrow, qb);  // behind q: zeros
-          }
-        }
-        for (int i = 0; i < w.nt && ok; ++i, ++g) {
-          const int b = g & 1, h = 2 * (w.tile0 + i) + static_cast<int>(rank);
-          int row = h < w.u.nh ? half_row(P, w.u, h, 0) : static_cast<int>(P.c.pool_rows);
-          for (int y = 0; y < 2; ++y) {  // two slabs at a time, as the O of the tile before last frees them
-            const int qr = 2 * y + x;
-            if (g >= 2 && !(ok = bar_wait_or_abort(&sm.kv_free[b][qr], ((g >> 1) - 1) & 1, abort))) break;
-            const uint32_t fb = in_cta(&sm.kv_full[b][qr], 0);
-            if (rank == 0) bar_expect_tx(&sm.kv_full[b][qr], 4 * SLAB);
-            for (int k = 0; k < boxes; ++k) {
-              if (boxes > 1) row = h < w.u.nh ? half_row(P, w.u, h, k) : static_cast<int>(P.c.pool_rows);
+      int row = tile_row(P, w.u, 2 * w.tile0 + static_cast<int>(rank), lane, boxes);
+      // Q follows the last S of the unit before
+      if (x == 0 && g > 0) ok = bar_wait_or_abort(&sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort);
+      if (x == 0 && ok && elect_one()) {
+        sm.unit_tiles[ord & 1] = w.nt;
+        const uint32_t qb = in_cta(&sm.q_full, 0);
+        if (rank == 0) bar_expect_tx(&sm.q_full, 2 * 8 * SLAB);
+        const int qrow = static_cast<int>(rank) < w.u.n ? (w.u.t0 + static_cast<int>(rank)) * HB : P.c.total * HB;
+        for (int e = 0; e < 8; ++e) load_pair(sm.q + e * SLAB, &P.q, e * 64, qrow, qb);  // behind q: zeros
+      }
+      __syncwarp();
+      for (int i = 0; i < w.nt && ok; ++i, ++g) {
+        const int b = g & 1;
+        const int next = i + 1 < w.nt ? tile_row(P, w.u, 2 * (w.tile0 + i + 1) + static_cast<int>(rank), lane, boxes) : 0;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {  // two slabs at a time, as the O of the tile before last frees them
+          const int qr = 2 * y + x;
+          if (g >= 2 && !(ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.kv_free[b][qr], ((g >> 1) - 1) & 1, abort)))) break;
+          const uint32_t fb = in_cta(&sm.kv_full[b][qr], 0);
+          const bool one = elect_one();
+          if (one && rank == 0) bar_expect_tx(&sm.kv_full[b][qr], 4 * SLAB);
+          for (int k = 0; k < boxes; ++k) {
+            const int at = __shfl_sync(0xffffffffu, row, k);
+            if (one) {
 #pragma unroll
               for (int e = 0; e < 2; ++e)
-                load_pair(sm.kv[b][x] + (2 * y + e) * SLAB + k * box_bytes, &P.pool, (4 * x + 2 * y + e) * 64, row, fb);
+                load_pair(sm.kv[b][x] + (2 * y + e) * SLAB + k * box_bytes, &P.pool, (4 * x + 2 * y + e) * 64, at, fb);
             }
-            ++issued;
           }
+          ++issued;
         }
-        if (!ok) {
-          set_abort(sm);
-          // what both CTAs have under way into the pair's tiles lands before the pair leaves
-          if (rank == 0) {
-            if (x == 0) bar_wait(&sm.q_full, ord & 1);
-            for (int e = max(0, issued - 4); e < issued; ++e)
-              bar_wait(&sm.kv_full[(e >> 1) & 1][2 * (e & 1) + x], (e >> 2) & 1);
-          }
+        row = next;
+      }
+      if (!ok) {
+        if (lane == 0) set_abort(sm);
+        // what both CTAs have under way into the pair's tiles lands before the pair leaves
+        if (rank == 0) {
+          if (x == 0) bar_wait(&sm.q_full, ord & 1);
+          for (int e = max(0, issued - 4); e < issued; ++e)
+            bar_wait(&sm.kv_full[(e >> 1) & 1][2 * (e & 1) + x], (e >> 2) & 1);
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok, leader);
-      g = __shfl_sync(0xffffffffu, g, leader);
-      issued = __shfl_sync(0xffffffffu, issued, leader);
       ++ord;
     }
-    if (x == 0 && ok && elect_one()) {
-      if (g > 0) ok = bar_wait_or_abort(&sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort);
+    if (x == 0 && ok && g > 0) ok = bar_wait_or_abort(&sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort);
+    if (x == 0 && lane == 0) {
       if (!ok) set_abort(sm);
       sm.unit_tiles[ord & 1] = -1;
-      bar_arrive(&sm.q_full);
+      if (ok) bar_arrive(&sm.q_full);
     }
   } else if (warp == 3) {
     // ---------------------------------------------------------------- the other half's rows as V
     bool ok = true;
     int g = 0;
-    Work w(P);
-    while (ok && w.next(P)) {
-      uint32_t leader;
-      if (elect_one(&leader)) {
-        for (int i = 0; i < w.nt; ++i, ++g) {
-          const int b = g & 1, h = 2 * (w.tile0 + i) + 1 - static_cast<int>(rank);
-          int row = h < w.u.nh ? half_row(P, w.u, h, 0) : static_cast<int>(P.c.pool_rows);
-          if (!(ok = bar_wait_or_abort(&sm.s_full[b], (g >> 1) & 1, abort))) break;
-          bar_expect_tx(&sm.v_full[b], SLOT);
-          uint8_t* slot = sm.kv[b][1 - rank];  // CTA 0: Y takes rows 64-127, CTA 1: X takes rows 0-63
-          for (int k = 0; k < boxes; ++k) {
-            if (k > 0) row = h < w.u.nh ? half_row(P, w.u, h, k) : static_cast<int>(P.c.pool_rows);
+    for (; ok && has; has = w.next(P)) {
+      if (w.nt == 0) continue;
+      int row = tile_row(P, w.u, 2 * w.tile0 + 1 - static_cast<int>(rank), lane, boxes);
+      for (int i = 0; i < w.nt; ++i, ++g) {
+        const int b = g & 1;
+        const int next = i + 1 < w.nt ? tile_row(P, w.u, 2 * (w.tile0 + i + 1) + 1 - static_cast<int>(rank), lane, boxes) : 0;
+        if (!(ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.s_full[b], (g >> 1) & 1, abort)))) break;
+        uint8_t* slot = sm.kv[b][1 - rank];  // CTA 0: Y takes rows 64-127, CTA 1: X takes rows 0-63
+        const bool one = elect_one();
+        if (one) bar_expect_tx(&sm.v_full[b], SLOT);
+        for (int k = 0; k < boxes; ++k) {
+          const int at = __shfl_sync(0xffffffffu, row, k);
+          if (one) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              tma_load_2d(slot + e * SLAB + k * box_bytes, &P.pool, (4 * static_cast<int>(rank) + e) * 64, row, &sm.v_full[b]);
+              tma_load_2d(slot + e * SLAB + k * box_bytes, &P.pool, (4 * static_cast<int>(rank) + e) * 64, at, &sm.v_full[b]);
           }
         }
-        if (!ok) {
-          set_abort(sm);
-          for (int e = max(0, g - 2); e < g; ++e) bar_wait(&sm.v_full[e & 1], (e >> 1) & 1);
-        }
+        row = next;
       }
-      ok = __shfl_sync(0xffffffffu, ok, leader);
-      g = __shfl_sync(0xffffffffu, g, leader);
+      if (!ok) {
+        if (lane == 0) set_abort(sm);
+        for (int e = max(0, g - 2); e < g; ++e) bar_wait(&sm.v_full[e & 1], (e >> 1) & 1);
+      }
     }
   } else if (warp == 0) {
     // ---------------------------------------------------------------- S (CTA 0, one thread)
@@ -472,8 +485,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       const uint64_t pd = sdesc(smem_u32(sm.p), 16, 1024), vd = sdesc(smem_u32(sm.kv), SLAB, 1024);
       bool ok = true;
       int g = 0, ord = 0;
-      Work w(P);
-      while (ok && w.next(P)) {
+      for (; ok && has; has = w.next(P)) {
         if (w.nt == 0) continue;
         uint32_t leader;
         if (elect_one(&leader)) {
@@ -512,8 +524,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     const float sink = P.sink[head] * LOG2E;
     bool ok = true;
     int g = 0;
-    Work w(P);
-    for (bool has = w.next(P); has;) {
+    while (has) {
       const Unit& u = w.u;
       const bool mine = static_cast<int>(rank) < u.n;  // this CTA has a token
       const int64_t token = u.t0 + rank;
@@ -644,36 +655,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       after_sync();
       const uint32_t src = tmem + lanes + COL_O + 128 * ch;
       const int d0 = 256 * kvh + 128 * ch, group = 2 * kvh + ch;
+      // Rows leave by way of P's space, which is out of use until the next unit's first P: 64 rows by 128 bytes
+      // of two warps at a time, 128-byte swizzled, to the tensor by TMA (16 bytes a lane straight from the
+      // registers took 5700 cycles a unit, 10000 for the fp32 partials).
+      uint8_t* const tile = sm.p[0] + group * SLAB;
+      const bool storer = (quad & 1) == 0 && lane == 0;
       if (P.splits > 1) {
-        if (ok && mine) {
-          const int64_t at = (token * P.splits + split) * HB + head;
-          float* po = P.part + at * D + d0;
+        const int64_t at = (token * P.splits + split) * HB;
 #pragma unroll 1
-          for (int c = 0; c < 128; c += 32) {
-            float v[32];
-            tmem_ld16(src + c, v);
-            tmem_ld16(src + c + 16, v + 16);
-            tmem_wait_ld();
+        for (int c = 0; c < 128; c += 32) {
+          float v[32];
+          tmem_ld16(src + c, v);
+          tmem_ld16(src + c + 16, v + 16);
+          tmem_wait_ld();
+          if (c > 0) {  // the columns before have left the space
+            if (storer) stores_read();
+            column_bar(group);
+          }
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              reinterpret_cast<float4*>(po + c)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-          }
-          if (group == 0) {
-            float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + at * 2;
-            ml[0] = m;
-            ml[1] = l;
-          }
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(tile + head * 128 + ((e ^ (head & 7)) << 4)) =
+                make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          fence_async_smem();
+          column_bar(group);
+          if (storer && ok && mine) store_tile(&P.o, d0 + c, static_cast<int>(at), tile);
         }
+        if (ok && mine && group == 0) {
+          float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + (at + head) * 2;
+          ml[0] = m;
+          ml[1] = l;
+        }
+        if (storer) stores_read();
       } else {
         const float inv = 1.f / (l + exp2f(sink - m));
         const int64_t off = (token * HB + head) * D + d0;
         float rc = 1.f, rs = 0.f;  // lane f: the rotation of pair f
         if (P.freqs != nullptr && d0 + 128 > D - P.rope_dim && lane < P.rope_dim / 2)
           rope_cos_sin(pos, P.freqs[lane], &rc, &rs);
-        // bf16: by way of P's space, which is out of use until the next unit's first P: 64 rows by 64 dims
-        // of two warps at a time, 128-byte swizzled, to the tensor by TMA (rows of 16 bytes a lane straight
-        // from the registers took 5700 cycles a unit)
-        uint8_t* const tile = sm.p[0] + group * SLAB;
         const bool store = mine && P.out_dtype == DSV4_BF16;
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
@@ -693,7 +711,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
           }
           if (P.out_dtype == DSV4_BF16) {
             if (c == 64) {  // the first 64 dims have left the space
-              if (store && (quad & 1) == 0 && lane == 0) stores_read();
+              if (storer) stores_read();
               column_bar(group);
             }
 #pragma unroll
@@ -704,7 +722,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
             if (c & 32) {
               fence_async_smem();
               column_bar(group);
-              if (store && ok && (quad & 1) == 0 && lane == 0)
+              if (store && ok && storer)
                 store_tile(&P.o, d0 + c - 32, static_cast<int>(token) * HB, tile);
             }
           } else if (ok && mine) {
@@ -713,7 +731,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
             for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
           }
         }
-        if (store && (quad & 1) == 0 && lane == 0) stores_read();
+        if (storer) stores_read();
       }
       if (!ok && lane == 0) set_abort(sm);
       // O has been read: the next unit's may be begun
@@ -738,14 +756,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
 }
 
 // One CTA per (token, head): the splits' partials weighed by 2^(m - max), the sink, the inverse
-// rotation. At most 64 splits.
-__global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ Params P) {
+// rotation. At most 64 splits; four groups of 128 threads take every fourth of them, all loads of a
+// group in flight together, so that a single token's 64 CTAs still draw on the whole L2.
+constexpr int MERGE = 4;
+__global__ void __launch_bounds__(128 * MERGE) chunk_merge_kernel(const __grid_constant__ Params P) {
+  pdl_wait();
   const int64_t t = blockIdx.x >> 6;
   const int head = blockIdx.x & 63;
   const ChunkToken k = chunk_token(P.c, static_cast<int>(t));
   if (k.seq < 0) return;
   __shared__ float w[64];
   __shared__ float inv;
+  __shared__ float4 sum[MERGE][128];
   const float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D);
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
@@ -753,9 +775,10 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int s = lane + 32 * e;
-      const int64_t at = ((t * P.splits + s) * HB + head) * 2;
-      m[e] = s < P.splits ? ml[at] : -INFINITY;
-      l[e] = s < P.splits ? ml[at + 1] : 0.f;
+      const float2 v = s < P.splits ? *reinterpret_cast<const float2*>(ml + ((t * P.splits + s) * HB + head) * 2)
+                                    : make_float2(-INFINITY, 0.f);
+      m[e] = v.x;
+      l[e] = v.y;
     }
     const float M = warp_max(fmaxf(m[0], m[1]));
     float L = 0.f;
@@ -769,22 +792,32 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
     if (lane == 0) inv = 1.f / (L + exp2f(P.sink[head] * LOG2E - M));
   }
   __syncthreads();
-  const int d = threadIdx.x * 4;
-  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  const int part = threadIdx.x >> 7, d = (threadIdx.x & 127) * 4;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   const float* src = P.part + (t * P.splits * HB + head) * D + d;
 #pragma unroll 4
-  for (int s = 0; s < P.splits; ++s) {
+  for (int s = part; s < P.splits; s += MERGE) {
     const float x = w[s];
     if (x != 0.f) {  // a split without rows has written no O
       const float4 v = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (HB * D));
-      o[0] = fmaf(x, v.x, o[0]);
-      o[1] = fmaf(x, v.y, o[1]);
-      o[2] = fmaf(x, v.z, o[2]);
-      o[3] = fmaf(x, v.w, o[3]);
+      o.x = fmaf(x, v.x, o.x);
+      o.y = fmaf(x, v.y, o.y);
+      o.z = fmaf(x, v.z, o.z);
+      o.w = fmaf(x, v.w, o.w);
     }
   }
+  sum[part][threadIdx.x & 127] = o;
+  __syncthreads();
+  if (part != 0) return;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] *= inv;
+  for (int e = 1; e < MERGE; ++e) {
+    const float4 v = sum[e][threadIdx.x];
+    o.x += v.x;
+    o.y += v.y;
+    o.z += v.z;
+    o.w += v.w;
+  }
+  float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
   if (P.freqs != nullptr) {
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
@@ -792,21 +825,21 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
       if (f >= 0) {
         float c, s;
         rope_cos_sin(k.pos, P.freqs[f], &c, &s);
-        rotate_pair(o[e], o[e + 1], c, s, true, &o[e], &o[e + 1]);
+        rotate_pair(y[e], y[e + 1], c, s, true, &y[e], &y[e + 1]);
       }
     }
   }
   const int64_t off = (t * HB + head) * D + d;
   if (P.out_dtype == DSV4_BF16)
     *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + off) =
-        make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+        make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
   else
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + off) = make_float4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + off) = make_float4(y[0], y[1], y[2], y[3]);
 }
 
 DSV4_ERROR_READER(chunk_attn)
 
-static int encode(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows) {
+static int encode(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows, bool fp32 = false) {
   static std::atomic<void*> fn{nullptr};
   void* f = fn.load(std::memory_order_acquire);
   if (!f) {
@@ -819,11 +852,11 @@ static int encode(CUtensorMap* map, const void* base, uint64_t rows, uint32_t bo
     fn.store(f, std::memory_order_release);
   }
   const cuuint64_t dims[2] = {D, rows};
-  const cuuint64_t strides[1] = {D * 2};
-  const cuuint32_t box[2] = {64, box_rows};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(fp32 ? D * 4 : D * 2)};
+  const cuuint32_t box[2] = {fp32 ? 32u : 64u, box_rows};  // 128 bytes of a row
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f)(
-      map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+      map, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
@@ -837,7 +870,7 @@ static int encode(CUtensorMap* map, const void* base, uint64_t rows, uint32_t bo
 // clusters of one wave shared out over the pairs of tokens, two tiles a split at least
 static int plan_splits(const dsv4_chunk_attn_params* p) {
   const int64_t units = (static_cast<int64_t>(p->chunk.total) + p->chunk.n) / 2;
-  const int tiles = p->chunk.max_comp / BN + 1;
+  const int tiles = (p->chunk.max_comp + 2 * p->chunk.window) / BN + 1;  // at most
   int want = p->num_splits;
   if (want <= 0) {
     want = static_cast<int>(std::max<int64_t>(1, num_sms() / 2 / std::max<int64_t>(1, units)));
@@ -891,10 +924,11 @@ int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
   if (st != DSV4_OK) return st;
   st = ca::encode(&P.q, p->q, static_cast<uint64_t>(p->chunk.total) * ca::HB, 64);
   if (st != DSV4_OK) return st;
-  if (p->out_dtype == DSV4_BF16) {
+  if (P.splits > 1)
+    st = ca::encode(&P.o, p->workspace, static_cast<uint64_t>(p->chunk.total) * P.splits * ca::HB, 64, true);
+  else if (p->out_dtype == DSV4_BF16)
     st = ca::encode(&P.o, p->out, static_cast<uint64_t>(p->chunk.total) * ca::HB, 64);
-    if (st != DSV4_OK) return st;
-  }
+  if (st != DSV4_OK) return st;
   P.c = p->chunk;
   P.sink = p->sink;
   P.out = p->out;
@@ -905,16 +939,15 @@ int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
   P.scale_log2 = p->scale * ca::LOG2E;
   // one cluster per pair of SMs, or per unit where there are fewer
   const int64_t units = (static_cast<int64_t>(P.c.total) + P.c.n) / 2 * P.splits;
-  DSV4_CHECK_ARG(units <= 0x3fffffffLL, "dsv4_chunk_attn: too many tokens");
+  DSV4_CHECK_ARG(static_cast<int64_t>(P.c.total) * P.splits * ca::HB <= 0x7fffffffLL, "dsv4_chunk_attn: too many tokens");
   static PerDeviceOnce attr;
   const int smem = static_cast<int>(sizeof(ca::Smem)) + 1024;
   DSV4_CUDA_CHECK(set_smem_once(attr, ca::chunk_attn_kernel, smem));
-  ca::chunk_attn_kernel<<<static_cast<unsigned>(2 * std::min<int64_t>(units, num_sms() / 2)), ca::THREADS, smem, as_stream(stream)>>>(P);
-  DSV4_LAUNCH_CHECK("chunk_attn_kernel");
-  if (P.splits > 1) {
-    ca::chunk_merge_kernel<<<static_cast<unsigned>(P.c.total) * 64, 128, 0, as_stream(stream)>>>(P);
-    DSV4_LAUNCH_CHECK("chunk_merge_kernel");
-  }
+  DSV4_CUDA_CHECK(launch_pdl(ca::chunk_attn_kernel, dim3(static_cast<unsigned>(2 * std::min<int64_t>(units, num_sms() / 2))),
+                             dim3(ca::THREADS), smem, as_stream(stream), P));
+  if (P.splits > 1)
+    DSV4_CUDA_CHECK(launch_pdl(ca::chunk_merge_kernel, dim3(static_cast<unsigned>(P.c.total) * 64), dim3(128 * ca::MERGE), 0,
+                               as_stream(stream), P));
   return DSV4_OK;
 }
 
