@@ -76,11 +76,11 @@ static_assert(sizeof(Smem) + 1024 <= 232448, "shared memory above the 227 KB a C
 struct Params {
   CUtensorMap pool;  // [pool_rows, 512] bf16, box 64 dims x box_rows
   CUtensorMap q;     // [total * 64, 512] bf16, box 64 dims x 64 rows
-  CUtensorMap o;     // out, if bf16: as q; the partials [total * splits * 64, 512] fp32 if split, box 32 dims x 64 rows
+  CUtensorMap o;     // out, if bf16 and not split: as q
   dsv4_chunk c;
   const float* sink;
   void* out;
-  float* part;       // splits > 1: O [total][splits][64][512], then (m, l) [total][splits][64][2]
+  float* part;       // splits > 1: O [total][splits][512 dims][64 heads], then (m, l) [total][splits][64][2]
   const float* freqs;
   int rope_dim, out_dtype, splits, box_rows;
   float scale_log2;
@@ -342,7 +342,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     tma_prefetch_map(&P.q);
   }
   pdl_wait();  // what follows reads memory that the kernels before may have written
-  pdl_trigger();
   Work w(P);
   bool has = w.next(P);
   before_sync();
@@ -655,40 +654,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       after_sync();
       const uint32_t src = tmem + lanes + COL_O + 128 * ch;
       const int d0 = 256 * kvh + 128 * ch, group = 2 * kvh + ch;
-      // Rows leave by way of P's space, which is out of use until the next unit's first P: 64 rows by 128 bytes
-      // of two warps at a time, 128-byte swizzled, to the tensor by TMA (16 bytes a lane straight from the
-      // registers took 5700 cycles a unit, 10000 for the fp32 partials).
-      uint8_t* const tile = sm.p[0] + group * SLAB;
-      const bool storer = (quad & 1) == 0 && lane == 0;
       if (P.splits > 1) {
-        const int64_t at = (token * P.splits + split) * HB;
+        // partials with the heads innermost: a warp stores a dim of 32 heads at a time
+        if (ok && mine) {
+          const int64_t at = token * P.splits + split;
+          float* po = P.part + (at * D + d0) * HB + head;
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          float v[32];
-          tmem_ld16(src + c, v);
-          tmem_ld16(src + c + 16, v + 16);
-          tmem_wait_ld();
-          if (c > 0) {  // the columns before have left the space
-            if (storer) stores_read();
-            column_bar(group);
-          }
+          for (int c = 0; c < 128; c += 32) {
+            float v[32];
+            tmem_ld16(src + c, v);
+            tmem_ld16(src + c + 16, v + 16);
+            tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<float4*>(tile + head * 128 + ((e ^ (head & 7)) << 4)) =
-                make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-          fence_async_smem();
-          column_bar(group);
-          if (storer && ok && mine) store_tile(&P.o, d0 + c, static_cast<int>(at), tile);
+            for (int e = 0; e < 32; ++e) po[(c + e) * HB] = v[e];
+          }
+          if (group == 0)
+            *reinterpret_cast<float2*>(P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + (at * HB + head) * 2) =
+                make_float2(m, l);
         }
-        if (ok && mine && group == 0) {
-          float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + (at + head) * 2;
-          ml[0] = m;
-          ml[1] = l;
-        }
-        if (storer) stores_read();
       } else {
         const float inv = 1.f / (l + exp2f(sink - m));
         const int64_t off = (token * HB + head) * D + d0;
+        // Rows leave by way of P's space, which is out of use until the next unit's first P: 64 rows by 64 dims
+        // of two warps at a time, 128-byte swizzled, to the tensor by TMA (16 bytes a lane straight from the
+        // registers took 5700 cycles a unit).
+        uint8_t* const tile = sm.p[0] + group * SLAB;
+        const bool storer = (quad & 1) == 0 && lane == 0;
         float rc = 1.f, rs = 0.f;  // lane f: the rotation of pair f
         if (P.freqs != nullptr && d0 + 128 > D - P.rope_dim && lane < P.rope_dim / 2)
           rope_cos_sin(pos, P.freqs[lane], &rc, &rs);
@@ -749,97 +740,115 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
   __syncwarp();
   before_sync();
   __syncthreads();
+  // (not earlier: the merging kernel's blocks would all be placed on the few SMs without a cluster)
+  pdl_trigger();
   cluster_sync();  // no CTA leaves while the pair's MMAs, loads or arrivals may touch it
   after_sync();
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(TMEM_COLS));
 }
 
-// One CTA per (token, head): the splits' partials weighed by 2^(m - max), the sink, the inverse
-// rotation. At most 64 splits; four groups of 128 threads take every fourth of them, all loads of a
-// group in flight together, so that a single token's 64 CTAs still draw on the whole L2.
-constexpr int MERGE = 4;
-__global__ void __launch_bounds__(128 * MERGE) chunk_merge_kernel(const __grid_constant__ Params P) {
+// One CTA per (token, MD dims): the splits' partials weighed by 2^(m - max), the sink, the inverse
+// rotation. At most 64 splits. A split's dims of 64 heads lie in a row, a float4 (four heads of a dim) per
+// thread of a group; MG groups take every MG-th split. <8, 4> for many splits, that is few tokens, so that
+// the 64 CTAs of a single token have enough loads in flight; <16, 1> otherwise, a quarter of the threads
+// (32 tokens in 3 splits: 21 us with the attention, against 33 us). The sum turns round in shared memory,
+// so that a head's dims leave together.
+template <int MD, int MG>
+__global__ void __launch_bounds__(MG * MD * HB / 4) chunk_merge_kernel(const __grid_constant__ Params P) {
+  constexpr int MT = MG * MD * HB / 4, MH = MT / HB, MS = 64 / MH;  // threads; per head; splits a thread weighs
   pdl_wait();
-  const int64_t t = blockIdx.x >> 6;
-  const int head = blockIdx.x & 63;
+  constexpr int BLOCKS = D / MD;
+  const int64_t t = blockIdx.x / BLOCKS;
+  const int d0 = static_cast<int>(blockIdx.x % BLOCKS) * MD;
   const ChunkToken k = chunk_token(P.c, static_cast<int>(t));
   if (k.seq < 0) return;
-  __shared__ float w[64];
-  __shared__ float inv;
-  __shared__ float4 sum[MERGE][128];
-  const float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D);
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    float m[2], l[2];
+  __shared__ float w[64][HB];   // [split][head]
+  __shared__ float red[2][MH][HB];
+  __shared__ float o[MG][MD][HB];
+  const int tid = threadIdx.x;
+  {
+    const int h = tid & (HB - 1), g = tid / HB;
+    const float2* ml = reinterpret_cast<const float2*>(P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D)) +
+                       t * P.splits * HB + h;
+    float2 v[MS];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int s = lane + 32 * e;
-      const float2 v = s < P.splits ? *reinterpret_cast<const float2*>(ml + ((t * P.splits + s) * HB + head) * 2)
-                                    : make_float2(-INFINITY, 0.f);
-      m[e] = v.x;
-      l[e] = v.y;
+    for (int i = 0; i < MS; ++i) {
+      const int s = g + i * MH;
+      v[i] = s < P.splits ? ml[s * HB] : make_float2(-INFINITY, 0.f);
     }
-    const float M = warp_max(fmaxf(m[0], m[1]));
+    float M = v[0].x;
+#pragma unroll
+    for (int i = 1; i < MS; ++i) M = fmaxf(M, v[i].x);
+    red[0][g][h] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MH; ++i) M = fmaxf(M, red[0][i][h]);
     float L = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float x = m[e] == -INFINITY ? 0.f : exp2f(m[e] - M);
-      w[lane + 32 * e] = x;
-      L += x * l[e];
+    for (int i = 0; i < MS; ++i) {
+      const int s = g + i * MH;
+      const float x = v[i].x == -INFINITY ? 0.f : exp2f(v[i].x - M);
+      if (s < P.splits) w[s][h] = x;
+      L = fmaf(x, v[i].y, L);
     }
-    L = warp_sum(L);
-    if (lane == 0) inv = 1.f / (L + exp2f(P.sink[head] * LOG2E - M));
+    red[1][g][h] = L;
+    __syncthreads();
+    if (g == 0) {
+      L = 0.f;
+#pragma unroll
+      for (int i = 0; i < MH; ++i) L += red[1][i][h];
+      red[0][0][h] = 1.f / (L + exp2f(P.sink[h] * LOG2E - M));
+    }
   }
-  __syncthreads();
-  const int part = threadIdx.x >> 7, d = (threadIdx.x & 127) * 4;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float* src = P.part + (t * P.splits * HB + head) * D + d;
+  {
+    const int g = tid / (MD * HB / 4), e = tid / (HB / 4) % MD, h = tid % (HB / 4) * 4;  // dim d0 + e, heads h .. h + 3
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* src = P.part + (t * P.splits * D + d0 + e) * HB + h;
 #pragma unroll 4
-  for (int s = part; s < P.splits; s += MERGE) {
-    const float x = w[s];
-    if (x != 0.f) {  // a split without rows has written no O
-      const float4 v = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (HB * D));
-      o.x = fmaf(x, v.x, o.x);
-      o.y = fmaf(x, v.y, o.y);
-      o.z = fmaf(x, v.z, o.z);
-      o.w = fmaf(x, v.w, o.w);
-    }
-  }
-  sum[part][threadIdx.x & 127] = o;
-  __syncthreads();
-  if (part != 0) return;
-#pragma unroll
-  for (int e = 1; e < MERGE; ++e) {
-    const float4 v = sum[e][threadIdx.x];
-    o.x += v.x;
-    o.y += v.y;
-    o.z += v.z;
-    o.w += v.w;
-  }
-  float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-  if (P.freqs != nullptr) {
-#pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-      const int f = (d + e - (D - P.rope_dim)) >> 1;
-      if (f >= 0) {
-        float c, s;
-        rope_cos_sin(k.pos, P.freqs[f], &c, &s);
-        rotate_pair(y[e], y[e + 1], c, s, true, &y[e], &y[e + 1]);
+    for (int s = g; s < P.splits; s += MG) {
+      const float4 x = *reinterpret_cast<const float4*>(&w[s][h]);
+      // a split without rows has written no O, and its weight is 0 for every head
+      if (x.x != 0.f || x.y != 0.f || x.z != 0.f || x.w != 0.f) {
+        const float4 v = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (HB * D));
+        a.x = fmaf(x.x, v.x, a.x);
+        a.y = fmaf(x.y, v.y, a.y);
+        a.z = fmaf(x.z, v.z, a.z);
+        a.w = fmaf(x.w, v.w, a.w);
       }
     }
+    *reinterpret_cast<float4*>(&o[g][e][h]) = a;
   }
-  const int64_t off = (t * HB + head) * D + d;
-  if (P.out_dtype == DSV4_BF16)
-    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + off) =
-        make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
-  else
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + off) = make_float4(y[0], y[1], y[2], y[3]);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MD * HB / 2; i += MT) {  // a pair of dims of a head
+    if (i + tid >= MD * HB / 2) break;
+    const int head = (i + tid) / (MD / 2), e = (i + tid) % (MD / 2) * 2;
+    float y = 0.f, z = 0.f;
+#pragma unroll
+    for (int g = 0; g < MG; ++g) {
+      y += o[g][e][head];
+      z += o[g][e + 1][head];
+    }
+    y *= red[0][0][head];
+    z *= red[0][0][head];
+    const int f = (d0 + e - (D - P.rope_dim)) >> 1;
+    if (P.freqs != nullptr && f >= 0) {
+      float c, s;
+      rope_cos_sin(k.pos, P.freqs[f], &c, &s);
+      rotate_pair(y, z, c, s, true, &y, &z);
+    }
+    const int64_t off = (t * HB + head) * D + d0 + e;
+    if (P.out_dtype == DSV4_BF16)
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<__nv_bfloat16*>(P.out) + off) = pack_bf16x2(y, z);
+    else
+      *reinterpret_cast<float2*>(reinterpret_cast<float*>(P.out) + off) = make_float2(y, z);
+  }
 }
 
 DSV4_ERROR_READER(chunk_attn)
 
-static int encode(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows, bool fp32 = false) {
+static int encode(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows) {
   static std::atomic<void*> fn{nullptr};
   void* f = fn.load(std::memory_order_acquire);
   if (!f) {
@@ -852,11 +861,11 @@ static int encode(CUtensorMap* map, const void* base, uint64_t rows, uint32_t bo
     fn.store(f, std::memory_order_release);
   }
   const cuuint64_t dims[2] = {D, rows};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(fp32 ? D * 4 : D * 2)};
-  const cuuint32_t box[2] = {fp32 ? 32u : 64u, box_rows};  // 128 bytes of a row
+  const cuuint64_t strides[1] = {D * 2};
+  const cuuint32_t box[2] = {64, box_rows};
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f)(
-      map, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+      map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
@@ -924,9 +933,7 @@ int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
   if (st != DSV4_OK) return st;
   st = ca::encode(&P.q, p->q, static_cast<uint64_t>(p->chunk.total) * ca::HB, 64);
   if (st != DSV4_OK) return st;
-  if (P.splits > 1)
-    st = ca::encode(&P.o, p->workspace, static_cast<uint64_t>(p->chunk.total) * P.splits * ca::HB, 64, true);
-  else if (p->out_dtype == DSV4_BF16)
+  if (P.splits == 1 && p->out_dtype == DSV4_BF16)
     st = ca::encode(&P.o, p->out, static_cast<uint64_t>(p->chunk.total) * ca::HB, 64);
   if (st != DSV4_OK) return st;
   P.c = p->chunk;
@@ -945,9 +952,12 @@ int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
   DSV4_CUDA_CHECK(set_smem_once(attr, ca::chunk_attn_kernel, smem));
   DSV4_CUDA_CHECK(launch_pdl(ca::chunk_attn_kernel, dim3(static_cast<unsigned>(2 * std::min<int64_t>(units, num_sms() / 2))),
                              dim3(ca::THREADS), smem, as_stream(stream), P));
-  if (P.splits > 1)
-    DSV4_CUDA_CHECK(launch_pdl(ca::chunk_merge_kernel, dim3(static_cast<unsigned>(P.c.total) * 64), dim3(128 * ca::MERGE), 0,
-                               as_stream(stream), P));
+  if (P.splits > 8)
+    DSV4_CUDA_CHECK(launch_pdl(ca::chunk_merge_kernel<8, 4>, dim3(static_cast<unsigned>(P.c.total) * (ca::D / 8)),
+                               dim3(4 * 8 * ca::HB / 4), 0, as_stream(stream), P));
+  else if (P.splits > 1)
+    DSV4_CUDA_CHECK(launch_pdl(ca::chunk_merge_kernel<16, 1>, dim3(static_cast<unsigned>(P.c.total) * (ca::D / 16)),
+                               dim3(16 * ca::HB / 4), 0, as_stream(stream), P));
   return DSV4_OK;
 }
 
