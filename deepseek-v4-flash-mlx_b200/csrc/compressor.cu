@@ -13,6 +13,7 @@
 
 #include "common.cuh"
 #include "key_image.cuh"
+#include "tcgen05.cuh"
 
 namespace dsv4 {
 namespace cmp {
@@ -506,6 +507,39 @@ struct ChunkSeq {
   int first, n, start, slot;  // first token, tokens, position of the first, cache slot
 };
 
+// where entry g of a slot goes; -1 (and the error word) past the cache, without a page or outside of out
+__device__ __forceinline__ int64_t chunk_row(const dsv4_compressor_chunk_params& p, int slot, int g) {
+  int64_t row = -1;
+  if (g < p.max_comp) {
+    if (p.block_table == nullptr) {
+      row = p.out_base + static_cast<int64_t>(slot) * p.max_comp + g;
+    } else {
+      const int32_t pg = p.block_table[static_cast<int64_t>(slot) * p.bt_stride + g / p.page];
+      if (pg >= 0) row = p.out_base + static_cast<int64_t>(pg) * p.page + g % p.page;
+    }
+  }
+  if (row < 0 || row >= p.out_rows) {
+    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+    return -1;
+  }
+  return row;
+}
+// one column of a row: the softmax over its 2 R slots
+template <int R>
+__device__ __forceinline__ float chunk_pool(const float2 (&K)[2 * R], const float2 (&S)[2 * R], int e) {
+  float m = e ? S[0].y : S[0].x;
+#pragma unroll
+  for (int i = 1; i < 2 * R; ++i) m = fmaxf(m, e ? S[i].y : S[i].x);
+  float den = 0.f, num = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2 * R; ++i) {
+    const float ex = expf((e ? S[i].y : S[i].x) - m);
+    den += ex;
+    num = fmaf(ex, e ? K[i].y : K[i].x, num);
+  }
+  return num / den;
+}
+
 template <int R>
 __device__ __forceinline__ void chunk_emit(const dsv4_compressor_chunk_params& p, const ChunkSeq<R>& q, int g,
                                            float* red, float* xch) {
@@ -513,6 +547,7 @@ __device__ __forceinline__ void chunk_emit(const dsv4_compressor_chunk_params& p
   const float* rk = p.ring_kv + static_cast<int64_t>(q.slot) * 2 * R * d2;
   const float* rs = p.ring_score + static_cast<int64_t>(q.slot) * 2 * R * d2;
   const int block = q.start / R * R;  // the block the chunk begins in
+  const int64_t orow = chunk_row(p, q.slot, g);
   float vals[2][2];
   float ss = 0.f;
 #pragma unroll
@@ -537,38 +572,12 @@ __device__ __forceinline__ void chunk_emit(const dsv4_compressor_chunk_params& p
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float m = e ? S[0].y : S[0].x;
-#pragma unroll
-      for (int i = 1; i < 2 * R; ++i) m = fmaxf(m, e ? S[i].y : S[i].x);
-      float den = 0.f, num = 0.f;
-#pragma unroll
-      for (int i = 0; i < 2 * R; ++i) {
-        const float ex = expf((e ? S[i].y : S[i].x) - m);
-        den += ex;
-        num = fmaf(ex, e ? K[i].y : K[i].x, num);
-      }
-      vals[np][e] = num / den;
+      vals[np][e] = chunk_pool<R>(K, S, e);
       ss = fmaf(vals[np][e], vals[np][e], ss);
     }
   }
   ss = block_sum(ss, red);
   const float rinv = rsqrtf(ss / static_cast<float>(d) + p.eps);
-  int64_t orow = -1;
-  if (g >= p.max_comp) {
-    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-  } else if (p.block_table == nullptr) {
-    orow = p.out_base + static_cast<int64_t>(q.slot) * p.max_comp + g;
-  } else {
-    const int32_t pg = p.block_table[static_cast<int64_t>(q.slot) * p.bt_stride + g / p.page];
-    if (pg >= 0)
-      orow = p.out_base + static_cast<int64_t>(pg) * p.page + g % p.page;
-    else
-      raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-  }
-  if (orow >= p.out_rows) {
-    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-    orow = -1;
-  }
 #pragma unroll
   for (int np = 0; np < 2; ++np) {
     const int c = 2 * (threadIdx.x + np * THREADS);
@@ -598,6 +607,177 @@ __device__ __forceinline__ ChunkSeq<R> chunk_seq(const dsv4_compressor_chunk_par
     q.n = 0;
   }
   return q;
+}
+
+// the rows of sequence b that read its ring (at most two), then the ring
+template <int R>
+__device__ __forceinline__ void chunk_sequence(const dsv4_compressor_chunk_params& p, int b, float* red, float* xch) {
+  const ChunkSeq<R> q = chunk_seq<R>(p, b);
+  if (q.n <= 0) return;
+  const int end = q.start + q.n, g0 = q.start / R, g1 = end / R;
+  for (int g = g0; g < g1 && (g - 1) * R < q.start; ++g) chunk_emit<R>(p, q, g, red, xch);
+  // the ring after the chunk: rows [0, R) the last complete block, rows R + p % R the newest token
+  const int d2 = 2 * p.head_dim;
+  float* rk = p.ring_kv + static_cast<int64_t>(q.slot) * 2 * R * d2;
+  float* rs = p.ring_score + static_cast<int64_t>(q.slot) * 2 * R * d2;
+  for (int c = 2 * threadIdx.x; c < d2; c += 2 * blockDim.x) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int last = end - 1 - (end - 1 - i + R) % R;  // newest position with p % R == i
+      if (g1 > g0) {
+        const int pos = (g1 - 1) * R + i;
+        if (pos >= q.start) {
+          const int64_t off = static_cast<int64_t>(q.first + (pos - q.start)) * d2 + c;
+          const float2 s = ld2(p.score + off), a = ld2(p.ape + i * d2 + c);
+          st2(rk + i * d2 + c, ld2(p.kv + off));
+          st2(rs + i * d2 + c, make_float2(s.x + a.x, s.y + a.y));
+        } else {
+          st2(rk + i * d2 + c, ld2(rk + (R + i) * d2 + c));
+          st2(rs + i * d2 + c, ld2(rs + (R + i) * d2 + c));
+        }
+      }
+      if (last >= q.start) {
+        const int64_t off = static_cast<int64_t>(q.first + (last - q.start)) * d2 + c;
+        const float2 s = ld2(p.score + off), a = ld2(p.ape + i * d2 + c);
+        st2(rk + (R + i) * d2 + c, ld2(p.kv + off));
+        st2(rs + (R + i) * d2 + c, make_float2(s.x + a.x, s.y + a.y));
+      }
+    }
+  }
+}
+
+// The long-chunk form of the rows that need no ring (R = 4, head_dim a multiple of 64 up to 512): a CTA
+// takes up to `run` blocks of a sequence one after the other. A block's tokens are consecutive, so one bulk
+// copy each brings kv and score (16 KB each at 512 dims) into a ring of RUN_STAGES buffers, three blocks
+// ahead of the one that is computed and without a thread waiting for any address; every block is read once
+// and serves two rows, but for the one before a run (half of its columns again, 1 / run). Two CTAs an SM
+// keep 192 KB under way, which HBM needs; the row-at-a-time form above looks its row up, loads, sums and
+// stores in turn and reached 2.6 TB/s (16384 tokens in 53 us).
+constexpr int RUN_STAGES = 3;
+__global__ void __launch_bounds__(THREADS, 2) chunk_run_kernel(dsv4_compressor_chunk_params p, int run) {
+  constexpr int R = 4;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float red[33];
+  __shared__ float xch[128];
+  if (static_cast<int>(blockIdx.x) < p.n) {
+    pdl_wait();
+    pdl_trigger();
+    chunk_sequence<R>(p, blockIdx.x, red, xch);
+    return;
+  }
+  __shared__ uint64_t full[RUN_STAGES];
+  __shared__ int unit[3];  // sequence, first block of the run, blocks
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int d = p.head_dim, d2 = 2 * d;
+  const uint32_t half = static_cast<uint32_t>(R * d2 * 4), stage = 2 * half;  // bytes of a block's kv, of both
+  if (tid == 0) {
+    for (int i = 0; i < RUN_STAGES; ++i) tc5::bar_init(&full[i], 1);
+    tc5::bar_init_fence();
+  }
+  pdl_wait();
+  pdl_trigger();
+  if (tid < 32) {  // the run of this CTA, counted through the sequences
+    int before = 0, seq = -1;
+    for (int b0 = 0; b0 < p.n; b0 += 32) {
+      const int b = b0 + lane;
+      int gs = 0, ge = 0;
+      if (b < p.n) {
+        const int first = p.cu_seqlens[b], n = p.cu_seqlens[b + 1] - first, start = p.start[b];
+        const int slot = p.seqs ? p.seqs[b] : b;
+        // the blocks whose row needs no token of before the chunk (invalid sequences: reported elsewhere)
+        if (first >= 0 && n > 0 && first + n <= p.total && start >= 0 && slot >= 0 && slot < p.slots) {
+          gs = (start + R - 1) / R + 1;
+          ge = max(gs, (start + n) / R);
+        }
+      }
+      const int cnt = (ge - gs + run - 1) / run;
+      int s = cnt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += x;
+      }
+      const int at = before + s - cnt, want = static_cast<int>(blockIdx.x) - p.n;
+      if (want >= at && want < at + cnt) {
+        unit[0] = b;
+        unit[1] = gs + (want - at) * run;
+        unit[2] = min(run, ge - unit[1]);
+        seq = b;
+      }
+      if (__any_sync(0xffffffffu, seq >= 0)) break;
+      before += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (!__any_sync(0xffffffffu, seq >= 0) && lane == 0) unit[2] = 0;
+  }
+  __syncthreads();
+  const int nb = unit[2];
+  if (nb == 0) return;
+  const int b = unit[0], g0 = unit[1];
+  const int first = p.cu_seqlens[b], start = p.start[b], slot = p.seqs ? p.seqs[b] : b;
+  const float* kv = p.kv + static_cast<int64_t>(first + (g0 - 1) * R - start) * d2;  // block g0 - 1
+  const float* sc = p.score + static_cast<int64_t>(first + (g0 - 1) * R - start) * d2;
+  auto load = [&](int i) {  // block g0 - 1 + i
+    uint8_t* dst = smem + (i % RUN_STAGES) * stage;
+    tc5::bar_expect_tx(&full[i % RUN_STAGES], stage);
+    tc5::bulk_g2s(dst, kv + static_cast<int64_t>(i) * R * d2, half, &full[i % RUN_STAGES]);
+    tc5::bulk_g2s(dst + half, sc + static_cast<int64_t>(i) * R * d2, half, &full[i % RUN_STAGES]);
+  };
+  int issued = min(RUN_STAGES, nb + 1);
+  if (tid == 0)
+    for (int i = 0; i < issued; ++i) load(i);
+  const int c = 2 * tid;  // this thread's columns c, c + 1 and d + c, d + c + 1
+  const bool mine = c < d;
+  float2 A[2 * R];
+#pragma unroll
+  for (int i = 0; i < 2 * R; ++i)
+    A[i] = mine ? ld2(p.ape + (i % R) * d2 + c + (i < R ? 0 : d)) : make_float2(0.f, 0.f);
+  bool ok = tc5::bar_wait(&full[0], 0);
+  for (int i = 1; i <= nb; ++i) {
+    const int g = g0 - 1 + i;
+    const int64_t orow = chunk_row(p, slot, g);
+    ok = ok && tc5::bar_wait(&full[i % RUN_STAGES], (i / RUN_STAGES) & 1);
+    if (__syncthreads_or(!ok)) {
+      if (tid == 0) raise_device_error(DSV4_ERR_WAIT_TIMEOUT);
+      break;
+    }
+    float vals[1][2] = {{0.f, 0.f}};
+    float ss = 0.f;
+    if (mine) {
+      float2 K[2 * R], S[2 * R];
+#pragma unroll
+      for (int j = 0; j < 2 * R; ++j) {
+        const uint8_t* src = smem + ((j < R ? i - 1 : i) % RUN_STAGES) * stage +
+                             static_cast<uint32_t>((j % R) * d2 + c + (j < R ? 0 : d)) * 4;
+        K[j] = *reinterpret_cast<const float2*>(src);
+        const float2 s = *reinterpret_cast<const float2*>(src + half);
+        S[j] = make_float2(s.x + A[j].x, s.y + A[j].y);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        vals[0][e] = chunk_pool<R>(K, S, e);
+        ss = fmaf(vals[0][e], vals[0][e], ss);
+      }
+    }
+    ss = block_sum(ss, red);  // its barriers: block i - 1 has been read
+    if (issued <= nb) {
+      if (tid == 0) load(issued);
+      ++issued;
+    }
+    const float rinv = rsqrtf(ss / static_cast<float>(d) + p.eps);
+    if (mine)
+      finish_pair(vals[0][0], vals[0][1], c, d, p.rope_dim, p.norm_w, p.norm_dtype, rinv, p.freqs, R * g, p.out, orow,
+                  p.out_dtype, p.act_quant);
+    if (p.act_quant == 2) {  // head_dim 128: threads 0..63 hold the row (uniform over the CTA)
+      hadamard_fp4_128(vals[0][0], vals[0][1], xch);
+      if (tid < 64) store_pair(vals[0][0], vals[0][1], c, d, p.out, orow, p.out_dtype);
+    }
+    if (p.key_image && g < p.max_comp) {
+      append_key_row(vals[0][0], vals[0][1], d, p.key_image, p.key_inv, p.key_norm_max, p.max_comp, slot, g, red);
+      __syncthreads();  // red is free for the next row
+    }
+  }
+  if (!ok && tid == 0)  // what was asked for lands before the CTA leaves
+    for (int i = max(0, issued - RUN_STAGES); i < issued; ++i) tc5::bar_wait(&full[i % RUN_STAGES], (i / RUN_STAGES) & 1);
 }
 
 template <int R>
@@ -636,38 +816,7 @@ __global__ void __launch_bounds__(THREADS) chunk_kernel(dsv4_compressor_chunk_pa
     }
     return;
   }
-  const ChunkSeq<R> q = chunk_seq<R>(p, blockIdx.x);
-  if (q.n <= 0) return;
-  const int end = q.start + q.n, g0 = q.start / R, g1 = end / R;
-  for (int g = g0; g < g1 && (g - 1) * R < q.start; ++g) chunk_emit<R>(p, q, g, red, xch);
-  // the ring after the chunk: rows [0, R) the last complete block, rows R + p % R the newest token
-  const int d2 = 2 * p.head_dim;
-  float* rk = p.ring_kv + static_cast<int64_t>(q.slot) * 2 * R * d2;
-  float* rs = p.ring_score + static_cast<int64_t>(q.slot) * 2 * R * d2;
-  for (int c = 2 * threadIdx.x; c < d2; c += 2 * blockDim.x) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int last = end - 1 - (end - 1 - i + R) % R;  // newest position with p % R == i
-      if (g1 > g0) {
-        const int pos = (g1 - 1) * R + i;
-        if (pos >= q.start) {
-          const int64_t off = static_cast<int64_t>(q.first + (pos - q.start)) * d2 + c;
-          const float2 s = ld2(p.score + off), a = ld2(p.ape + i * d2 + c);
-          st2(rk + i * d2 + c, ld2(p.kv + off));
-          st2(rs + i * d2 + c, make_float2(s.x + a.x, s.y + a.y));
-        } else {
-          st2(rk + i * d2 + c, ld2(rk + (R + i) * d2 + c));
-          st2(rs + i * d2 + c, ld2(rs + (R + i) * d2 + c));
-        }
-      }
-      if (last >= q.start) {
-        const int64_t off = static_cast<int64_t>(q.first + (last - q.start)) * d2 + c;
-        const float2 s = ld2(p.score + off), a = ld2(p.ape + i * d2 + c);
-        st2(rk + (R + i) * d2 + c, ld2(p.kv + off));
-        st2(rs + (R + i) * d2 + c, make_float2(s.x + a.x, s.y + a.y));
-      }
-    }
-  }
+  chunk_sequence<R>(p, blockIdx.x, red, xch);
 }
 
 DSV4_ERROR_READER(compressor)
@@ -790,6 +939,21 @@ extern "C" int dsv4_compressor_chunk(const dsv4_compressor_chunk_params* p, void
                  "dsv4_compressor_chunk: a key image needs head_dim 128, fp32 out, inv, norm_max and a 16-byte aligned image");
   if (p->n == 0 || p->total == 0) return DSV4_OK;
   const int threads = std::min(cmp::THREADS, (p->head_dim / 2 + 31) / 32 * 32);
+  // Long chunks: runs of blocks, as many CTAs as keep 192 KB an SM under way (two at 512 dims), all resident at
+  // once. Below two blocks a run there is nothing to stream ahead; the bulk copies want 16-byte alignment.
+  int run = 0;
+  if (p->ratio == 4 && p->head_dim % 64 == 0 && p->head_dim <= 2 * cmp::THREADS) {
+    const int ctas = 2 * (2 * cmp::THREADS / p->head_dim) * num_sms() - 2 * p->n;
+    run = ctas > 0 ? (p->total / 4 + ctas - 1) / ctas : 0;
+  }
+  if (run >= 2 && ((reinterpret_cast<uintptr_t>(p->kv) | reinterpret_cast<uintptr_t>(p->score)) & 15) == 0) {
+    static PerDeviceOnce attr;
+    DSV4_CUDA_CHECK(set_smem_once(attr, cmp::chunk_run_kernel, cmp::RUN_STAGES * 4 * 2 * 2 * cmp::THREADS * 8));
+    // at most one run a sequence is not full
+    DSV4_CUDA_CHECK(launch_pdl(cmp::chunk_run_kernel, dim3(p->n + p->total / 4 / run + p->n), dim3(threads),
+                               cmp::RUN_STAGES * 4 * 2 * p->head_dim * 8, as_stream(stream), *p, run));
+    return DSV4_OK;
+  }
   const dim3 grid(p->n + (p->total + 3) / 4);
   void (*k)(dsv4_compressor_chunk_params) = nullptr;
   switch (p->ratio) {

@@ -326,6 +326,42 @@ def test_compressor_chunk_equals_the_steps(d, ratio, lens, start, quant):
         assert torch.equal(a, b), name
 
 
+@pytest.mark.parametrize("d,lens,start,quant", [(512, [5000, 3, 0, 40], [3, 8, 1, 5], 0), (512, [2600], [0], 1), (128, [9999, 777], [1, 30], 2),
+                                               (128, [12000], [4], 0), (64, [4, 20000], [2, 7], 0)])
+def test_compressor_chunk_long(d, lens, start, quant):
+    """Chunks long enough to be streamed, bit for bit the same as in pieces of at most 37 tokens, which are
+    not; padding behind the last sequence, several sequences, odd starts, a paged table and keys."""
+    pkg, _, L = _mods()
+    I = importlib.import_module(PKG + ".indexer")
+    g = torch.Generator(device="cuda").manual_seed(d)
+    f, page = _freqs().cuda(), 16
+    most = max((s + n) // 4 for n, s in zip(lens, start)) + 1
+    slots, per = len(lens), -(-most // page)
+    table = torch.randperm(slots * per, generator=torch.Generator().manual_seed(2)).to(torch.int32).view(slots, per).cuda()
+    total = sum(lens) + 9
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    kv, sc, ape, nw = rnd(total, 2 * d), rnd(total, 2 * d), rnd(4, 2 * d), 1 + 0.1 * rnd(d)
+    keys = d == 128
+    out = torch.zeros(slots * per * page if not keys else slots * most, d, device="cuda", dtype=torch.float32 if keys else torch.bfloat16)
+    state = [rnd(slots, 8, 2 * d), rnd(slots, 8, 2 * d), out, *(I.key_image_buffers(slots, most, "cuda") if keys else ())]
+    a, b = [t.clone() for t in state], [t.clone() for t in state]
+    kw = lambda st: dict(key_image=st[3:]) if keys else dict(block_table=table, page=page)  # noqa: E731
+    q = dict(act_quant=quant == 1, rotate=quant == 2, rope_head_dim=min(64, d) if d > 64 or not quant else 0)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pkg.compressor_chunk((kv, sc), i32(np.concatenate([[0], np.cumsum(lens)])), i32(start), ape, nw, a[0], a[1], a[2], most, head_dim=d,
+                         freqs=f, **kw(a), **q)
+    at = 0
+    for slot, (n, s) in enumerate(zip(lens, start)):
+        for o in range(0, n, 37):
+            m = min(37, n - o)
+            pkg.compressor_chunk((kv[at + o:at + o + m], sc[at + o:at + o + m]), i32([0, m]), i32([s + o]), ape, nw, b[0], b[1], b[2], most,
+                                 seqs=i32([slot]), head_dim=d, freqs=f, **kw(b), **q)
+        at += n
+    assert L.device_error() == 0
+    for name, x, y in zip(("ring_kv", "ring_score", "rows", "image", "inv", "norm_max"), a, b):
+        assert torch.equal(x, y), name
+
+
 def test_compressor_chunk_against_the_definition():
     """Rows in 64 bits: eight-slot softmax, norm and rotation. fp32 arithmetic: at most 40 roundings of
     2^-24 on values of the row's scale (each output is a normalised weighted mean; the norm divides by the
