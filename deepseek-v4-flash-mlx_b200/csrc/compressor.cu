@@ -507,17 +507,16 @@ struct ChunkSeq {
   int first, n, start, slot;  // first token, tokens, position of the first, cache slot
 };
 
+// the table's word on entry g of a slot (0 without a table), to be asked for well before chunk_row needs it
+__device__ __forceinline__ int32_t chunk_page(const dsv4_compressor_chunk_params& p, int slot, int g) {
+  return p.block_table != nullptr && g < p.max_comp ? p.block_table[static_cast<int64_t>(slot) * p.bt_stride + g / p.page] : 0;
+}
 // where entry g of a slot goes; -1 (and the error word) past the cache, without a page or outside of out
-__device__ __forceinline__ int64_t chunk_row(const dsv4_compressor_chunk_params& p, int slot, int g) {
+__device__ __forceinline__ int64_t chunk_row(const dsv4_compressor_chunk_params& p, int slot, int g, int32_t page) {
   int64_t row = -1;
-  if (g < p.max_comp) {
-    if (p.block_table == nullptr) {
-      row = p.out_base + static_cast<int64_t>(slot) * p.max_comp + g;
-    } else {
-      const int32_t pg = p.block_table[static_cast<int64_t>(slot) * p.bt_stride + g / p.page];
-      if (pg >= 0) row = p.out_base + static_cast<int64_t>(pg) * p.page + g % p.page;
-    }
-  }
+  if (g < p.max_comp && page >= 0)
+    row = p.out_base + (p.block_table == nullptr ? static_cast<int64_t>(slot) * p.max_comp + g
+                                                 : static_cast<int64_t>(page) * p.page + g % p.page);
   if (row < 0 || row >= p.out_rows) {
     raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
     return -1;
@@ -547,7 +546,7 @@ __device__ __forceinline__ void chunk_emit(const dsv4_compressor_chunk_params& p
   const float* rk = p.ring_kv + static_cast<int64_t>(q.slot) * 2 * R * d2;
   const float* rs = p.ring_score + static_cast<int64_t>(q.slot) * 2 * R * d2;
   const int block = q.start / R * R;  // the block the chunk begins in
-  const int64_t orow = chunk_row(p, q.slot, g);
+  const int32_t page = chunk_page(p, q.slot, g);
   float vals[2][2];
   float ss = 0.f;
 #pragma unroll
@@ -577,6 +576,7 @@ __device__ __forceinline__ void chunk_emit(const dsv4_compressor_chunk_params& p
     }
   }
   ss = block_sum(ss, red);
+  const int64_t orow = chunk_row(p, q.slot, g, page);
   const float rinv = rsqrtf(ss / static_cast<float>(d) + p.eps);
 #pragma unroll
   for (int np = 0; np < 2; ++np) {
@@ -610,6 +610,7 @@ __device__ __forceinline__ ChunkSeq<R> chunk_seq(const dsv4_compressor_chunk_par
 }
 
 // the rows of sequence b that read its ring (at most two), then the ring
+// (any number of threads that covers a row: those past it add nothing)
 template <int R>
 __device__ __forceinline__ void chunk_sequence(const dsv4_compressor_chunk_params& p, int b, float* red, float* xch) {
   const ChunkSeq<R> q = chunk_seq<R>(p, b);
@@ -647,17 +648,27 @@ __device__ __forceinline__ void chunk_sequence(const dsv4_compressor_chunk_param
 }
 
 // The long-chunk form of the rows that need no ring (R = 4, head_dim a multiple of 64 up to 512): a CTA
-// takes up to `run` blocks of a sequence one after the other. A block's tokens are consecutive, so one bulk
-// copy each brings kv and score (16 KB each at 512 dims) into a ring of RUN_STAGES buffers, three blocks
-// ahead of the one that is computed and without a thread waiting for any address; every block is read once
-// and serves two rows, but for the one before a run (half of its columns again, 1 / run). Two CTAs an SM
-// keep 192 KB under way, which HBM needs; the row-at-a-time form above looks its row up, loads, sums and
-// stores in turn and reached 2.6 TB/s (16384 tokens in 53 us).
-constexpr int RUN_STAGES = 3;
-__global__ void __launch_bounds__(THREADS, 2) chunk_run_kernel(dsv4_compressor_chunk_params p, int run) {
-  constexpr int R = 4;
+// takes up to `run` blocks of a sequence one after the other, G rows at a time, a group of threads each. A
+// block's tokens are consecutive, so one bulk copy each brings kv and score (16 KB each at 512 dims) into a
+// ring of 2 G + 1 buffers, G blocks ahead of those that are computed and without a thread waiting for any
+// address; every block is read once and serves two rows, but for the one before a run (half of its columns
+// again, 1 / run). The arithmetic (about 500 instructions a warp and row: 16 exponentials and 2 divisions
+// a thread, as the decode step has them) is as long as the reads, so as many warps as registers allow run
+// at once: 512 dims with G = 3 (24 warps, 224 KB) in one CTA an SM. The row-at-a-time form above looks its
+// row up, loads, sums and stores in turn: 53 us for 16384 tokens; two CTAs of G = 1 took 33 us.
+template <int D, int G>  // D: head_dim where it is known (addresses fold into the loads), 0: any
+struct Run {
+  static constexpr int STAGES = 2 * G + 1;
+};
+template <int D, int G>
+__global__ void __launch_bounds__(G == 1 ? THREADS : G * D / 2, G == 1 ? 2 : 1)
+    chunk_run_kernel(dsv4_compressor_chunk_params p, int run) {
+  constexpr int R = 4, STAGES = Run<D, G>::STAGES;
+  static_assert(G == 1 || D == 2 * THREADS, "groups of THREADS");
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red[33];
+  __shared__ float sums[G][THREADS / 32];
+  __shared__ int64_t where[G];
   __shared__ float xch[128];
   if (static_cast<int>(blockIdx.x) < p.n) {
     pdl_wait();
@@ -665,20 +676,22 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_run_kernel(dsv4_compressor_c
     chunk_sequence<R>(p, blockIdx.x, red, xch);
     return;
   }
-  __shared__ uint64_t full[RUN_STAGES];
+  __shared__ uint64_t full[STAGES];
   __shared__ int unit[3];  // sequence, first block of the run, blocks
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int d = p.head_dim, d2 = 2 * d;
+  const int lane = threadIdx.x & 31, group = G == 1 ? 0 : threadIdx.x / THREADS;
+  const int tid = G == 1 ? threadIdx.x : threadIdx.x % THREADS;  // in the group
+  const int d = D ? D : p.head_dim, d2 = 2 * d;
   const uint32_t half = static_cast<uint32_t>(R * d2 * 4), stage = 2 * half;  // bytes of a block's kv, of both
-  if (tid == 0) {
-    for (int i = 0; i < RUN_STAGES; ++i) tc5::bar_init(&full[i], 1);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) tc5::bar_init(&full[i], 1);
     tc5::bar_init_fence();
   }
   pdl_wait();
   pdl_trigger();
-  if (tid < 32) {  // the run of this CTA, counted through the sequences
-    int before = 0, seq = -1;
-    for (int b0 = 0; b0 < p.n; b0 += 32) {
+  if (threadIdx.x < 32) {  // the run of this CTA, counted through the sequences
+    int before = 0;
+    bool found = false;
+    for (int b0 = 0; b0 < p.n && !found; b0 += 32) {
       const int b = b0 + lane;
       int gs = 0, ge = 0;
       if (b < p.n) {
@@ -698,16 +711,16 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_run_kernel(dsv4_compressor_c
         if (lane >= o) s += x;
       }
       const int at = before + s - cnt, want = static_cast<int>(blockIdx.x) - p.n;
-      if (want >= at && want < at + cnt) {
+      const bool hit = want >= at && want < at + cnt;
+      if (hit) {
         unit[0] = b;
         unit[1] = gs + (want - at) * run;
         unit[2] = min(run, ge - unit[1]);
-        seq = b;
       }
-      if (__any_sync(0xffffffffu, seq >= 0)) break;
+      found = __any_sync(0xffffffffu, hit);
       before += __shfl_sync(0xffffffffu, s, 31);
     }
-    if (!__any_sync(0xffffffffu, seq >= 0) && lane == 0) unit[2] = 0;
+    if (!found && lane == 0) unit[2] = 0;
   }
   __syncthreads();
   const int nb = unit[2];
@@ -716,68 +729,92 @@ __global__ void __launch_bounds__(THREADS, 2) chunk_run_kernel(dsv4_compressor_c
   const int first = p.cu_seqlens[b], start = p.start[b], slot = p.seqs ? p.seqs[b] : b;
   const float* kv = p.kv + static_cast<int64_t>(first + (g0 - 1) * R - start) * d2;  // block g0 - 1
   const float* sc = p.score + static_cast<int64_t>(first + (g0 - 1) * R - start) * d2;
-  auto load = [&](int i) {  // block g0 - 1 + i
-    uint8_t* dst = smem + (i % RUN_STAGES) * stage;
-    tc5::bar_expect_tx(&full[i % RUN_STAGES], stage);
-    tc5::bulk_g2s(dst, kv + static_cast<int64_t>(i) * R * d2, half, &full[i % RUN_STAGES]);
-    tc5::bulk_g2s(dst + half, sc + static_cast<int64_t>(i) * R * d2, half, &full[i % RUN_STAGES]);
+  int issued = 0;
+  auto load_to = [&](int end) {  // blocks g0 - 1 + issued .. g0 - 1 + end - 1
+    if (threadIdx.x == 0)
+      for (int i = issued; i < end; ++i) {
+        uint8_t* dst = smem + (i % STAGES) * stage;
+        tc5::bar_expect_tx(&full[i % STAGES], stage);
+        tc5::bulk_g2s(dst, kv + static_cast<int64_t>(i) * R * d2, half, &full[i % STAGES]);
+        tc5::bulk_g2s(dst + half, sc + static_cast<int64_t>(i) * R * d2, half, &full[i % STAGES]);
+      }
+    issued = max(issued, end);
   };
-  int issued = min(RUN_STAGES, nb + 1);
-  if (tid == 0)
-    for (int i = 0; i < issued; ++i) load(i);
+  load_to(min(STAGES, nb + 1));
   const int c = 2 * tid;  // this thread's columns c, c + 1 and d + c, d + c + 1
   const bool mine = c < d;
   float2 A[2 * R];
 #pragma unroll
   for (int i = 0; i < 2 * R; ++i)
     A[i] = mine ? ld2(p.ape + (i % R) * d2 + c + (i < R ? 0 : d)) : make_float2(0.f, 0.f);
-  bool ok = tc5::bar_wait(&full[0], 0);
-  for (int i = 1; i <= nb; ++i) {
-    const int g = g0 - 1 + i;
-    const int64_t orow = chunk_row(p, slot, g);
-    ok = ok && tc5::bar_wait(&full[i % RUN_STAGES], (i / RUN_STAGES) & 1);
+  // one thread of a group finds where its rows go, a round ahead
+  int32_t next_page = tid == 0 && group < nb ? chunk_page(p, slot, g0 + group) : 0;
+  bool ok = true;
+  int sp = group, sc_ = group + 1;          // buffers of the row's two blocks, and their phases
+  uint32_t pp = 0, pc = 0;
+  for (int i0 = 1; i0 <= nb; i0 += G) {
+    const int i = i0 + group, g = g0 - 1 + i;
+    const bool row = i <= nb;
+    float2 K[2 * R], S[2 * R];
+    if (row) {
+      if (tid == 0) {
+        where[group] = chunk_row(p, slot, g, next_page);
+        if (i + G <= nb) next_page = chunk_page(p, slot, g + G);
+      }
+      ok = tc5::bar_wait(&full[sp], pp) && tc5::bar_wait(&full[sc_], pc);
+      if (mine) {
+        const uint8_t* prev = smem + sp * stage + c * 4;
+        const uint8_t* cur = smem + sc_ * stage + (d + c) * 4;
+#pragma unroll
+        for (int j = 0; j < 2 * R; ++j) {
+          const uint8_t* src = (j < R ? prev : cur) + (j % R) * d2 * 4;
+          K[j] = *reinterpret_cast<const float2*>(src);
+          const float2 s = *reinterpret_cast<const float2*>(src + half);
+          S[j] = make_float2(s.x + A[j].x, s.y + A[j].y);
+        }
+      }
+    }
+    sp += G;
+    if (sp >= STAGES) sp -= STAGES, pp ^= 1;
+    sc_ += G;
+    if (sc_ >= STAGES) sc_ -= STAGES, pc ^= 1;
     if (__syncthreads_or(!ok)) {
-      if (tid == 0) raise_device_error(DSV4_ERR_WAIT_TIMEOUT);
+      if (threadIdx.x == 0) raise_device_error(DSV4_ERR_WAIT_TIMEOUT);
       break;
     }
+    load_to(min(nb + 1, i0 + G - 1 + STAGES));  // blocks up to i0 + G - 2 have been read
+    if (!row) continue;
     float vals[1][2] = {{0.f, 0.f}};
     float ss = 0.f;
     if (mine) {
-      float2 K[2 * R], S[2 * R];
-#pragma unroll
-      for (int j = 0; j < 2 * R; ++j) {
-        const uint8_t* src = smem + ((j < R ? i - 1 : i) % RUN_STAGES) * stage +
-                             static_cast<uint32_t>((j % R) * d2 + c + (j < R ? 0 : d)) * 4;
-        K[j] = *reinterpret_cast<const float2*>(src);
-        const float2 s = *reinterpret_cast<const float2*>(src + half);
-        S[j] = make_float2(s.x + A[j].x, s.y + A[j].y);
-      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         vals[0][e] = chunk_pool<R>(K, S, e);
         ss = fmaf(vals[0][e], vals[0][e], ss);
       }
     }
-    ss = block_sum(ss, red);  // its barriers: block i - 1 has been read
-    if (issued <= nb) {
-      if (tid == 0) load(issued);
-      ++issued;
-    }
+    // the group's sum, in block_sum's order; the next round's barrier frees sums
+    ss = warp_sum(ss);
+    if (lane == 0) sums[group][tid >> 5] = ss;
+    if (G == 1)
+      __syncthreads();
+    else
+      asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(THREADS) : "memory");
+    ss = warp_sum(lane < (d + 63) / 64 ? sums[group][lane] : 0.f);
+    const int64_t orow = where[group];
     const float rinv = rsqrtf(ss / static_cast<float>(d) + p.eps);
     if (mine)
       finish_pair(vals[0][0], vals[0][1], c, d, p.rope_dim, p.norm_w, p.norm_dtype, rinv, p.freqs, R * g, p.out, orow,
                   p.out_dtype, p.act_quant);
-    if (p.act_quant == 2) {  // head_dim 128: threads 0..63 hold the row (uniform over the CTA)
+    if (G == 1 && p.act_quant == 2) {  // head_dim 128: threads 0..63 hold the row (uniform over the CTA)
       hadamard_fp4_128(vals[0][0], vals[0][1], xch);
       if (tid < 64) store_pair(vals[0][0], vals[0][1], c, d, p.out, orow, p.out_dtype);
     }
-    if (p.key_image && g < p.max_comp) {
+    if (G == 1 && p.key_image && g < p.max_comp)
       append_key_row(vals[0][0], vals[0][1], d, p.key_image, p.key_inv, p.key_norm_max, p.max_comp, slot, g, red);
-      __syncthreads();  // red is free for the next row
-    }
   }
-  if (!ok && tid == 0)  // what was asked for lands before the CTA leaves
-    for (int i = max(0, issued - RUN_STAGES); i < issued; ++i) tc5::bar_wait(&full[i % RUN_STAGES], (i / RUN_STAGES) & 1);
+  if (!ok && threadIdx.x == 0)  // what was asked for lands before the CTA leaves
+    for (int i = max(0, issued - STAGES); i < issued; ++i) tc5::bar_wait(&full[i % STAGES], (i / STAGES) & 1);
 }
 
 template <int R>
@@ -939,19 +976,26 @@ extern "C" int dsv4_compressor_chunk(const dsv4_compressor_chunk_params* p, void
                  "dsv4_compressor_chunk: a key image needs head_dim 128, fp32 out, inv, norm_max and a 16-byte aligned image");
   if (p->n == 0 || p->total == 0) return DSV4_OK;
   const int threads = std::min(cmp::THREADS, (p->head_dim / 2 + 31) / 32 * 32);
-  // Long chunks: runs of blocks, as many CTAs as keep 192 KB an SM under way (two at 512 dims), all resident at
-  // once. Below two blocks a run there is nothing to stream ahead; the bulk copies want 16-byte alignment.
+  // Long chunks: runs of blocks, all CTAs resident at once: one an SM at 512 dims, as many as keep 192 KB an SM
+  // under way below. Under two blocks a run there is nothing to stream ahead; the bulk copies want 16-byte
+  // alignment.
   int run = 0;
+  const bool wide = p->head_dim == 512 && p->act_quant != 2 && p->key_image == nullptr;
   if (p->ratio == 4 && p->head_dim % 64 == 0 && p->head_dim <= 2 * cmp::THREADS) {
-    const int ctas = 2 * (2 * cmp::THREADS / p->head_dim) * num_sms() - 2 * p->n;
+    const int ctas = (wide ? 1 : 2 * (2 * cmp::THREADS / p->head_dim)) * num_sms() - 2 * p->n;
     run = ctas > 0 ? (p->total / 4 + ctas - 1) / ctas : 0;
   }
   if (run >= 2 && ((reinterpret_cast<uintptr_t>(p->kv) | reinterpret_cast<uintptr_t>(p->score)) & 15) == 0) {
-    static PerDeviceOnce attr;
-    DSV4_CUDA_CHECK(set_smem_once(attr, cmp::chunk_run_kernel, cmp::RUN_STAGES * 4 * 2 * 2 * cmp::THREADS * 8));
+    using cmp::Run;
+    const int which = wide ? 0 : p->head_dim == 128 ? 1 : 2;
+    void (*k)(dsv4_compressor_chunk_params, int) =
+        wide ? cmp::chunk_run_kernel<512, 3> : which == 1 ? cmp::chunk_run_kernel<128, 1> : cmp::chunk_run_kernel<0, 1>;
+    const int smem = (wide ? Run<512, 3>::STAGES : Run<0, 1>::STAGES) * 4 * 2 * p->head_dim * 8;
+    static PerDeviceOnce attr[3];
+    DSV4_CUDA_CHECK(set_smem_once(attr[which], k, which == 2 ? Run<0, 1>::STAGES * 4 * 2 * 2 * cmp::THREADS * 8 : smem));
     // at most one run a sequence is not full
-    DSV4_CUDA_CHECK(launch_pdl(cmp::chunk_run_kernel, dim3(p->n + p->total / 4 / run + p->n), dim3(threads),
-                               cmp::RUN_STAGES * 4 * 2 * p->head_dim * 8, as_stream(stream), *p, run));
+    DSV4_CUDA_CHECK(launch_pdl(k, dim3(p->n + p->total / 4 / run + p->n), dim3(wide ? 3 * cmp::THREADS : threads), smem,
+                               as_stream(stream), *p, run));
     return DSV4_OK;
   }
   const dim3 grid(p->n + (p->total + 3) / 4);
