@@ -64,20 +64,20 @@ __device__ __forceinline__ int lowest_free(const int32_t* refs, int n_pages, int
   return have < want ? have : want;
 }
 
-// one warp per sequence: its pages given back (its count lowered), its table row emptied
-__global__ void free_kernel(dsv4_pages p, const int32_t* seqs, int n) {
+// one CTA per sequence: its pages given back (its count lowered), its table row emptied. Bound by two
+// dependent reads (the row, then nothing waits for the counts).
+__global__ void __launch_bounds__(COPY) free_kernel(dsv4_pages p, const int32_t* seqs, int n) {
   pdl_wait();
   pdl_trigger();
-  const int k = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (k >= n) return;
-  const int s = seqs[k];
-  if (s < 0 || s >= p.slots) {
-    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-    return;
-  }
-  for (int j = threadIdx.x & 31; j < p.bt_stride; j += 32) {
-    // the exchange lets a sequence named twice give its pages back once
-    const int32_t pg = atomicExch(p.block_table + static_cast<int64_t>(s) * p.bt_stride + j, -1);
+  const int k = blockIdx.x, s = seqs[k];
+  bool skip = s < 0 || s >= p.slots;
+  if (skip && threadIdx.x == 0) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+  for (int i = threadIdx.x; i < k; i += COPY) skip |= seqs[i] == s;  // a sequence named twice gives its pages back once
+  if (__syncthreads_or(skip)) return;
+  for (int j = threadIdx.x; j < p.bt_stride; j += COPY) {
+    int32_t* cell = p.block_table + static_cast<int64_t>(s) * p.bt_stride + j;
+    const int32_t pg = *cell;
+    *cell = -1;
     if (pg >= 0 && pg < p.n_pages) atomicSub(p.refs + pg, 1);
   }
 }
@@ -209,10 +209,12 @@ __global__ void __launch_bounds__(PLAN) fork_plan_kernel(dsv4_pages p, const int
     } else {
       const int pages = (e + p.page - 1) / p.page;
       // every page of the source there, the branch's row empty, and no slot written twice or read after
+      const int32_t *ra = p.block_table + static_cast<int64_t>(a) * p.bt_stride;
+      const int32_t *rb = p.block_table + static_cast<int64_t>(b) * p.bt_stride;
+#pragma unroll 8
       for (int j = lane; j < p.bt_stride; j += 32) {
-        const int32_t pg = p.block_table[static_cast<int64_t>(a) * p.bt_stride + j];
-        bad |= j < pages && (pg < 0 || pg >= p.n_pages);
-        bad |= p.block_table[static_cast<int64_t>(b) * p.bt_stride + j] >= 0;
+        const int32_t pg = ra[j], own = rb[j];
+        bad |= (j < pages && (pg < 0 || pg >= p.n_pages)) | (own >= 0);
       }
       for (int i = lane; i < n; i += 32) bad |= (i < k && dst[i] == b) || src[i] == b;
     }
@@ -256,10 +258,20 @@ __global__ void __launch_bounds__(PLAN) fork_plan_kernel(dsv4_pages p, const int
   for (int k = w; k < n; k += PLAN / 32) {
     const Fork f = forks[k];
     if (!f.ok) continue;
-    for (int j = lane; j < f.entries / p.page; j += 32) {
-      const int32_t pg = p.block_table[static_cast<int64_t>(f.src) * p.bt_stride + j];
-      p.block_table[static_cast<int64_t>(f.dst) * p.bt_stride + j] = pg;
-      atomicAdd(p.refs + pg, 1);
+    const int32_t* ra = p.block_table + static_cast<int64_t>(f.src) * p.bt_stride;
+    int32_t* rb = p.block_table + static_cast<int64_t>(f.dst) * p.bt_stride;
+    const int full = f.entries / p.page;
+    for (int j0 = lane; j0 < full; j0 += 8 * 32) {
+      int32_t pg[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (j0 + 32 * i < full) pg[i] = ra[j0 + 32 * i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (j0 + 32 * i < full) {
+          rb[j0 + 32 * i] = pg[i];
+          atomicAdd(p.refs + pg[i], 1);
+        }
     }
   }
   // copy units before each part
@@ -292,24 +304,32 @@ __device__ __forceinline__ void copy_unit(const uint8_t* src, uint8_t* dst, int 
     if (static_cast<int>(threadIdx.x) + i * COPY < n16) __stcs(d + threadIdx.x + i * COPY, v[i]);
 }
 
+// A CTA takes neighbouring units: it looks its first part up and walks on from there.
 __global__ void __launch_bounds__(COPY) fork_copy_kernel(dsv4_pages p, int n, Fork* forks) {
   pdl_wait();
   pdl_trigger();
   const int64_t* starts = unit_starts(forks, n);
   const int parts = n * (SEGS + 1);
   const int64_t units = starts[parts];
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    int lo = 0, hi = parts - 1;  // the last part that starts at or before u (parts without units are passed over)
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (starts[mid] <= u)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
+  const int64_t u1 = units * (blockIdx.x + 1) / gridDim.x;
+  int64_t u = units * blockIdx.x / gridDim.x;
+  if (u >= u1) return;
+  int lo = 0, hi = parts - 1;  // the last part that starts at or before u (parts without units are passed over)
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (starts[mid] <= u)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  while (u < u1) {
+    while (starts[lo + 1] <= u) ++lo;  // u < units = starts[parts]
     const Part q = part(p, forks[lo / (SEGS + 1)], lo % (SEGS + 1));
-    const int64_t off = (u - starts[lo]) * UNIT;
-    copy_unit(q.src + off, q.dst + off, static_cast<int>(min(static_cast<int64_t>(UNIT), q.bytes - off)));
+    const int64_t first = starts[lo], end = min(starts[lo + 1], u1);
+    for (; u < end; ++u) {
+      const int64_t off = (u - first) * UNIT;
+      copy_unit(q.src + off, q.dst + off, static_cast<int>(min(static_cast<int64_t>(UNIT), q.bytes - off)));
+    }
   }
 }
 
@@ -318,23 +338,28 @@ __global__ void __launch_bounds__(PLAN) compact_plan_kernel(dsv4_pages p, int32_
                                                             int32_t* to, int32_t* n_moves) {
   pdl_wait();
   pdl_trigger();
+  // a stretch of pages per thread, in order
+  const int per = (p.n_pages + PLAN - 1) / PLAN;
+  const int i0 = min(p.n_pages, per * static_cast<int>(threadIdx.x)), i1 = min(p.n_pages, i0 + per);
   int live = 0;
-  for (int i = threadIdx.x; i < p.n_pages; i += PLAN) live += p.refs[i] > 0;
-  int total;
-  block_scan(live, &total);
-  const int nl = total;
-  int nh = 0, nm = 0;
-  for (int base = 0; base < p.n_pages; base += PLAN) {
-    const int i = base + threadIdx.x;
-    const int r = i < p.n_pages ? p.refs[i] : 0;
-    const bool hole = i < nl && r <= 0, mover = i >= nl && i < p.n_pages && r > 0;
-    // holes lie below nl and movers above: one scan serves both, but for the stretch that holds nl
-    int th, tm;
-    const int rh = block_scan(hole ? 1 : 0, &th), rm = block_scan(mover ? 1 : 0, &tm);
-    if (hole) holes[nh + rh] = i;
-    if (mover) movers[nm + rm] = i;
-    nh += th;
-    nm += tm;
+#pragma unroll 8
+  for (int i = i0; i < i1; ++i) live += p.refs[i] > 0;
+  int nl, nh, nm;
+  block_scan(live, &nl);
+  int h = 0, m = 0;
+#pragma unroll 8
+  for (int i = i0; i < i1; ++i) {
+    const bool used = p.refs[i] > 0;
+    h += !used && i < nl;
+    m += used && i >= nl;
+  }
+  h = block_scan(h, &nh);
+  m = block_scan(m, &nm);
+#pragma unroll 8
+  for (int i = i0; i < i1; ++i) {
+    const bool used = p.refs[i] > 0;
+    if (!used && i < nl) holes[h++] = i;
+    if (used && i >= nl) movers[m++] = i;
   }
   __syncthreads();
   for (int k = threadIdx.x; k < nm; k += PLAN) {  // nh == nm
@@ -411,7 +436,7 @@ int dsv4_pages_free(const dsv4_pages* p, const int32_t* seqs, int32_t n, void* s
   if (rc != DSV4_OK) return rc;
   DSV4_CHECK_ARG(n >= 0 && (n == 0 || seqs), "dsv4_pages_free: NULL sequences");
   if (n == 0) return DSV4_OK;
-  DSV4_CUDA_CHECK(launch_pdl(pg::free_kernel, dim3((n + 7) / 8), dim3(256), 0, as_stream(stream), *p, seqs, n));
+  DSV4_CUDA_CHECK(launch_pdl(pg::free_kernel, dim3(n), dim3(pg::COPY), 0, as_stream(stream), *p, seqs, n));
   return DSV4_OK;
 }
 
