@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // the 128-byte swizzle pattern is anchored to 1024-byte boundaries
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // the same register in every lane
   // CTA = (query, split): tiles [tbase, tbase + ntiles) of the query's list
   const int64_t qi = blockIdx.x / P.splits;
   const int split = static_cast<int>(blockIdx.x % P.splits);
@@ -247,13 +248,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
 
   if (warp == 0) {
     // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t id_s = idesc_bf16<128, HB>(false, false);
       constexpr uint32_t id_o = idesc_bf16<128, HB>(true, true);
       constexpr uint32_t id_l = idesc_bf16<128, HB>(false, true);
-      const uint32_t ks = smem_u32(sm.kv), qs = smem_u32(sm.q), ps = smem_u32(sm.p);
+      // operand descriptors, advanced by adding to the address field (16-byte units)
+      const uint64_t kd = sdesc(smem_u32(sm.kv), 16, 1024), qd = sdesc(smem_u32(sm.q), 16, 1024);
+      const uint64_t vd = sdesc(smem_u32(sm.kv), SLAB_KV, 1024), pd = sdesc(smem_u32(sm.p), 1024, 1024);
       bool ok = true;
       for (int i = 0; i < ntiles && ok; ++i) {
+#pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
           if (!(ok = bar_wait_or_abort(&sm.bar_full[mt], i & 1, abort))) break;
           fence_async_smem();  // the cp.async writes (generic proxy) are read by the tensor cores
@@ -262,23 +266,25 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
           for (int sl = 2 * mt; sl < 2 * mt + 2; ++sl)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              mma16(tmem + COL_S, sdesc(ks + sl * SLAB_KV + kk * 32, 16, 1024),
-                    sdesc(qs + sl * SLAB_Q + kk * 32, 16, 1024), id_s, (sl | kk) ? 1u : 0u);
+              mma16(tmem + COL_S, kd + ((sl * SLAB_KV + kk * 32) >> 4), qd + ((sl * SLAB_Q + kk * 32) >> 4), id_s,
+                    (sl | kk) ? 1u : 0u);
         }
         if (!ok) break;
         mma_commit(&sm.bar_s);
         if (!(ok = bar_wait_or_abort(&sm.bar_p, i & 1, abort))) break;
         after_sync();
+        const uint32_t acc = i > 0 ? 1u : 0u;
+#pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            mma16(tmem + COL_O + mt * HB, sdesc(ks + 2 * mt * SLAB_KV + kk * 2048, SLAB_KV, 1024),
-                  sdesc(ps + kk * 2048, 1024, 1024), id_o, (i > 0 || kk > 0) ? 1u : 0u);
+            mma16(tmem + COL_O + mt * HB, vd + ((2 * mt * SLAB_KV + kk * 2048) >> 4), pd + (kk * 2048 >> 4), id_o,
+                  kk > 0 ? 1u : acc);
           mma_commit(&sm.bar_empty[mt]);
         }
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          mma16_ta(tmem + COL_L, tmem + COL_ONES, sdesc(ps + kk * 2048, 1024, 1024), id_l, (i > 0 || kk > 0) ? 1u : 0u);
+          mma16_ta(tmem + COL_L, tmem + COL_ONES, pd + (kk * 2048 >> 4), id_l, kk > 0 ? 1u : acc);
       }
       mma_commit(&sm.bar_fin);  // also on abort, so that the drain below can wait for everything issued
       if (!ok) set_abort(sm);

@@ -87,16 +87,6 @@ struct Params {
 };
 
 // ---- the pair
-// One lane of the warp, chosen so that the compiler knows it: with the role's warp index the same in
-// every lane, the MMAs' descriptors stay in uniform registers (issued from a plain "lane == 0" branch
-// every MMA cost 70 to 130 cycles of the issuing thread, whatever its shape; this way 33 and 65 for
-// the N = 128 and N = 256 forms, their full rate).
-__device__ __forceinline__ bool elect_one(uint32_t* leader = nullptr) {
-  uint32_t p, l;
-  asm volatile("{\n.reg .pred e;\nelect.sync %1|e, 0xffffffff;\nselp.u32 %0, 1, 0, e;\n}\n" : "=r"(p), "=r"(l));
-  if (leader) *leader = l;
-  return p != 0;
-}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));

@@ -16,6 +16,17 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// One lane of the warp, chosen so that the compiler knows it: with the role's warp index the same in
+// every lane, the MMAs' descriptors stay in uniform registers (issued from a plain "lane == 0" branch
+// every MMA cost 70 to 130 cycles of the issuing thread, whatever its shape; this way 33 and 65 for
+// the N = 128 and N = 256 forms, their full rate).
+__device__ __forceinline__ bool elect_one(uint32_t* leader = nullptr) {
+  uint32_t p, l;
+  asm volatile("{\n.reg .pred e;\nelect.sync %1|e, 0xffffffff;\nselp.u32 %0, 1, 0, e;\n}\n" : "=r"(p), "=r"(l));
+  if (leader) *leader = l;
+  return p != 0;
+}
+
 // 64-bit shared-memory matrix descriptor: start, leading / stride byte offsets, version 1 (sm_100),
 // layout 2 = 128-byte swizzle
 __device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
