@@ -96,11 +96,9 @@ __global__ void __launch_bounds__(PLAN) reserve_kernel(dsv4_pages p, const int32
       const int s = seqs ? seqs[base + k] : base + k;
       int need = 0, have = 0;
       if (s >= 0 && s < p.slots) {
-        int e = max(0, (tokens[base + k] + add) / p.ratio);
-        if (e > p.max_comp) {
-          if (lane == 0) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-          e = p.max_comp;
-        }
+        const int64_t all = max(static_cast<int64_t>(0), static_cast<int64_t>(tokens[base + k]) + add) / p.ratio;
+        if (all > p.max_comp && lane == 0) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+        const int e = static_cast<int>(min(all, static_cast<int64_t>(p.max_comp)));
         need = (e + p.page - 1) / p.page;
         // pages fill a row from the left
         for (int j = lane; j < p.bt_stride; j += 32)
@@ -202,7 +200,7 @@ __global__ void __launch_bounds__(PLAN) fork_plan_kernel(dsv4_pages p, const int
   // a warp per branch: what it asks for, and whether it may have it
   for (int k = w; k < n; k += PLAN / 32) {
     const int a = src[k], b = dst[k];
-    const int e = tokens[k] / p.ratio;
+    const int e = p.max_comp == 0 ? 0 : tokens[k] / p.ratio;  // a window-only cache has rings alone
     int bad = 0;
     if (a < 0 || a >= p.slots || b < 0 || b >= p.slots || a == b || tokens[k] < 0 || e > p.max_comp) {
       bad = 1;
@@ -360,6 +358,7 @@ __global__ void __launch_bounds__(PLAN) compact_plan_kernel(dsv4_pages p, int32_
     const bool used = p.refs[i] > 0;
     if (!used && i < nl) holes[h++] = i;
     if (used && i >= nl) movers[m++] = i;
+    if (!used) to[i] = -1;  // for a cell that names a page which is not counted
   }
   __syncthreads();
   for (int k = threadIdx.x; k < nm; k += PLAN) {  // nh == nm
@@ -399,9 +398,12 @@ __global__ void __launch_bounds__(COPY) compact_copy_kernel(dsv4_pages p, const 
 DSV4_ERROR_READER(pages)
 
 static int check_pages(const dsv4_pages* p, const char* who) {
-  DSV4_CHECK_ARG(p && p->pool && p->block_table && p->refs && p->win_base, "%s: NULL pointer in the cache", who);
-  DSV4_CHECK_ARG(p->slots > 0 && p->n_pages >= 0 && p->page > 0 && p->max_comp > 0 && p->ratio > 0 && p->window > 0 &&
-                     p->bt_stride * static_cast<int64_t>(p->page) >= p->max_comp && p->comp_base >= 0,
+  DSV4_CHECK_ARG(p && p->pool && p->win_base && (p->max_comp == 0 || (p->block_table && p->refs)),
+                 "%s: NULL pointer in the cache", who);
+  DSV4_CHECK_ARG(p->slots > 0 && p->n_pages >= 0 && p->page > 0 && p->max_comp >= 0 && p->ratio > 0 && p->window > 0 &&
+                     (p->max_comp == 0 ? p->bt_stride == 0 && p->n_pages == 0
+                                       : p->bt_stride * static_cast<int64_t>(p->page) >= p->max_comp) &&
+                     p->comp_base >= 0,
                  "%s: bad sizes", who);
   DSV4_CHECK_ARG(p->head_dim > 0 && p->head_dim % 8 == 0 && p->idx_dim >= 0 && p->idx_dim % 4 == 0,
                  "%s: rows must be a multiple of 16 bytes", who);
@@ -445,7 +447,7 @@ int dsv4_pages_reserve(const dsv4_pages* p, const int32_t* seqs, const int32_t* 
   const int rc = pg::check_pages(p, "dsv4_pages_reserve");
   if (rc != DSV4_OK) return rc;
   DSV4_CHECK_ARG(n >= 0 && (n == 0 || tokens) && (seqs || n <= p->slots), "dsv4_pages_reserve: bad sequences");
-  if (n == 0) return DSV4_OK;
+  if (n == 0 || p->max_comp == 0) return DSV4_OK;
   if (workspace == nullptr || workspace_bytes < dsv4_pages_workspace_size(p, n)) {
     set_error("dsv4_pages_reserve: workspace missing or too small");
     return DSV4_ERR_WORKSPACE;

@@ -51,7 +51,7 @@ class SparseMLACache:
         if n_pages is not None and (n_pages < 0 or page_order is not None):
             raise ValueError("SparseMLACache: n_pages is a number of pages, and a paged cache hands them out itself "
                              "(no page_order)")
-        n_pages = n_pages if n_pages is not None else batch * self.pages_per_seq
+        n_pages = n_pages if paged else batch * self.pages_per_seq
         self.comp_base = batch * window
         self.max_chunk = int(max_chunk)
         if self.max_chunk < 0:

@@ -7,7 +7,8 @@ which are laid out by slot. Tables and counts stay on the device: every call is 
 current stream, can be captured in a CUDA graph, and gives the same tables for the same input. What a
 call cannot do for one sequence it leaves out for that sequence, and raises the device error word
 (`_lib.device_error`): NO_PAGES, or INDEX_OUT_OF_RANGE for a slot that does not exist, more tokens
-than the cache holds, or a branch onto a slot that has pages.
+than the cache holds, or a branch onto a slot that has pages. A window-only cache (no compressed rows)
+has no pages: it is branched by a copy of the window ring, and the other calls leave it as it is.
 """
 import ctypes
 
@@ -17,6 +18,11 @@ from . import _lib as L
 
 
 def _params(cache):
+    if not cache.compressed:   # window rings alone: nothing is paged, a branch is a copy of its ring
+        L.require_cuda(cache.kv_pool)
+        p = L.Pages(pool=cache.kv_pool.data_ptr(), win_base=cache.win_base.data_ptr(), comp_base=cache.comp_base)
+        p.slots, p.page, p.window, p.head_dim, p.ratio = cache.batch, 1, cache.window, cache.head_dim, 1
+        return p
     if cache.page_refs is None:
         raise ValueError("SparseMLACache: pages are handed out and shared only in a paged cache (n_pages=...)")
     L.require_cuda(cache.kv_pool)

@@ -404,7 +404,8 @@ typedef struct {
 DSV4_API int dsv4_chunk_rows(const dsv4_chunk* c, int32_t* positions, int64_t* stage_rows, int32_t* index,
                              int64_t index_stride, int32_t cols, const int32_t* given, void* stream);
 /* the chunk's last rows (at most window per sequence) from the stage into the window rings; pool is
- * the bf16 pool of rows of dim elements */
+ * the bf16 pool of rows of dim elements. The second sequence with tokens that names a slot is left out
+ * and raises DSV4_ERR_INDEX_OUT_OF_RANGE. */
 DSV4_API int dsv4_chunk_commit(const dsv4_chunk* c, void* pool, int32_t dim, void* stream);
 
 /* Attention of the chunk, every token over its window and all the compressed entries it sees; the
@@ -435,7 +436,8 @@ DSV4_API int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream);
  * (oracle/decode_engine.py:96-105 for a run of tokens; the reference takes one token at a time). Entry g of
  * slot s goes to row out_base + block_table[s, g / page] * page + g % page, or without a table to row
  * out_base + s * max_comp + g (the indexer keys). An entry past max_comp or without a page raises
- * DSV4_ERR_INDEX_OUT_OF_RANGE and is not stored. */
+ * DSV4_ERR_INDEX_OUT_OF_RANGE and is not stored; so does a slot that two sequences with tokens name,
+ * whose ring and entries are then not defined. */
 typedef struct {
   const float* kv;            /* [total, 2 * head_dim] */
   const float* score;         /* [total, 2 * head_dim], before ape */
@@ -469,8 +471,8 @@ DSV4_API int dsv4_compressor_chunk(const dsv4_compressor_chunk_params* p, void* 
 typedef struct {
   void* pool;               /* bf16 rows of head_dim: window rings at win_base, pages from comp_base */
   const int64_t* win_base;  /* [slots] */
-  int32_t* block_table;     /* [slots, bt_stride] */
-  int32_t* refs;            /* [n_pages] */
+  int32_t* block_table;     /* [slots, bt_stride]; NULL with max_comp, bt_stride and n_pages 0 (a window-only */
+  int32_t* refs;            /* [n_pages]                     cache: a branch is a copy of the window ring) */
   float* k_idx;             /* [slots, max_comp, idx_dim] or NULL */
   uint8_t* key_image;       /* dsv4_key_image_params layout, or NULL */
   float* key_inv;

@@ -317,3 +317,51 @@ def test_step_on_a_paged_cache():
     for s in range(2):
         other[c.comp_rows(s, torch.arange(16, device="cuda")) - c.comp_base] = False
     assert torch.equal(c.kv_pool[c.comp_base:][other], pool[other])
+
+
+def test_branches_of_a_window_only_cache():
+    """No pages: a branch is a copy of the window ring; handing out, giving back and compacting do nothing."""
+    pkg, Dm, L = _mods()
+    c = Dm.SparseMLACache(4, 0, n_pages=3, max_chunk=2)
+    c.kv_pool.copy_(torch.randn(c.kv_pool.shape, device="cuda").to(torch.bfloat16))
+    want = c.kv_pool.clone()
+    c.reserve([0, 1], [1000, 5])
+    c.free([3])
+    assert c.compact().item() == 0 and torch.equal(c.kv_pool, want)
+    c.fork([0, 0], [1, 3], [5000, 7])
+    want[W:2 * W] = want[:W]
+    want[3 * W:4 * W] = want[:W]
+    assert torch.equal(c.kv_pool, want) and L.device_error() == 0
+    c.fork([0], [4], [1])
+    assert torch.equal(c.kv_pool, want) and L.device_error() == OUT_OF_RANGE
+
+
+def test_reserve_at_the_ends():
+    """More sequences than the planning CTA has threads, a slot named again in the next thousand, counts at the
+    end of their type."""
+    pkg, Dm, L = _mods()
+    c = Dm.SparseMLACache(1100, 8, window=64, page=8, n_pages=1101, idx_dim=128)
+    order = list(np.random.default_rng(3).permutation(1100)) + [7, 8]
+    c.reserve([int(s) for s in order], [32] * 1102)
+    assert L.device_error() == 0
+    assert c.block_table[order[:1100], 0].tolist() == list(range(1100))
+    assert c.page_refs.tolist() == [1] * 1100 + [0]
+    c.free([5])
+    c.reserve([5], [2 ** 31 - 1], add=2 ** 31 - 1)   # past the cache: all that it has, and the error word
+    assert L.device_error() == OUT_OF_RANGE and int(c.block_table[5, 0]) >= 0
+    c.free([5])
+    c.reserve([5], [-2 ** 31], add=-2 ** 31)
+    c.reserve([5], [-8], add=7)
+    assert L.device_error() == 0 and int(c.block_table[5, 0]) == -1
+
+
+def test_compact_with_a_cell_that_is_not_counted():
+    """A table that names a page nobody counted (not one that these calls leave): the cell is emptied."""
+    pkg, Dm, L = _mods()
+    c = _cache(3, 128, 64, 6)
+    c.reserve([0, 1], [512, 256])
+    c.free([0])
+    c.block_table[2, 0] = 5
+    assert c.compact().item() == 1
+    assert c.block_table.tolist() == [[-1, -1], [0, -1], [-1, -1]] and c.page_refs.tolist() == [1, 0, 0, 0, 0, 0]
+    assert L.device_error() == 0
