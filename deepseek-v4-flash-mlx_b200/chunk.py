@@ -39,10 +39,9 @@ def _f32(t):
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
-def _chunk(cache, cu_seqlens, start, seqs, total):
-    """dsv4_chunk of the cache, and the tensors it points to."""
-    pool, table = cache.kv_pool, cache.block_table
-    dev = pool.device
+def _sequences(cache, cu_seqlens, start, seqs, total):
+    """The chunk's sequences as int32 tensors, checked against the cache."""
+    dev = cache.kv_pool.device
     cu = _index_tensor("cu_seqlens", cu_seqlens, dev, None)
     n = cu.numel() - 1
     if n < 0:
@@ -54,10 +53,21 @@ def _chunk(cache, cu_seqlens, start, seqs, total):
         raise ValueError(f"a chunk of {n} sequences, the cache has {cache.batch} slots")
     if total > cache.max_chunk:
         raise ValueError(f"a chunk of {total} tokens, the cache stages {cache.max_chunk} (SparseMLACache(max_chunk=...))")
-    c = L.Chunk(cu.data_ptr(), start.data_ptr(), None if seqs is None else seqs.data_ptr(), cache.win_base.data_ptr(),
-                table.data_ptr() if cache.compressed else None, cache.comp_base, cache.stage_base, pool.shape[0], n, total,
-                cache.batch, cache.window, cache.ratio, cache.page, table.shape[1], cache.max_comp)
+    return cu, start, seqs
+
+
+def _chunk(cache, cu_seqlens, start, seqs, total):
+    """dsv4_chunk of the cache, and the tensors it points to."""
+    cu, start, seqs = _sequences(cache, cu_seqlens, start, seqs, total)
+    c = _layout(cache.kv_pool, cache.block_table, cache.win_base, cu, start, seqs, total, cache.comp_base, cache.stage_base,
+                cache.window, cache.ratio, cache.page, cache.max_comp)
     return c, (cu, start, seqs)
+
+
+def _layout(pool, table, win_base, cu, start, seqs, total, comp_base, stage_base, window, ratio, page, max_comp):
+    return L.Chunk(cu.data_ptr(), start.data_ptr(), None if seqs is None else seqs.data_ptr(), win_base.data_ptr(),
+                   table.data_ptr() if max_comp else None, comp_base, stage_base, pool.shape[0], cu.numel() - 1, total,
+                   win_base.numel(), window, ratio, page, table.shape[1], max_comp)
 
 
 def chunk_rows(cache, cu_seqlens, start, total, seqs=None):
@@ -78,17 +88,46 @@ def chunk_rows(cache, cu_seqlens, start, total, seqs=None):
 
 def chunk_commit(cache, cu_seqlens, start, total, seqs=None):
     """Move the chunk's rows into the window rings (the last `window` of each sequence), after its
-    attention: what the decode steps and the next chunk see."""
+    attention: what the decode steps and the next chunk see. A slot takes one sequence of a call: the second
+    one that names it is left out and raises INDEX_OUT_OF_RANGE on the device error word."""
     c, keep = _chunk(cache, cu_seqlens, start, seqs, total)
     with L.device_of(cache.kv_pool):
         L.check(L.lib().dsv4_chunk_commit(ctypes.byref(c), L.ptr(cache.kv_pool), cache.head_dim,
                                           L.stream_of(cache.kv_pool)))
 
 
-def _attend(cache, c, q, sink, scale, freqs, out_dtype, num_splits):
+@torch.library.custom_op("dsv4::chunk_attention", mutates_args=(), device_types="cuda")
+def _chunk_attention_op(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tensor, win_base: torch.Tensor,
+                        sink: torch.Tensor, cu_seqlens: torch.Tensor, start: torch.Tensor, seqs: torch.Tensor | None,
+                        rows: torch.Tensor | None, freqs: torch.Tensor, comp_base: int, stage_base: int, window: int,
+                        ratio: int, page: int, max_comp: int, scale: float, out_dtype: torch.dtype,
+                        num_splits: int) -> torch.Tensor:
+    return _attention(q, kv_pool, block_table, win_base, sink, cu_seqlens, start, seqs, rows, freqs, comp_base, stage_base,
+                      window, ratio, page, max_comp, scale, out_dtype, num_splits)
+
+
+@_chunk_attention_op.register_fake
+def _(q, kv_pool, block_table, win_base, sink, cu_seqlens, start, seqs, rows, freqs, comp_base, stage_base, window, ratio,
+      page, max_comp, scale, out_dtype, num_splits):
+    return torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
+
+
+def _attention(q, kv_pool, block_table, win_base, sink, cu_seqlens, start, seqs, rows, freqs, comp_base, stage_base, window,
+               ratio, page, max_comp, scale, out_dtype, num_splits):
+    c = _layout(kv_pool, block_table, win_base, cu_seqlens, start, seqs, q.shape[0], comp_base, stage_base, window, ratio,
+                page, max_comp)
+    with L.device_of(q):
+        # lists differ from token to token, and pages that no box of rows divides have no run to load: those
+        # go through an index, token by token
+        if rows is None and (page % 8 == 0 or not max_comp) and window <= 1024:
+            return _attend(kv_pool, c, q, sink, scale, freqs, out_dtype, num_splits)
+        return _attend_listed(kv_pool, c, q, sink, rows, scale, freqs, out_dtype)
+
+
+def _attend(kv_pool, c, q, sink, scale, freqs, out_dtype, num_splits):
     """All visible rows: dsv4_chunk_attn, which finds them by itself."""
     out = torch.empty_like(q, dtype=out_dtype)
-    p = L.ChunkAttnParams(c, q.data_ptr(), cache.kv_pool.data_ptr(), sink.data_ptr(), out.data_ptr(), freqs.data_ptr(),
+    p = L.ChunkAttnParams(c, q.data_ptr(), kv_pool.data_ptr(), sink.data_ptr(), out.data_ptr(), freqs.data_ptr(),
                           2 * freqs.numel(), L.dtype_code(out), scale, num_splits)
     lib, ref = L.lib(), ctypes.byref(p)
     nbytes = lib.dsv4_chunk_attn_workspace_size(ref)
@@ -99,16 +138,16 @@ def _attend(cache, c, q, sink, scale, freqs, out_dtype, num_splits):
     return out
 
 
-def _attend_listed(cache, c, q, sink, rows, scale, freqs, out_dtype):
+def _attend_listed(kv_pool, c, q, sink, rows, scale, freqs, out_dtype):
     """Every token's list as an index tensor, and the sparse attention over it."""
     total = q.shape[0]
-    cols = cache.max_comp if rows is None else rows.shape[1]
-    idx = torch.empty((total, cache.window + cols), dtype=torch.int32, device=q.device)
+    cols = c.max_comp if rows is None else rows.shape[1]
+    idx = torch.empty((total, c.window + cols), dtype=torch.int32, device=q.device)
     pos = torch.empty(total, dtype=torch.int32, device=q.device)
     L.check(L.lib().dsv4_chunk_rows(ctypes.byref(c), L.ptr(pos), None, L.ptr(idx), idx.shape[1], cols, L.ptr(rows),
                                     L.stream_of(q)))
     out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    return sparse_attn_into(out, q, cache.kv_pool, sink, idx, scale, freqs, pos, 2 * freqs.numel())
+    return sparse_attn_into(out, q, kv_pool, sink, idx, scale, freqs, pos, 2 * freqs.numel())
 
 
 def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, scale=None, freqs=None,
@@ -122,7 +161,10 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
     oracle/decode_engine.py:110-116), or with `rows` (int32 [total, k] pool rows, -1 for none: the
     indexer's selection) those instead. `num_splits`: over how many CTA pairs the rows of two tokens are split
     (0: automatic; all visible rows only). Returns o [total, 64, 512] after the inverse RoPE; what it holds
-    behind the last sequence is not defined."""
+    behind the last sequence, and for a sequence that the error word reports (a slot that does not exist, tokens
+    outside of q), is not defined. Without `rows` the tokens of a sequence are taken in pairs: a row that is
+    not finite and seen by the second token of a pair reaches the first one's output too. The custom op
+    `dsv4::chunk_attention`."""
     L.require_cuda(q, sink, rows, freqs)
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
         raise ValueError(f"chunk_attention: q must be [total, heads, {cache.head_dim}], got {tuple(q.shape)}")
@@ -146,13 +188,11 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
     if not 0 <= num_splits <= 64:
         raise ValueError(f"chunk_attention: 0 to 64 splits, got {num_splits}")
     scale = cache.head_dim ** -0.5 if scale is None else float(scale)
-    c, keep = _chunk(cache, cu_seqlens, start, seqs, total)
-    if total == 0 or c.n == 0:
+    cu, start, seqs = _sequences(cache, cu_seqlens, start, seqs, total)
+    if total == 0 or cu.numel() == 1:
         return torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    q, sink = q.contiguous(), _f32(sink)
-    with L.device_of(q):
-        # lists differ from token to token, and pages that no box of rows divides have no run to load: those
-        # go through an index, token by token
-        if rows is None and (cache.page % 8 == 0 or not cache.compressed) and cache.window <= 1024:
-            return _attend(cache, c, q, sink, scale, freqs, out_dtype, int(num_splits))
-        return _attend_listed(cache, c, q, sink, rows, scale, freqs, out_dtype)
+    # traced programs see the custom op; an eager call goes straight to it
+    f = _chunk_attention_op if torch.compiler.is_compiling() else _attention
+    return f(q.contiguous(), cache.kv_pool, cache.block_table, cache.win_base, _f32(sink), cu, start, seqs, rows, freqs,
+             cache.comp_base, cache.stage_base, cache.window, cache.ratio, cache.page, cache.max_comp, scale, out_dtype,
+             int(num_splits))

@@ -295,7 +295,8 @@ def compressor_chunk(proj, cu_seqlens, start, ape, norm_w, ring_kv, ring_score, 
     int32 tensors on the device. Entry j of slot s goes to row out_base + block_table[s, j // page] *
     page + j % page of `out`, or without a table (the indexer keys) to row out_base + s * max_comp + j.
     An entry past max_comp, or whose page the table does not have, raises INDEX_OUT_OF_RANGE on the
-    device error word and is not stored. `key_image` (image, inv, norm_max: the cache's), `act_quant` and
+    device error word and is not stored; so does a slot named by two sequences that have tokens, whose ring
+    and rows are then not defined. `key_image` (image, inv, norm_max: the cache's), `act_quant` and
     `rotate` as in `compressor_decode_step`. The custom op `dsv4::compressor_chunk`."""
     kv, score = proj
     L.require_cuda(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, freqs)

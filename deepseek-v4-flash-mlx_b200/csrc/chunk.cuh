@@ -11,17 +11,14 @@ struct ChunkToken {
   int pos;    // position of this token
 };
 
-// cache slot of the chunk's sequence b; -1 (and the error word) when seqs names none
-__device__ __forceinline__ int chunk_slot(const dsv4_chunk& c, int b) {
-  const int s = c.seqs ? c.seqs[b] : b;
-  if (s < 0 || s >= c.slots) {
-    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-    return -1;
-  }
-  return s;
+// whether a sequence is one that can be read: its tokens in the batch, positions that stay far from
+// the end of an int, a slot of the cache
+__device__ __forceinline__ bool chunk_valid(int first, int end, int total, int start, int slot, int slots) {
+  return first >= 0 && end >= first && end <= total && start >= 0 && start <= 0x7fff0000 - total && slot >= 0 && slot < slots;
 }
 
-// the sequence of token t: the last b with cu_seqlens[b] <= t (empty sequences own no token)
+// the sequence of token t: the last b with cu_seqlens[b] <= t (empty sequences own no token); a token
+// of a sequence that is not valid belongs to none
 __device__ __forceinline__ ChunkToken chunk_token(const dsv4_chunk& c, int t) {
   ChunkToken k = {-1, 0, 0, 0};
   if (t >= c.cu_seqlens[c.n]) return k;
@@ -35,8 +32,14 @@ __device__ __forceinline__ ChunkToken chunk_token(const dsv4_chunk& c, int t) {
   }
   k.first = c.cu_seqlens[lo];
   k.start = c.start[lo];
-  k.pos = k.start + (t - k.first);
-  if (t >= k.first && k.start >= 0 && (c.seqs == nullptr || (c.seqs[lo] >= 0 && c.seqs[lo] < c.slots))) k.seq = lo;
+  const int end = c.cu_seqlens[lo + 1];
+  if (t < k.first || t >= end) return k;
+  if (chunk_valid(k.first, end, c.total, k.start, c.seqs ? c.seqs[lo] : lo, c.slots)) {
+    k.seq = lo;
+    k.pos = k.start + (t - k.first);
+  } else {
+    raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+  }
   return k;
 }
 

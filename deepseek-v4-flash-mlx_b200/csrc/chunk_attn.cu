@@ -254,13 +254,15 @@ struct Work {
     Seq q = {0, 0, 0, 0, 0};
     if (b < P.c.n) {
       q.first = P.c.cu_seqlens[b];
-      q.len = P.c.cu_seqlens[b + 1] - q.first;
+      const int end = P.c.cu_seqlens[b + 1];
       q.start = P.c.start[b];
       q.slot = P.c.seqs ? P.c.seqs[b] : b;
-      if (q.first >= 0 && q.len >= 0 && q.first + q.len <= P.c.total && q.start >= 0 && q.slot >= 0 && q.slot < P.c.slots)
+      if (chunk_valid(q.first, end, P.c.total, q.start, q.slot, P.c.slots)) {
+        q.len = end - q.first;
         q.pairs = (q.len + 1) / 2;
-      else
+      } else {
         raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+      }
     }
     return q;
   }

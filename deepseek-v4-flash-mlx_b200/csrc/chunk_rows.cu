@@ -23,12 +23,12 @@ __global__ void chunk_rows_kernel(dsv4_chunk c, int32_t* positions, int64_t* sta
   const int t = blockIdx.x;
   const ChunkToken k = chunk_token(c, t);
   if (threadIdx.x == 0) {
-    if (positions) positions[t] = k.seq < 0 ? 0 : k.pos;
+    if (positions) positions[t] = k.pos;
     if (stage_rows) stage_rows[t] = c.stage_base + t;
   }
   if (index == nullptr) return;
   int32_t* row = index + t * index_stride;
-  const int slot = k.seq < 0 ? 0 : chunk_slot(c, k.seq);
+  const int slot = k.seq < 0 ? 0 : c.seqs ? c.seqs[k.seq] : k.seq;
   for (int j = threadIdx.x; j < c.window; j += blockDim.x) {
     const int p = k.pos - c.window + 1 + j;
     int64_t r = -1;
@@ -51,15 +51,23 @@ __global__ void chunk_rows_kernel(dsv4_chunk c, int32_t* positions, int64_t* sta
   }
 }
 
-// one CTA per (sequence, ring slot): the slot's newest token of the chunk, if it has one
+// one CTA per (sequence, ring slot): the slot's newest token of the chunk, if it has one. A slot named
+// twice has no newest token: DSV4_ERR_INDEX_OUT_OF_RANGE, and the first to name it has the ring.
 __global__ void chunk_commit_kernel(dsv4_chunk c, uint4* pool, int row16) {
   pdl_wait();
   pdl_trigger();
   const int b = blockIdx.y, j = blockIdx.x;
-  const int first = c.cu_seqlens[b], n = c.cu_seqlens[b + 1] - first;
-  const int slot = chunk_slot(c, b);
-  if (n <= 0 || first < 0 || first + n > c.total || slot < 0) return;
-  const int end = c.start[b] + n;  // the largest p < end with p % window == j
+  const int first = c.cu_seqlens[b], last = c.cu_seqlens[b + 1];
+  const int slot = c.seqs ? c.seqs[b] : b;
+  bool bad = !chunk_valid(first, last, c.total, c.start[b], slot, c.slots);
+  if (c.seqs != nullptr && last > first)
+    for (int i = threadIdx.x; i < b; i += blockDim.x) bad |= c.seqs[i] == slot && c.cu_seqlens[i + 1] > c.cu_seqlens[i];
+  if (__syncthreads_or(bad)) {
+    if (j == 0 && threadIdx.x == 0) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+    return;
+  }
+  if (last == first) return;
+  const int end = c.start[b] + (last - first);  // the largest p < end with p % window == j
   const int p = end - 1 - (end - 1 - j % c.window + c.window) % c.window;
   if (p < c.start[b]) return;
   const uint4* src = pool + (c.stage_base + first + (p - c.start[b])) * row16;

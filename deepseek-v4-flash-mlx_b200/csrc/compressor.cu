@@ -11,6 +11,7 @@
 // dims (up to 256 threads, whole warps). The decode kernel keeps the per-sequence ring [2*ratio, 2d] on the device.
 #include <algorithm>
 
+#include "chunk.cuh"
 #include "common.cuh"
 #include "key_image.cuh"
 #include "tcgen05.cuh"
@@ -599,10 +600,11 @@ template <int R>
 __device__ __forceinline__ ChunkSeq<R> chunk_seq(const dsv4_compressor_chunk_params& p, int b) {
   ChunkSeq<R> q;
   q.first = p.cu_seqlens[b];
-  q.n = p.cu_seqlens[b + 1] - q.first;
+  const int end = p.cu_seqlens[b + 1];
   q.start = p.start[b];
   q.slot = p.seqs ? p.seqs[b] : b;
-  if (q.first < 0 || q.first + q.n > p.total || q.start < 0 || q.slot < 0 || q.slot >= p.slots) {
+  q.n = end - q.first;
+  if (!chunk_valid(q.first, end, p.total, q.start, q.slot, p.slots)) {
     raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
     q.n = 0;
   }
@@ -615,6 +617,10 @@ template <int R>
 __device__ __forceinline__ void chunk_sequence(const dsv4_compressor_chunk_params& p, int b, float* red, float* xch) {
   const ChunkSeq<R> q = chunk_seq<R>(p, b);
   if (q.n <= 0) return;
+  // a slot named twice: an error (nothing waits for the look), and the rows and ring of that slot are either's
+  if (p.seqs != nullptr)
+    for (int i = threadIdx.x; i < b; i += blockDim.x)
+      if (p.seqs[i] == q.slot && p.cu_seqlens[i + 1] > p.cu_seqlens[i]) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
   const int end = q.start + q.n, g0 = q.start / R, g1 = end / R;
   for (int g = g0; g < g1 && (g - 1) * R < q.start; ++g) chunk_emit<R>(p, q, g, red, xch);
   // the ring after the chunk: rows [0, R) the last complete block, rows R + p % R the newest token
@@ -695,12 +701,12 @@ __global__ void __launch_bounds__(G == 1 ? THREADS : G * D / 2, G == 1 ? 2 : 1)
       const int b = b0 + lane;
       int gs = 0, ge = 0;
       if (b < p.n) {
-        const int first = p.cu_seqlens[b], n = p.cu_seqlens[b + 1] - first, start = p.start[b];
+        const int first = p.cu_seqlens[b], last = p.cu_seqlens[b + 1], start = p.start[b];
         const int slot = p.seqs ? p.seqs[b] : b;
         // the blocks whose row needs no token of before the chunk (invalid sequences: reported elsewhere)
-        if (first >= 0 && n > 0 && first + n <= p.total && start >= 0 && slot >= 0 && slot < p.slots) {
+        if (chunk_valid(first, last, p.total, start, slot, p.slots)) {
           gs = (start + R - 1) / R + 1;
-          ge = max(gs, (start + n) / R);
+          ge = max(gs, (start + last - first) / R);
         }
       }
       const int cnt = (ge - gs + run - 1) / run;

@@ -263,6 +263,8 @@ class DecodeBlock:
             raise ValueError(f"extend: slots {slots} of a cache with {c.batch}")
         if total > c.max_chunk:
             raise ValueError(f"extend: {total} rows, the cache stages {c.max_chunk} (max_chunk)")
+        if not sum(lengths):
+            return torch.zeros((total, d.dim), dtype=torch.float32, device=dev)
         if c.compressed and any((p + n) // d.ratio > c.max_comp for n, p in zip(lengths, start)):
             raise ValueError(f"extend: a sequence grows past the cache's {c.max_comp} compressed rows")
         meta, at = [0], 0

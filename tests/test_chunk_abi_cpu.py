@@ -160,3 +160,69 @@ def test_python_refusals():
     paged.page_refs[1] = 2
     other.load_state_dict(paged.state_dict())
     assert other.page_refs.tolist() == [0, 2, 0] and paged.clone().page_refs.tolist() == [0, 2, 0]
+
+
+def _attn(**kw):
+    p = L.ChunkAttnParams()
+    buf = ctypes.create_string_buffer(64)
+    at = (ctypes.addressof(buf) + 15) // 16 * 16
+    chunk = {k: kw.pop(k) for k in list(kw) if hasattr(p.chunk, k)}
+    p.chunk = _chunk(**chunk)
+    p.q = p.pool = p.sink = p.out = p.rope_freqs = p.workspace = at
+    p.rope_dim, p.out_dtype, p.scale, p.num_splits, p.workspace_bytes = 64, 1, 0.04, 1, 0
+    for k, v in kw.items():
+        setattr(p, k, at + 4 if v == "misaligned" else v)
+    p._keep = buf
+    return p
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(window=1088), 1), (dict(window=100), 1), (dict(page=36), 1), (dict(page=4), 1), (dict(q=None), 1), (dict(sink=None), 1),
+    (dict(out=None), 1), (dict(pool=None), 1), (dict(q="misaligned"), 1), (dict(pool="misaligned"), 1), (dict(out="misaligned"), 1),
+    (dict(out_dtype=2), 2), (dict(rope_dim=66), 1), (dict(rope_dim=0), 1), (dict(rope_dim=7), 1), (dict(num_splits=65), 1),
+    (dict(num_splits=-1), 1), (dict(num_splits=2), 6), (dict(num_splits=2, workspace=None, workspace_bytes=1 << 40), 6),
+    (dict(num_splits=2, workspace="misaligned", workspace_bytes=1 << 40), 6)])
+def test_attention_refusals_of_the_c_entry(bad, code):
+    """Each is refused on the host, before any launch."""
+    assert L.lib().dsv4_chunk_attn(ctypes.byref(_attn(**bad)), None) == code
+
+
+def test_attention_workspace_and_nothing_to_do():
+    lib = L.lib()
+    assert lib.dsv4_chunk_attn_workspace_size(ctypes.byref(_attn())) == 0
+    total = _attn().chunk.total
+    assert lib.dsv4_chunk_attn_workspace_size(ctypes.byref(_attn(num_splits=5))) == total * 5 * (64 * 512 + 128) * 4
+    assert lib.dsv4_chunk_attn_workspace_size(ctypes.byref(_attn(num_splits=5, n=0))) == 0
+    assert lib.dsv4_chunk_attn(ctypes.byref(_attn(num_splits=5, n=0)), None) == 0
+    assert lib.dsv4_chunk_attn(None, None) == 1
+
+
+def test_pages_of_a_window_only_cache():
+    """No table and no counts, only the window rings: nothing to reserve, and no half of a paged cache."""
+    none = dict(block_table=None, refs=None, max_comp=0, n_pages=0, bt_stride=0)
+    p, lib = _pages(**none), L.lib()
+    at = p.win_base
+    assert lib.dsv4_pages_reserve(ctypes.byref(p), at, at, 0, 1, at, 1 << 20, None) == 0
+    for bad in (dict(n_pages=4), dict(bt_stride=2), dict(pool=None), dict(win_base=None)):
+        assert lib.dsv4_pages_reserve(ctypes.byref(_pages(**{**none, **bad})), at, at, 0, 1, at, 1 << 20, None) == 1
+    D = importlib.import_module(PKG + ".decode")
+    c = D.SparseMLACache(2, 0, device="cpu", n_pages=7)   # a window-only layer of a paged model holds no pages
+    assert c.kv_pool.shape[0] == 2 * 128 and c.page_refs is None
+    with pytest.raises(RuntimeError, match="CUDA"):
+        c.fork([0], [1], [4])
+
+
+def test_chunk_ops_trace_on_fake_tensors():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    importlib.import_module(PKG)
+    with FakeTensorMode():
+        e = lambda *s, dtype=torch.int32: torch.empty(*s, dtype=dtype, device="cuda")  # noqa: E731
+        f32, bf16 = torch.float32, torch.bfloat16
+        o = torch.ops.dsv4.chunk_attention(e(7, 64, 512, dtype=bf16), e(1000, 512, dtype=bf16), e(2, 3),
+                                           e(2, dtype=torch.int64), e(64, dtype=f32), e(3), e(2), None, None, e(32, dtype=f32),
+                                           256, 640, 128, 4, 64, 100, 0.04, f32, 0)
+        assert o.shape == (7, 64, 512) and o.dtype == f32 and o.device.type == "cuda"
+        assert torch.ops.dsv4.compressor_chunk(
+            e(7, 1024, dtype=f32), e(7, 1024, dtype=f32), e(3), e(2), None, e(4, 1024, dtype=f32), None,
+            e(2, 8, 1024, dtype=f32), e(2, 8, 1024, dtype=f32), e(1000, 512, dtype=bf16), e(2, 3), 64, 256, 100, 512, 4, 64,
+            e(32, dtype=f32), 1e-6, None, None, None, 0) is None

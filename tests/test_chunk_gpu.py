@@ -503,3 +503,198 @@ def test_extend_continues_a_prefill_and_refuses():
             blk.extend(x[:4], **kw)
     with pytest.raises(ValueError, match="max_chunk"):
         blk.extend(x[:200], [200], [300])
+
+
+# ---- calls at the edges of what the entry points allow ----
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 7, 8, 9, 33, 64])
+def test_chunk_attention_any_number_of_splits(splits):
+    """More splits than a token has tiles leave some without rows."""
+    pkg, _, L = _mods()
+    lens, start = [3, 0, 2], [1700, 9, 20]
+    c, q, sink, cu, st, _ = _case(lens, start, seed=31)
+    want, tol = _attention64(c, q, sink, lens, start, range(3))
+    for dtype in (torch.bfloat16, torch.float32):
+        _check(pkg.chunk_attention(c, q, sink, cu, st, freqs=_freqs().cuda(), num_splits=splits, out_dtype=dtype), want, tol)
+    assert L.device_error() == 0
+
+
+def test_chunk_attention_many_sequences():
+    """More sequences than a warp looks at together, and more pairs of tokens than clusters."""
+    pkg, _, L = _mods()
+    rng = np.random.default_rng(5)
+    lens, start = [int(n) for n in rng.integers(0, 6, 75)], [int(p) for p in rng.integers(0, 400, 75)]
+    seqs = [int(b) for b in rng.permutation(80)[:75]]
+    c, q, sink, cu, st, sq = _case(lens, start, seed=32, seqs=seqs, slots=80, page=16, paged=True, pad=5)
+    o = pkg.chunk_attention(c, q, sink, cu, st, seqs=sq, freqs=_freqs().cuda())
+    assert L.device_error() == 0
+    want, tol = _attention64(c, q, sink, lens, start, seqs)
+    _check(o, want, tol)
+
+
+@pytest.mark.parametrize("window", [64, 192, 1024, 2048])
+def test_chunk_attention_windows(window):
+    pkg, _, L = _mods()
+    lens, start = [3, 70, 1], [window + 11, 2 * window - 30, window - 1]
+    c, q, sink, cu, st, _ = _case(lens, start, seed=33, window=window)
+    o = pkg.chunk_attention(c, q, sink, cu, st, freqs=_freqs().cuda())
+    assert L.device_error() == 0
+    want, tol = _attention64(c, q, sink, lens, start, range(3))
+    _check(o, want, tol)
+
+
+def test_rows_past_32_bit_offsets():
+    """Pages and stage behind 4 GB and 2^31 elements of pool: attention both ways, compressor, commit."""
+    pkg, Dm, L = _mods()
+    n_pages, n, s = 70000, 9, 1001
+    c = Dm.SparseMLACache(1, 260, n_pages=n_pages, max_chunk=n)
+    g = torch.Generator(device="cuda").manual_seed(34)
+    c.block_table.copy_(torch.arange(n_pages - 1, n_pages - 6, -1, dtype=torch.int32)[None])
+    assert c.stage_base * 512 > 1 << 31
+    hi = c.comp_base + (n_pages - 5) * 64
+    c.kv_pool[hi:] = torch.randn(c.kv_pool[hi:].shape, generator=g, device="cuda").to(torch.bfloat16)
+    c.kv_pool[:W] = torch.randn(W, D, generator=g, device="cuda").to(torch.bfloat16)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    cu, st = i32(0, n), i32(s)
+    kv, sc = (torch.randn(n, 1024, generator=g, device="cuda") for _ in range(2))
+    ape, nw, f = torch.randn(4, 1024, generator=g, device="cuda"), torch.ones(512, device="cuda"), _freqs().cuda()
+    low, rings = torch.zeros(260, 512, dtype=torch.bfloat16, device="cuda"), []
+    for out, base, table in ((c.kv_pool, c.comp_base, c.block_table), (low, 0, None)):
+        rings.append((torch.zeros(1, 8, 1024, device="cuda"), torch.zeros(1, 8, 1024, device="cuda")))
+        pkg.compressor_chunk((kv, sc), cu, st, ape, nw, *rings[-1], out, 260, block_table=table, page=64, out_base=base, freqs=f)
+    e = torch.arange((s + n) // 4, device="cuda")
+    rows = c.comp_rows(0, e)
+    new = e[s // 4:]
+    assert new.numel() == 2 and torch.equal(c.kv_pool[rows[new]], low[new])
+    q = torch.randn(n, H, D, generator=g, device="cuda").to(torch.bfloat16) / 8
+    sink = torch.randn(H, generator=g, device="cuda")
+    want, tol = _attention64(c, q, sink, [n], [s], [0])
+    _check(pkg.chunk_attention(c, q, sink, cu, st, freqs=f), want, tol)
+    given = torch.full((n, e.numel()), -1, dtype=torch.int32, device="cuda")
+    for i in range(n):
+        given[i, :(s + i + 1) // 4] = rows[:(s + i + 1) // 4].to(torch.int32)
+    _check(pkg.chunk_attention(c, q, sink, cu, st, rows=given, freqs=f), want, tol)
+    pkg.chunk_commit(c, cu, st, n)
+    assert torch.equal(c.kv_pool[[(s + i) % W for i in range(n)]], c.kv_pool[c.stage_base:])
+    assert L.device_error() == 0
+
+
+BAD = [dict(start=-1), dict(start=2 ** 31 - 5), dict(start=2 ** 31 - 1), dict(slot=9), dict(slot=-1), dict(end=99)]
+
+
+@pytest.mark.parametrize("bad", BAD)
+def test_sequences_that_are_not_valid_are_reported_and_left_out(bad):
+    """The first sequence is a good one: it comes out as if alone, and nothing of the second is written."""
+    pkg, _, L = _mods()
+    lens, start = [5, 12], [601, 8]
+    c, q, sink, cu, st, sq = _case(lens, start, seed=35)
+    f, (want, tol) = _freqs().cuda(), _attention64(c, q, sink, lens, start, range(2))
+    st[1], sq[1], cu[2] = bad.get("start", 8), bad.get("slot", 1), bad.get("end", 17)
+    pos, _ = pkg.chunk_rows(c, cu, st, 17, sq)
+    assert L.device_error() == 4
+    assert pos.tolist() == list(range(601, 606)) + [0] * 12
+    for rows in (None, torch.full((17, 1), -1, dtype=torch.int32, device="cuda")):
+        o = pkg.chunk_attention(c, q, sink, cu, st, seqs=sq, rows=rows, freqs=f)
+        assert L.device_error() == 4
+        if rows is None:
+            _check(o[:5], want[:5], tol[:5])
+    for total in (17, 4 * 4000):   # few tokens and long chunks take different kernels
+        kv = torch.randn(total, 1024, device="cuda")
+        ape, nw = torch.zeros(4, 1024, device="cuda"), torch.ones(512, device="cuda")
+        rings = [torch.zeros(2, 8, 1024, device="cuda") for _ in range(2)]
+        out = torch.zeros(2 * 5000, 512, device="cuda")
+        cu2, st2 = cu.clone(), st.clone()
+        cu2[2], st2[0] = total + 7 if "end" in bad else total, 1
+        pkg.compressor_chunk((kv, kv), cu2, st2, ape, nw, *rings, out, 5000, seqs=sq, freqs=f)
+        assert L.device_error() == 4
+        assert out[0].any() and not out[1:].any() and not rings[0][1].any() and not rings[1][1].any()
+    before = c.kv_pool.clone()
+    pkg.chunk_commit(c, cu, st, 17, sq)
+    assert L.device_error() == 4
+    for i in range(5):
+        before[(601 + i) % W] = before[c.stage_base + i]
+    assert torch.equal(c.kv_pool, before)
+
+
+def test_a_slot_named_twice():
+    """Reading it twice is a call like any other; the ring takes the first, and the second is reported. Empty
+    sequences (a batch padded to a fixed number of them) name what they like."""
+    pkg, _, L = _mods()
+    lens, start = [3, 2], [300, 300]
+    c, q, sink, cu, st, sq = _case(lens, start, seed=36, seqs=[1, 1], slots=2)
+    _check(pkg.chunk_attention(c, q, sink, cu, st, seqs=sq, freqs=_freqs().cuda()), *_attention64(c, q, sink, lens, start, [1, 1]))
+    assert L.device_error() == 0
+    before = c.kv_pool.clone()
+    pkg.chunk_commit(c, cu, st, 5, sq)
+    assert L.device_error() == 4
+    for i in range(3):
+        before[W + (300 + i) % W] = before[c.stage_base + i]
+    assert torch.equal(c.kv_pool, before)
+    kv = torch.randn(5, 1024, device="cuda")
+    ape, nw, out = torch.zeros(4, 1024, device="cuda"), torch.ones(512, device="cuda"), torch.zeros(200, 512, device="cuda")
+    rings = [torch.zeros(2, 8, 1024, device="cuda") for _ in range(2)]
+    pkg.compressor_chunk((kv, kv), cu, st, ape, nw, *rings, out, 100, seqs=sq)
+    assert L.device_error() == 4
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    cu, st, sq = i32(0, 3, 3, 3, 5), i32(300, 0, 0, 300), i32(1, 1, 0, 0)
+    pkg.chunk_commit(c, cu, st, 5, sq)
+    pkg.compressor_chunk((kv, kv), cu, st, ape, nw, *rings, out, 100, seqs=sq)
+    assert L.device_error() == 0
+
+
+def test_chunk_ops_compile_as_one_graph():
+    """Traced whole (a graph break raises), the compressor writing what the attention then reads: the eager bits."""
+    import torch._dynamo
+    torch._dynamo.reset()
+    pkg, _, L = _mods()
+    lens, start = [9, 6], [400, 31]
+    c, q, sink, cu, st, _ = _case(lens, start, seed=37, paged=True)
+    g = torch.Generator(device="cuda").manual_seed(38)
+    kv, sc = (torch.randn(15, 1024, generator=g, device="cuda") for _ in range(2))
+    ape, nw, f = torch.randn(4, 1024, generator=g, device="cuda"), torch.ones(512, device="cuda"), _freqs().cuda()
+
+    def run(c, kv, sc, q, sink, cu, st):
+        pkg.compressor_chunk((kv, sc), cu, st, ape, nw, c.ring_kv, c.ring_score, c.kv_pool, c.max_comp,
+                             block_table=c.block_table, page=c.page, out_base=c.comp_base, freqs=f)
+        return pkg.chunk_attention(c, q, sink, cu, st, freqs=f)
+
+    other = c.clone()
+    want = run(c, kv, sc, q, sink, cu, st)
+    got = torch.compile(run, fullgraph=True, backend="aot_eager")(other, kv, sc, q, sink, cu, st)
+    assert torch.equal(got, want) and torch.equal(other.kv_pool, c.kv_pool) and torch.equal(other.ring_kv, c.ring_kv)
+    assert L.device_error() == 0
+
+
+def test_two_graphs_and_an_eager_call_share_nothing():
+    """Split attentions have a workspace: two captured graphs replayed on two streams at once, and eager calls
+    between, each keep their own."""
+    pkg, _, L = _mods()
+    lens, start, f = [2], [9000], _freqs().cuda()
+    cases = [_case(lens, start, seed=40 + i) for i in range(3)]
+    wants = [pkg.chunk_attention(c, q, sink, cu, st, freqs=f) for c, q, sink, cu, st, _ in cases]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for c, q, sink, cu, st, _ in cases[:2]:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(pkg.chunk_attention(c, q, sink, cu, st, freqs=f))
+        graphs.append(gr)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for gr, sm in zip(graphs, streams):
+            with torch.cuda.stream(sm):
+                gr.replay()
+        c, q, sink, cu, st, _ = cases[2]
+        assert torch.equal(pkg.chunk_attention(c, q, sink, cu, st, freqs=f), wants[2])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], wants[0]) and torch.equal(outs[1], wants[1])
+    assert L.device_error() == 0
+
+
+def test_extend_by_nothing():
+    blk, _, dims, _ = _block(4, 2, 256, 512, n_pages=3, max_chunk=8)
+    before = {k: v.clone() for k, v in blk.cache.state_dict().items()}
+    for x, lengths, start in ((torch.zeros(0, dims.dim, device="cuda"), [], []), (torch.zeros(3, dims.dim, device="cuda"), [0, 0], [4, 9])):
+        assert blk.extend(x, lengths, start).shape == x.shape
+    for k, v in blk.cache.state_dict().items():
+        assert torch.equal(v, before[k]), k
