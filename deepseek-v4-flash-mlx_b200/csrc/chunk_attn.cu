@@ -73,6 +73,23 @@ struct Smem {
 };
 static_assert(sizeof(Smem) + 1024 <= 232448, "shared memory above the 227 KB a CTA may opt into");
 
+// Division by a number of the call, as a product: floor(x / d) = x * ceil(2^(31 + s) / d) >> (31 + s) for
+// 0 <= x < 2^31 and s = ceil(log2 d): the rounding up adds less than x / 2^(31 + s) < 2^-s <= 1 / d to the quotient.
+// (A division takes over 100 cycles, and a unit needs a dozen before its first load: 2000 of 5000 cycles.)
+struct Div {
+  uint32_t mul;
+  int32_t d, shift;
+  Div() = default;
+  explicit Div(int by) : d(by), shift(31) {
+    while ((1LL << (shift - 31)) < by) ++shift;
+    mul = static_cast<uint32_t>(((1ULL << shift) + by - 1) / by);
+  }
+  __device__ __forceinline__ int quot(int x) const {
+    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * mul >> shift);
+  }
+  __device__ __forceinline__ int rem(int x) const { return x - quot(x) * d; }
+};
+
 struct Params {
   CUtensorMap pool;  // [pool_rows, 512] bf16, box 64 dims x box_rows
   CUtensorMap q;     // [total * 64, 512] bf16, box 64 dims x 64 rows
@@ -80,10 +97,11 @@ struct Params {
   dsv4_chunk c;
   const float* sink;
   void* out;
-  float* part;       // splits > 1: O [total][splits][512 dims][64 heads], then (m, l) [total][splits][64][2]
+  float* part;       // splits > 1: O [total][splits][512 / 4][64 heads][4 dims], then (m, l) [total][splits][64][2]
   const float* freqs;
   int rope_dim, out_dtype, splits, box_rows;
   float scale_log2;
+  Div by_window, by_ratio, by_page, by_splits;
 };
 
 // ---- the pair
@@ -97,9 +115,8 @@ __device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 // Arrive on a barrier of either CTA. What it tells of is read by the tensor cores from the arriving
 // CTA's own shared memory, and its writes there are complete for them once fence.proxy.async has been
 // passed, so the arrival need not release at cluster scope (which took 1000 to 1800 cycles a tile).
@@ -114,7 +131,8 @@ __device__ __forceinline__ void load_pair(void* dst, const void* map, int x, int
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-// a 64 x 64 tile of this CTA's shared memory to a tensor, and the wait until such tiles have been read
+// a 64 x 64 tile of this CTA's shared memory to a tensor, and the wait until such tiles have been read (what
+// was written is complete with the grid)
 __device__ __forceinline__ void store_tile(const void* map, int x, int y, const void* src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -123,7 +141,6 @@ __device__ __forceinline__ void store_tile(const void* map, int x, int y, const 
   asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
 }
 __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
-__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
   asm volatile(
       "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
@@ -174,11 +191,16 @@ struct Unit {
   int p0;                 // its position
   int slot;               // cache slot
   int stage_pos;          // position of the first staged row it sees
+  int newest;             // ring slot of the newest row of before the chunk
   int nring, nstage, nh;  // halves: ring, stage, all
   uint64_t ring;          // the ring's halves, 4 bits each
   int seen[2];            // compressed entries that the first and the last token see
 };
-__device__ __forceinline__ Unit make_unit(const dsv4_chunk& c, int first, int start, int slot, int t0, int n) {
+__device__ __forceinline__ int entries_seen(const Params& P, int pos) {  // as chunk_seen
+  return P.c.max_comp == 0 ? 0 : min(P.by_ratio.quot(pos + 1), P.c.max_comp);
+}
+__device__ __forceinline__ Unit make_unit(const Params& P, int first, int start, int slot, int t0, int n) {
+  const dsv4_chunk& c = P.c;
   Unit u;
   u.first = first;
   u.start = start;
@@ -190,15 +212,17 @@ __device__ __forceinline__ Unit make_unit(const dsv4_chunk& c, int first, int st
   u.ring = 0;
   u.nring = 0;
   const int old = u.start - lo;                // rows of before the chunk: slots lo % window .., cyclic
+  const int oldest = P.by_window.rem(lo);
+  u.newest = u.start > 0 ? P.by_window.rem(u.start - 1) : 0;
   if (old > 0)
-    for (int h = 0; h < c.window / 64; ++h) {
-      const int gap = (h * 64 - lo % c.window + c.window) % c.window;  // slots from the oldest row to the half
+    for (int h = 0; 64 * h < c.window; ++h) {
+      const int gap = h * 64 - oldest + (h * 64 < oldest ? c.window : 0);  // slots from the oldest row to the half
       if (gap < old || gap > c.window - 64) u.ring |= static_cast<uint64_t>(h) << (4 * u.nring++);
     }
   u.stage_pos = max(u.start, lo);
   u.nstage = (u.p0 + n - u.stage_pos + 63) / 64;
-  u.seen[0] = chunk_seen(c, u.p0);
-  u.seen[1] = chunk_seen(c, u.p0 + n - 1);
+  u.seen[0] = entries_seen(P, u.p0);
+  u.seen[1] = entries_seen(P, u.p0 + n - 1);
   u.nh = u.nring + u.nstage + (u.seen[1] + 63) / 64;
   return u;
 }
@@ -211,12 +235,13 @@ __device__ __forceinline__ int half_row(const Params& P, const Unit& u, int h, i
   if (h < u.nstage) return static_cast<int>(c.stage_base) + u.first + (u.stage_pos - u.start) + 64 * h + r;
   const int e = 64 * (h - u.nstage) + r;
   if (e >= u.seen[1]) return static_cast<int>(c.pool_rows);
-  const int32_t pg = c.block_table[static_cast<int64_t>(u.slot) * c.bt_stride + e / c.page];
+  const int j = P.by_page.quot(e);
+  const int32_t pg = c.block_table[static_cast<int64_t>(u.slot) * c.bt_stride + j];
   if (pg < 0) {
     raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
     return static_cast<int>(c.pool_rows);
   }
-  const int64_t row = c.comp_base + static_cast<int64_t>(pg) * c.page + e % c.page;
+  const int64_t row = c.comp_base + static_cast<int64_t>(pg) * c.page + (e - j * c.page);
   return row < c.pool_rows ? static_cast<int>(row) : static_cast<int>(c.pool_rows);
 }
 // the same for lane `b` of a warp that loads a half together; nothing to load past the last half or box
@@ -226,7 +251,7 @@ __device__ __forceinline__ int tile_row(const Params& P, const Unit& u, int h, i
 // whether the token at position p (entries: what it sees of them) sees row j of half h
 __device__ __forceinline__ bool half_sees(const dsv4_chunk& c, const Unit& u, int h, int j, int p, int entries) {
   if (h < u.nring) {
-    const int back = (u.start - 1 - 64 * static_cast<int>((u.ring >> (4 * h)) & 15) - j) % c.window;
+    const int back = u.newest - 64 * static_cast<int>((u.ring >> (4 * h)) & 15) - j;
     const int pos = u.start - 1 - (back < 0 ? back + c.window : back);
     return pos >= 0 && pos > p - c.window;
   }
@@ -240,14 +265,15 @@ __device__ __forceinline__ bool half_sees(const dsv4_chunk& c, const Unit& u, in
 
 // The work of a cluster: units (pair of tokens, split) number `at`, at + clusters, ...; the pairs are counted
 // through the sequences and taken from the last to the first, since the last see the most rows. A warp looks
-// together, a lane per sequence, 32 at a time.
+// together, a lane per sequence, 32 at a time (and keeps the first 32).
 struct Work {
-  Unit u;
-  int pairs, at, split, tile0, nt;
-
   struct Seq {
     int first, len, start, slot, pairs;
   };
+  Unit u;
+  Seq head;
+  int pairs, at, split, tile0, nt;
+
   // this lane's sequence of those from b0 on
   static __device__ __forceinline__ Seq load(const Params& P, int b0) {
     const int b = b0 + (threadIdx.x & 31);
@@ -266,37 +292,41 @@ struct Work {
     }
     return q;
   }
-  __device__ __forceinline__ explicit Work(const Params& P) : pairs(0), at(static_cast<int>(blockIdx.x >> 1)) {
-    for (int b0 = 0; b0 < P.c.n; b0 += 32) pairs += __reduce_add_sync(0xffffffffu, load(P, b0).pairs);
+  __device__ __forceinline__ explicit Work(const Params& P) : head(load(P, 0)), at(static_cast<int>(blockIdx.x >> 1)) {
+    pairs = __reduce_add_sync(0xffffffffu, head.pairs);
+    for (int b0 = 32; b0 < P.c.n; b0 += 32) pairs += __reduce_add_sync(0xffffffffu, load(P, b0).pairs);
   }
   __device__ __forceinline__ bool next(const Params& P) {
     if (at >= pairs * P.splits) return false;
-    split = at % P.splits;
-    const int find = pairs - 1 - at / P.splits;
+    const int pair = P.by_splits.quot(at);
+    split = at - pair * P.splits;
+    const int find = pairs - 1 - pair;
     at += gridDim.x >> 1;
     int before = 0;
     for (int b0 = 0;; b0 += 32) {  // ends: find < pairs
-      const Seq q = load(P, b0);
+      const Seq q = b0 == 0 ? head : load(P, b0);
       int s = q.pairs;
+      if (P.c.n > 1) {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, s, o);
-        if ((threadIdx.x & 31) >= o) s += x;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, s, o);
+          if ((threadIdx.x & 31) >= o) s += x;
+        }
       }
       const int own = before + s - q.pairs;
       const uint32_t hit = __ballot_sync(0xffffffffu, find >= own && find < own + q.pairs);
       if (hit != 0) {
         const int l = __ffs(hit) - 1, t0 = q.first + 2 * (find - own);
-        u = make_unit(P.c, __shfl_sync(0xffffffffu, q.first, l), __shfl_sync(0xffffffffu, q.start, l),
+        u = make_unit(P, __shfl_sync(0xffffffffu, q.first, l), __shfl_sync(0xffffffffu, q.start, l),
                       __shfl_sync(0xffffffffu, q.slot, l), __shfl_sync(0xffffffffu, t0, l),
                       __shfl_sync(0xffffffffu, min(2, q.first + q.len - t0), l));
         break;
       }
       before += __shfl_sync(0xffffffffu, s, 31);
     }
-    const int tiles = (u.nh + 1) / 2;
-    tile0 = static_cast<int>(static_cast<int64_t>(tiles) * split / P.splits);
-    nt = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / P.splits) - tile0;
+    const int tiles = (u.nh + 1) / 2;  // below 2^24 + 16: 64 times that is an int
+    tile0 = P.by_splits.quot(tiles * split);
+    nt = P.by_splits.quot(tiles * (split + 1)) - tile0;
     return true;
   }
 };
@@ -333,16 +363,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     tma_prefetch_map(&P.pool);
     tma_prefetch_map(&P.q);
   }
-  pdl_wait();  // what follows reads memory that the kernels before may have written
-  Work w(P);
-  bool has = w.next(P);
   before_sync();
   __syncthreads();
-  cluster_sync();
+  cluster_arrive();
+  pdl_wait();  // what follows reads memory that the kernels before may have written
+  // one launch: the next kernel may move in beside it (the merging kernel: see the end)
+  if (P.splits == 1) pdl_trigger();
+  Work w(P);
+  bool has = w.next(P);
+  // the loading warps' first rows (the table's words) are on their way while the pair meets
+  const int boxes = 64 / P.box_rows;
+  int first_row = 0;
+  if (warp >= 1 && warp <= 3 && has) first_row = tile_row(P, w.u, 2 * w.tile0 + static_cast<int>(warp == 3 ? 1 - rank : rank), lane, boxes);
+  cluster_wait();
   after_sync();
   const uint32_t tmem = sm.tmem_base;
   const volatile int* abort = &sm.abort;
-  const int boxes = 64 / P.box_rows;
   const uint32_t box_bytes = static_cast<uint32_t>(P.box_rows) * 128;
 
   // Tiles and units are counted through the whole work (g, ord): a barrier of two buffers is in phase
@@ -351,11 +387,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     // ---------------------------------------------------------------- the tiles as K: slot X (and Q), slot Y
     // (the warp goes together: lane k finds the row of box k, a tile ahead; one lane issues the loads)
     const int x = warp - 1;
-    bool ok = true;
+    bool ok = true, looked = true;  // looked: first_row is the unit's
     int g = 0, ord = 0, issued = 0;
-    for (; ok && has; has = w.next(P)) {
+    for (; ok && has; has = w.next(P), looked = false) {
       if (w.nt == 0) continue;
-      int row = tile_row(P, w.u, 2 * w.tile0 + static_cast<int>(rank), lane, boxes);
+      int row = looked ? first_row : tile_row(P, w.u, 2 * w.tile0 + static_cast<int>(rank), lane, boxes);
       // Q follows the last S of the unit before
       if (x == 0 && g > 0) ok = bar_wait_or_abort(&sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1, abort);
       if (x == 0 && ok && elect_one()) {
@@ -368,7 +404,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       __syncwarp();
       for (int i = 0; i < w.nt && ok; ++i, ++g) {
         const int b = g & 1;
-        const int next = i + 1 < w.nt ? tile_row(P, w.u, 2 * (w.tile0 + i + 1) + static_cast<int>(rank), lane, boxes) : 0;
 #pragma unroll
         for (int y = 0; y < 2; ++y) {  // two slabs at a time, as the O of the tile before last frees them
           const int qr = 2 * y + x;
@@ -386,7 +421,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
           }
           ++issued;
         }
-        row = next;
+        if (i + 1 < w.nt) row = tile_row(P, w.u, 2 * (w.tile0 + i + 1) + static_cast<int>(rank), lane, boxes);
       }
       if (!ok) {
         if (lane == 0) set_abort(sm);
@@ -407,14 +442,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     }
   } else if (warp == 3) {
     // ---------------------------------------------------------------- the other half's rows as V
-    bool ok = true;
+    bool ok = true, looked = true;
     int g = 0;
-    for (; ok && has; has = w.next(P)) {
+    for (; ok && has; has = w.next(P), looked = false) {
       if (w.nt == 0) continue;
-      int row = tile_row(P, w.u, 2 * w.tile0 + 1 - static_cast<int>(rank), lane, boxes);
+      int row = looked ? first_row : tile_row(P, w.u, 2 * w.tile0 + 1 - static_cast<int>(rank), lane, boxes);
       for (int i = 0; i < w.nt; ++i, ++g) {
         const int b = g & 1;
-        const int next = i + 1 < w.nt ? tile_row(P, w.u, 2 * (w.tile0 + i + 1) + 1 - static_cast<int>(rank), lane, boxes) : 0;
         if (!(ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.s_full[b], (g >> 1) & 1, abort)))) break;
         uint8_t* slot = sm.kv[b][1 - rank];  // CTA 0: Y takes rows 64-127, CTA 1: X takes rows 0-63
         const bool one = elect_one();
@@ -427,7 +461,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
               tma_load_2d(slot + e * SLAB + k * box_bytes, &P.pool, (4 * static_cast<int>(rank) + e) * 64, at, &sm.v_full[b]);
           }
         }
-        row = next;
+        if (i + 1 < w.nt) row = tile_row(P, w.u, 2 * (w.tile0 + i + 1) + 1 - static_cast<int>(rank), lane, boxes);
       }
       if (!ok) {
         if (lane == 0) set_abort(sm);
@@ -647,10 +681,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       const uint32_t src = tmem + lanes + COL_O + 128 * ch;
       const int d0 = 256 * kvh + 128 * ch, group = 2 * kvh + ch;
       if (P.splits > 1) {
-        // partials with the heads innermost: a warp stores a dim of 32 heads at a time
+        // partials by four dims of every head: a warp stores 512 bytes at a time
         if (ok && mine) {
           const int64_t at = token * P.splits + split;
-          float* po = P.part + (at * D + d0) * HB + head;
+          float4* po = reinterpret_cast<float4*>(P.part) + (at * (D / 4) + d0 / 4) * HB + head;
 #pragma unroll 1
           for (int c = 0; c < 128; c += 32) {
             float v[32];
@@ -658,7 +692,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
             tmem_ld16(src + c + 16, v + 16);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) po[(c + e) * HB] = v[e];
+            for (int e = 0; e < 8; ++e) po[(c / 4 + e) * HB] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
           }
           if (group == 0)
             *reinterpret_cast<float2*>(P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + (at * HB + head) * 2) =
@@ -722,7 +756,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       __syncwarp();
       if (lane == 0) arrive_at(in_cta(&sm.o_free, 0));
     }
-    if (lane == 0) stores_done();
     // every commit of the last two tiles has arrived here before the CTA leaves
     for (int e = max(0, g - 2); e < g; ++e)
       for (int x = 0; x < 4; ++x)
@@ -733,34 +766,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
   before_sync();
   __syncthreads();
   // (not earlier: the merging kernel's blocks would all be placed on the few SMs without a cluster)
-  pdl_trigger();
-  cluster_sync();  // no CTA leaves while the pair's MMAs, loads or arrivals may touch it
+  if (P.splits > 1) pdl_trigger();
+  cluster_arrive();
+  cluster_wait();  // no CTA leaves while the pair's MMAs, loads or arrivals may touch it
   after_sync();
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(TMEM_COLS));
 }
 
 // One CTA per (token, MD dims): the splits' partials weighed by 2^(m - max), the sink, the inverse
-// rotation. At most 64 splits. A split's dims of 64 heads lie in a row, a float4 (four heads of a dim) per
-// thread of a group; MG groups take every MG-th split. <8, 4> for many splits, that is few tokens, so that
-// the 64 CTAs of a single token have enough loads in flight; <16, 1> otherwise, a quarter of the threads
-// (32 tokens in 3 splits: 21 us with the attention, against 33 us). The sum turns round in shared memory,
-// so that a head's dims leave together.
-template <int MD, int MG>
+// rotation. At most 64 splits. A float4 (four dims of a head) per thread of a group and split; MG groups take
+// every MG-th split, the first PF of a thread's loads on their way before the weights are known. <8, 4> for
+// as many tokens as have all their CTAs resident at once (2 an SM), so that the 64 CTAs of a single token have
+// enough loads in flight; <16, 1> otherwise. The sum turns round in shared memory, so that a head's dims leave
+// together. What the attention kernel had to wait for is complete before this one starts (its launch is
+// triggered behind that wait), so the sequences are looked up before its own wait.
+template <int MD, int MG, int PF>
 __global__ void __launch_bounds__(MG * MD * HB / 4) chunk_merge_kernel(const __grid_constant__ Params P) {
   constexpr int MT = MG * MD * HB / 4, MH = MT / HB, MS = 64 / MH;  // threads; per head; splits a thread weighs
-  pdl_wait();
   constexpr int BLOCKS = D / MD;
   const int64_t t = blockIdx.x / BLOCKS;
   const int d0 = static_cast<int>(blockIdx.x % BLOCKS) * MD;
   const ChunkToken k = chunk_token(P.c, static_cast<int>(t));
-  if (k.seq < 0) return;
   __shared__ float w[64][HB];   // [split][head]
   __shared__ float red[2][MH][HB];
-  __shared__ float o[MG][MD][HB];
-  const int tid = threadIdx.x;
+  __shared__ float4 o[MG][MD / 4][HB];
+  const int tid = threadIdx.x, h = tid & (HB - 1);
+  const float sink = P.sink[h] * LOG2E;
+  pdl_wait();
+  if (k.seq < 0) return;
+  // this thread's four dims of head h, splits gd, gd + MG, ...
+  const int gd = tid / (MD * HB / 4), quad = tid / HB % (MD / 4);
+  const float4* src = reinterpret_cast<const float4*>(P.part) + (t * P.splits * (D / 4) + d0 / 4 + quad) * HB + h;
+  float4 x[PF];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < PF; ++i)
+      if (s0 + i * MG < P.splits) x[i] = src[static_cast<int64_t>(s0 + i * MG) * (HB * D / 4)];
+  };
   {
-    const int h = tid & (HB - 1), g = tid / HB;
+    const int g = tid / HB;
     const float2* ml = reinterpret_cast<const float2*>(P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D)) +
                        t * P.splits * HB + h;
     float2 v[MS];
@@ -769,6 +814,7 @@ __global__ void __launch_bounds__(MG * MD * HB / 4) chunk_merge_kernel(const __g
       const int s = g + i * MH;
       v[i] = s < P.splits ? ml[s * HB] : make_float2(-INFINITY, 0.f);
     }
+    fetch(gd);
     float M = v[0].x;
 #pragma unroll
     for (int i = 1; i < MS; ++i) M = fmaxf(M, v[i].x);
@@ -780,9 +826,9 @@ __global__ void __launch_bounds__(MG * MD * HB / 4) chunk_merge_kernel(const __g
 #pragma unroll
     for (int i = 0; i < MS; ++i) {
       const int s = g + i * MH;
-      const float x = v[i].x == -INFINITY ? 0.f : exp2f(v[i].x - M);
-      if (s < P.splits) w[s][h] = x;
-      L = fmaf(x, v[i].y, L);
+      const float e = v[i].x == -INFINITY ? 0.f : exp2f(v[i].x - M);
+      if (s < P.splits) w[s][h] = e;
+      L = fmaf(e, v[i].y, L);
     }
     red[1][g][h] = L;
     __syncthreads();
@@ -790,27 +836,25 @@ __global__ void __launch_bounds__(MG * MD * HB / 4) chunk_merge_kernel(const __g
       L = 0.f;
 #pragma unroll
       for (int i = 0; i < MH; ++i) L += red[1][i][h];
-      red[0][0][h] = 1.f / (L + exp2f(P.sink[h] * LOG2E - M));
+      red[0][0][h] = 1.f / (L + exp2f(sink - M));
     }
   }
-  {
-    const int g = tid / (MD * HB / 4), e = tid / (HB / 4) % MD, h = tid % (HB / 4) * 4;  // dim d0 + e, heads h .. h + 3
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float* src = P.part + (t * P.splits * D + d0 + e) * HB + h;
-#pragma unroll 4
-    for (int s = g; s < P.splits; s += MG) {
-      const float4 x = *reinterpret_cast<const float4*>(&w[s][h]);
-      // a split without rows has written no O, and its weight is 0 for every head
-      if (x.x != 0.f || x.y != 0.f || x.z != 0.f || x.w != 0.f) {
-        const float4 v = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (HB * D));
-        a.x = fmaf(x.x, v.x, a.x);
-        a.y = fmaf(x.y, v.y, a.y);
-        a.z = fmaf(x.z, v.z, a.z);
-        a.w = fmaf(x.w, v.w, a.w);
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = gd; s0 < P.splits; s0 += PF * MG) {
+    if (s0 != gd) fetch(s0);
+#pragma unroll
+    for (int i = 0; i < PF; ++i) {
+      const int s = s0 + i * MG;
+      const float f = s < P.splits ? w[s][h] : 0.f;
+      if (f != 0.f) {  // a split without rows has written no O
+        a.x = fmaf(f, x[i].x, a.x);
+        a.y = fmaf(f, x[i].y, a.y);
+        a.z = fmaf(f, x[i].z, a.z);
+        a.w = fmaf(f, x[i].w, a.w);
       }
     }
-    *reinterpret_cast<float4*>(&o[g][e][h]) = a;
   }
+  o[gd][quad][h] = a;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < MD * HB / 2; i += MT) {  // a pair of dims of a head
@@ -819,8 +863,9 @@ __global__ void __launch_bounds__(MG * MD * HB / 4) chunk_merge_kernel(const __g
     float y = 0.f, z = 0.f;
 #pragma unroll
     for (int g = 0; g < MG; ++g) {
-      y += o[g][e][head];
-      z += o[g][e + 1][head];
+      const float2 v = *(reinterpret_cast<const float2*>(&o[g][e / 4][head]) + (e / 2 & 1));
+      y += v.x;
+      z += v.y;
     }
     y *= red[0][0][head];
     z *= red[0][0][head];
@@ -868,16 +913,24 @@ static int encode(CUtensorMap* map, const void* base, uint64_t rows, uint32_t bo
   return DSV4_OK;
 }
 
-// clusters of one wave shared out over the pairs of tokens, two tiles a split at least
+// Over how many clusters the rows of a pair are split: the number with the least time, by this account in
+// hundredths of a tile (1.43 us for 128 rows): the tiles of a split in every round of the clusters, 1.4 a round
+// after the first, and for a split 2.4 for the merging kernel and 0.05 a token and split for its partials.
+// Measured (us): 32 tokens at 2048: 19.0 whole, 23.1 in 3; 1 at 65536: 196 whole, 20.6 in 44, 21.8 in 64; 80 at
+// 64548 (40 pairs for 74 clusters): 199 whole, 161 in 3, 177 in 8; 300 at 16384: 173 whole, 217 in 2.
 static int plan_splits(const dsv4_chunk_attn_params* p) {
-  const int64_t units = (static_cast<int64_t>(p->chunk.total) + p->chunk.n) / 2;
-  const int tiles = (p->chunk.max_comp + 2 * p->chunk.window) / BN + 1;  // at most
-  int want = p->num_splits;
-  if (want <= 0) {
-    want = static_cast<int>(std::max<int64_t>(1, num_sms() / 2 / std::max<int64_t>(1, units)));
-    want = std::min(want, std::max(1, tiles / 2));
+  if (p->num_splits > 0) return std::min(p->num_splits, 64);
+  const int64_t units = (static_cast<int64_t>(p->chunk.total) + p->chunk.n) / 2, clusters = std::max(1, num_sms() / 2);
+  const int64_t tiles = (static_cast<int64_t>(p->chunk.max_comp) + 2 * p->chunk.window) / BN + 1;  // at most
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= 64; ++s) {
+    const int64_t rounds = (units * s + clusters - 1) / clusters, each = (tiles + s - 1) / s;
+    const int64_t cost = rounds * each * 100 + (rounds - 1) * 140 + (s > 1 ? 240 + 5 * s * static_cast<int64_t>(p->chunk.total) : 0);
+    if (cost < least) least = cost, best = s;
+    if (each == 1) break;
   }
-  return std::min(want, 64);
+  return best;
 }
 
 }  // namespace ca
@@ -936,6 +989,10 @@ int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
   P.rope_dim = p->rope_freqs ? p->rope_dim : 0;
   P.out_dtype = p->out_dtype;
   P.scale_log2 = p->scale * ca::LOG2E;
+  P.by_window = ca::Div(P.c.window);
+  P.by_ratio = ca::Div(std::max(1, P.c.ratio));
+  P.by_page = ca::Div(std::max(1, P.c.page));
+  P.by_splits = ca::Div(P.splits);
   // one cluster per pair of SMs, or per unit where there are fewer
   const int64_t units = (static_cast<int64_t>(P.c.total) + P.c.n) / 2 * P.splits;
   DSV4_CHECK_ARG(static_cast<int64_t>(P.c.total) * P.splits * ca::HB <= 0x7fffffffLL, "dsv4_chunk_attn: too many tokens");
@@ -944,11 +1001,11 @@ int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
   DSV4_CUDA_CHECK(set_smem_once(attr, ca::chunk_attn_kernel, smem));
   DSV4_CUDA_CHECK(launch_pdl(ca::chunk_attn_kernel, dim3(static_cast<unsigned>(2 * std::min<int64_t>(units, num_sms() / 2))),
                              dim3(ca::THREADS), smem, as_stream(stream), P));
-  if (P.splits > 8)
-    DSV4_CUDA_CHECK(launch_pdl(ca::chunk_merge_kernel<8, 4>, dim3(static_cast<unsigned>(P.c.total) * (ca::D / 8)),
+  if (P.splits > 1 && P.c.total * (ca::D / 8) <= 2 * num_sms())
+    DSV4_CUDA_CHECK(launch_pdl(ca::chunk_merge_kernel<8, 4, 8>, dim3(static_cast<unsigned>(P.c.total) * (ca::D / 8)),
                                dim3(4 * 8 * ca::HB / 4), 0, as_stream(stream), P));
   else if (P.splits > 1)
-    DSV4_CUDA_CHECK(launch_pdl(ca::chunk_merge_kernel<16, 1>, dim3(static_cast<unsigned>(P.c.total) * (ca::D / 16)),
+    DSV4_CUDA_CHECK(launch_pdl(ca::chunk_merge_kernel<16, 1, 4>, dim3(static_cast<unsigned>(P.c.total) * (ca::D / 16)),
                                dim3(16 * ca::HB / 4), 0, as_stream(stream), P));
   return DSV4_OK;
 }
