@@ -72,7 +72,7 @@ struct Params {
   void* out;
   int64_t s, n;
   int h, t;
-  int idx_dtype, out_dtype;
+  int out_dtype;
   float scale_log2;
   const float* rope_freqs;
   const int32_t* positions;
@@ -81,35 +81,64 @@ struct Params {
   int win_stride, window, window_linear;
 };
 
-// pool row of logical list entry u of query qi ([implicit window | idx]); -1 = masked
-__device__ __forceinline__ int64_t list_row(const Params& P, int64_t qi, int u) {
-  if (P.win_base != nullptr) {
-    if (u < P.window) {
-      const int p = P.positions[qi];
-      const int W = P.window;
-      int slot;
-      if (P.window_linear) {
-        const int lo = p - W + 1 > 0 ? p - W + 1 : 0;
-        slot = (lo + u <= p) ? lo + u : -1;
-      } else if (p >= W - 1) {
-        const int sp = p % W;
-        slot = (u < W - sp - 1) ? (sp + 1 + u) : (u - (W - sp - 1));
-      } else {
-        slot = (u <= p) ? u : -1;
-      }
-      return slot < 0 ? -1 : P.win_base[qi * P.win_stride] + slot;
-    }
-    u -= P.window;
-  }
-  if (P.idx_dtype == DSV4_I64) return __ldg(reinterpret_cast<const long long*>(P.idx) + qi * P.t + u);
-  return __ldg(reinterpret_cast<const int32_t*>(P.idx) + qi * P.t + u);
-}
+// The list of a query, [implicit window | idx]: what an entry's row follows from, read once.
+template <bool WIDE>  // 64-bit idx
+struct List {
+  const int32_t* idx;     // the query's row of idx
+  int64_t win;            // its window's first pool row
+  int window, len;        // implicit rows, all entries
+  int first, sp, linear;  // window entry u: linear: row first + u while <= sp; else ring slot from sp + 1 on
+  int64_t n;
 
-__device__ __forceinline__ bool row_valid(const Params& P, int64_t qi, int u, int L) {
-  if (u >= L) return false;
-  const int64_t v = list_row(P, qi, u);
-  return v >= 0 && v < P.n;
-}
+  __device__ __forceinline__ List(const Params& P, int64_t qi) {
+    window = P.window;
+    len = window + P.t;
+    n = P.n;
+    idx = reinterpret_cast<const int32_t*>(P.idx) + (WIDE ? 2 : 1) * (qi * P.t);
+    win = 0;
+    first = sp = 0;
+    linear = 1;
+    if (window > 0) {
+      const int p = P.positions[qi];
+      win = P.win_base[qi * P.win_stride];
+      linear = P.window_linear || p < window - 1;
+      first = P.window_linear && p - window + 1 > 0 ? p - window + 1 : 0;
+      sp = linear ? p : p % window;
+    }
+  }
+  // what is read for entry u, asked for early: nothing here waits for it
+  struct Raw {
+    int32_t lo, hi;
+  };
+  __device__ __forceinline__ Raw ask(int u) const {
+    Raw w = {0, 0};
+    if (u >= window && u < len) {
+      const int32_t* at = idx + (WIDE ? 2 : 1) * static_cast<int64_t>(u - window);
+      w.lo = __ldg(at);
+      if (WIDE) w.hi = __ldg(at + 1);
+    }
+    return w;
+  }
+  // its pool row, -1 if masked; an index past the pool raises the error word
+  __device__ __forceinline__ int32_t row(int u, Raw w) const {
+    if (u >= len) return -1;
+    int64_t v;
+    if (u < window) {
+      if (linear)
+        v = first + u <= sp ? win + first + u : -1;
+      else
+        v = win + (u < window - sp - 1 ? sp + 1 + u : u - (window - sp - 1));
+    } else {
+      v = WIDE ? static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(w.hi)) << 32 | static_cast<uint32_t>(w.lo))
+               : static_cast<int64_t>(w.lo);
+    }
+    if (v >= n) {
+      raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
+      v = -1;
+    }
+    return static_cast<int32_t>(v < 0 ? -1 : v);
+  }
+};
 
 // D (+)= A . B with A in tensor memory (K-major, 16-bit), B from shared memory
 __device__ __forceinline__ void mma16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t id, uint32_t acc) {
@@ -169,7 +198,8 @@ __device__ __forceinline__ float warp_col_max32(const float* v) {
   return a[0];
 }
 
-__global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
+template <bool WIDE>
+__global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(const __grid_constant__ Params P) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // the 128-byte swizzle pattern is anchored to 1024-byte boundaries
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
@@ -178,7 +208,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
   // CTA = (query, split): tiles [tbase, tbase + ntiles) of the query's list
   const int64_t qi = blockIdx.x / P.splits;
   const int split = static_cast<int>(blockIdx.x % P.splits);
-  const int L = (P.win_base ? P.window : 0) + P.t;
+  const int L = P.window + P.t;
   const int tiles_all = (L + BN - 1) / BN;
   const int per = (tiles_all + P.splits - 1) / P.splits;
   const int tbase = split * per;
@@ -202,44 +232,31 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
   int nown = 0;
 #pragma unroll
   for (int k = 0; k < W_CHUNKS; ++k) nown += (wt + W_THREADS * k < BN * 16);
-  auto load_rows = [&](int i, int* rr) {
+  pdl_wait();  // the kernel before is complete from here
+  const List<WIDE> list(P, qi);
+  typename List<WIDE>::Raw raw[W_CHUNKS], raw_s = {0, 0};  // of the next tile: this worker's rows, this softmax thread's row
+  auto ask_rows = [&](int i) {
 #pragma unroll
-    for (int k = 0; k < W_CHUNKS; ++k) {
-      const int c = wt + W_THREADS * k;
-      int32_t v = 0;
-      if (k < nown) {
-        const int u = (tbase + i) * BN + (c >> 4);
-        int64_t r = u < L ? list_row(P, qi, u) : -1;
-        if (r >= P.n) {
-          raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-          r = -1;
-        }
-        v = static_cast<int32_t>(r < 0 ? 0 : r);  // masked rows fetch row 0; their p is 0
-      }
-      rr[k] = v;
-    }
+    for (int k = 0; k < W_CHUNKS; ++k)
+      if (k < nown) raw[k] = list.ask((tbase + i) * BN + ((wt + W_THREADS * k) >> 4));
+    if (warp >= SM_WARP0) raw_s = list.ask((tbase + i) * BN + (warp & 3) * 32 + lane);
   };
-  // Q -> 8 swizzled slabs (64 heads x 128 B); the first tile's row numbers and the softmax rows'
-  // validity (dependent index loads) are fetched while Q lands
+  // Q -> 8 swizzled slabs (64 heads x 128 B), by the gather workers: their arrivals on the first tile's
+  // barriers come after it
   int rr[W_CHUNKS];
-  bool valid0 = false;
-  {
+  if (warp >= W_WARP0) {
+    if (ntiles > 0) ask_rows(0);
     const uint32_t qs = smem_u32(sm.q);
     const __nv_bfloat16* qg = P.q + qi * HB * D;
-    for (int c = tid; c < HB * 64; c += THREADS) {
+    for (int c = wt; c < HB * 64 && ntiles > 0; c += W_THREADS) {
       const int hh = c >> 6, ch = c & 63;
       cp_async16(qs + slab_off(hh, ch, SLAB_Q), qg + hh * D + ch * 8, true);
     }
-    asm volatile("cp.async.commit_group;\n" ::);
-    if (warp >= W_WARP0 && ntiles > 0) load_rows(0, rr);
-    if (warp >= SM_WARP0) valid0 = row_valid(P, qi, tbase * BN + (warp & 3) * 32 + lane, L);
+  } else if (P.rope_freqs != nullptr && P.rope_dim <= 64 && lane < P.rope_dim / 2) {
     // the RoPE angles of the query's position, once per CTA (one sincosf per lane of warp 0, which
     // is idle here): the epilogue's inverse rotation reads them from shared memory
-    if (warp == 0 && P.rope_freqs != nullptr && P.rope_dim <= 64 && lane < P.rope_dim / 2)
-      rope_cos_sin(P.positions[qi], P.rope_freqs[lane], &sm.rope_c[lane], &sm.rope_s[lane]);
-    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    rope_cos_sin(P.positions[qi], P.rope_freqs[lane], &sm.rope_c[lane], &sm.rope_s[lane]);
   }
-  fence_async_smem();
   before_sync();
   __syncthreads();
   after_sync();
@@ -315,10 +332,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
       }
       before_sync();
       sm_bar();
-      valid = valid0;
     }
     bool ok = true;
     for (int i = 0; i < ntiles; ++i) {
+      // the tile's rows have been asked for a tile ahead; the next tile's are asked for before this one is fetched
+#pragma unroll
+      for (int k = 0; k < W_CHUNKS; ++k)
+        if (k < nown) rr[k] = list.row((tbase + i) * BN + ((wt + W_THREADS * k) >> 4), raw[k]);
+      if (smx) valid = list.row((tbase + i) * BN + row, raw_s) >= 0;
+      if (i + 1 < ntiles) ask_rows(i + 1);
       // gather tile i, pair by pair
       for (int mt = 0; mt < 4 && ok; ++mt) {
         if (i > 0) ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.bar_empty[mt], (i - 1) & 1, abort));
@@ -330,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
             const int r = c >> 4, j = c & 15;
             const int sl = 2 * mt + (j >> 3), ch = j & 7;
             cp_async16(ks + static_cast<uint32_t>(sl * SLAB_KV + r * 128 + ((ch ^ (r & 7)) << 4)),
-                       P.kv + static_cast<int64_t>(rr[k]) * D + sl * 64 + ch * 8, true);
+                       P.kv + static_cast<int64_t>(max(rr[k], 0)) * D + sl * 64 + ch * 8, rr[k] >= 0);
           }
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(&sm.bar_full[mt]))
@@ -340,7 +362,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
         if (lane == 0) set_abort(sm);
         if (!smx) break;
       }
-      if (i + 1 < ntiles) load_rows(i + 1, rr);
       if (!smx) continue;
 
       // ---------------------------------------------------------- softmax of tile i (warps 4-11)
@@ -432,7 +453,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
       fence_async_smem();
       before_sync();
       bar_arrive(&sm.bar_p);
-      valid = row_valid(P, qi, (tbase + i + 1) * BN + row, L);
     }
 
     if (smx) {
@@ -514,7 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
 #pragma unroll 1
         for (int mt = 0; mt < 4; ++mt) {
           const int d = mt * 128 + qd * 32 + lane;
-          const bool do_rope = rope && d >= D - P.rope_dim;
+          const bool do_rope = rope && d >= D - P.rope_dim;  // the same for a pair (rope_dim is even)
           float cs = 1.f, sn = 0.f;
           if (do_rope) {
             const int f = (d - (D - P.rope_dim)) >> 1;
@@ -529,26 +549,32 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(Params P) {
           tmem_ld16(tmem + lq + COL_O + mt * HB + half * 32, v);
           tmem_ld16(tmem + lq + COL_O + mt * HB + half * 32 + 16, v + 16);
           tmem_wait_ld();
+          // Lanes hold neighbouring dims; two of them swap every other head, so that each has the pair (d, d + 1)
+          // of one head, rotates it, and for bf16 four lanes swap pairs: 8 bytes of a head a lane, 4 heads a
+          // store. (A value a lane and store took 8600 cycles for the query's 64 KB.)
+          const bool odd = lane & 1, upper = lane & 2;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            float xo = v[c] * inv[c];
-            if (do_rope) {
-              // the pair (d, d+1) sits in lanes (even, odd)
-              const float other = __shfl_xor_sync(0xffffffffu, xo, 1);
-              float y0, y1;
-              if ((d & 1) == 0) {
-                rotate_pair(xo, other, cs, sn, true, &y0, &y1);
-                xo = y0;
-              } else {
-                rotate_pair(other, xo, cs, sn, true, &y0, &y1);
-                xo = y1;
-              }
+          for (int c = 0; c < 32; c += 4) {
+            float y[2], z[2];  // heads c + odd, c + 2 + odd
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float a = v[c + 2 * k] * inv[c + 2 * k], b = v[c + 2 * k + 1] * inv[c + 2 * k + 1];
+              const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+              y[k] = odd ? other : a;
+              z[k] = odd ? b : other;
+              if (do_rope) rotate_pair(y[k], z[k], cs, sn, true, &y[k], &z[k]);
             }
-            const int64_t off = (qi * P.h + half * 32 + c) * D + d;
-            if (bf)
-              reinterpret_cast<__nv_bfloat16*>(P.out)[off] = __float2bfloat16_rn(xo);
-            else
-              reinterpret_cast<float*>(P.out)[off] = xo;
+            const int64_t row0 = (qi * P.h + half * 32 + c + odd) * D;
+            if (bf) {
+              const uint32_t p0 = pack_bf16x2(y[0], z[0]), p1 = pack_bf16x2(y[1], z[1]);
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, upper ? p0 : p1, 2);
+              *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + row0 + (upper ? 2 * D : 0) + (d & ~3)) =
+                  upper ? make_uint2(other, p1) : make_uint2(p0, other);
+            } else {
+              float* o = reinterpret_cast<float*>(P.out) + row0 + (d & ~1);
+              *reinterpret_cast<float2*>(o) = make_float2(y[0], z[0]);
+              *reinterpret_cast<float2*>(o + 2 * D) = make_float2(y[1], z[1]);
+            }
           }
         }
       }
@@ -587,7 +613,6 @@ int dsv4_sparse_attn_tc(const dsv4_sparse_attn_params* p, int splits, float* par
   P.n = p->n;
   P.h = p->h;
   P.t = p->t;
-  P.idx_dtype = p->idx_dtype;
   P.out_dtype = p->out_dtype;
   P.scale_log2 = p->scale * tc::LOG2E;
   P.rope_freqs = p->rope_freqs;
@@ -601,10 +626,12 @@ int dsv4_sparse_attn_tc(const dsv4_sparse_attn_params* p, int splits, float* par
   DSV4_CHECK_ARG((reinterpret_cast<uintptr_t>(p->kv) & 15) == 0, "dsv4_sparse_attn: kv must be 16-byte aligned");
   P.kv = reinterpret_cast<const __nv_bfloat16*>(p->kv);
   const int smem = static_cast<int>(sizeof(tc::Smem)) + 1024;
-  static PerDeviceOnce attr;
-  DSV4_CUDA_CHECK(set_smem_once(attr, tc::attn_tc_kernel, smem));
+  static PerDeviceOnce attr[2];
+  const bool wide = p->idx_dtype == DSV4_I64;
+  void (*const k)(tc::Params) = wide ? tc::attn_tc_kernel<true> : tc::attn_tc_kernel<false>;
+  DSV4_CUDA_CHECK(set_smem_once(attr[wide], k, smem));
   DSV4_CHECK_ARG(splits >= 1 && (splits == 1 || part != nullptr), "dsv4_sparse_attn: split partials need a workspace");
-  tc::attn_tc_kernel<<<static_cast<unsigned>(p->s * splits), tc::THREADS, smem, as_stream(stream)>>>(P);
-  DSV4_LAUNCH_CHECK("attn_tc_kernel");
+  DSV4_CUDA_CHECK(launch_pdl(k, dim3(static_cast<unsigned>(p->s * splits)), dim3(tc::THREADS), smem,
+                             as_stream(stream), P));
   return DSV4_OK;
 }

@@ -53,9 +53,10 @@ __global__ void chunk_rows_kernel(dsv4_chunk c, int32_t* positions, int64_t* sta
 
 // one CTA per (sequence, ring slot): the slot's newest token of the chunk, if it has one. A slot named
 // twice has no newest token: DSV4_ERR_INDEX_OUT_OF_RANGE, and the first to name it has the ring.
+// No early launch of the next kernel: the decode attention reads window rows before it waits for the
+// kernel before it, and counts on those that wrote them being complete.
 __global__ void chunk_commit_kernel(dsv4_chunk c, uint4* pool, int row16) {
   pdl_wait();
-  pdl_trigger();
   const int b = blockIdx.y, j = blockIdx.x;
   const int first = c.cu_seqlens[b], last = c.cu_seqlens[b + 1];
   const int slot = c.seqs ? c.seqs[b] : b;

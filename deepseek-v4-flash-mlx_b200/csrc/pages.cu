@@ -302,10 +302,10 @@ __device__ __forceinline__ void copy_unit(const uint8_t* src, uint8_t* dst, int 
     if (static_cast<int>(threadIdx.x) + i * COPY < n16) __stcs(d + threadIdx.x + i * COPY, v[i]);
 }
 
-// A CTA takes neighbouring units: it looks its first part up and walks on from there.
+// A CTA takes neighbouring units: it looks its first part up and walks on from there. No early launch of
+// the next kernel: the decode attention reads window rows before it waits for the kernel before it.
 __global__ void __launch_bounds__(COPY) fork_copy_kernel(dsv4_pages p, int n, Fork* forks) {
   pdl_wait();
-  pdl_trigger();
   const int64_t* starts = unit_starts(forks, n);
   const int parts = n * (SEGS + 1);
   const int64_t units = starts[parts];
