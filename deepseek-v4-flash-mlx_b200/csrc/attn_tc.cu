@@ -40,6 +40,8 @@ constexpr int SM_WARP0 = 4;                 // first softmax warp
 constexpr int SM_THREADS = 256;             // softmax warps 4-11 (warp w: lane quadrant w % 4)
 constexpr int W_WARP0 = 1, W_THREADS = 352;  // gather workers: warps 1-11
 constexpr int W_CHUNKS = 6;                 // ceil(128 rows x 16 chunks per slab pair / 352)
+constexpr int W_ROWS = W_THREADS / 16;      // a worker's chunks of a slab pair are W_ROWS rows apart, in one column
+static_assert(W_THREADS % 16 == 0, "a worker stays in its column");
 constexpr int SLAB_Q = HB * 128;            // 8 KB: one 64-dim slab of Q (64 rows x 128 B)
 constexpr int SLAB_KV = BN * 128;           // 16 KB: one 64-dim slab of the tile (128 rows x 128 B)
 constexpr int TMEM_COLS = 512;
@@ -88,12 +90,12 @@ struct List {
   int64_t win;            // its window's first pool row
   int window, len;        // implicit rows, all entries
   int first, sp, linear;  // window entry u: linear: row first + u while <= sp; else ring slot from sp + 1 on
-  int64_t n;
+  int32_t n;              // rows of the pool (below 2^31)
 
   __device__ __forceinline__ List(const Params& P, int64_t qi) {
     window = P.window;
     len = window + P.t;
-    n = P.n;
+    n = static_cast<int32_t>(P.n);
     idx = reinterpret_cast<const int32_t*>(P.idx) + (WIDE ? 2 : 1) * (qi * P.t);
     win = 0;
     first = sp = 0;
@@ -119,24 +121,16 @@ struct List {
     }
     return w;
   }
-  // its pool row, -1 if masked; an index past the pool raises the error word
-  __device__ __forceinline__ int32_t row(int u, Raw w) const {
+  // its pool row, -1 if masked; an index past the pool is masked too, and noted in *bad
+  __device__ __forceinline__ int32_t row(int u, Raw w, bool* bad) const {
     if (u >= len) return -1;
-    int64_t v;
     if (u < window) {
-      if (linear)
-        v = first + u <= sp ? win + first + u : -1;
-      else
-        v = win + (u < window - sp - 1 ? sp + 1 + u : u - (window - sp - 1));
-    } else {
-      v = WIDE ? static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(w.hi)) << 32 | static_cast<uint32_t>(w.lo))
-               : static_cast<int64_t>(w.lo);
+      if (linear) return first + u <= sp ? static_cast<int32_t>(win + first + u) : -1;
+      return static_cast<int32_t>(win + (u < window - sp - 1 ? sp + 1 + u : u - (window - sp - 1)));
     }
-    if (v >= n) {
-      raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-      v = -1;
-    }
-    return static_cast<int32_t>(v < 0 ? -1 : v);
+    const bool over = WIDE ? w.hi > 0 || (w.hi == 0 && (w.lo < 0 || w.lo >= n)) : w.lo >= n;
+    *bad |= over;
+    return over || (WIDE ? w.hi < 0 : w.lo < 0) ? -1 : w.lo;
   }
 };
 
@@ -226,19 +220,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(const __grid_consta
     sm.abort = 0;
     bar_init_fence();
   }
-  // gather workers (warps 1-11): this worker's (row, chunk) positions within a slab pair: c = wt + 352 k
-  // < 2048; row c / 16, chunk c % 16 (slab 2mt + chunk / 8, 16-byte chunk chunk % 8 of the row's 128 B)
-  const int wt = tid - W_WARP0 * 32;
-  int nown = 0;
-#pragma unroll
-  for (int k = 0; k < W_CHUNKS; ++k) nown += (wt + W_THREADS * k < BN * 16);
+  // gather workers (warps 1-11): this worker's rows r0 + W_ROWS k < 128 of a slab pair, of each the 16-byte
+  // chunk wj (slab 2 mt + wj / 8, chunk wj % 8 of the row's 128 B)
+  const int wt = tid - W_WARP0 * 32, r0 = wt >> 4, wj = wt & 15;
   pdl_wait();  // the kernel before is complete from here
   const List<WIDE> list(P, qi);
   typename List<WIDE>::Raw raw[W_CHUNKS], raw_s = {0, 0};  // of the next tile: this worker's rows, this softmax thread's row
   auto ask_rows = [&](int i) {
 #pragma unroll
     for (int k = 0; k < W_CHUNKS; ++k)
-      if (k < nown) raw[k] = list.ask((tbase + i) * BN + ((wt + W_THREADS * k) >> 4));
+      if (r0 + W_ROWS * k < BN) raw[k] = list.ask((tbase + i) * BN + r0 + W_ROWS * k);
     if (warp >= SM_WARP0) raw_s = list.ask((tbase + i) * BN + (warp & 3) * 32 + lane);
   };
   // Q -> 8 swizzled slabs (64 heads x 128 B), by the gather workers: their arrivals on the first tile's
@@ -309,7 +300,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(const __grid_consta
   } else {
     // ---------------------------------------------------------------- gather workers (warps 1-11)
     const bool smx = warp >= SM_WARP0;
-    const uint32_t ks = smem_u32(sm.kv);
+    const uint32_t kd = smem_u32(sm.kv) + static_cast<uint32_t>((wj >> 3) * SLAB_KV + r0 * 128);
+    const __nv_bfloat16* const kg = P.kv + wj * 8;
 
     // softmax state (warps 4-11)
     const int qd = warp & 3;                    // TMEM lane quadrant: rows / dims qd*32 + lane
@@ -319,7 +311,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(const __grid_consta
     float m[32];
 #pragma unroll
     for (int c = 0; c < 32; ++c) m[c] = -INFINITY;
-    bool valid = false;
+    bool valid = false, bad = false;
     if (smx) {
       {  // the ones operand (bf16 pairs) of the L MMA
         float ones[16];
@@ -333,35 +325,37 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(const __grid_consta
       before_sync();
       sm_bar();
     }
-    bool ok = true;
-    for (int i = 0; i < ntiles; ++i) {
-      // the tile's rows have been asked for a tile ahead; the next tile's are asked for before this one is fetched
+    bool ok = true, next_valid = false;
+    auto find_rows = [&](int i) {
 #pragma unroll
       for (int k = 0; k < W_CHUNKS; ++k)
-        if (k < nown) rr[k] = list.row((tbase + i) * BN + ((wt + W_THREADS * k) >> 4), raw[k]);
-      if (smx) valid = list.row((tbase + i) * BN + row, raw_s) >= 0;
-      if (i + 1 < ntiles) ask_rows(i + 1);
+        if (r0 + W_ROWS * k < BN) rr[k] = list.row((tbase + i) * BN + r0 + W_ROWS * k, raw[k], &bad);
+      if (smx) next_valid = list.row((tbase + i) * BN + row, raw_s, &bad) >= 0;
+    };
+    if (ntiles > 0) find_rows(0);
+    for (int i = 0; i < ntiles; ++i) {
+      valid = next_valid;
       // gather tile i, pair by pair
       for (int mt = 0; mt < 4 && ok; ++mt) {
         if (i > 0) ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.bar_empty[mt], (i - 1) & 1, abort));
         if (!ok) break;
 #pragma unroll
         for (int k = 0; k < W_CHUNKS; ++k) {
-          if (k < nown) {
-            const int c = wt + W_THREADS * k;
-            const int r = c >> 4, j = c & 15;
-            const int sl = 2 * mt + (j >> 3), ch = j & 7;
-            cp_async16(ks + static_cast<uint32_t>(sl * SLAB_KV + r * 128 + ((ch ^ (r & 7)) << 4)),
-                       P.kv + static_cast<int64_t>(max(rr[k], 0)) * D + sl * 64 + ch * 8, rr[k] >= 0);
-          }
+          const int r = r0 + W_ROWS * k;
+          if (r < BN)
+            cp_async16(kd + static_cast<uint32_t>(2 * mt * SLAB_KV + W_ROWS * k * 128 + ((wj ^ r) & 7) * 16),
+                       kg + static_cast<int64_t>(max(rr[k], 0)) * D + mt * 128, rr[k] >= 0);
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(&sm.bar_full[mt]))
                      : "memory");
+        // the next tile's row numbers, asked for and taken up while others are waited for
+        if (mt == 0 && i + 1 < ntiles) ask_rows(i + 1);
       }
       if (!ok) {
         if (lane == 0) set_abort(sm);
         if (!smx) break;
       }
+      if (i + 1 < ntiles) find_rows(i + 1);
       if (!smx) continue;
 
       // ---------------------------------------------------------- softmax of tile i (warps 4-11)
@@ -455,6 +449,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(const __grid_consta
       bar_arrive(&sm.bar_p);
     }
 
+    if (bad) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
     if (smx) {
       if (ok) {
         ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.bar_fin, 0, abort));
