@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(PLAN) reserve_kernel(dsv4_pages p, const int32
 // ---- a branch: what one (src, dst) pair copies
 struct Fork {
   int32_t src, dst, entries, ok;
-  int32_t from, to;  // the partly filled last page and its copy, -1: none
+  int32_t from, to;    // the partly filled last page and its copy, -1: none
+  int32_t lead, next;  // the first branch that copies the same, the one after this, -1: none
 };
 
 struct Part {
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(PLAN) fork_plan_kernel(dsv4_pages p, const int
     bad = __any_sync(0xffffffffu, bad);
     if (lane == 0) {
       if (bad) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
-      forks[k] = {a, b, e, bad ? 0 : 1, -1, -1};
+      forks[k] = {a, b, e, bad ? 0 : 1, -1, -1, 0, -1};
     }
   }
   __syncthreads();
@@ -256,6 +257,20 @@ __global__ void __launch_bounds__(PLAN) fork_plan_kernel(dsv4_pages p, const int
   for (int k = w; k < n; k += PLAN / 32) {
     const Fork f = forks[k];
     if (!f.ok) continue;
+    // the other branches of what this one copies
+    bool before = false;
+    int next = -1;
+    for (int i0 = 0; i0 < n && next < 0; i0 += 32) {
+      const int i = i0 + lane;
+      const bool same = i < n && forks[i].ok && forks[i].src == f.src && forks[i].entries == f.entries;
+      before |= __any_sync(0xffffffffu, same && i < k);
+      const uint32_t after = __ballot_sync(0xffffffffu, same && i > k);
+      if (after != 0) next = i0 + __ffs(after) - 1;
+    }
+    if (lane == 0) {
+      forks[k].lead = !before;
+      forks[k].next = next;
+    }
     const int32_t* ra = p.block_table + static_cast<int64_t>(f.src) * p.bt_stride;
     int32_t* rb = p.block_table + static_cast<int64_t>(f.dst) * p.bt_stride;
     const int full = f.entries / p.page;
@@ -272,13 +287,14 @@ __global__ void __launch_bounds__(PLAN) fork_plan_kernel(dsv4_pages p, const int
         }
     }
   }
+  __syncthreads();
   // copy units before each part
   int64_t before = 0;
   const int parts = n * (SEGS + 1);
   for (int base = 0; base < parts; base += PLAN) {
     const int i = base + threadIdx.x;
     int units = 0;
-    if (i < parts && forks[i / (SEGS + 1)].ok)
+    if (i < parts && forks[i / (SEGS + 1)].lead)
       units = static_cast<int>((part_bytes(p, forks[i / (SEGS + 1)], i % (SEGS + 1)) + UNIT - 1) / UNIT);
     int total;
     const int r = block_scan(units, &total);
@@ -289,20 +305,26 @@ __global__ void __launch_bounds__(PLAN) fork_plan_kernel(dsv4_pages p, const int
 }
 
 // up to UNIT bytes (a multiple of 16): all of a thread's loads before its first store
-__device__ __forceinline__ void copy_unit(const uint8_t* src, uint8_t* dst, int bytes) {
-  const uint4* s = reinterpret_cast<const uint4*>(src);
-  uint4* d = reinterpret_cast<uint4*>(dst);
-  const int n16 = bytes / 16;
+struct Piece {
   uint4 v[UNIT / 16 / COPY];
+  __device__ __forceinline__ void load(const uint8_t* src, int bytes) {
+    const uint4* s = reinterpret_cast<const uint4*>(src) + threadIdx.x;
+    const int n16 = bytes / 16 - static_cast<int>(threadIdx.x);
 #pragma unroll
-  for (int i = 0; i < UNIT / 16 / COPY; ++i)
-    if (static_cast<int>(threadIdx.x) + i * COPY < n16) v[i] = __ldcs(s + threadIdx.x + i * COPY);
+    for (int i = 0; i < UNIT / 16 / COPY; ++i)
+      if (i * COPY < n16) v[i] = __ldcs(s + i * COPY);
+  }
+  __device__ __forceinline__ void store(uint8_t* dst, int bytes) const {
+    uint4* d = reinterpret_cast<uint4*>(dst) + threadIdx.x;
+    const int n16 = bytes / 16 - static_cast<int>(threadIdx.x);
 #pragma unroll
-  for (int i = 0; i < UNIT / 16 / COPY; ++i)
-    if (static_cast<int>(threadIdx.x) + i * COPY < n16) __stcs(d + threadIdx.x + i * COPY, v[i]);
-}
+    for (int i = 0; i < UNIT / 16 / COPY; ++i)
+      if (i * COPY < n16) __stcs(d + i * COPY, v[i]);
+  }
+};
 
-// A CTA takes neighbouring units: it looks its first part up and walks on from there. No early launch of
+// A CTA takes neighbouring units: it looks its first part up and walks on from there. A unit is read once for
+// all branches of it (eight branches of 16384 entries: 30.7 us when each read it, with HBM at 40%). No early launch of
 // the next kernel: the decode attention reads window rows before it waits for the kernel before it.
 __global__ void __launch_bounds__(COPY) fork_copy_kernel(dsv4_pages p, int n, Fork* forks) {
   pdl_wait();
@@ -322,11 +344,16 @@ __global__ void __launch_bounds__(COPY) fork_copy_kernel(dsv4_pages p, int n, Fo
   }
   while (u < u1) {
     while (starts[lo + 1] <= u) ++lo;  // u < units = starts[parts]
-    const Part q = part(p, forks[lo / (SEGS + 1)], lo % (SEGS + 1));
+    const int lead = lo / (SEGS + 1), seg = lo % (SEGS + 1);
+    const Part q = part(p, forks[lead], seg);
     const int64_t first = starts[lo], end = min(starts[lo + 1], u1);
     for (; u < end; ++u) {
       const int64_t off = (u - first) * UNIT;
-      copy_unit(q.src + off, q.dst + off, static_cast<int>(min(static_cast<int64_t>(UNIT), q.bytes - off)));
+      const int bytes = static_cast<int>(min(static_cast<int64_t>(UNIT), q.bytes - off));
+      Piece x;
+      x.load(q.src + off, bytes);
+      x.store(q.dst + off, bytes);
+      for (int k = forks[lead].next; k >= 0; k = forks[k].next) x.store(part(p, forks[k], seg).dst + off, bytes);
     }
   }
 }
@@ -386,8 +413,10 @@ __global__ void __launch_bounds__(COPY) compact_copy_kernel(dsv4_pages p, const 
   uint8_t* base = reinterpret_cast<uint8_t*>(p.pool) + p.comp_base * p.head_dim * 2;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int64_t k = u / per, off = (u - k * per) * UNIT;
-    copy_unit(base + movers[nl - nm + k] * bytes + off, base + holes[k] * bytes + off,
-              static_cast<int>(min(static_cast<int64_t>(UNIT), bytes - off)));
+    const int some = static_cast<int>(min(static_cast<int64_t>(UNIT), bytes - off));
+    Piece x;
+    x.load(base + movers[nl - nm + k] * bytes + off, some);
+    x.store(base + holes[k] * bytes + off, some);
   }
   const int64_t cells = static_cast<int64_t>(p.slots) * p.bt_stride;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * COPY + threadIdx.x; i < cells;
