@@ -9,6 +9,9 @@ Drop-in ops with the reference's call signatures (ref_torch / v4mlx), each a tor
   q_down, perhead_norm, q_up, kv_proj,        v4mlx/mla.py
   o_grouped
   indexer_topk                                lightning-indexer selection (absent from the reference)
+  chunk_rows, compressor_chunk,               several new tokens of several sequences at once over the
+  chunk_attention, chunk_commit               decode cache (oracle/v4_fast.py:82-122 in a loop)
+  pages_reserve / free / fork / compact       pages of a cache that sequences share (oracle/v4_fast.py:150-159)
 
 There is no CPU path: the ops raise on CPU tensors and when libdsv4.so is missing.
 """

@@ -24,6 +24,9 @@
 //    and the epilogue. The running maximum m is lazy: it is recomputed (exact tile maximum per head)
 //    only when some score exceeds m + 8 (log2 units) or on the first tile, in which case O^T and L
 //    are rescaled in TMEM; otherwise p may reach 2^8, which bf16 P and the fp32 sums absorb.
+// Measured on a B200: 4096 queries of 1152 rows 1.06 ms (585 TFLOP/s, the tensor pipe active 31% of the time),
+// 256 queries of 640 rows 49.8 us. A tile takes 6100 cycles, 3364 of them MMAs (N = 64 reads shared memory at its
+// full rate): the gather of the next tile, S^T, the softmax and O^T follow one another in the single buffer.
 // The sink enters only the denominator, as in ref_torch/sparse_attn.py:33. All waits are bounded
 // (1 s); a timeout raises DSV4_ERR_WAIT_TIMEOUT, the roles stop, and the CTA drains what it issued.
 #include "common.cuh"

@@ -6,7 +6,7 @@
 // tokens of the same chunk still see. So the chunk's rows are staged behind the pages of the pool,
 // token i of the chunk at row stage_base + i, and reach the ring only after the attention.
 //
-// All three kernels move a few words per token and are bound by their launch.
+// Both kernels move a few words or rows per token and are bound by their launch (256 lists of 640 entries: 4.8 us).
 #include "chunk.cuh"
 #include "common.cuh"
 

@@ -24,6 +24,11 @@
  *   dsv4_indexer_topk         <- no reference code: the reference attends to every visible compressed row
  *                                (oracle/decode_engine.py:112-114); this is the lightning-indexer selection
  *                                that replaces that list when more than top_k rows are visible.
+ *   dsv4_chunk_attn, dsv4_chunk_rows, dsv4_chunk_commit, dsv4_compressor_chunk
+ *                             <- oracle/v4_fast.py:82-122 (the decode step's rows, ring, list and attention)
+ *                                in a loop over several tokens of several sequences
+ *   dsv4_pages_*              <- no reference code: the reference copies whole states
+ *                                (oracle/v4_fast.py:150-159 clone_states)
  *   dsv4_decode_window_indices<- oracle/v4_fast.py:108-117 (window rows of the attended list, ring order
  *                                of ref_torch/sparse_attn.py:11-13)
  */
