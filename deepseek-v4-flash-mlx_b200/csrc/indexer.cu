@@ -419,12 +419,14 @@ constexpr int SEL_BINS = 4096;
 constexpr int SEL_RANK_MAX = 1024;   // candidates resolved by O(c^2) rank counting up to this many
 static_assert(SEL_BINS % SEL_THREADS == 0, "whole bins per thread");
 
+// the pool row of key j; -1 for a key whose page the sequence does not have (a paged cache that ran out:
+// reported when the page was asked for)
 __device__ __forceinline__ int32_t map_key(const SelectParams& P, int b, int j) {
   int64_t row;
   if (P.block_table != nullptr) {
-    int pg = j / P.page;
-    row = static_cast<int64_t>(P.block_table[static_cast<int64_t>(b) * P.table_stride + pg]) * P.page +
-          (j % P.page);
+    const int32_t pg = P.block_table[static_cast<int64_t>(b) * P.table_stride + j / P.page];
+    if (pg < 0) return -1;
+    row = static_cast<int64_t>(pg) * P.page + (j % P.page);
   } else {
     row = j;
   }
@@ -447,14 +449,15 @@ struct KeyMap {
       const int pg0 = min(j0 / P.page, last);
       const int pg1 = min((j0 + per - 1) / P.page, last);
       const int32_t* t = P.block_table + static_cast<int64_t>(b) * P.table_stride;
-      off0 = (static_cast<int64_t>(__ldg(t + pg0)) - pg0) * P.page + P.out_offset;
-      off1 = (static_cast<int64_t>(__ldg(t + pg1)) - pg1) * P.page + P.out_offset;
+      const int32_t a0 = __ldg(t + pg0), a1 = __ldg(t + pg1);
+      off0 = a0 < 0 ? INT64_MIN / 2 : (static_cast<int64_t>(a0) - pg0) * P.page + P.out_offset;
+      off1 = a1 < 0 ? INT64_MIN / 2 : (static_cast<int64_t>(a1) - pg1) * P.page + P.out_offset;
       split = (pg0 + 1) * P.page;
     }
   }
   __device__ __forceinline__ int32_t map(const SelectParams& P, int b, int j) const {
     if (!direct) return map_key(P, b, j);
-    return static_cast<int32_t>(j + (j < split ? off0 : off1));
+    return static_cast<int32_t>(max(static_cast<int64_t>(-1), j + (j < split ? off0 : off1)));
   }
 };
 

@@ -698,3 +698,63 @@ def test_extend_by_nothing():
         assert blk.extend(x, lengths, start).shape == x.shape
     for k, v in blk.cache.state_dict().items():
         assert torch.equal(v, before[k]), k
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("window", [False, True])
+def test_listed_rows_that_are_masked_may_hold_anything(dtype, window):
+    """The gathered kernel: row 0 of the pool and the rows that no list names hold no numbers, and masked entries
+    stand everywhere in the lists."""
+    S = importlib.import_module(PKG + ".sparse_attn")
+    _, _, L = _mods()
+    g = torch.Generator(device="cuda").manual_seed(50)
+    n, s, t = 900, 20, 300
+    pool = torch.randn(n, D, generator=g, device="cuda").to(torch.bfloat16)
+    idx = torch.randint(200, n, (s, t), generator=g, device="cuda")
+    idx[torch.rand(s, t, generator=g, device="cuda") < 0.4] = -1
+    idx[3], idx[4, :200] = -1, -1
+    idx[3, 299] = 777
+    named = torch.zeros(n, dtype=torch.bool, device="cuda")
+    named[idx[idx >= 0]] = True
+    pos = torch.arange(20, 20 + s, dtype=torch.int32, device="cuda")
+    if window:
+        named[1:129] = True                     # the ring's rows 1 ..
+    pool[~named] = torch.tensor([float("nan"), float("inf"), -float("inf")], device="cuda").to(torch.bfloat16)[
+        torch.arange(int((~named).sum()), device="cuda") % 3][:, None]
+    q = torch.randn(s, H, D, generator=g, device="cuda").to(torch.bfloat16) / 4
+    sink, f = torch.randn(H, generator=g, device="cuda"), _freqs().cuda()
+    out = torch.empty(s, H, D, dtype=torch.bfloat16, device="cuda")
+    kw = dict(window=128, win_base=torch.ones(s, dtype=torch.int64, device="cuda")) if window else {}
+    S.sparse_attn_into(out, q, pool, sink, idx.to(dtype), D ** -0.5, f, pos, 64, kernel=2, **kw)
+    assert L.device_error() == 0
+    kv, want, tol = pool.double(), [], []
+    for i in range(s):
+        r = idx[i][idx[i] >= 0]
+        if window:
+            r = torch.cat([1 + torch.arange(int(pos[i]) + 1, device="cuda"), r])
+        x = torch.cat([q[i].double() @ kv[r].T * D ** -0.5, sink.double()[:, None]], 1)
+        w = torch.softmax(x, -1)[:, :-1]
+        a = w @ kv[r].abs()
+        a[:, -64:] = a[:, -64:] + a[:, -64:].reshape(H, 32, 2).flip(-1).reshape(H, 64)
+        want.append(_rotate64((w @ kv[r])[None], pos[i:i + 1], f, -1)[0])
+        tol.append(4 * EPS * a)
+    _check(out, torch.stack(want), torch.stack(tol))
+
+
+def test_a_replay_takes_what_its_tensors_then_hold():
+    """Lengths, positions, slots and the table are read on the device: one captured chunk serves others that fit."""
+    pkg, _, L = _mods()
+    c, q, sink, cu, st, sq = _case([5, 3], [900, 40], seed=51, seqs=[1, 0], slots=3, pad=2)
+    f = _freqs().cuda()
+    pkg.chunk_attention(c, q, sink, cu, st, seqs=sq, freqs=f)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        pos, rows = pkg.chunk_rows(c, cu, st, 10, sq)
+        o = pkg.chunk_attention(c, q, sink, cu, st, seqs=sq, freqs=f)
+    for lens, start, seqs in (([5, 3], [900, 40], [1, 0]), ([1, 9], [700, 3], [2, 1]), ([0, 4], [5, 0], [0, 2]), ([10, 0], [333, 1], [0, 0])):
+        cu.copy_(torch.tensor([0, lens[0], sum(lens)])), st.copy_(torch.tensor(start)), sq.copy_(torch.tensor(seqs))
+        gr.replay()
+        assert L.device_error() == 0
+        assert pos.tolist() == [p + i for n, p in zip(lens, start) for i in range(n)] + [0] * (10 - sum(lens))
+        _check(o, *_attention64(c, q, sink, lens, start, seqs))

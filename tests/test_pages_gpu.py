@@ -365,3 +365,62 @@ def test_compact_with_a_cell_that_is_not_counted():
     assert c.compact().item() == 1
     assert c.block_table.tolist() == [[-1, -1], [0, -1], [-1, -1]] and c.page_refs.tolist() == [1, 0, 0, 0, 0, 0]
     assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("n_keys,page", [(300, 8), (300, 64), (5000, 64), (20000, 8), (20000, 256)])
+def test_selection_leaves_out_keys_without_a_page(n_keys, page, rows):
+    """Every visible key selected: those on pages that the sequence has, mapped to their rows, and -1 for the
+    others (a cache that ran out of pages may hold keys whose rows were never stored)."""
+    I = importlib.import_module(PKG + ".indexer")  # noqa: E741
+    _, _, L = _mods()
+    g = torch.Generator(device="cuda").manual_seed(n_keys + page)
+    q, w = torch.randn(1, rows, 64, 128, generator=g, device="cuda"), torch.randn(1, rows, 64, generator=g, device="cuda")
+    k = torch.randn(1, n_keys, 128, generator=g, device="cuda")
+    pages = -(-n_keys // page)
+    table = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table[torch.rand(pages, generator=g, device="cuda") < 0.3] = -1
+    pos = torch.full((1, rows), 4 * n_keys, dtype=torch.int32, device="cuda")
+    out = torch.empty(1, rows, n_keys, dtype=torch.int32, device="cuda")
+    I.indexer_topk_into(out, q, w, k, n_keys, positions=pos, ratio=4, out_offset=1000, block_table=table[None], page=page)
+    j = torch.arange(n_keys, device="cuda")
+    pg = table[j // page]
+    want = torch.where(pg >= 0, 1000 + pg * page + (j % page).to(torch.int32), -1).sort().values.to(torch.int32)
+    assert torch.equal(out[0].sort(-1).values, want.expand(rows, -1)) and L.device_error() == 0
+
+
+def test_forks_of_one_source_at_several_lengths():
+    """More branches than a warp looks at together, some of the same rows (read once for all), some shorter, some
+    refused."""
+    c = _cache(45, 96, 16, 200, seed=9)
+    c.reserve([0, 1], [384, 200])
+    m = Model(c)
+    src = [0 if k % 3 else 1 for k in range(40)]
+    tokens = [200 if s == 1 else (384, 100, 131, 64)[k % 4] for k, s in enumerate(src)]
+    dst = list(range(2, 42))
+    m.fork(src, dst, tokens)
+    at = 20                                   # and one onto a slot that has pages, left out alone
+    c.fork(src[:at] + [0] + src[at:], dst[:at] + [1] + dst[at:], tokens[:at] + [384] + tokens[at:])
+    assert _mods()[2].device_error() == OUT_OF_RANGE
+    m.check()
+
+
+def test_serving_runner_on_a_paged_cache():
+    """The captured step hands out its pages at every replay: the runner's outputs are those of a fixed cache."""
+    Lm = importlib.import_module(PKG + ".layer")
+    _, _, L = _mods()
+    Wt = Lm.make_attention_weights(61).to("cuda")
+    runs = [Lm.BlockRunner(Lm.DecodeBlock(Wt, 2, 256, page=8, **kw)) for kw in ({}, dict(n_pages=9))]
+    x = torch.randn(90, 2, 4096, generator=torch.Generator().manual_seed(2))
+    for p in range(90):
+        outs = []
+        for r in runs:
+            hx, hp = r.host_inputs()
+            hx.copy_(x[p]), hp.copy_(torch.tensor([p, p + 40], dtype=torch.int32))
+            o = r.step_host()
+            r.synchronize()
+            outs.append(o.clone())
+        assert torch.equal(*outs), p
+    assert L.device_error() == 0
+    t = runs[1].block.cache.block_table
+    assert (t >= 0).sum(1).tolist() == [3, 4]   # 22 and 32 entries
