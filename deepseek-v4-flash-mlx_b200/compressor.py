@@ -271,14 +271,15 @@ def _(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out,
 
 def _chunk_into(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, page, out_base,
                 max_comp, head_dim, ratio, rope_head_dim, freqs, eps, key_image, key_inv, key_norm_max, act_quant):
-    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     p = L.CompressorChunkParams(
-        kv.data_ptr(), score.data_ptr(), ape.data_ptr(), at(norm_w), ring_kv.data_ptr(), ring_score.data_ptr(), out.data_ptr(),
-        freqs.data_ptr(), cu_seqlens.data_ptr(), start.data_ptr(), at(seqs), at(block_table), out_base, out.numel() // head_dim,
-        cu_seqlens.numel() - 1, kv.shape[0], ring_kv.shape[0], block_table.shape[1] if block_table is not None else 0,
-        page if block_table is not None else 1, max_comp, head_dim, ratio, rope_head_dim,
-        L.dtype_code(norm_w) if norm_w is not None else L.F32, L.dtype_code(out), act_quant, eps, at(key_image), at(key_inv),
-        at(key_norm_max))
+        kv.data_ptr(), score.data_ptr(), ape.data_ptr(), None if norm_w is None else norm_w.data_ptr(), ring_kv.data_ptr(),
+        ring_score.data_ptr(), out.data_ptr(), freqs.data_ptr(), cu_seqlens.data_ptr(), start.data_ptr(),
+        None if seqs is None else seqs.data_ptr(), None if block_table is None else block_table.data_ptr(), out_base,
+        out.numel() // head_dim, cu_seqlens.numel() - 1, kv.size(0), ring_kv.size(0),
+        0 if block_table is None else block_table.size(1), 1 if block_table is None else page, max_comp, head_dim, ratio,
+        rope_head_dim, L.F32 if norm_w is None else L.dtype_code(norm_w), L.dtype_code(out), act_quant, eps)
+    if key_image is not None:
+        p.key_image, p.key_inv, p.key_norm_max = key_image.data_ptr(), key_inv.data_ptr(), key_norm_max.data_ptr()
     with L.device_of(kv):
         L.check(L.lib().dsv4_compressor_chunk(ctypes.byref(p), L.stream_of(kv)))
 
@@ -300,38 +301,42 @@ def compressor_chunk(proj, cu_seqlens, start, ape, norm_w, ring_kv, ring_score, 
     `rotate` as in `compressor_decode_step`. The custom op `dsv4::compressor_chunk`."""
     kv, score = proj
     L.require_cuda(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, freqs)
-    if kv.dtype != torch.float32 or score.dtype != torch.float32 or kv.shape != score.shape or kv.dim() != 2 or \
-            kv.shape[1] != 2 * head_dim:
+    f32 = torch.float32
+    if kv.dtype != f32 or score.dtype != f32 or kv.shape != score.shape or kv.dim() != 2 or kv.size(1) != 2 * head_dim:
         raise ValueError(f"compressor_chunk: kv and score must be float32 [total, {2 * head_dim}]")
-    for name, r in (("ring_kv", ring_kv), ("ring_score", ring_score)):
-        if r.dtype != torch.float32 or r.dim() != 3 or r.shape[1:] != (2 * ratio, 2 * head_dim) or not r.is_contiguous():
-            raise ValueError(f"compressor_chunk: {name} must be contiguous float32 [slots, {2 * ratio}, {2 * head_dim}]")
-    if ring_kv.shape[0] != ring_score.shape[0]:
-        raise ValueError("compressor_chunk: ring_kv and ring_score have different slots")
-    if out.shape[-1] != head_dim or not out.is_contiguous() or out.dtype not in (torch.float32, torch.bfloat16):
+    if ring_kv.dtype != f32 or ring_kv.dim() != 3 or ring_kv.size(1) != 2 * ratio or ring_kv.size(2) != 2 * head_dim or \
+            not ring_kv.is_contiguous():
+        raise ValueError(f"compressor_chunk: ring_kv must be contiguous float32 [slots, {2 * ratio}, {2 * head_dim}]")
+    if ring_score.dtype != f32 or ring_score.shape != ring_kv.shape or not ring_score.is_contiguous():
+        raise ValueError("compressor_chunk: ring_score must be contiguous float32 of ring_kv's shape")
+    if out.size(-1) != head_dim or not out.is_contiguous() or (out.dtype != torch.bfloat16 and out.dtype != f32):
         raise ValueError(f"compressor_chunk: out must be contiguous rows of {head_dim} float32 or bfloat16")
-    n, slots = cu_seqlens.numel() - 1, ring_kv.shape[0]
+    n, slots = cu_seqlens.numel() - 1, ring_kv.size(0)
     if n < 0 or start.numel() != n or (seqs is not None and seqs.numel() != n) or (seqs is None and n > slots):
         raise ValueError(f"compressor_chunk: cu_seqlens, start and seqs name {n}, {start.numel()} and "
                          f"{None if seqs is None else seqs.numel()} sequences ({slots} slots)")
-    for name, t in (("cu_seqlens", cu_seqlens), ("start", start), ("seqs", seqs), ("block_table", block_table)):
-        if t is not None and t.dtype != torch.int32:
-            raise TypeError(f"compressor_chunk: {name} must be int32, got {t.dtype}")
-    if block_table is not None and (block_table.dim() != 2 or block_table.shape[0] < slots or page <= 0 or
-                                    not block_table.is_contiguous()):
+    i32 = torch.int32
+    if cu_seqlens.dtype != i32 or start.dtype != i32 or (seqs is not None and seqs.dtype != i32):
+        raise TypeError("compressor_chunk: cu_seqlens, start and seqs must be int32")
+    if block_table is None:
+        if out_base + slots * max_comp > out.numel() // head_dim:
+            raise ValueError(f"compressor_chunk: out has {out.numel() // head_dim} rows, {slots} slots of {max_comp} entries "
+                             f"need {out_base + slots * max_comp}")
+    elif block_table.dtype != i32:
+        raise TypeError(f"compressor_chunk: block_table must be int32, got {block_table.dtype}")
+    elif block_table.dim() != 2 or block_table.size(0) < slots or page <= 0 or not block_table.is_contiguous():
         raise ValueError("compressor_chunk: block_table must be contiguous int32 [slots, pages] with a page size")
-    rows = out.numel() // head_dim
-    if block_table is None and out_base + slots * max_comp > rows:
-        raise ValueError(f"compressor_chunk: out has {rows} rows, {slots} slots of {max_comp} entries need "
-                         f"{out_base + slots * max_comp}")
-    if ape.shape != (ratio, 2 * head_dim) or ape.dtype != torch.float32:
+    if ape.dim() != 2 or ape.size(0) != ratio or ape.size(1) != 2 * head_dim or ape.dtype != f32:
         raise ValueError(f"compressor_chunk: ape must be float32 [{ratio}, {2 * head_dim}]")
     if norm_w is not None and norm_w.numel() != head_dim:
         raise ValueError(f"compressor_chunk: norm_w must have {head_dim} values")
-    freqs = rope_freqs(rope_head_dim, kv.device) if freqs is None else freqs.float().contiguous()
+    if freqs is None:
+        freqs = rope_freqs(rope_head_dim, kv.device)
+    elif freqs.dtype != f32 or not freqs.is_contiguous():
+        freqs = freqs.float().contiguous()
     if 2 * freqs.numel() < rope_head_dim:
         raise ValueError("compressor_chunk: fewer rotation frequencies than rope_head_dim needs")
-    if norm_w is not None and norm_w.dtype not in (torch.float32, torch.bfloat16):
+    if norm_w is not None and norm_w.dtype != f32 and norm_w.dtype != torch.bfloat16:
         norm_w = norm_w.float()
     img, inv, nmax = key_image if key_image is not None else (None, None, None)
     # traced programs see the custom op; an eager call goes straight to it

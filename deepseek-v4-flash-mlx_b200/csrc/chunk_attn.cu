@@ -45,8 +45,9 @@
 // two buffers one is being refilled (a load's latency, S behind the other tile's O, softmax), and a third does
 // not fit. A pair of tokens costs 7000 cycles beside its tiles (the last O, the epilogue, the next unit's first
 // softmax, by the same warps). Few tokens are bound by latency: 32 at position 2048 take 17.6 us and one at
-// 65536 17.8 us (16 MB of rows, 2.6 us of HBM), of which the launch and the first rows are 5, the partials'
-// stores 2 (an SM writes 32 bytes a cycle) and the merging kernel 6.
+// 65536 16.9 us (16 MB of rows, 2.6 us of HBM), of which the launch and the first rows are 5, the partials'
+// stores 1 (an SM writes 32 bytes a cycle; 17.8 us when one CTA of the pair stored them all) and the merging
+// kernel 6.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -253,6 +254,9 @@ __device__ __forceinline__ int half_row(const Params& P, const Unit& u, int h, i
   const int64_t row = c.comp_base + static_cast<int64_t>(pg) * c.page + (e - j * c.page);
   return row < c.pool_rows ? static_cast<int>(row) : static_cast<int>(c.pool_rows);
 }
+// One token and split: each CTA has 32 of its heads in rows 0-31, since storing the partials (32 bytes a cycle
+// and SM) is what the pair is slow at; otherwise each has its own token.
+__device__ __forceinline__ bool heads_shared(const Params& P, const Unit& u) { return P.splits > 1 && u.n == 1; }
 // the same for lane `b` of a warp that loads a half together; nothing to load past the last half or box
 __device__ __forceinline__ int tile_row(const Params& P, const Unit& u, int h, int b, int boxes) {
   return h < u.nh && b < boxes ? half_row(P, u, h, b) : static_cast<int>(P.c.pool_rows);
@@ -407,7 +411,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
         sm.unit_tiles[ord & 1] = w.nt;
         const uint32_t qb = in_cta(&sm.q_full, 0);
         if (rank == 0) bar_expect_tx(&sm.q_full, 2 * 8 * SLAB);
-        const int qrow = static_cast<int>(rank) < w.u.n ? (w.u.t0 + static_cast<int>(rank)) * HB : P.c.total * HB;
+        const int qrow = heads_shared(P, w.u) ? w.u.t0 * HB + 32 * static_cast<int>(rank)
+                                    : static_cast<int>(rank) < w.u.n ? (w.u.t0 + static_cast<int>(rank)) * HB : P.c.total * HB;
         for (int e = 0; e < 8; ++e) load_pair(sm.q + e * SLAB, &P.q, e * 64, qrow, qb);  // behind q: zeros
       }
       __syncwarp();
@@ -560,12 +565,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     int g = 0;
     while (has) {
       const Unit& u = w.u;
-      const bool mine = static_cast<int>(rank) < u.n;  // this CTA has a token
-      const int64_t token = u.t0 + rank;
+      const bool shared = heads_shared(P, u);
+      const bool second = rank != 0 && !shared;  // this CTA has the pair's second token
+      const int token = u.t0 + second;
+      // the row's head, -1: none of a token
+      const int whose = shared ? ((quad & 1) == 0 ? 32 * static_cast<int>(rank) + lane : -1) : second >= u.n ? -1 : head;
       const int pos = u.p0 + static_cast<int>(rank), split = w.split;
       if (w.nt == 0) {  // splits > 1: no rows for this one, its O is not read
-        if (mine && kvh == 0 && ch == 0) {
-          float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + ((token * P.splits + split) * HB + head) * 2;
+        if (whose >= 0 && kvh == 0 && ch == 0) {
+          float* ml = P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) +
+                      ((static_cast<int64_t>(token) * P.splits + split) * HB + whose) * 2;
           ml[0] = -INFINITY;
           ml[1] = 0.f;
         }
@@ -583,7 +592,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
           const int j = 32 * ch + lane;
           const bool v0 = h < u.nh && half_sees(P.c, u, h, j, u.p0, u.seen[0]);
           const bool v1 = h < u.nh && u.n > 1 && half_sees(P.c, u, h, j, u.p0 + 1, u.seen[1]);
-          see = __ballot_sync(0xffffffffu, rank == 0 ? v0 : v1);
+          see = __ballot_sync(0xffffffffu, second ? v1 : v0);
           either = __ballot_sync(0xffffffffu, v0 || v1);
         }
         // a wait that ran out takes the CTA's warps to the end together, from the next smx_any
@@ -691,9 +700,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
       const int d0 = 256 * kvh + 128 * ch, group = 2 * kvh + ch;
       if (P.splits > 1) {
         // partials by four dims of every head: a warp stores 512 bytes at a time
-        if (ok && mine) {
-          const int64_t at = token * P.splits + split;
-          float4* po = reinterpret_cast<float4*>(P.part) + (at * (D / 4) + d0 / 4) * HB + head;
+        if (ok && whose >= 0) {
+          const int64_t at = static_cast<int64_t>(token) * P.splits + split;
+          float4* po = reinterpret_cast<float4*>(P.part) + (at * (D / 4) + d0 / 4) * HB + whose;
 #pragma unroll 1
           for (int c = 0; c < 128; c += 32) {
             float v[32];
@@ -704,12 +713,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
             for (int e = 0; e < 8; ++e) po[(c / 4 + e) * HB] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
           }
           if (group == 0)
-            *reinterpret_cast<float2*>(P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + (at * HB + head) * 2) =
+            *reinterpret_cast<float2*>(P.part + static_cast<int64_t>(P.c.total) * P.splits * (HB * D) + (at * HB + whose) * 2) =
                 make_float2(m, l);
         }
       } else {
         const float inv = 1.f / (l + exp2f(sink - m));
-        const int64_t off = (token * HB + head) * D + d0;
+        const int64_t off = (static_cast<int64_t>(token) * HB + head) * D + d0;
         // Rows leave by way of P's space, which is out of use until the next unit's first P: 64 rows by 64 dims
         // of two warps at a time, 128-byte swizzled, to the tensor by TMA (16 bytes a lane straight from the
         // registers took 5700 cycles a unit).
@@ -718,7 +727,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
         float rc = 1.f, rs = 0.f;  // lane f: the rotation of pair f
         if (P.freqs != nullptr && d0 + 128 > D - P.rope_dim && lane < P.rope_dim / 2)
           rope_cos_sin(pos, P.freqs[lane], &rc, &rs);
-        const bool store = mine && P.out_dtype == DSV4_BF16;
+        const bool store = whose >= 0 && P.out_dtype == DSV4_BF16;
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
           float v[32];
@@ -749,9 +758,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
               fence_async_smem();
               column_bar(group);
               if (store && ok && storer)
-                store_tile(&P.o, d0 + c - 32, static_cast<int>(token) * HB, tile);
+                store_tile(&P.o, d0 + c - 32, token * HB, tile);
             }
-          } else if (ok && mine) {
+          } else if (ok && whose >= 0) {
             float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + off + c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);

@@ -37,7 +37,8 @@ def _params(cache):
 
 def _ints(name, cache, *ts):
     """Sequences and token counts (lists, or tensors on the cache's device) as int32 tensors of one length."""
-    dev, out = cache.block_table.device, []
+    dev, index, out = cache.block_table.device, cache.block_table.get_device(), []
+    n = None
     for t in ts:
         if not isinstance(t, torch.Tensor):
             t = torch.tensor(t, dtype=torch.int32, device=dev)
@@ -46,14 +47,14 @@ def _ints(name, cache, *ts):
                 L.require_cuda(t)
                 raise TypeError(f"{name}: sequences and token counts are integers, got {t.dtype}")
             t = t.reshape(-1).to(torch.int32).contiguous()
-        if t.device != dev:
+        if t.get_device() != index:
             L.require_cuda(t)
             raise ValueError(f"{name}: tensors on {t.device}, the cache is on {dev}")
+        if n is None:
+            n = t.numel()
+        elif t.numel() != n:
+            raise ValueError(f"{name}: {n} sequences, {t.numel()} of their counts")
         out.append(t)
-    n = out[0].numel()
-    for t in out:
-        if t.numel() != n:
-            raise ValueError(f"{name}: {[t.numel() for t in out]} sequences and counts")
     return out
 
 
