@@ -936,16 +936,23 @@ static int encode(CUtensorMap* map, const void* base, uint64_t rows, uint32_t bo
 // after the first, and for a split 2.4 for the merging kernel and 0.05 a token and split for its partials.
 // Measured (us): 32 tokens at 2048: 19.0 whole, 23.1 in 3; 1 at 65536: 196 whole, 20.6 in 44, 21.8 in 64; 80 at
 // 64548 (40 pairs for 74 clusters): 199 whole, 161 in 3, 177 in 8; 300 at 16384: 173 whole, 217 in 2.
+// A last round of eight or more that is not full is not worth it. Of the splits with as many tiles each the
+// fewest are the best, so only those are looked at.
 static int plan_splits(const dsv4_chunk_attn_params* p) {
   if (p->num_splits > 0) return std::min(p->num_splits, 64);
-  const int64_t units = (static_cast<int64_t>(p->chunk.total) + p->chunk.n) / 2, clusters = std::max(1, num_sms() / 2);
-  const int64_t tiles = (static_cast<int64_t>(p->chunk.max_comp) + 2 * p->chunk.window) / BN + 1;  // at most
+  const int64_t total = p->chunk.total;
+  const uint32_t clusters = std::max(1, num_sms() / 2);
+  if ((total + p->chunk.n) / 2 >= 8 * static_cast<int64_t>(clusters)) return 1;
+  const uint32_t units = static_cast<uint32_t>((total + p->chunk.n) / 2);
+  const uint32_t tiles = (static_cast<uint32_t>(p->chunk.max_comp) + 2u * p->chunk.window) / BN + 1;  // at most
   int best = 1;
   int64_t least = INT64_MAX;
-  for (int s = 1; s <= 64; ++s) {
-    const int64_t rounds = (units * s + clusters - 1) / clusters, each = (tiles + s - 1) / s;
-    const int64_t cost = rounds * each * 100 + (rounds - 1) * 140 + (s > 1 ? 240 + 5 * s * static_cast<int64_t>(p->chunk.total) : 0);
-    if (cost < least) least = cost, best = s;
+  for (uint32_t s = 1, each = tiles; s <= 64; s = (tiles + each - 2) / (each - 1)) {  // the fewest with fewer tiles each
+    each = (tiles + s - 1) / s;
+    const uint32_t rounds = (units * s + clusters - 1) / clusters;
+    const int64_t cost = static_cast<int64_t>(rounds) * each * 100 + (static_cast<int64_t>(rounds) - 1) * 140 +
+                         (s > 1 ? 240 + 5 * s * total : 0);
+    if (cost < least) least = cost, best = static_cast<int>(s);
     if (each == 1) break;
   }
   return best;
@@ -958,10 +965,12 @@ using namespace dsv4;
 
 extern "C" {
 
+static size_t partial_bytes(const dsv4_chunk_attn_params* p, int splits) {
+  return splits == 1 ? 0 : static_cast<size_t>(p->chunk.total) * splits * (ca::HB * ca::D + ca::HB * 2) * sizeof(float);
+}
 size_t dsv4_chunk_attn_workspace_size(const dsv4_chunk_attn_params* p) {
   if (p == nullptr || p->chunk.total <= 0 || p->chunk.n <= 0) return 0;
-  const int splits = ca::plan_splits(p);
-  return splits == 1 ? 0 : static_cast<size_t>(p->chunk.total) * splits * (ca::HB * ca::D + ca::HB * 2) * sizeof(float);
+  return partial_bytes(p, ca::plan_splits(p));
 }
 
 int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
@@ -983,7 +992,7 @@ int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream) {
   if (p->chunk.n == 0 || p->chunk.total == 0) return DSV4_OK;
   ca::Params P = {};
   P.splits = ca::plan_splits(p);
-  const size_t need = dsv4_chunk_attn_workspace_size(p);
+  const size_t need = partial_bytes(p, P.splits);
   if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need ||
                    (reinterpret_cast<uintptr_t>(p->workspace) & 15) != 0)) {
     set_error("dsv4_chunk_attn: workspace of %zu bytes needed, %zu given", need, p->workspace_bytes);
