@@ -24,12 +24,12 @@ from .norm_rope import rope_freqs
 from .sparse_attn import sparse_attn_into
 
 
-def _index_tensor(name, t, dev, n):
-    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.dim() != 1:
+def _index_tensor(name, t, pool, n):
+    if not isinstance(t, torch.Tensor) or t.dim() != 1 or (t.dtype != torch.int32 and t.dtype != torch.int64):
         raise TypeError(f"{name} must be a 1-d int32 tensor")
-    if t.device != dev:
+    if t.get_device() != pool.get_device():
         L.require_cuda(t)
-        raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+        raise ValueError(f"{name} is on {t.device}, the cache on {pool.device}")
     if n is not None and t.numel() != n:
         raise ValueError(f"{name} has {t.numel()} values, the chunk has {n} sequences")
     return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
@@ -41,14 +41,14 @@ def _f32(t):
 
 def _sequences(cache, cu_seqlens, start, seqs, total):
     """The chunk's sequences as int32 tensors, checked against the cache."""
-    dev = cache.kv_pool.device
-    cu = _index_tensor("cu_seqlens", cu_seqlens, dev, None)
+    pool = cache.kv_pool
+    cu = _index_tensor("cu_seqlens", cu_seqlens, pool, None)
     n = cu.numel() - 1
     if n < 0:
         raise ValueError("cu_seqlens holds one value more than there are sequences")
-    start = _index_tensor("start", start, dev, n)
+    start = _index_tensor("start", start, pool, n)
     if seqs is not None:
-        seqs = _index_tensor("seqs", seqs, dev, n)
+        seqs = _index_tensor("seqs", seqs, pool, n)
     elif n > cache.batch:
         raise ValueError(f"a chunk of {n} sequences, the cache has {cache.batch} slots")
     if total > cache.max_chunk:
@@ -166,23 +166,24 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
     not finite and seen by the second token of a pair reaches the first one's output too. The custom op
     `dsv4::chunk_attention`."""
     L.require_cuda(q, sink, rows, freqs)
-    if q.dim() != 3 or q.shape[2] != cache.head_dim:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim:
         raise ValueError(f"chunk_attention: q must be [total, heads, {cache.head_dim}], got {tuple(q.shape)}")
     if q.dtype != torch.bfloat16:
         raise TypeError(f"chunk_attention: q is the bf16 output of norm_rope, got {q.dtype}")
-    if q.shape[1] != 64 or sink.numel() != 64:
+    if shape[1] != 64 or sink.numel() != 64:
         raise ValueError(f"chunk_attention: 64 heads, got q {tuple(q.shape)} and {sink.numel()} sinks")
-    if out_dtype not in (torch.bfloat16, torch.float32):
+    if out_dtype != torch.bfloat16 and out_dtype != torch.float32:
         raise TypeError(f"chunk_attention: out_dtype must be bfloat16 or float32, got {out_dtype}")
-    dev = cache.kv_pool.device
-    if q.device != dev or sink.device != dev or (rows is not None and rows.device != dev):
+    index = cache.kv_pool.get_device()
+    if q.get_device() != index or sink.get_device() != index or (rows is not None and rows.get_device() != index):
         raise ValueError("chunk_attention: q, sink and rows must be on the cache's device")
-    total = q.shape[0]
+    total = shape[0]
     if rows is not None:
         if rows.dim() != 2 or rows.shape[0] != total or rows.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"chunk_attention: rows must be int32 [{total}, k], got {rows.dtype} {tuple(rows.shape)}")
         rows = rows.to(torch.int32).contiguous()
-    freqs = rope_freqs(64, dev) if freqs is None else _f32(freqs)
+    freqs = rope_freqs(64, q.device) if freqs is None else _f32(freqs)
     if not 0 < freqs.numel() <= 32:
         raise ValueError(f"chunk_attention: 1 to 32 rotation frequencies, got {freqs.numel()}")
     if not 0 <= num_splits <= 64:
