@@ -222,8 +222,10 @@ def check(status):
         raise Dsv4Error(status, msg.decode() if msg else "")
 
 
+# an address as ctypes takes it (every entry point declares its arguments; a c_void_p object made for each
+# took half a microsecond)
 def ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def dtype_code(t):

@@ -21,7 +21,6 @@ import torch
 
 from . import _lib as L
 from .norm_rope import rope_freqs
-from .sparse_attn import sparse_attn_into
 
 
 def _index_tensor(name, t, pool, n):
@@ -139,15 +138,25 @@ def _attend(kv_pool, c, q, sink, scale, freqs, out_dtype, num_splits):
 
 
 def _attend_listed(kv_pool, c, q, sink, rows, scale, freqs, out_dtype):
-    """Every token's list as an index tensor, and the sparse attention over it."""
-    total = q.shape[0]
+    """Every token's list and position (one allocation), and the sparse attention over them."""
+    lib, stream = L.lib(), L.stream_of(q)
+    total, heads, dim = q.shape
     cols = c.max_comp if rows is None else rows.shape[1]
-    idx = torch.empty((total, c.window + cols), dtype=torch.int32, device=q.device)
-    pos = torch.empty(total, dtype=torch.int32, device=q.device)
-    L.check(L.lib().dsv4_chunk_rows(ctypes.byref(c), L.ptr(pos), None, L.ptr(idx), idx.shape[1], cols, L.ptr(rows),
-                                    L.stream_of(q)))
-    out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    return sparse_attn_into(out, q, kv_pool, sink, idx, scale, freqs, pos, 2 * freqs.numel())
+    t = c.window + cols
+    lists = torch.empty(total * (t + 1), dtype=torch.int32, device=q.device)
+    idx = lists.data_ptr()
+    pos = idx + 4 * total * t
+    L.check(lib.dsv4_chunk_rows(ctypes.byref(c), pos, None, idx, t, cols, None if rows is None else rows.data_ptr(), stream))
+    out = torch.empty_like(q, dtype=out_dtype)
+    p = L.SparseAttnParams(q.data_ptr(), kv_pool.data_ptr(), sink.data_ptr(), idx, out.data_ptr(), total, c.pool_rows, heads,
+                           dim, t, L.BF16, L.I32, L.dtype_code(out), scale, freqs.data_ptr(), pos, 2 * freqs.numel())
+    ref = ctypes.byref(p)
+    nbytes = lib.dsv4_sparse_attn_workspace_size(ref)
+    if nbytes:
+        ws = L.workspace(nbytes, q.device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+    L.check(lib.dsv4_sparse_attn(ref, stream))
+    return out
 
 
 def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, scale=None, freqs=None,
