@@ -424,3 +424,15 @@ def test_serving_runner_on_a_paged_cache():
     assert L.device_error() == 0
     t = runs[1].block.cache.block_table
     assert (t >= 0).sum(1).tolist() == [3, 4]   # 22 and 32 entries
+
+
+def test_hundreds_of_branches():
+    c = _cache(300, 40, 16, 700, seed=10)
+    c.reserve([0, 1, 2], [160, 100, 64])
+    m = Model(c)
+    src, dst = [k % 3 for k in range(270)], list(range(20, 290))
+    tokens = [(160, 100, 64)[k] for k in src]
+    m.fork(src, dst, tokens)
+    c.fork(src, dst, tokens)
+    assert _mods()[2].device_error() == 0
+    m.check()
