@@ -758,3 +758,52 @@ def test_a_replay_takes_what_its_tensors_then_hold():
         assert L.device_error() == 0
         assert pos.tolist() == [p + i for n, p in zip(lens, start) for i in range(n)] + [0] * (10 - sum(lens))
         _check(o, *_attention64(c, q, sink, lens, start, seqs))
+
+
+@pytest.mark.parametrize("quant,act_quant", [(True, False), (False, True), (True, True)])
+def test_extend_with_8_bit_weights_and_quantised_rows(quant, act_quant):
+    """Chunks above and below the 64 tokens at which the projections change kernels."""
+    Lm, C = importlib.import_module(PKG + ".layer"), importlib.import_module(PKG + ".configs")
+    _, _, L = _mods()
+    dims = C.LayerDims(ratio=4)
+    Wt = Lm.make_attention_weights(70, dims=dims, quant=quant).to("cuda")
+    a = Lm.DecodeBlock(Wt, 2, 256, dims=dims, act_quant=act_quant, max_chunk=80, n_pages=8)
+    b = Lm.DecodeBlock(Wt, 2, 256, dims=dims, act_quant=act_quant)
+    x = torch.randn(2, 80, 4096, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    got = [torch.cat([a.extend(x[0, :75], [75], [0]), a.extend(x[0, 75:], [5], [75])]), a.extend(x[1], [80], [0], seqs=[1])]
+    ref = torch.stack([b.step(x[:, p], torch.full((2,), p, dtype=torch.int32, device="cuda")) for p in range(80)], 1)
+    assert L.device_error() == 0
+    for s in range(2):
+        # a cached row that an fp32 sum in another order moves across a border of its 4-bit grid moves by a step, 2^-3 of
+        # its value (e4m3); the rows are a mean over the list, so few of those show in an output
+        assert rel_rms(got[s], ref[s]) <= (2 if act_quant else 1) * BLOCK_REL
+
+
+def test_a_conversation_with_branches():
+    """A prompt in chunks, branches of it that each go their own way while pages move, drafts on a branch that are
+    dropped, and the same tokens one at a time on fixed caches."""
+    pkg, _, L = _mods()
+    a, Wt, dims, Lm = _block(4, 4, 512, 512, max_chunk=200, page=16, n_pages=24)
+    c = a.cache
+    g = torch.Generator(device="cuda").manual_seed(7)
+    prompt, ways, drafts = (torch.randn(n, 4096, generator=g, device="cuda") for n in (190, 90, 6))
+    outs = {0: [a.extend(prompt[:101], [101], [0]), a.extend(prompt[101:], [89], [101])]}
+    c.fork([0, 0], [2, 3], [190, 190])
+    a.extend(drafts, [6], [190], seqs=[3])                   # not taken: the branch is given back
+    c.free([3])
+    c.fork([2], [3], [190])
+    o = a.extend(torch.cat([ways[:33], ways[40:50], ways[60:61]]), [33, 10, 1], [190, 190, 190], seqs=[0, 2, 3])
+    outs[0].append(o[:33]), outs.update({2: [o[33:43]], 3: [o[43:]]})
+    c.free([0])                                              # the branches keep the shared pages
+    live = int(c.compact())
+    assert live == int((c.page_refs > 0).sum()) and (c.page_refs[:live] > 0).all()
+    o = a.extend(torch.cat([ways[50:60], ways[61:90]]), [10, 29], [200, 191], seqs=[2, 3])
+    outs[2].append(o[:10]), outs[3].append(o[10:])
+    assert L.device_error() == 0
+    for s, own in ((0, ways[:33]), (2, ways[40:60]), (3, ways[60:90])):
+        b, _, _, _ = _block(4, 1, 512, 512, page=16)
+        x = torch.cat([prompt, own])
+        ref = torch.cat([b.step(x[p:p + 1], torch.tensor([p], dtype=torch.int32, device="cuda")) for p in range(x.shape[0])])
+        got = torch.cat(outs[s]) if s == 0 else torch.cat([torch.cat(outs[0])[:190], *outs[s]])
+        assert rel_rms(got, ref) <= BLOCK_REL, s
+        assert rel_rms(got[190:], ref[190:]) <= BLOCK_REL, s
