@@ -807,3 +807,23 @@ def test_a_conversation_with_branches():
         got = torch.cat(outs[s]) if s == 0 else torch.cat([torch.cat(outs[0])[:190], *outs[s]])
         assert rel_rms(got, ref) <= BLOCK_REL, s
         assert rel_rms(got[190:], ref[190:]) <= BLOCK_REL, s
+
+
+@pytest.mark.parametrize("lens,start", [([151], [9000]), ([301], [4100]), ([2] * 80, [3000] * 80), ([1] * 76, list(range(2900, 2976))),
+                                        ([1, 0, 3] * 30, [4000, 7, 3900] * 30), ([40, 1, 120], [6000, 5, 2500])])
+def test_chunk_attention_a_little_more_than_a_round(lens, start):
+    """A few pairs of tokens more than the clusters take in whole rounds, and fewer in a replay's lengths."""
+    pkg, _, L = _mods()
+    c, q, sink, cu, st, _ = _case(lens, start, seed=60, page=32)
+    want, tol = _attention64(c, q, sink, lens, start, range(len(lens)))
+    for dtype in (torch.bfloat16, torch.float32):
+        _check(pkg.chunk_attention(c, q, sink, cu, st, freqs=_freqs().cuda(), out_dtype=dtype), want, tol)
+    assert L.device_error() == 0
+    # lengths that a replay may find: fewer pairs than clusters, or none
+    for keep in (5, 0):
+        few = torch.clamp(cu, max=keep)
+        o = pkg.chunk_attention(c, q, sink, few, st, freqs=_freqs().cuda())
+        if keep:
+            n = [int(b - a) for a, b in zip(few[:-1], few[1:])]
+            _check(o[:keep], *[x[:keep] for x in _attention64(c, q, sink, n, start, range(len(n)))])
+    assert L.device_error() == 0
