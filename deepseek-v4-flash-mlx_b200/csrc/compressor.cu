@@ -791,6 +791,9 @@ __global__ void __launch_bounds__(G == 1 ? THREADS : G * D / 2, G == 1 ? 2 : 1)
     }
     load_to(min(nb + 1, i0 + G - 1 + STAGES));  // blocks up to i0 + G - 2 have been read
     if (!row) continue;
+    // Between the CTA's barrier above, behind which the write of `where` lies, and the group's barrier below, ahead
+    // of the next round's write: read behind the group's barrier it would race with that write.
+    const int64_t orow = where[group];
     float vals[1][2] = {{0.f, 0.f}};
     float ss = 0.f;
     if (mine) {
@@ -800,7 +803,7 @@ __global__ void __launch_bounds__(G == 1 ? THREADS : G * D / 2, G == 1 ? 2 : 1)
         ss = fmaf(vals[0][e], vals[0][e], ss);
       }
     }
-    // the group's sum, in block_sum's order; the next round's barrier frees sums
+    // the group's sum, in block_sum's order; the next round writes sums behind its CTA barrier, so that frees them
     ss = warp_sum(ss);
     if (lane == 0) sums[group][tid >> 5] = ss;
     if (G == 1)
@@ -808,7 +811,6 @@ __global__ void __launch_bounds__(G == 1 ? THREADS : G * D / 2, G == 1 ? 2 : 1)
     else
       asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(THREADS) : "memory");
     ss = warp_sum(lane < (d + 63) / 64 ? sums[group][lane] : 0.f);
-    const int64_t orow = where[group];
     const float rinv = rsqrtf(ss / static_cast<float>(d) + p.eps);
     if (mine)
       finish_pair(vals[0][0], vals[0][1], c, d, p.rope_dim, p.norm_w, p.norm_dtype, rinv, p.freqs, R * g, p.out, orow,
