@@ -172,7 +172,8 @@ def compressor_decode_step(x, wkv, wgate, ape, norm_w, ring_kv, ring_score, posi
     `proj` may pass precomputed projections (kv, score) [b, 2*head_dim] fp32. `key_image`
     (image, inv, norm_max, keys_per_entry) also adds each emitted indexer key (out viewed as
     [entries * keys_per_entry, 128] fp32) to a decode cache's key image. `act_quant`: the fp8-e4m3
-    act-quant simulation of the emitted row's nope dims (oracle/decode_engine.py:105). `rotate`
+    act-quant simulation of the emitted row's nope dims (oracle/decode_engine.py:105). The block of
+    position 0 has none before it: ring rows [0, ratio) count as empty there, whatever they hold. `rotate`
     (head_dim 128): the Hadamard + fp4-e2m1 key simulation of `compressor_prefill(rotate=True)`."""
     wkv_t, wkv_s = _w_parts(wkv)
     wg_t, wg_s = _w_parts(wgate)

@@ -259,7 +259,9 @@ __global__ void ring_seed_kernel(dsv4_compressor_params p) {
 }
 
 // one decode token per sequence: ring row R + p%R <- (kv, score + ape[p%R]); when (p+1)%R == 0
-// emit the pooled row at position p+1-R and shift rows [R,2R) to [0,R).
+// emit the pooled row at position p+1-R and shift rows [R,2R) to [0,R). Block 0 has none before it: rows
+// [0,R) then count as empty (kv 0, score -inf) whatever they hold, so that a slot that begins again takes
+// nothing from the sequence it held.
 // ratio 4 (the model's): the same step with every thread owning column pairs (c, c+1) of both
 // halves. The ring rows it reads were written by earlier steps and the current token's row stays
 // in registers, so all of a thread's loads go out at once and the only barrier is the norm's
@@ -334,8 +336,8 @@ __device__ __forceinline__ void decode_r4_row(const dsv4_compressor_decode_param
     if (emit) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        K[np][r] = ld2(rk + r * d2 + c);
-        S[np][r] = ld2(rs + r * d2 + c);
+        K[np][r] = pos < R ? make_float2(0.f, 0.f) : ld2(rk + r * d2 + c);
+        S[np][r] = pos < R ? make_float2(-INFINITY, -INFINITY) : ld2(rs + r * d2 + c);
       }
 #pragma unroll
       for (int r = 0; r < R - 1; ++r) {
@@ -453,8 +455,8 @@ __global__ void __launch_bounds__(THREADS) decode_kernel(dsv4_compressor_decode_
       const int cc = c + e;
       float kv8[16], sc8[16];
       for (int r = 0; r < R; ++r) {
-        kv8[r] = rk[r * d2 + cc];
-        sc8[r] = rs[r * d2 + cc];
+        kv8[r] = pos < R ? 0.f : rk[r * d2 + cc];
+        sc8[r] = pos < R ? -INFINITY : rs[r * d2 + cc];
         kv8[R + r] = rk[(R + r) * d2 + d + cc];
         sc8[R + r] = rs[(R + r) * d2 + d + cc];
       }
@@ -493,7 +495,8 @@ __global__ void __launch_bounds__(THREADS) decode_kernel(dsv4_compressor_decode_
 // decode step per emitted row would leave, in one launch. Block g of a sequence is emitted when its
 // last token, position R g + R - 1, is in the chunk; its tokens and those of block g - 1 come from
 // the chunk where it has them and from the ring otherwise (rows [0, R): the last complete block,
-// rows R + p % R: the tokens of the block begun before the chunk).
+// rows R + p % R: the tokens of the block begun before the chunk; before position 0 there are none, kv 0 and
+// score -inf whatever the ring holds).
 //
 // Every element of the projections is used once (the first half of a token's columns by the next
 // block's row, the second half by its own), so the kernel is a stream of 16 * head_dim bytes per
@@ -564,8 +567,11 @@ __device__ __forceinline__ void chunk_emit(const dsv4_compressor_chunk_params& p
         K[i] = ld2(p.kv + off);
         const float2 s = ld2(p.score + off), a = ld2(p.ape + (i % R) * d2 + col);
         S[i] = make_float2(s.x + a.x, s.y + a.y);
+      } else if (pos < 0) {  // not the ring's rows: they may be those of another sequence
+        K[i] = make_float2(0.f, 0.f);
+        S[i] = make_float2(-INFINITY, -INFINITY);
       } else {
-        const int row = (pos >= block ? R : 0) + i % R;  // positions below 0 are the ring's empty rows
+        const int row = (pos >= block ? R : 0) + i % R;
         K[i] = ld2(rk + row * d2 + col);
         S[i] = ld2(rs + row * d2 + col);
       }

@@ -65,7 +65,9 @@ def _workspace(p, n, device):
 
 def pages_free(cache, seqs):
     """Give back the pages of slots `seqs` (a page shared with another slot stays with that one) and
-    empty their table rows. A slot named twice gives its pages back once."""
+    empty their table rows. A slot named twice gives its pages back once. The slot's next sequence begins at
+    position 0: nothing else of the last one is read from there (window rows and entries are seen by position,
+    and the first block has none before it)."""
     p = _params(cache)
     seqs, = _ints("pages_free", cache, seqs)
     with L.device_of(seqs):

@@ -327,8 +327,8 @@ typedef struct {
   const float* score;     /* [b, 2*head_dim] this token's x.wgate^T (before ape) */
   const float* ape;       /* [ratio, 2*head_dim] */
   const void* norm_w;     /* [head_dim] */
-  float* ring_kv;         /* [b, 2*ratio, 2*head_dim] */
-  float* ring_score;      /* [b, 2*ratio, 2*head_dim] */
+  float* ring_kv;         /* [b, 2*ratio, 2*head_dim]; rows [0, ratio) count as empty (kv 0, score -inf) */
+  float* ring_score;      /*   at positions below ratio, which have no block before theirs, whatever they hold */
   const int32_t* positions; /* [b] decode position p of this token */
   void* out;              /* pool base [*, head_dim] out_dtype */
   const int64_t* out_rows;/* [b] pool row where the emitted row goes (written only when (p+1)%ratio==0) */
@@ -440,7 +440,8 @@ DSV4_API int dsv4_chunk_attn(const dsv4_chunk_attn_params* p, void* stream);
  * per token would leave in the rings, the emitted rows and the key image, in one launch
  * (oracle/decode_engine.py:96-105 for a run of tokens; the reference takes one token at a time). Entry g of
  * slot s goes to row out_base + block_table[s, g / page] * page + g % page, or without a table to row
- * out_base + s * max_comp + g (the indexer keys). An entry past max_comp or without a page raises
+ * out_base + s * max_comp + g (the indexer keys). Positions below 0 count as kv 0 and score -inf whatever the
+ * ring holds. An entry past max_comp or without a page raises
  * DSV4_ERR_INDEX_OUT_OF_RANGE and is not stored; so does a slot that two sequences with tokens name,
  * whose ring and entries are then not defined. */
 typedef struct {

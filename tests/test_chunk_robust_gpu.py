@@ -50,3 +50,69 @@ def test_long_chunks_again_and_again(d, quant, start):
         for name, a, b in zip(("rows", "ring_kv", "ring_score"), run((kv, sc)), want):
             assert torch.equal(a, b), name
     assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("paged", [True, False])
+@pytest.mark.parametrize("how", ["extend", "step", "both"])
+def test_a_slot_begins_again(paged, how):
+    """A slot that held another conversation starts from position 0 as a slot of a new cache does, bit for bit:
+    outputs, compressed rows, keys and rings."""
+    Lm = importlib.import_module(PKG + ".layer")
+    _, _, L = _mods()
+    Wt = Lm.make_attention_weights(90).to("cuda")
+    used, new = (Lm.DecodeBlock(Wt, 2, 512, page=16, max_chunk=160, **(dict(n_pages=40) if paged else {})) for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(140, 4096, generator=g, device="cuda")
+    used.extend(x, [70, 70], [0, 0])                       # both slots, the second in the middle of a block
+    new.extend(x[:70], [70], [0])
+    if paged:
+        used.cache.free([1])
+    y, other = torch.randn(41, 4096, generator=g, device="cuda"), torch.randn(41, 4096, generator=g, device="cuda")
+    sizes = {"extend": [2, 1, 30, 8], "step": [1] * 41, "both": [3, 1, 1, 33, 1, 1, 1]}[how]
+    at = 0
+    for n in sizes:
+        outs = []
+        for blk in (used, new):
+            if n == 1:   # a step takes both slots
+                outs.append(blk.step(torch.stack([other[at], y[at]]), _i32(70 + at, at))[1])
+            else:
+                outs.append(blk.extend(y[at:at + n], [n], [at], seqs=[1]))
+        assert torch.equal(*outs), at
+        at += n
+    assert at == 41 and L.device_error() == 0
+    a, b, e = used.cache, new.cache, torch.arange(10, device="cuda")
+    assert torch.equal(a.kv_pool[a.comp_rows(1, e)], b.kv_pool[b.comp_rows(1, e)])
+    assert torch.equal(a.k_idx[1, :10], b.k_idx[1, :10])
+    assert torch.equal(a.key_image[1].view(2, -1)[1, :10], b.key_image[1].view(2, -1)[1, :10])
+    for name in ("ring_kv", "ring_score", "ring_k_idx", "ring_s_idx"):
+        assert torch.equal(getattr(a, name)[1, :5], getattr(b, name)[1, :5]), name
+
+
+@pytest.mark.parametrize("ratio,d", [(1, 64), (2, 512), (3, 128), (4, 128), (4, 512), (4, 1024), (8, 512)])
+def test_the_first_block_has_none_before_it(ratio, d):
+    """The row of block 0 is that of an empty ring, whatever the ring holds of a sequence before: steps and chunks."""
+    pkg, _, L = _mods()
+    g = torch.Generator(device="cuda").manual_seed(ratio)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    n = 2 * ratio + 1
+    kv, sc, ape, nw, freqs = rnd(n, 2 * d), rnd(n, 2 * d), rnd(ratio, 2 * d), 1 + 0.1 * rnd(d), rnd(32)
+    empty = (torch.zeros(1, 2 * ratio, 2 * d, device="cuda"), torch.full((1, 2 * ratio, 2 * d), -float("inf"), device="cuda"))
+    rope, outs = min(64, d), []
+    for ring in (empty, (rnd(1, 2 * ratio, 2 * d), 5 * rnd(1, 2 * ratio, 2 * d))):
+        for sizes in ([n], [1] * n, [ratio, ratio + 1], [-n]):
+            rk, rs = (t.clone() for t in ring)
+            out, at = torch.zeros(3, d, device="cuda"), 0
+            if sizes[0] < 0:    # one token at a time
+                for p in range(n):
+                    pkg.compressor_decode_step(rk, None, None, ape, nw, rk, rs, _i32(p), out, torch.tensor([p // ratio], device="cuda"),
+                                               head_dim=d, ratio=ratio, rope_head_dim=rope, freqs=freqs, proj=(kv[p:p + 1], sc[p:p + 1]))
+            else:
+                for m in sizes:
+                    pkg.compressor_chunk((kv[at:at + m], sc[at:at + m]), _i32(0, m), _i32(at), ape, nw, rk, rs, out, 3, head_dim=d,
+                                         ratio=ratio, rope_head_dim=rope, freqs=freqs)
+                    at += m
+            outs.append((out, rk[:, :ratio + 1], rs[:, :ratio + 1]))
+    assert L.device_error() == 0 and outs[0][0][:2].any(-1).all()
+    for o in outs[1:]:
+        for x, y in zip(o, outs[0]):
+            assert torch.equal(x, y)
