@@ -124,12 +124,14 @@ struct List {
     }
     return w;
   }
-  // its pool row, -1 if masked; an index past the pool is masked too, and noted in *bad
+  // its pool row, -1 if masked; a row past the pool, of the window or listed, is masked too, and noted in *bad
   __device__ __forceinline__ int32_t row(int u, Raw w, bool* bad) const {
     if (u >= len) return -1;
     if (u < window) {
-      if (linear) return first + u <= sp ? static_cast<int32_t>(win + first + u) : -1;
-      return static_cast<int32_t>(win + (u < window - sp - 1 ? sp + 1 + u : u - (window - sp - 1)));
+      if (linear && first + u > sp) return -1;
+      const int64_t r = win + (linear ? first + u : u < window - sp - 1 ? sp + 1 + u : u - (window - sp - 1));
+      *bad |= r >= n;
+      return r < 0 || r >= n ? -1 : static_cast<int32_t>(r);
     }
     const bool over = WIDE ? w.hi > 0 || (w.hi == 0 && (w.lo < 0 || w.lo >= n)) : w.lo >= n;
     *bad |= over;

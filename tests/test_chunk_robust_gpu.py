@@ -116,3 +116,58 @@ def test_the_first_block_has_none_before_it(ratio, d):
     for o in outs[1:]:
         for x, y in zip(o, outs[0]):
             assert torch.equal(x, y)
+
+
+def _plain64(q, kv, sink, lists, pos, freqs, scale=512 ** -0.5):
+    """Attention of each query over its list of pool rows in 64 bits, and the bound of each element: probabilities and
+    output are rounded to bf16, half a step of 2^-8 each, 3 * 2^-8 of the weighted mean of |kv| with the denominator's
+    share, and one more for the sums in 32 bits; the rotation adds up the two of a pair."""
+    want, tol, eps = [], [], torch.finfo(torch.bfloat16).eps / 2
+    for i, rows in enumerate(lists):
+        r = torch.tensor([x for x in rows if x >= 0], device="cuda", dtype=torch.long)
+        v = kv[r].double()
+        w = torch.softmax(torch.cat([q[i].double() @ v.T * scale, sink.double()[:, None]], 1), -1)[:, :-1]
+        o, a = w @ v, w @ v.abs()
+        t = (pos[i].float() * freqs).double()
+        y, x = o.clone(), o[:, -64:].reshape(-1, 32, 2)
+        y[:, -64::2] = x[..., 0] * t.cos() + x[..., 1] * t.sin()
+        y[:, -63::2] = x[..., 1] * t.cos() - x[..., 0] * t.sin()
+        a[:, -64:] += a[:, -64:].reshape(-1, 32, 2).flip(-1).reshape(-1, 64)
+        want.append(y), tol.append(4 * eps * a)
+    return torch.stack(want), torch.stack(tol)
+
+
+@pytest.mark.parametrize("kernel,s", [(0, 3), (0, 20), (1, 3), (1, 20), (2, 3), (2, 20), (2, 200), (3, 3)])
+@pytest.mark.parametrize("linear", [False, True])
+def test_window_rows_past_the_pool(kernel, s, linear):
+    """Rows of the implicit window that are no rows of kv are left out, those past its end reported, by every kernel.
+    kv lies inside a larger tensor of NaN, so that a row that is read all the same shows."""
+    pkg, _, L = _mods()
+    g = torch.Generator(device="cuda").manual_seed(s)
+    n, window, off, t = 500, 128, 600, 40
+    big = torch.full((off + n + 600, 512), float("nan"), device="cuda", dtype=torch.bfloat16)
+    kv = big[off:off + n]
+    kv.copy_(torch.randn(n, 512, generator=g, device="cuda"))
+    q, sink = torch.randn(s, 64, 512, generator=g, device="cuda").to(torch.bfloat16), torch.randn(64, generator=g, device="cuda")
+    freqs = 1.0 / (160000.0 ** (torch.arange(0, 64, 2, dtype=torch.float32, device="cuda") / 64))
+    idx = torch.randint(0, n, (s, t), generator=g, device="cuda", dtype=torch.int32)
+    # (window base, position): inside; past the end by some rows or all; below 0; the ring not yet full; before position 0
+    kinds = [(7, 300, False), (n - 40, 300, True), (n, 300, True), (2 ** 33, 300, True), (-30, 300, False), (-500, 300, False),
+             (-2 ** 33, 300, False), (n - 10, 20, True), (n - 10, 9, False), (3, -1, False), (n - 128, 127, False)]
+    if linear:
+        kinds = [(0, 300, False), (0, n, True), (0, n + 100, True), (0, n + 400, True), (0, 2 ** 30, True), (0, 5, False), (40, n - 41, False),
+                 (40, n - 40, True), (-300, 350, False), (-2 ** 33, 350, False), (0, -1, False)]
+    for base, p, over in kinds:
+        pos = torch.full((s,), p, dtype=torch.int32, device="cuda")
+        if linear:
+            rows = [base + u for u in range(max(0, p - window + 1), p + 1)]
+        else:
+            rows = [base + u % window for u in range(max(0, p - window + 1), p + 1)]
+        assert any(r >= n for r in rows) == over
+        lists = [[r if 0 <= r < n else -1 for r in rows] + idx[i].tolist() for i in range(s)]
+        o = pkg.sparse_attn_rope(q, kv, sink, idx, 512 ** -0.5, pos, freqs, win_base=torch.full((s,), base, device="cuda"), window=window,
+                                 window_linear=linear, kernel=kernel)
+        assert L.device_error() == (4 if over else 0), (base, p)
+        want, tol = _plain64(q, kv, sink, lists, pos, freqs)
+        assert torch.isfinite(o).all(), (base, p)
+        assert ((o.double() - want).abs() <= tol).all(), (base, p)
