@@ -101,6 +101,7 @@ def _chunk_attention_op(q: torch.Tensor, kv_pool: torch.Tensor, block_table: tor
                         rows: torch.Tensor | None, freqs: torch.Tensor, comp_base: int, stage_base: int, window: int,
                         ratio: int, page: int, max_comp: int, scale: float, out_dtype: torch.dtype,
                         num_splits: int) -> torch.Tensor:
+    _check_rows(q, kv_pool)
     return _attention(q, kv_pool, block_table, win_base, sink, cu_seqlens, start, seqs, rows, freqs, comp_base, stage_base,
                       window, ratio, page, max_comp, scale, out_dtype, num_splits)
 
@@ -108,7 +109,17 @@ def _chunk_attention_op(q: torch.Tensor, kv_pool: torch.Tensor, block_table: tor
 @_chunk_attention_op.register_fake
 def _(q, kv_pool, block_table, win_base, sink, cu_seqlens, start, seqs, rows, freqs, comp_base, stage_base, window, ratio,
       page, max_comp, scale, out_dtype, num_splits):
+    _check_rows(q, kv_pool)
     return torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
+
+
+def _check_rows(q, kv_pool):
+    """What the custom op, called by itself, has to hold: the kernels' tiles take 64 heads of 512 bf16 whatever the
+    tensors are (`chunk_attention` checks it with the rest)."""
+    if q.dim() != 3 or q.shape[1] != 64 or q.shape[2] != 512 or kv_pool.dim() != 2 or kv_pool.shape[1] != 512:
+        raise ValueError(f"dsv4::chunk_attention: q [total, 64, 512] over rows of 512, got {tuple(q.shape)} and {tuple(kv_pool.shape)}")
+    if q.dtype != torch.bfloat16 or kv_pool.dtype != torch.bfloat16:
+        raise TypeError(f"dsv4::chunk_attention: q and the pool are bf16, got {q.dtype} and {kv_pool.dtype}")
 
 
 def _attention(q, kv_pool, block_table, win_base, sink, cu_seqlens, start, seqs, rows, freqs, comp_base, stage_base, window,
@@ -176,8 +187,9 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
     `dsv4::chunk_attention`."""
     L.require_cuda(q, sink, rows, freqs)
     shape = q.shape
-    if len(shape) != 3 or shape[2] != cache.head_dim:
-        raise ValueError(f"chunk_attention: q must be [total, heads, {cache.head_dim}], got {tuple(q.shape)}")
+    if len(shape) != 3 or shape[2] != 512 or cache.head_dim != 512:
+        raise ValueError(f"chunk_attention: q must be [total, 64, 512] over a cache of 512-wide rows, got {tuple(q.shape)} and "
+                         f"head_dim {cache.head_dim}")
     if q.dtype != torch.bfloat16:
         raise TypeError(f"chunk_attention: q is the bf16 output of norm_rope, got {q.dtype}")
     if shape[1] != 64 or sink.numel() != 64:
