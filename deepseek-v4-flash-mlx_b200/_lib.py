@@ -261,6 +261,14 @@ def device_of(t):
     return _HERE_ALREADY if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def through_op(*ts):
+    """Whether a call has to go through its custom op rather than straight to its body: inside a trace or a mode that
+    takes torch's calls (fake tensors, make_fx), or with tensors that are of another class."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
+        return True
+    return any(type(t) is not torch.Tensor for t in ts)
+
+
 def require_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:

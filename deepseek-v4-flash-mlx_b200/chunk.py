@@ -213,8 +213,8 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
     cu, start, seqs = _sequences(cache, cu_seqlens, start, seqs, total)
     if total == 0 or cu.numel() == 1:
         return torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    # traced programs see the custom op; an eager call goes straight to it
-    f = _chunk_attention_op if torch.compiler.is_compiling() else _attention
+    # traced programs see the custom op; an eager call goes straight to its body
+    f = _chunk_attention_op if L.through_op(q, cache.kv_pool, sink, cu) else _attention
     return f(q.contiguous(), cache.kv_pool, cache.block_table, cache.win_base, _f32(sink), cu, start, seqs, rows, freqs,
              cache.comp_base, cache.stage_base, cache.window, cache.ratio, cache.page, cache.max_comp, scale, out_dtype,
              int(num_splits))

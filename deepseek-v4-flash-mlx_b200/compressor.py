@@ -340,8 +340,8 @@ def compressor_chunk(proj, cu_seqlens, start, ape, norm_w, ring_kv, ring_score, 
     if norm_w is not None and norm_w.dtype != f32 and norm_w.dtype != torch.bfloat16:
         norm_w = norm_w.float()
     img, inv, nmax = key_image if key_image is not None else (None, None, None)
-    # traced programs see the custom op; an eager call goes straight to it
-    f = _compressor_chunk_op if torch.compiler.is_compiling() else _chunk_into
+    # traced programs see the custom op; an eager call goes straight to its body
+    f = _compressor_chunk_op if L.through_op(kv, score, ring_kv, out) else _chunk_into
     f(kv.contiguous(), score.contiguous(), cu_seqlens.contiguous(), start.contiguous(),
       None if seqs is None else seqs.contiguous(), ape.contiguous(), None if norm_w is None else norm_w.contiguous(),
       ring_kv, ring_score, out, block_table, int(page), int(out_base), int(max_comp), int(head_dim), int(ratio),

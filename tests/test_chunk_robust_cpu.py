@@ -34,3 +34,44 @@ def test_chunk_attention_takes_rows_of_512(head_dim):
                 with pytest.raises((ValueError, TypeError)):
                     torch.ops.dsv4.chunk_attention(_e(4, heads, qd, dtype=qt), _e(1000, pd, dtype=pt), c.block_table, c.win_base, sink, cu, start,
                                                    None, rows, freqs, 256, 384, 128, 4, 64, 64, 0.04, BF16, 0)
+
+
+def _attention_args():
+    _, D = _mods()
+    c = D.SparseMLACache(2, 64, max_chunk=8)
+    return c, (_e(7, 64, 512, dtype=BF16), _e(64), _e(3, dtype=I32), _e(2, dtype=I32))
+
+
+def _compressor_args(c):
+    return ((_e(7, 1024), _e(7, 1024)), _e(3, dtype=I32), _e(2, dtype=I32), _e(4, 1024), _e(512), c.ring_kv, c.ring_score, c.kv_pool, 64)
+
+
+def test_chunk_calls_on_fake_tensors():
+    """The public calls, as a mode that holds no data sees them: inside it, and on its tensors outside of it."""
+    pkg, _ = _mods()
+    mode = FakeTensorMode()
+    with mode:
+        c, args = _attention_args()
+        freqs, comp = _e(32), _compressor_args(c)
+        kw = dict(block_table=c.block_table, page=64, out_base=256)
+        for rows in (None, _e(7, 5, dtype=I32)):
+            o = pkg.chunk_attention(c, *args, rows=rows, freqs=freqs, out_dtype=F32)
+            assert o.shape == (7, 64, 512) and o.dtype == F32 and o.is_cuda
+        assert pkg.compressor_chunk(*comp, freqs=freqs, **kw) is None
+    assert pkg.chunk_attention(c, *args, freqs=freqs).shape == (7, 64, 512)
+    assert pkg.compressor_chunk(*comp, freqs=freqs, **kw) is None
+
+
+def test_chunk_calls_are_one_op_in_a_graph():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    pkg, _ = _mods()
+    with FakeTensorMode():
+        c, args = _attention_args()
+        freqs, comp = _e(32), _compressor_args(c)
+
+        def f(q, kv):
+            pkg.compressor_chunk((kv, comp[0][1]), *comp[1:], freqs=freqs, block_table=c.block_table, page=64, out_base=256)
+            return pkg.chunk_attention(c, q, *args[1:], freqs=freqs)
+
+        names = [str(n.target) for n in make_fx(f)(args[0], comp[0][0]).graph.nodes if n.op == "call_function"]
+    assert names == ["dsv4.compressor_chunk.default", "dsv4.chunk_attention.default"]
