@@ -197,8 +197,9 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
     if out_dtype != torch.bfloat16 and out_dtype != torch.float32:
         raise TypeError(f"chunk_attention: out_dtype must be bfloat16 or float32, got {out_dtype}")
     index = cache.kv_pool.get_device()
-    if q.get_device() != index or sink.get_device() != index or (rows is not None and rows.get_device() != index):
-        raise ValueError("chunk_attention: q, sink and rows must be on the cache's device")
+    if q.get_device() != index or sink.get_device() != index or (rows is not None and rows.get_device() != index) or \
+            (freqs is not None and freqs.get_device() != index):
+        raise ValueError("chunk_attention: q, sink, rows and freqs must be on the cache's device")
     total = shape[0]
     if rows is not None:
         if rows.dim() != 2 or rows.shape[0] != total or rows.dtype not in (torch.int32, torch.int64):

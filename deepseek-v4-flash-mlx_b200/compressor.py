@@ -301,7 +301,10 @@ def compressor_chunk(proj, cu_seqlens, start, ape, norm_w, ring_kv, ring_score, 
     and rows are then not defined. `key_image` (image, inv, norm_max: the cache's), `act_quant` and
     `rotate` as in `compressor_decode_step`. The custom op `dsv4::compressor_chunk`."""
     kv, score = proj
-    L.require_cuda(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, freqs)
+    tensors, index = (kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, freqs), kv.get_device()
+    if index < 0 or any(t is not None and t.get_device() != index for t in tensors):
+        L.require_cuda(*tensors)
+        raise ValueError("compressor_chunk: every tensor must be on the projections' device")
     f32 = torch.float32
     if kv.dtype != f32 or score.dtype != f32 or kv.shape != score.shape or kv.dim() != 2 or kv.size(1) != 2 * head_dim:
         raise ValueError(f"compressor_chunk: kv and score must be float32 [total, {2 * head_dim}]")

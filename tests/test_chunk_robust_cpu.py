@@ -75,3 +75,28 @@ def test_chunk_calls_are_one_op_in_a_graph():
 
         names = [str(n.target) for n in make_fx(f)(args[0], comp[0][0]).graph.nodes if n.op == "call_function"]
     assert names == ["dsv4.compressor_chunk.default", "dsv4.chunk_attention.default"]
+
+
+def test_chunk_calls_refuse_tensors_of_another_device():
+    pkg, D = _mods()
+    with FakeTensorMode():
+        c, (q, sink, cu, start) = _attention_args()
+        ok = dict(cache=c, q=q, sink=sink, cu_seqlens=cu, start=start, seqs=_e(2, dtype=I32), rows=_e(7, 5, dtype=I32), freqs=_e(32))
+        for name in ("q", "sink", "cu_seqlens", "start", "seqs", "rows", "freqs"):
+            for device, err in (("cuda:1", ValueError), ("cpu", RuntimeError)):
+                with pytest.raises(err):
+                    pkg.chunk_attention(**{**ok, name: torch.empty_like(ok[name], device=device)})
+        proj, _, _, ape, nw, rk, rs, out, most = _compressor_args(c)
+        ok = dict(proj=proj, cu_seqlens=cu, start=start, ape=ape, norm_w=nw, ring_kv=rk, ring_score=rs, out=out, max_comp=most,
+                  block_table=c.block_table, page=64, out_base=256, seqs=_e(2, dtype=I32), freqs=_e(32))
+        for name in ok:
+            for device, err in (("cuda:1", ValueError), ("cpu", RuntimeError)):
+                if name == "proj":
+                    with pytest.raises(err):
+                        pkg.compressor_chunk(**{**ok, name: (proj[0], torch.empty_like(proj[1], device=device))})
+                elif isinstance(ok[name], torch.Tensor):
+                    with pytest.raises(err):
+                        pkg.compressor_chunk(**{**ok, name: torch.empty_like(ok[name], device=device)})
+        with pytest.raises(RuntimeError):   # all of them on the CPU
+            cpu = {k: torch.empty_like(v, device="cpu") if isinstance(v, torch.Tensor) else v for k, v in ok.items()}
+            pkg.compressor_chunk(**{**cpu, "proj": tuple(torch.empty_like(t, device="cpu") for t in proj)})
