@@ -285,6 +285,19 @@ def _chunk_into(kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_s
         L.check(L.lib().dsv4_compressor_chunk(ctypes.byref(p), L.stream_of(kv)))
 
 
+def _slot_image(key_image, slots, max_comp, index):
+    """The parts of a key image that a chunk of `slots` slots of `max_comp` entries writes to by slot and entry."""
+    if len(key_image) != 3:
+        raise ValueError("compressor_chunk: a key image has three parts (image, inv, norm_max)")
+    tiles = -(-max_comp // 128)
+    for t, dtype, need in zip(key_image, (torch.uint8, torch.float32, torch.float32),
+                              (slots * tiles * L.KEY_TILE_BYTES, slots * tiles * 128, slots)):
+        if t.dtype != dtype or t.get_device() != index or not t.is_contiguous() or t.numel() < need:
+            raise ValueError(f"compressor_chunk: the key image of {slots} slots of {max_comp} entries (key_image_buffers) needs "
+                             f"contiguous {dtype} of {need} values on the projections' device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return key_image
+
+
 def compressor_chunk(proj, cu_seqlens, start, ape, norm_w, ring_kv, ring_score, out, max_comp, block_table=None, page=0,
                      out_base=0, seqs=None, head_dim=512, ratio=4, rope_head_dim=64, freqs=None, eps=1e-6, key_image=None,
                      act_quant=False, rotate=False):
@@ -342,7 +355,7 @@ def compressor_chunk(proj, cu_seqlens, start, ape, norm_w, ring_kv, ring_score, 
         raise ValueError("compressor_chunk: fewer rotation frequencies than rope_head_dim needs")
     if norm_w is not None and norm_w.dtype != f32 and norm_w.dtype != torch.bfloat16:
         norm_w = norm_w.float()
-    img, inv, nmax = key_image if key_image is not None else (None, None, None)
+    img, inv, nmax = _slot_image(key_image, slots, max_comp, index) if key_image is not None else (None, None, None)
     # traced programs see the custom op; an eager call goes straight to its body
     f = _compressor_chunk_op if L.through_op(kv, score, ring_kv, out) else _chunk_into
     f(kv.contiguous(), score.contiguous(), cu_seqlens.contiguous(), start.contiguous(),

@@ -100,3 +100,27 @@ def test_chunk_calls_refuse_tensors_of_another_device():
         with pytest.raises(RuntimeError):   # all of them on the CPU
             cpu = {k: torch.empty_like(v, device="cpu") if isinstance(v, torch.Tensor) else v for k, v in ok.items()}
             pkg.compressor_chunk(**{**cpu, "proj": tuple(torch.empty_like(t, device="cpu") for t in proj)})
+
+
+def test_a_chunk_of_keys_refuses_an_image_that_is_not_the_slots():
+    """The image is written by slot and entry without a look at its size."""
+    pkg, _ = _mods()
+    I = importlib.import_module(PKG + ".indexer")  # noqa: E741
+    with FakeTensorMode():
+        slots, most = 2, 300
+        ring = _e(slots, 8, 256), _e(slots, 8, 256)
+        call = lambda image: pkg.compressor_chunk(  # noqa: E731
+            (_e(7, 256), _e(7, 256)), _e(3, dtype=I32), _e(2, dtype=I32), _e(4, 256), _e(128), *ring, _e(slots, most, 128), most,
+            head_dim=128, freqs=_e(32), key_image=image)
+        img, inv, nmax = I.key_image_buffers(slots, most, "cuda")
+        assert call((img, inv, nmax)) is None
+        small = I.key_image_buffers(slots, 256, "cuda")
+        for bad in ((small[0], inv, nmax), (img, small[1], nmax), (img, inv, nmax[:1]), (img.view(torch.int8), inv, nmax),
+                    (img, inv.half(), nmax), (img, inv, nmax.double()), (img[::2], inv, nmax), (img, inv)):
+            with pytest.raises((ValueError, TypeError)):
+                call(bad)
+        for k in range(3):
+            image = [img, inv, nmax]
+            image[k] = torch.empty_like(image[k], device="cuda:1")
+            with pytest.raises(ValueError):
+                call(tuple(image))
