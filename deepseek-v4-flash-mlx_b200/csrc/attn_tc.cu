@@ -531,6 +531,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(const __grid_consta
         const bool rope = P.rope_freqs != nullptr;
         const int pos = rope ? P.positions[qi] : 0;
         const bool bf = P.out_dtype == DSV4_BF16;
+        const bool by8 = (reinterpret_cast<uintptr_t>(P.out) & 7) == 0;  // else out goes element by element
 #pragma unroll 1
         for (int mt = 0; mt < 4; ++mt) {
           const int d = mt * 128 + qd * 32 + lane;
@@ -568,12 +569,22 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tc_kernel(const __grid_consta
             if (bf) {
               const uint32_t p0 = pack_bf16x2(y[0], z[0]), p1 = pack_bf16x2(y[1], z[1]);
               const uint32_t other = __shfl_xor_sync(0xffffffffu, upper ? p0 : p1, 2);
-              *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(P.out) + row0 + (upper ? 2 * D : 0) + (d & ~3)) =
-                  upper ? make_uint2(other, p1) : make_uint2(p0, other);
+              uint16_t* o = reinterpret_cast<uint16_t*>(P.out) + row0 + (upper ? 2 * D : 0) + (d & ~3);
+              const uint32_t lo = upper ? other : p0, hi = upper ? p1 : other;
+              if (by8) {
+                *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
+              } else {
+                o[0] = static_cast<uint16_t>(lo), o[1] = static_cast<uint16_t>(lo >> 16);
+                o[2] = static_cast<uint16_t>(hi), o[3] = static_cast<uint16_t>(hi >> 16);
+              }
             } else {
               float* o = reinterpret_cast<float*>(P.out) + row0 + (d & ~1);
-              *reinterpret_cast<float2*>(o) = make_float2(y[0], z[0]);
-              *reinterpret_cast<float2*>(o + 2 * D) = make_float2(y[1], z[1]);
+              if (by8) {
+                *reinterpret_cast<float2*>(o) = make_float2(y[0], z[0]);
+                *reinterpret_cast<float2*>(o + 2 * D) = make_float2(y[1], z[1]);
+              } else {
+                o[0] = y[0], o[1] = z[0], o[2 * D] = y[1], o[2 * D + 1] = z[1];
+              }
             }
           }
         }

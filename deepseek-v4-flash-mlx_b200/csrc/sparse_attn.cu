@@ -717,7 +717,7 @@ bool dsv4_hg_cluster_fits(int splits);
 // one CTA per (query, split). The plan (kernel and split count) is made in one place, for the
 // workspace size and for the launch.
 static bool tc_shape_ok(const dsv4_sparse_attn_params* p) {
-  return p->h == sa::HB && (p->q_dtype == DSV4_BF16 || p->q_norm_rope) && (reinterpret_cast<uintptr_t>(p->out) & 7) == 0;
+  return p->h == sa::HB && (p->q_dtype == DSV4_BF16 || p->q_norm_rope);
 }
 struct AttnPlan {
   bool tc;

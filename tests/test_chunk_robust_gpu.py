@@ -171,3 +171,28 @@ def test_window_rows_past_the_pool(kernel, s, linear):
         want, tol = _plain64(q, kv, sink, lists, pos, freqs)
         assert torch.isfinite(o).all(), (base, p)
         assert ((o.double() - want).abs() <= tol).all(), (base, p)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("s,kernel", [(20, 0), (20, 2), (3, 2), (200, 2)])
+def test_gathered_attention_into_an_output_at_any_element(dtype, s, kernel):
+    """An output that starts at any element of a tensor, and nothing beside it."""
+    S = importlib.import_module(PKG + ".sparse_attn")
+    _, _, L = _mods()
+    g = torch.Generator(device="cuda").manual_seed(s)
+    n, t = 700, 300
+    kv = torch.randn(n, 512, generator=g, device="cuda").to(torch.bfloat16)
+    q, sink = torch.randn(s, 64, 512, generator=g, device="cuda").to(torch.bfloat16), torch.randn(64, generator=g, device="cuda")
+    idx = torch.randint(-1, n, (s, t), generator=g, device="cuda", dtype=torch.int32)
+    pos = torch.arange(s, dtype=torch.int32, device="cuda")
+    freqs = 1.0 / (160000.0 ** (torch.arange(0, 64, 2, dtype=torch.float32, device="cuda") / 64))
+    size = s * 64 * 512
+    want = S.sparse_attn_into(torch.empty(s, 64, 512, device="cuda", dtype=dtype), q, kv, sink, idx, 512 ** -0.5, freqs, pos, 64,
+                              num_splits=1, kernel=2)
+    for at in (1, 2, 3, 4):
+        all_ = torch.full((size + 8,), 7.0, device="cuda", dtype=dtype)
+        out = all_[at:at + size].view(s, 64, 512)
+        S.sparse_attn_into(out, q, kv, sink, idx, 512 ** -0.5, freqs, pos, 64, num_splits=1, kernel=kernel)
+        assert torch.equal(out, want), at
+        assert (all_[:at] == 7).all() and (all_[at + size:] == 7).all()
+    assert L.device_error() == 0
