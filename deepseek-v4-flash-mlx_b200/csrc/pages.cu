@@ -86,13 +86,15 @@ __global__ void __launch_bounds__(COPY) free_kernel(dsv4_pages p, const int32_t*
 }
 
 // pages of its own for the entries of `tokens[k] + add` tokens of sequence seqs[k]; a sequence that
-// finds too few free pages gets none of them (DSV4_ERR_NO_PAGES on the error word)
+// finds too few free pages gets none of them (DSV4_ERR_NO_PAGES on the error word), and those behind it are
+// served from what it leaves. There are enough pages for all almost always, and then a scan hands them out; one
+// thread goes through the sequences in order where there are not.
 __global__ void __launch_bounds__(PLAN) reserve_kernel(dsv4_pages p, const int32_t* seqs, const int32_t* tokens, int add,
                                                        int n, int32_t* free_list) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  __shared__ int want[PLAN], held[PLAN];
+  __shared__ int want[PLAN], held[PLAN], from[PLAN];
   for (int base = 0; base < n; base += PLAN) {  // PLAN sequences at a time
     const int m = min(PLAN, n - base);
     for (int k = w; k < m; k += PLAN / 32) {
@@ -125,13 +127,24 @@ __global__ void __launch_bounds__(PLAN) reserve_kernel(dsv4_pages p, const int32
     const int at = block_scan(mine, &total);
     if (total == 0) continue;  // uniform
     const int got = lowest_free(p.refs, p.n_pages, total, free_list);
+    from[threadIdx.x] = at;
+    __syncthreads();
+    if (got < total && threadIdx.x == 0) {
+      for (int k = 0, used = 0; k < m; ++k) {
+        const bool fits = want[k] <= got - used;
+        from[k] = fits ? used : -1;
+        if (fits) used += want[k];
+      }
+    }
+    __syncthreads();
     if (mine > 0) {
-      if (at + mine > got) {
+      const int first = from[threadIdx.x];
+      if (first < 0) {
         raise_device_error(DSV4_ERR_NO_PAGES);
       } else {
         const int s = seqs ? seqs[base + threadIdx.x] : base + static_cast<int>(threadIdx.x);
         for (int j = 0; j < mine; ++j) {
-          const int32_t pg = free_list[at + j];
+          const int32_t pg = free_list[first + j];
           p.block_table[static_cast<int64_t>(s) * p.bt_stride + held[threadIdx.x] + j] = pg;
           p.refs[pg] = 1;
         }

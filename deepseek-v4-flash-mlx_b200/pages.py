@@ -76,7 +76,8 @@ def pages_free(cache, seqs):
 
 def pages_reserve(cache, seqs, tokens, add=0):
     """Pages for the compressed rows of `tokens + add` tokens of slots `seqs` (None: slot k for the
-    k-th count); pages they have stay. A slot that finds too few free pages gets none."""
+    k-th count); pages they have stay. A slot that finds too few free pages gets none, and those behind it
+    are served from what it leaves."""
     p = _params(cache)
     if seqs is None:
         tokens, = _ints("pages_reserve", cache, tokens)

@@ -196,3 +196,37 @@ def test_gathered_attention_into_an_output_at_any_element(dtype, s, kernel):
         assert torch.equal(out, want), at
         assert (all_[:at] == 7).all() and (all_[at + size:] == 7).all()
     assert L.device_error() == 0
+
+
+def _paged(slots, max_comp, page, n_pages):
+    _, Dm, _ = _mods()
+    return Dm.SparseMLACache(slots, max_comp, page=page, n_pages=n_pages)
+
+
+def test_a_reservation_that_cannot_be_met_leaves_the_others_theirs():
+    """In the order of the call, each sequence gets its pages if there are as many left; one that finds too few gets
+    none, and those behind it are served from what it left."""
+    _, _, L = _mods()
+    for wants in ([10, 2], [2, 10, 3], [10, 5], [6, 6, 6], [1, 5, 4, 1], [5], [0, 7, 0, 5], [3, 3, 2]):
+        c = _paged(len(wants) + 1, 640, 64, 5)
+        c.reserve(list(range(len(wants), 0, -1)), [256 * n for n in wants])
+        left, table, failed = 5, [[] for _ in range(len(wants) + 1)], False
+        for k, n in enumerate(wants):
+            if n <= left:
+                table[len(wants) - k] = list(range(5 - left, 5 - left + n))
+                left -= n
+            else:
+                failed = True
+        assert L.device_error() == (7 if failed else 0), wants
+        assert [[int(p) for p in row if p >= 0] for row in c.block_table.tolist()] == table, wants
+        assert c.page_refs.tolist() == [1] * (5 - left) + [0] * left, wants
+    # over a thousand sequences: the same in every planning batch
+    c = _paged(3000, 16, 8, 1500)
+    c.reserve(list(range(3000)), [64 if k % 3 == 1 else 32 for k in range(3000)])
+    left, at = 1500, []
+    for k in range(3000):
+        n = 2 if k % 3 == 1 else 1
+        at.append(n if n <= left else 0)
+        left -= at[-1]
+    assert L.device_error() == 7 and left == 0
+    assert (c.block_table >= 0).sum(1).tolist() == at and c.page_refs.tolist() == [1] * 1500
