@@ -100,8 +100,20 @@ __global__ void __launch_bounds__(PLAN) reserve_kernel(dsv4_pages p, const int32
     for (int k = w; k < m; k += PLAN / 32) {
       const int s = seqs ? seqs[base + k] : base + k;
       int need = 0, have = 0;
+      // a sequence named twice asks once, by its first mention, for the largest count (and again among the next
+      // PLAN, for what it does not have by then)
+      bool again = false;
+      int count = tokens[base + k];
+      if (seqs != nullptr)
+        for (int i = lane; i < m; i += 32)
+          if (seqs[base + i] == s) {
+            again |= i < k;
+            count = max(count, tokens[base + i]);
+          }
+      again = __any_sync(0xffffffffu, again);
+      count = __reduce_max_sync(0xffffffffu, count);
       if (s >= 0 && s < p.slots) {
-        const int64_t all = max(static_cast<int64_t>(0), static_cast<int64_t>(tokens[base + k]) + add) / p.ratio;
+        const int64_t all = max(static_cast<int64_t>(0), static_cast<int64_t>(count) + add) / p.ratio;
         if (all > p.max_comp && lane == 0) raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
         const int e = static_cast<int>(min(all, static_cast<int64_t>(p.max_comp)));
         need = (e + p.page - 1) / p.page;
@@ -112,12 +124,8 @@ __global__ void __launch_bounds__(PLAN) reserve_kernel(dsv4_pages p, const int32
       } else if (lane == 0) {
         raise_device_error(DSV4_ERR_INDEX_OUT_OF_RANGE);
       }
-      // a sequence named twice asks once: the later mention finds the earlier one
-      bool again = false;
-      for (int i = lane; i < k; i += 32) again |= (seqs ? seqs[base + i] : base + i) == s;
-      if (__any_sync(0xffffffffu, again)) need = 0;
       if (lane == 0) {
-        want[k] = max(0, need - have);
+        want[k] = again ? 0 : max(0, need - have);
         held[k] = have;
       }
     }

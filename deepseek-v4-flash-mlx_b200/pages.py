@@ -6,8 +6,8 @@ will write to (the last partial page, the window ring, the compressor rings) and
 which are laid out by slot. Tables and counts stay on the device: every call is asynchronous on the
 current stream, can be captured in a CUDA graph, and gives the same tables for the same input. What a
 call cannot do for one sequence it leaves out for that sequence, and raises the device error word
-(`_lib.device_error`): NO_PAGES, or INDEX_OUT_OF_RANGE for a slot that does not exist, more tokens
-than the cache holds, or a branch onto a slot that has pages. A window-only cache (no compressed rows)
+(`_lib.device_error`): NO_PAGES, or INDEX_OUT_OF_RANGE for a slot that does not exist, a branch of more
+tokens than the cache or its source's pages hold, or a branch onto a slot that has pages. A window-only cache (no compressed rows)
 has no pages: it is branched by a copy of the window ring, and the other calls leave it as it is.
 """
 import ctypes
@@ -77,7 +77,8 @@ def pages_free(cache, seqs):
 def pages_reserve(cache, seqs, tokens, add=0):
     """Pages for the compressed rows of `tokens + add` tokens of slots `seqs` (None: slot k for the
     k-th count); pages they have stay. A slot that finds too few free pages gets none, and those behind it
-    are served from what it leaves."""
+    are served from what it leaves; one named twice gets the pages of the larger count. A count past the
+    cache gets all the pages that the slot has entries for, and raises INDEX_OUT_OF_RANGE; one below 0 is none."""
     p = _params(cache)
     if seqs is None:
         tokens, = _ints("pages_reserve", cache, tokens)

@@ -492,7 +492,10 @@ typedef struct {
 DSV4_API size_t dsv4_pages_workspace_size(const dsv4_pages* p, int32_t n);
 /* the slots' pages given back, their table rows emptied */
 DSV4_API int dsv4_pages_free(const dsv4_pages* p, const int32_t* seqs, int32_t n, void* stream);
-/* pages for the entries of tokens[k] + add tokens of slot seqs[k] (NULL: slot k) */
+/* pages for the entries of tokens[k] + add tokens of slot seqs[k] (NULL: slot k). In the order of the call:
+ * a slot that finds too few free pages gets none (DSV4_ERR_NO_PAGES), and those behind it are served from
+ * what it leaves. A slot named twice gets the pages of its largest count; a count past the cache all that
+ * max_comp entries need, and DSV4_ERR_INDEX_OUT_OF_RANGE; one below 0 none. */
 DSV4_API int dsv4_pages_reserve(const dsv4_pages* p, const int32_t* seqs, const int32_t* tokens, int32_t add, int32_t n,
                                 void* workspace, size_t workspace_bytes, void* stream);
 /* slot dst[k] (its table row empty) becomes a branch of slot src[k], which holds tokens[k] tokens: full

@@ -230,3 +230,19 @@ def test_a_reservation_that_cannot_be_met_leaves_the_others_theirs():
         left -= at[-1]
     assert L.device_error() == 7 and left == 0
     assert (c.block_table >= 0).sum(1).tolist() == at and c.page_refs.tolist() == [1] * 1500
+
+
+def test_a_slot_named_twice_gets_the_pages_of_its_largest_count():
+    _, _, L = _mods()
+    c = _paged(3, 640, 64, 20)
+    c.reserve([0, 1, 0, 2, 0], [4, 256, 1000, 300, 512])
+    assert L.device_error() == 0
+    assert c.block_table.tolist() == [[0, 1, 2, 3] + [-1] * 6, [4] + [-1] * 9, [5, 6] + [-1] * 8]
+    assert c.page_refs.tolist() == [1] * 7 + [0] * 13
+    c.reserve([1, 1], [8, 256 * 10], add=0)
+    assert (c.block_table[1] >= 0).all() and L.device_error() == 0
+    c.free([0, 1, 2])
+    # mentions more than a planning batch apart
+    big = _paged(1100, 16, 8, 1200)
+    big.reserve([7] + list(range(1100)) + [7], [4] + [4] * 1100 + [64])
+    assert L.device_error() == 0 and big.block_table[7].tolist() == [0, 1100]
