@@ -161,8 +161,14 @@ class SparseMLACache:
         return self.win_base[b] + positions % self.window
 
     def fill_compressed(self, b, rows_bf16, keys_f32):
-        """Place n compressed rows (and their indexer keys) of sequence b (prefill hand-off)."""
+        """Place n compressed rows (and their indexer keys) of sequence b (prefill hand-off). In a paged cache
+        the slot must hold their pages (`reserve`), and hold them alone (a look at the table, so a wait for the device)."""
         n = rows_bf16.shape[0]
+        if self.page_refs is not None:
+            pages = self.block_table[b, :math.ceil(n / self.page)].long()
+            if n > self.max_comp or bool((pages < 0).any()) or bool((self.page_refs[pages] > 1).any()):
+                raise ValueError(f"SparseMLACache.fill_compressed: slot {b} does not hold the pages of {n} compressed rows, "
+                                 "or shares one with another slot")
         j = torch.arange(n, device=rows_bf16.device)
         self.kv_pool[self.comp_rows(b, j)] = rows_bf16.to(torch.bfloat16)
         self.k_idx[b, :n] = keys_f32

@@ -124,3 +124,27 @@ def test_a_chunk_of_keys_refuses_an_image_that_is_not_the_slots():
             image[k] = torch.empty_like(image[k], device="cuda:1")
             with pytest.raises(ValueError):
                 call(tuple(image))
+
+
+def test_rows_are_filled_into_pages_that_the_slot_holds_alone():
+    """A cell without a page is -1: rows put there would land in front of the pages, in the window rings."""
+    _, D = _mods()
+    c = D.SparseMLACache(3, 100, device="cpu", page=16, n_pages=9)
+    rows, keys = torch.ones(20, 512), torch.ones(20, 128)
+    for table in ([-1] * 7, [4, -1, -1, -1, -1, -1, -1]):
+        c.block_table[1] = torch.tensor(table, dtype=I32)
+        with pytest.raises(ValueError, match="page"):
+            c.fill_compressed(1, rows, keys)
+        assert not c.kv_pool.any() and not c.k_idx.any() and not c.image_stale
+    c.block_table[1, :2] = torch.tensor([4, 2], dtype=I32)
+    c.page_refs[4], c.page_refs[2] = 2, 1
+    with pytest.raises(ValueError, match="page"):
+        c.fill_compressed(1, rows, keys)          # another slot reads the first page
+    assert not c.kv_pool.any()
+    c.fill_compressed(1, rows[:0], keys[:0])
+    c.page_refs[4] = 1
+    c.fill_compressed(1, rows, keys)
+    at = c.comp_base + torch.cat([4 * 16 + torch.arange(16), 2 * 16 + torch.arange(4)])
+    assert (c.kv_pool[at] == 1).all() and c.kv_pool.float().sum() == 20 * 512 and c.k_idx.sum() == 20 * 128
+    with pytest.raises(ValueError):
+        c.fill_compressed(1, torch.ones(101, 512), torch.ones(101, 128))
