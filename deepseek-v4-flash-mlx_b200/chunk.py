@@ -185,7 +185,10 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
     outside of q), is not defined. Without `rows` the tokens of a sequence are taken in pairs: a row that is
     not finite and seen by the second token of a pair reaches the first one's output too. The custom op
     `dsv4::chunk_attention`."""
-    L.require_cuda(q, sink, rows, freqs)
+    index = cache.kv_pool.get_device()
+    if not L.one_device(index, (q, sink, rows, freqs)):
+        L.require_cuda(q, sink, rows, freqs)
+        raise ValueError("chunk_attention: q, sink, rows and freqs must be on the cache's device")
     shape = q.shape
     if len(shape) != 3 or shape[2] != 512 or cache.head_dim != 512:
         raise ValueError(f"chunk_attention: q must be [total, 64, 512] over a cache of 512-wide rows, got {tuple(q.shape)} and "
@@ -196,10 +199,6 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
         raise ValueError(f"chunk_attention: 64 heads, got q {tuple(q.shape)} and {sink.numel()} sinks")
     if out_dtype != torch.bfloat16 and out_dtype != torch.float32:
         raise TypeError(f"chunk_attention: out_dtype must be bfloat16 or float32, got {out_dtype}")
-    index = cache.kv_pool.get_device()
-    if q.get_device() != index or sink.get_device() != index or (rows is not None and rows.get_device() != index) or \
-            (freqs is not None and freqs.get_device() != index):
-        raise ValueError("chunk_attention: q, sink, rows and freqs must be on the cache's device")
     total = shape[0]
     if rows is not None:
         if rows.dim() != 2 or rows.shape[0] != total or rows.dtype not in (torch.int32, torch.int64):

@@ -315,7 +315,7 @@ def compressor_chunk(proj, cu_seqlens, start, ape, norm_w, ring_kv, ring_score, 
     `rotate` as in `compressor_decode_step`. The custom op `dsv4::compressor_chunk`."""
     kv, score = proj
     tensors, index = (kv, score, cu_seqlens, start, seqs, ape, norm_w, ring_kv, ring_score, out, block_table, freqs), kv.get_device()
-    if index < 0 or any(t is not None and t.get_device() != index for t in tensors):
+    if not L.one_device(index, tensors):
         L.require_cuda(*tensors)
         raise ValueError("compressor_chunk: every tensor must be on the projections' device")
     f32 = torch.float32
