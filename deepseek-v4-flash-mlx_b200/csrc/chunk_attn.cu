@@ -23,7 +23,10 @@
 // brings it in (boxes of min(64, the power of two that divides the page) rows), coordinates past the
 // pool for what is not there (TMA fills zeros). Visibility is a 64-bit mask per half and token. Rows
 // that neither token of the pair sees are zeroed in shared memory before they are used as values, so
-// that whatever they hold stays out; a row that one of the two sees is finite or spoils both.
+// that whatever they hold stays out. A row that one of the two sees alone (the window's oldest, the second
+// token's own, the entry that it completes: at least 32 rows apart) is a value of both, with a weight of 0 for the
+// other. If it is not finite, neither is any head's score of it: that is looked at while V is loaded, and then what
+// of the row is not finite is zeroed too, and the weight of the token that sees it made NaN.
 //
 // The kernel is persistent: a cluster takes pairs of tokens from a static list, the longest first, and
 // the next pair's loads and S run under the last pair's epilogue.
@@ -174,6 +177,12 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, relative error about 2^
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+// a pair of bf16 with 0 in place of what is not finite
+__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t v) {
+  if ((v & 0x7f80u) == 0x7f80u) v &= 0xffff0000u;
+  if ((v & 0x7f800000u) == 0x7f800000u) v &= 0xffffu;
+  return v;
 }
 __device__ __forceinline__ void smx_bar() { asm volatile("bar.sync 1, %0;\n" ::"n"(SMX_THREADS) : "memory"); }
 // the two warps that hold the same columns of O
@@ -587,13 +596,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
         // what of this warp's 32 rows is seen, by the CTA's token and by either token of the pair: all of
         // them, but for the ring, the stage and the last entries
         const int h = 2 * (w.tile0 + i) + kvh;
-        uint32_t see = 0xffffffffu, either = 0xffffffffu;
+        uint32_t see = 0xffffffffu, either = 0xffffffffu, one = 0;  // one: seen by one of two tokens alone, a row at most
         if (h < u.nring + u.nstage || 64 * (h - u.nring - u.nstage) + 64 > u.seen[0]) {
           const int j = 32 * ch + lane;
           const bool v0 = h < u.nh && half_sees(P.c, u, h, j, u.p0, u.seen[0]);
           const bool v1 = h < u.nh && u.n > 1 && half_sees(P.c, u, h, j, u.p0 + 1, u.seen[1]);
           see = __ballot_sync(0xffffffffu, second ? v1 : v0);
           either = __ballot_sync(0xffffffffu, v0 || v1);
+          one = __ballot_sync(0xffffffffu, u.n > 1 && v0 != v1);
         }
         // a wait that ran out takes the CTA's warps to the end together, from the next smx_any
         ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.s_full[b], (g >> 1) & 1, abort));
@@ -668,15 +678,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
           *reinterpret_cast<uint4*>(prow + (((ch * 4 + c4) ^ (head & 7)) << 4)) = make_uint4(e2[0], e2[1], e2[2], e2[3]);
         }
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        if (one != 0 && ok) {
+          // Is that row finite? If it is not, none of the heads' scores of it is. (While V is on its way.)
+          const int e = __ffs(one) - 1;
+          const float s = tmem_ld1(tmem + lanes + COL_S + 64 * b + 32 * ch + e);
+          const bool off = s * 0.f != 0.f;
+          if (!__any_sync(0xffffffffu, off)) {
+            one = 0;
+          } else if (off && (see & one) != 0) {  // this CTA's token has it, whatever its weight came out as
+            *reinterpret_cast<uint16_t*>(prow + (((ch * 4 + (e >> 3)) ^ (head & 7)) << 4) + 2 * (e & 7)) = 0x7fff;
+            l = __int_as_float(0x7fc00000);
+          }
+        }
         ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.v_full[b], (g >> 1) & 1, abort));
         if (!ok) {  // the CTA's other warps end at their next wait or at smx_any
           if (lane == 0) set_abort(sm);
-        } else if (either != 0xffffffffu && h < u.nh) {
-          // values of rows that neither token sees: two slabs of the slot for this warp, 16 lanes a row
+        } else if ((either != 0xffffffffu || one != 0) && h < u.nh) {
+          // values of rows that neither token sees, two slabs of the slot for this warp, 16 lanes a row; and what is not
+          // finite of those that one alone sees
           uint8_t* slab = sm.kv[b][kvh] + (2 * (quad & 1) + ((lane >> 3) & 1)) * SLAB;
           for (int e = lane >> 4; e < 32; e += 2)
             if (!((either >> e) & 1))
               *reinterpret_cast<uint4*>(slab + (32 * ch + e) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+          if (one != 0 && lane < 16) {
+            uint4* at = reinterpret_cast<uint4*>(slab + (32 * ch + __ffs(one) - 1) * 128 + (lane & 7) * 16);
+            *at = make_uint4(finite_bf16x2(at->x), finite_bf16x2(at->y), finite_bf16x2(at->z), finite_bf16x2(at->w));
+          }
         }
         fence_async_smem();
         before_sync();

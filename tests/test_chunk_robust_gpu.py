@@ -246,3 +246,41 @@ def test_a_slot_named_twice_gets_the_pages_of_its_largest_count():
     big = _paged(1100, 16, 8, 1200)
     big.reserve([7] + list(range(1100)) + [7], [4] + [4] * 1100 + [64])
     assert L.device_error() == 0 and big.block_table[7].tolist() == [0, 1100]
+
+
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("start,n", [(1000, 2), (1002, 2), (1022, 2), (130, 3), (4, 2), (5000, 1), (2047, 64)])
+@pytest.mark.parametrize("splits", [0, 1, 3])
+def test_rows_that_only_one_of_two_tokens_sees(what, start, n, splits):
+    """A row that is not finite reaches the tokens that see it and no others: a later draft's row, the entry that a later
+    token completes, the ring's row that has left a later token's window; in one dim or in all."""
+    pkg, Dm, L = _mods()
+    g = torch.Generator(device="cuda").manual_seed(start)
+    c = Dm.SparseMLACache(1, (start + n) // 4 + 1, page=16, max_chunk=n)
+    c.kv_pool.copy_(torch.randn(c.kv_pool.shape, generator=g, device="cuda"))
+    q, sink = torch.randn(n, 64, 512, generator=g, device="cuda").to(torch.bfloat16), torch.randn(64, generator=g, device="cuda")
+    call = lambda: pkg.chunk_attention(c, q, sink, _i32(0, n), _i32(start), num_splits=splits)  # noqa: E731
+    clean = call()
+    assert torch.isfinite(clean).all()
+    e = torch.arange((start + n) // 4, device="cuda")
+    # (pool row, the first and the last token that see it)
+    rows = [(c.stage_base + i, i, n - 1) for i in range(n)]
+    rows += [(int(c.comp_rows(0, e[-1])), max(0, 4 * int(e[-1]) + 3 - start), n - 1)]
+    if start >= 127:
+        rows += [((start - 127) % 128, 0, 0), ((start - 126) % 128, 0, min(1, n - 1))]
+    for row, first, last in rows[-5:]:
+        for dims in (slice(0, 512), slice(77, 78), slice(300, 301), slice(511, 512)):
+            was = c.kv_pool[row].clone()
+            c.kv_pool[row, dims] = what
+            o = call()
+            for i in range(n):
+                if first <= i <= last:
+                    # every head has it in its score, as NaN or as an infinity; where all tokens of a pair see the row, a
+                    # head whose score is -inf gives it a weight of 0, and may leave it out
+                    finite = torch.isfinite(o[i]).all(-1)
+                    alone = i // 2 * 2 < first or min(i // 2 * 2 + 1, n - 1) > last
+                    assert not finite.any() if alone else not finite.all(), (row, i)
+                else:
+                    assert torch.equal(o[i], clean[i]), (row, i)
+            c.kv_pool[row] = was
+    assert torch.equal(call(), clean) and L.device_error() == 0
