@@ -793,6 +793,7 @@ __global__ void __launch_bounds__(G == 1 ? THREADS : G * D / 2, G == 1 ? 2 : 1)
     if (sc_ >= STAGES) sc_ -= STAGES, pc ^= 1;
     if (__syncthreads_or(!ok)) {
       if (threadIdx.x == 0) raise_device_error(DSV4_ERR_WAIT_TIMEOUT);
+      ok = false;  // of every thread: the one that waits for the copies below is not the one whose wait ran out
       break;
     }
     load_to(min(nb + 1, i0 + G - 1 + STAGES));  // blocks up to i0 + G - 2 have been read
