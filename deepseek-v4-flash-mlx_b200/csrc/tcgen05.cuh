@@ -93,16 +93,6 @@ __device__ __forceinline__ bool bar_try(uint32_t a, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// whether the phase with the given parity has completed, without waiting
-__device__ __forceinline__ bool bar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
 // The time limit of a wait. Reading %globaltimer takes several hundred cycles, so it is looked at only
 // every 64th unsuccessful try.
 struct WaitLimit {
