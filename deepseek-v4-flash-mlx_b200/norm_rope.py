@@ -48,9 +48,13 @@ _freq_cache = {}
 
 
 def rope_freqs(rope_dim=64, device="cuda", **yarn):
-    """Device copy of the YaRN frequency table (cached per device and settings)."""
+    """Device copy of the YaRN frequency table (cached per device and settings, but for modes that take torch's
+    calls: fake tensors stay with them)."""
     cfg = dict(YARN_COMPRESSED)
     cfg.update(yarn)
+    if not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() > 0:
+        return precompute_freqs(rope_dim, 0, cfg["original_seq_len"], cfg["base"], cfg["factor"], cfg["beta_fast"],
+                                cfg["beta_slow"]).to(device)
     key = (rope_dim, str(torch.device(device)), tuple(sorted(cfg.items())))
     t = _freq_cache.get(key)
     if t is None:

@@ -148,3 +148,18 @@ def test_rows_are_filled_into_pages_that_the_slot_holds_alone():
     assert (c.kv_pool[at] == 1).all() and c.kv_pool.float().sum() == 20 * 512 and c.k_idx.sum() == 20 * 128
     with pytest.raises(ValueError):
         c.fill_compressed(1, torch.ones(101, 512), torch.ones(101, 128))
+
+
+def test_default_frequencies_are_kept_for_real_calls_only():
+    """The table that a call without `freqs` takes is kept between calls; not one without data, nor one for a mode."""
+    pkg, _ = _mods()
+    N = importlib.import_module(PKG + ".norm_rope")
+    real = N.rope_freqs(64, "cpu", base=12345.0)
+    with FakeTensorMode():
+        c, args = _attention_args()
+        assert pkg.chunk_attention(c, *args).shape == (7, 64, 512)
+        assert type(N.rope_freqs(64, "cpu", base=12345.0)) is not torch.Tensor
+        assert type(N.rope_freqs(32, "cpu", base=12345.0)) is not torch.Tensor
+    assert N.rope_freqs(64, "cpu", base=12345.0) is real
+    assert type(N.rope_freqs(32, "cpu", base=12345.0)) is torch.Tensor
+    assert all(type(t) is torch.Tensor for t in N._freq_cache.values())
