@@ -182,8 +182,8 @@ def chunk_attention(cache, q, sink, cu_seqlens, start, seqs=None, rows=None, sca
     indexer's selection) those instead. `num_splits`: over how many CTA pairs the rows of two tokens are split
     (0: automatic; all visible rows only). Returns o [total, 64, 512] after the inverse RoPE; what it holds
     behind the last sequence, and for a sequence that the error word reports (a slot that does not exist, tokens
-    outside of q), is not defined. A row that is not finite reaches the tokens that see it and no others. The
-    custom op `dsv4::chunk_attention`."""
+    outside of q), is not defined. A row that is not finite reaches the tokens that see it and no others (a
+    head that scores it -inf weighs it 0 and may leave it out). The custom op `dsv4::chunk_attention`."""
     index = cache.kv_pool.get_device()
     if not L.one_device(index, (q, sink, rows, freqs)):
         L.require_cuda(q, sink, rows, freqs)

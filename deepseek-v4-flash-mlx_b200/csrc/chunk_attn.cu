@@ -24,9 +24,11 @@
 // pool for what is not there (TMA fills zeros). Visibility is a 64-bit mask per half and token. Rows
 // that neither token of the pair sees are zeroed in shared memory before they are used as values, so
 // that whatever they hold stays out. A row that one of the two sees alone (the window's oldest, the second
-// token's own, the entry that it completes: at least 32 rows apart) is a value of both, with a weight of 0 for the
-// other. If it is not finite, neither is any head's score of it: that is looked at while V is loaded, and then what
-// of the row is not finite is zeroed too, and the weight of the token that sees it made NaN.
+// token's own, the entry that it completes) is a value of both, with a weight of 0 for the other: what of it
+// is not finite is zeroed too, by the warp that loads V, which knows these rows for the whole unit (2,048 tokens at
+// 16,384 at full clock: 948 us, 933 without; in the softmax warps, whichever way it was written, 960 to 978, in a
+// warp of its own 970, since one more that looks at a barrier slows the others). The token that sees the row has it
+// from its scores, which are not finite either; a head that scores it -inf weighs it 0 and leaves it out.
 //
 // The kernel is persistent: a cluster takes pairs of tokens from a static list, the longest first, and
 // the next pair's loads and S run under the last pair's epilogue.
@@ -285,6 +287,21 @@ __device__ __forceinline__ bool half_sees(const dsv4_chunk& c, const Unit& u, in
   return 64 * (h - u.nstage) + j < entries;
 }
 
+// The rows of a pair's halves (64 * half + row) that one of its two tokens alone sees, a lane each: 0 the oldest of the
+// first's window, 1 the second's own, 2 the entry that it completes. -1 where there is none.
+__device__ __forceinline__ int alone_row(const Params& P, const Unit& u, int lane) {
+  if (u.n < 2 || lane > 2) return -1;
+  if (lane == 1) return 64 * u.nring + (u.p0 + 1 - u.stage_pos);
+  if (lane == 2) return u.seen[1] > u.seen[0] ? 64 * (u.nring + u.nstage) + u.seen[0] : -1;
+  const int pos = u.p0 - P.c.window + 1;
+  if (pos < 0) return -1;
+  if (pos >= u.start) return 64 * u.nring + (pos - u.stage_pos);
+  const int slot = P.by_window.rem(pos);
+  for (int k = 0; k < u.nring; ++k)
+    if (static_cast<int>((u.ring >> (4 * k)) & 15) == slot >> 6) return 64 * k + (slot & 63);
+  return -1;
+}
+
 // The work of a cluster: units (pair of tokens, split) number `at`, at + clusters, ...; the pairs are counted
 // through the sequences and taken from the last to the first, since the last see the most rows. A warp looks
 // together, a lane per sequence, 32 at a time (and keeps the first 32).
@@ -377,7 +394,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
         bar_init(&sm.kv_free[i][x], 1);
       }
       bar_init(&sm.s_full[i], 1);
-      bar_init(&sm.p_full[i], 2 * SMX_WARPS);
+      bar_init(&sm.p_full[i], 2 * (SMX_WARPS + 1));  // and the warps that load V
       bar_init(&sm.v_full[i], 1);
     }
     sm.abort = 0;
@@ -470,6 +487,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
     for (; ok && has; has = w.next(P), looked = false) {
       if (w.nt == 0) continue;
       int row = looked ? first_row : tile_row(P, w.u, 2 * w.tile0 + 1 - static_cast<int>(rank), lane, boxes);
+      int alone = alone_row(P, w.u, lane);  // lanes 0 to 2
+      if (alone >= 0) alone -= 128 * w.tile0;
       for (int i = 0; i < w.nt; ++i, ++g) {
         const int b = g & 1;
         if (!(ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.s_full[b], (g >> 1) & 1, abort)))) break;
@@ -485,6 +504,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
           }
         }
         if (i + 1 < w.nt) row = tile_row(P, w.u, 2 * (w.tile0 + i + 1) + 1 - static_cast<int>(rank), lane, boxes);
+        uint32_t here = __ballot_sync(0xffffffffu, alone >> 7 == i);
+        if (here != 0) {  // rows of this tile that one token alone sees: 512 bytes of this CTA's dims each, 16 a lane
+          if (!(ok = __all_sync(0xffffffffu, bar_wait_or_abort(&sm.v_full[b], (g >> 1) & 1, abort)))) {
+            ++g;  // its load is under way
+            break;
+          }
+          for (; here != 0; here &= here - 1) {
+            const int r = __shfl_sync(0xffffffffu, alone, __ffs(here) - 1) & 127;
+            uint4* at = reinterpret_cast<uint4*>(sm.kv[b][r >> 6] + (lane >> 3) * SLAB + (r & 63) * 128 + (lane & 7) * 16);
+            const uint4 v = *at;
+            *at = make_uint4(finite_bf16x2(v.x), finite_bf16x2(v.y), finite_bf16x2(v.z), finite_bf16x2(v.w));
+          }
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) arrive_at(in_cta(&sm.p_full[b], 0));
       }
       if (!ok) {
         if (lane == 0) set_abort(sm);
@@ -596,14 +631,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
         // what of this warp's 32 rows is seen, by the CTA's token and by either token of the pair: all of
         // them, but for the ring, the stage and the last entries
         const int h = 2 * (w.tile0 + i) + kvh;
-        uint32_t see = 0xffffffffu, either = 0xffffffffu, one = 0;  // one: seen by one of two tokens alone, a row at most
+        uint32_t see = 0xffffffffu, either = 0xffffffffu;
         if (h < u.nring + u.nstage || 64 * (h - u.nring - u.nstage) + 64 > u.seen[0]) {
           const int j = 32 * ch + lane;
           const bool v0 = h < u.nh && half_sees(P.c, u, h, j, u.p0, u.seen[0]);
           const bool v1 = h < u.nh && u.n > 1 && half_sees(P.c, u, h, j, u.p0 + 1, u.seen[1]);
           see = __ballot_sync(0xffffffffu, second ? v1 : v0);
           either = __ballot_sync(0xffffffffu, v0 || v1);
-          one = __ballot_sync(0xffffffffu, u.n > 1 && v0 != v1);
         }
         // a wait that ran out takes the CTA's warps to the end together, from the next smx_any
         ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.s_full[b], (g >> 1) & 1, abort));
@@ -678,32 +712,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) chunk_at
           *reinterpret_cast<uint4*>(prow + (((ch * 4 + c4) ^ (head & 7)) << 4)) = make_uint4(e2[0], e2[1], e2[2], e2[3]);
         }
         l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-        if (one != 0 && ok) {
-          // Is that row finite? If it is not, none of the heads' scores of it is. (While V is on its way.)
-          const int e = __ffs(one) - 1;
-          const float s = tmem_ld1(tmem + lanes + COL_S + 64 * b + 32 * ch + e);
-          const bool off = s * 0.f != 0.f;
-          if (!__any_sync(0xffffffffu, off)) {
-            one = 0;
-          } else if (off && (see & one) != 0) {  // this CTA's token has it, whatever its weight came out as
-            *reinterpret_cast<uint16_t*>(prow + (((ch * 4 + (e >> 3)) ^ (head & 7)) << 4) + 2 * (e & 7)) = 0x7fff;
-            l = __int_as_float(0x7fc00000);
-          }
-        }
         ok = ok && __all_sync(0xffffffffu, bar_wait_or_abort(&sm.v_full[b], (g >> 1) & 1, abort));
         if (!ok) {  // the CTA's other warps end at their next wait or at smx_any
           if (lane == 0) set_abort(sm);
-        } else if ((either != 0xffffffffu || one != 0) && h < u.nh) {
-          // values of rows that neither token sees, two slabs of the slot for this warp, 16 lanes a row; and what is not
-          // finite of those that one alone sees
+        } else if (either != 0xffffffffu && h < u.nh) {
+          // values of rows that neither token sees: two slabs of the slot for this warp, 16 lanes a row
           uint8_t* slab = sm.kv[b][kvh] + (2 * (quad & 1) + ((lane >> 3) & 1)) * SLAB;
           for (int e = lane >> 4; e < 32; e += 2)
             if (!((either >> e) & 1))
               *reinterpret_cast<uint4*>(slab + (32 * ch + e) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-          if (one != 0 && lane < 16) {
-            uint4* at = reinterpret_cast<uint4*>(slab + (32 * ch + __ffs(one) - 1) * 128 + (lane & 7) * 16);
-            *at = make_uint4(finite_bf16x2(at->x), finite_bf16x2(at->y), finite_bf16x2(at->z), finite_bf16x2(at->w));
-          }
         }
         fence_async_smem();
         before_sync();
