@@ -44,13 +44,13 @@
 // Long lists with few tokens are split over clusters; fp32 partials and a merging kernel follow.
 // All waits inside a CTA are bounded (1 s): DSV4_ERR_WAIT_TIMEOUT, and the pair drains and leaves.
 //
-// Measured on a B200: 2048 tokens at position 16384 (1.2 TFLOP) take 0.91 ms, 1.32 PFLOP/s or 0.79 of a large
-// library product's burst rate, with the tensor pipe active 72% of the time and HBM at 3%; 1.02 ms under the power cap
-// (1545 MHz), 0.84 of the same product's sustained rate. A tile's MMAs take 2093 cycles and a tile 2900: of
+// Measured on a B200: 2048 tokens at position 16384 (1.2 TFLOP) take 0.95 ms at full clock, 1.27 PFLOP/s or 0.76 of a
+// large library product's burst rate, with the tensor pipe active 72% of the time and HBM at 3%; 1.03 ms under the power
+// cap (1545 MHz), 0.83 of the same product's sustained rate. A tile's MMAs take 2093 cycles and a tile 2900: of
 // two buffers one is being refilled (a load's latency, S behind the other tile's O, softmax), and a third does
 // not fit. A pair of tokens costs 7000 cycles beside its tiles (the last O, the epilogue, the next unit's first
-// softmax, by the same warps). Few tokens are bound by latency: 32 at position 2048 take 17.6 us and one at
-// 65536 16.9 us (16 MB of rows, 2.6 us of HBM), of which the launch and the first rows are 5, the partials'
+// softmax, by the same warps). Few tokens are bound by latency: 32 at position 2048 take 17.9 us and one at
+// 65536 17.0 us (16 MB of rows, 2.6 us of HBM), of which the launch and the first rows are 5, the partials'
 // stores 1 (an SM writes 32 bytes a cycle; 17.8 us when one CTA of the pair stored them all) and the merging
 // kernel 6.
 #include <cudaTypedefs.h>

@@ -664,11 +664,12 @@ __device__ __forceinline__ void chunk_sequence(const dsv4_compressor_chunk_param
 // block's tokens are consecutive, so one bulk copy each brings kv and score (16 KB each at 512 dims) into a
 // ring of 2 G + 1 buffers, G blocks ahead of those that are computed and without a thread waiting for any
 // address; every block is read once and serves two rows, but for the one before a run (half of its columns
-// again, 1 / run). The arithmetic (about 500 instructions a warp and row: 16 exponentials and 2 divisions
-// a thread, as the decode step has them) is as long as the reads, so as many warps as registers allow run
-// at once: 512 dims with G = 3 (24 warps, 224 KB) in one CTA an SM. The row-at-a-time form above looks its
-// row up, loads, sums and stores in turn: 53 us for 16384 tokens; two CTAs of G = 1 took 33 us, this 30 (139 MB,
-// 4.6 TB/s).
+// again, 1 / run). The arithmetic is about 490 instructions a warp and row (16 exponentials and 2 divisions
+// a thread, as the decode step has them), so as many warps as registers allow run at once: 512 dims with G = 3
+// (24 warps, 224 KB) in one CTA an SM. The row-at-a-time form above looks its row up, loads, sums and stores in
+// turn: 53 us for 16384 tokens; two CTAs of G = 1 took 33 us, this 30 (139 MB, 4.6 TB/s). Neither the issue slots
+// (40% used) nor HBM (50%) bound it: the CTA's barrier of every round, at which three groups wait for the slowest, is the
+// longest stall.
 template <int D, int G>  // D: head_dim where it is known (addresses fold into the loads), 0: any
 struct Run {
   static constexpr int STAGES = 2 * G + 1;

@@ -417,7 +417,8 @@ DSV4_API int dsv4_chunk_commit(const dsv4_chunk* c, void* pool, int32_t dim, voi
  * rows staged and the entries written. q after the per-head norm and RoPE; o after the inverse RoPE of
  * its last rope_dim dims (rope_freqs == NULL: none). 64 heads of 512, a window of at most 1024, pages of
  * a multiple of 8 rows. Rows of out behind the last sequence are not written. A row that is not finite
- * reaches the tokens that see it and no others (a head that scores it -inf weighs it 0 and may leave it out). An entry whose page the sequence does not have counts as a row of zeros and raises
+ * reaches the tokens that see it and no others (a head that scores it -inf weighs it 0 and may leave it
+ * out). An entry whose page the sequence does not have counts as a row of zeros and raises
  * DSV4_ERR_INDEX_OUT_OF_RANGE. */
 typedef struct {
   dsv4_chunk chunk;
